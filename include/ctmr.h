@@ -431,6 +431,51 @@ int64_t ctmr_flash_attention_f16x2_workspace_bytes(const ctmr_attn_desc* desc);
 int ctmr_flash_attention_f16x2(const ctmr_attn_desc* desc, const float* q, const float* k, const float* v,
                                float* out, void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * Differentiable operators of the attention blocks, for activations of fp32,
+ * bf16 or fp16.  No counterparts in the reference, which is inference only.
+ * Sums, statistics and softmax are held in fp32 or fp64; each output is rounded
+ * once.  No atomics: results are bit-identical run to run.  Like every entry
+ * point they neither allocate nor synchronise, so calls may be captured into a
+ * graph; two captures need workspaces of their own.
+ */
+enum ctmr_elem { CTMR_ELEM_F32 = 0, CTMR_ELEM_BF16 = 1, CTMR_ELEM_F16 = 2 };
+
+/* Group norm (+ SiLU) of channels-last rows x (n, s voxels, c), statistics over
+ * s x (c / groups) values, biased variance.  gamma and beta (c) are of type
+ * param_elem.  saved (n, groups, 4) fp32, 16-byte aligned, is what the backward
+ * call reads: the mean as two floats, 1 / sqrt(var + eps), and one unused.
+ * y may equal x.  The workspace is 16-byte aligned (0 bytes for small groups). */
+int64_t ctmr_norm_workspace_bytes(int32_t n, int64_t s, int32_t c, int32_t groups, int32_t elem, int32_t backward);
+int ctmr_norm_forward(int32_t n, int64_t s, int32_t c, int32_t groups, float eps, int32_t elem, const void* x,
+                      int32_t param_elem, const void* gamma, const void* beta, int32_t silu, void* y, float* saved,
+                      void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients of x, gamma and beta from dy (x's type); dx, or dgamma and dbeta together, may be NULL.
+ * dgamma and dbeta have type param_elem.  dx may equal dy or x. */
+int ctmr_norm_backward(int32_t n, int64_t s, int32_t c, int32_t groups, int32_t elem, const void* x, const void* dy,
+                       int32_t param_elem, const void* gamma, const void* beta, int32_t silu, const float* saved,
+                       void* dx, void* dgamma, void* dbeta, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotary positions.  q (n, q_heads, l, head_dim) and k (n, k_heads, l, head_dim;
+ * k_heads 0: none) have strides in values for the first three axes and a unit
+ * last one.  The head's first values are a section of widths[a] values for each
+ * axis a; value i < widths[a] / 2 of it and value i + widths[a] / 2 turn by
+ * positions[b][row][a] * turns[..] full turns (turns: host memory, one for each
+ * pair in order, base^(-2 i / widths[a]) / (2 pi)), backwards with `inverse`
+ * (the gradient).  positions (n or 1, l, axes); position_batch_stride 0 shares
+ * one item's.  Outputs may equal the inputs where the strides do. */
+#define CTMR_ROTARY_MAX_PAIRS 256
+enum ctmr_position_type { CTMR_POS_I32 = 0, CTMR_POS_I64 = 1, CTMR_POS_F32 = 2 };
+typedef struct ctmr_rotary_desc {
+  int32_t n, l, q_heads, k_heads, head_dim, axes;
+  int32_t widths[4];
+  int32_t elem, position_type, inverse, reserved;
+  int64_t position_batch_stride;
+  int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3]; /* batch, head, row */
+} ctmr_rotary_desc;
+int ctmr_rotary(const ctmr_rotary_desc* desc, const void* q, const void* k, const void* positions,
+                const double* turns, void* q_out, void* k_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,6 +25,9 @@ DT_F32, DT_BF16, DT_F16X2 = 0, 1, 2
 KERNEL_NAMES = ("stream", "stream_direct", "lds", "lds_bf16", "pointwise", "split_waves", "tap_expand", "lds_small",
                 "small_cout", "lds_f16x2", "march")
 AVGPOOL2, NEAREST2X, TRILINEAR2X = 0, 1, 2
+ELEM_F32, ELEM_BF16, ELEM_F16 = 0, 1, 2
+POS_I32, POS_I64, POS_F32 = 0, 1, 2
+ROTARY_MAX_PAIRS = 256
 ABI_VERSION = 5
 NOALLOC_SCRATCH_BYTES = 256 << 20  # CTMR_NOALLOC_SCRATCH_BYTES
 
@@ -45,6 +48,18 @@ class AttnDesc(ctypes.Structure):
     _fields_ = [(name, ctypes.c_int32) for name in ("n", "lq", "lk", "heads", "head_dim", "query_tiles")] + [
         (name, ctypes.c_int64) for name in ("ldq", "ldk", "ldv", "ldo")
     ] + [("scale", ctypes.c_float)]
+
+
+class RotaryDesc(ctypes.Structure):
+    """``ctmr_rotary_desc``."""
+
+    _fields_ = (
+        [(name, ctypes.c_int32) for name in ("n", "l", "q_heads", "k_heads", "head_dim", "axes")]
+        + [("widths", ctypes.c_int32 * 4)]
+        + [(name, ctypes.c_int32) for name in ("elem", "position_type", "inverse", "reserved")]
+        + [("position_batch_stride", ctypes.c_int64)]
+        + [(name, ctypes.c_int64 * 3) for name in ("q_strides", "k_strides", "q_out_strides", "k_out_strides")]
+    )
 
 
 _c_int, _c_i32, _c_i64 = ctypes.c_int, ctypes.c_int32, ctypes.c_int64
@@ -86,6 +101,12 @@ _PROTOTYPES = {
     "ctmr_flash_attention": (_c_int, [ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _vp, _vp]),
     "ctmr_flash_attention_f16x2_workspace_bytes": (_c_i64, [ctypes.POINTER(AttnDesc)]),
     "ctmr_flash_attention_f16x2": (_c_int, [ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _vp, _vp, _c_i64, _vp]),
+    "ctmr_norm_workspace_bytes": (_c_i64, [_c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32]),
+    "ctmr_norm_forward": (_c_int, [_c_i32, _c_i64, _c_i32, _c_i32, _f, _c_i32, _vp, _c_i32, _vp, _vp, _c_i32, _vp, _vp,
+                                   _vp, _sz, _vp]),
+    "ctmr_norm_backward": (_c_int, [_c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _vp, _vp, _c_i32, _vp, _vp, _c_i32, _vp,
+                                    _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ctmr_rotary": (_c_int, [ctypes.POINTER(RotaryDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,210 @@
+"""Operators of the networks' attention blocks with gradients, on fp32, bf16 and fp16 tensors.
+
+The reference is inference only; these are what fine-tuning its UNet and ControlNet (``unet.py``,
+``attention.py``) needs beside the fp32 surface of ``fast_fp32``:
+
+* ``group_norm``  channels-last group norm + SiLU
+* ``rotary``      rotary positions over one to four axes (depth, height, width) for q and k
+"""
+
+from __future__ import annotations
+
+import math
+import weakref
+from collections.abc import Sequence
+from typing import Optional
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+# Autograd graphs recorded outside any capture that hold leaves, by what each saved (see _graph_token).
+_eager_graphs: "weakref.WeakSet[_EagerGraph]" = weakref.WeakSet()
+
+
+class _EagerGraph:
+    """The leaves of one recorded call; lives as long as the call's autograd node."""
+
+    __slots__ = ("leaves", "__weakref__")
+
+    def __init__(self, leaves: list[Tensor]):
+        self.leaves = [weakref.ref(t) for t in leaves]
+
+
+def _graph_token(*tensors: Optional[Tensor]) -> Optional[_EagerGraph]:
+    """What an autograd node keeps while it lives: a mark on the leaves of a call made outside a capture.
+
+    A leaf has one gradient accumulator for all graphs that hold it, bound to the stream of the first.  A
+    backward pass captured into a HIP graph while an eager graph of the same leaf lives would make the
+    capture wait for a stream outside it, which ends the process; such a call is refused here.
+
+    Raises:
+        RuntimeError: in a capture, if a leaf belongs to a living graph recorded outside it."""
+    leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
+    if not leaves:
+        return None
+    if not torch.cuda.is_current_stream_capturing():
+        token = _EagerGraph(leaves)
+        _eager_graphs.add(token)
+        return token
+    for token in list(_eager_graphs):
+        for ref in token.leaves:
+            held = ref()
+            if held is not None and any(held is t for t in leaves):
+                raise RuntimeError("an autograd graph recorded outside this capture still holds one of its leaves; "
+                                   "drop that graph (its outputs and losses) before capturing, or capture a detached "
+                                   "copy of the leaf")
+    return None
+
+
+def _check_capture(captured: bool) -> None:
+    """Refuses a backward pass in another capture state than its forward pass."""
+    if torch.cuda.is_current_stream_capturing() != captured:
+        raise RuntimeError("forward and backward must both be inside a graph capture or both outside")
+
+
+def _activation(t, name: str, ndim: Optional[int] = None) -> Tensor:
+    if not isinstance(t, Tensor):
+        raise ValueError(f"{name} must be a torch.Tensor")
+    if ndim is not None and t.dim() != ndim:
+        raise ValueError(f"{name} must be {ndim}-D; got shape {tuple(t.shape)}")
+    if t.dtype not in ops.ELEMENTS:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16; got {t.dtype}")
+    return t
+
+
+def _on_gpu(t: Tensor, name: str) -> None:
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be on the GPU (there is no CPU path); got {t.device}")
+
+
+def _like(t, like: Tensor, name: str, ndim: Optional[int] = None) -> Tensor:
+    _activation(t, name, ndim)
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} is {t.dtype} on {t.device}; expected {like.dtype} on {like.device}")
+    return t
+
+
+# ---------------------------------------------------------------------------
+# group norm
+# ---------------------------------------------------------------------------
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, silu):
+        y, saved = ops.norm_forward(x, weight, bias, groups, eps, silu)
+        ctx.save_for_backward(x, weight, bias, saved)
+        ctx.silu = silu
+        ctx.token, ctx.captured = _graph_token(x, weight, bias), torch.cuda.is_current_stream_capturing()
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _check_capture(ctx.captured)
+        x, weight, bias, saved = ctx.saved_tensors
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        dx, dw, db = ops.norm_backward(x, dy.contiguous(), weight, bias, saved, ctx.silu, want_x, want_w or want_b)
+        return dx if want_x else None, dw if want_w else None, db if want_b else None, None, None, None
+
+
+def group_norm(x: Tensor, weight: Tensor, bias: Tensor, *, num_groups: int, eps: float,
+               apply_silu: bool = False) -> Tensor:
+    """Group norm, and SiLU with ``apply_silu``, of channels-last ``x`` ``(N, ..., C)``; differentiable.
+
+    ``x`` is fp32, bf16 or fp16 (a copy is made where it is not contiguous); ``weight`` and ``bias`` ``(C,)``
+    are fp32 or ``x``'s type.  Statistics are fp64 sums over each batch item's voxels and ``C / num_groups``
+    channels with the biased variance; the output has ``x``'s type, the gradients their inputs' types.
+
+    Raises:
+        ValueError: on other types, devices or shapes, channels that the groups do not divide, or an ``eps``
+            that is negative or not finite."""
+    _activation(x, "x")
+    if x.dim() < 2:
+        raise ValueError(f"x must be (N, ..., C); got shape {tuple(x.shape)}")
+    c, groups, eps = int(x.shape[-1]), int(num_groups), float(eps)
+    if groups < 1 or c < 1 or c % groups:
+        raise ValueError(f"{c} channels are not divisible by {num_groups} groups")
+    if not (math.isfinite(eps) and eps >= 0.0):
+        raise ValueError(f"eps must be finite and not negative; got {eps}")
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        _activation(t, name, 1)
+        if int(t.shape[0]) != c or t.device != x.device or t.dtype not in (torch.float32, x.dtype):
+            raise ValueError(f"{name} must be ({c},) in float32 or {x.dtype} on {x.device}; got "
+                             f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    if weight.dtype != bias.dtype:
+        raise ValueError(f"weight and bias differ in type: {weight.dtype} and {bias.dtype}")
+    _on_gpu(x, "x")
+    x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias.requires_grad):
+        return _GroupNorm.apply(x, weight, bias, groups, eps, bool(apply_silu))
+    return ops.norm_forward(x, weight, bias, groups, eps, bool(apply_silu))[0]
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+def _heads(t: Tensor) -> Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, sections, base):
+        out, k_out = ops.rotary(q, k, positions, sections, base, False)
+        ctx.save_for_backward(positions)
+        ctx.sections, ctx.base, ctx.with_k = sections, base, k is not None
+        ctx.token, ctx.captured = _graph_token(q, k), torch.cuda.is_current_stream_capturing()
+        return out, (k_out if k is not None else None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        _check_capture(ctx.captured)
+        positions, = ctx.saved_tensors
+        if not ctx.with_k:
+            dk = None
+        dq, dk_out = ops.rotary(_heads(dq), None if dk is None else _heads(dk), positions, ctx.sections, ctx.base, True)
+        return dq, (dk_out if ctx.with_k else None), None, None, None
+
+
+def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, *, sections: Sequence[int],
+           base: float = 10000.0) -> tuple[Tensor, Optional[Tensor]]:
+    """Rotary positions of ``(B, H, L, D)`` heads over one to four axes; differentiable in ``q`` and ``k``.
+
+    ``positions`` ``(L, A)`` or ``(B, L, A)`` (int32, int64 or fp32; fractions are allowed) holds a token's place on
+    each axis, such as a voxel's (depth, height, width).  The first ``sum(sections)`` values of a head are a
+    section per axis; value ``i`` of a section of width ``w`` and value ``i + w / 2`` turn by ``position * base **
+    (-2 i / w)``; the rest of the head passes.  ``k`` may have fewer heads than ``q``, or be None.  Angles are
+    computed in 64 bits.  The outputs have the inputs' type and lie as ``(B, L, H, D)`` in memory.
+
+    Raises:
+        ValueError: on other types, devices or shapes, sections that are odd, not positive, wider than the head
+            or not one for each axis, or a base that is not positive and finite."""
+    _activation(q, "q", 4)
+    b, _, l, d = (int(v) for v in q.shape)
+    if k is not None:
+        _like(k, q, "k", 4)
+        if int(k.shape[0]) != b or int(k.shape[2]) != l or int(k.shape[3]) != d:
+            raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in more than their heads")
+    sections = tuple(int(w) for w in sections)
+    if not 1 <= len(sections) <= 4 or any(w < 2 or w % 2 for w in sections):
+        raise ValueError(f"sections must be one to four positive even widths; got {sections}")
+    if d % 2 or sum(sections) > d or d > 2 * ops._lib.ROTARY_MAX_PAIRS:
+        raise ValueError(f"sections {sections} do not fit heads of {d} values (even, at most 512)")
+    base = float(base)
+    if not (math.isfinite(base) and base > 0.0):
+        raise ValueError(f"base must be positive and finite; got {base}")
+    if not isinstance(positions, Tensor) or positions.dtype not in ops.POSITION_TYPES or positions.device != q.device:
+        raise ValueError("positions must be an int32, int64 or float32 tensor on q's device")
+    if tuple(positions.shape) not in ((l, len(sections)), (1, l, len(sections)), (b, l, len(sections))):
+        raise ValueError(f"positions must be ({l}, {len(sections)}) or ({b}, {l}, {len(sections)}); got "
+                         f"{tuple(positions.shape)}")
+    _on_gpu(q, "q")
+    positions = positions.detach().contiguous()
+    q, k = _heads(q), None if k is None else _heads(k)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, positions, sections, base)
+    out, k_out = ops.rotary(q, k, positions, sections, base, False)
+    return out, (None if k is None else k_out)

@@ -16,9 +16,11 @@ operator.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
-from typing import Callable, Optional
+import math
+from typing import Callable, Optional, Sequence
 
 import torch
 from torch import Tensor
@@ -556,3 +558,119 @@ def flash_attention_f16x2(q: Tensor, k: Tensor, v: Tensor, heads: int, scale: fl
 @flash_attention_f16x2.register_fake
 def _(q, k, v, heads, scale, query_tiles=0):
     return q.new_empty(q.shape)
+
+
+# ---------------------------------------------------------------------------
+# differentiable operators (fp32, bf16 and fp16 activations; autograd in ``differentiable``)
+# ---------------------------------------------------------------------------
+ELEMENTS = {torch.float32: _lib.ELEM_F32, torch.bfloat16: _lib.ELEM_BF16, torch.float16: _lib.ELEM_F16}
+POSITION_TYPES = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64, torch.float32: _lib.POS_F32}
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on(t: Tensor):
+    """Makes ``t``'s device current for a launch (a stream's kernels launch on its own device)."""
+    return _SAME_DEVICE if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+
+
+def _workspace(nbytes: int, device: torch.device) -> Optional[Tensor]:
+    return torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
+
+
+@_custom_op("ctmr::norm_forward")
+def norm_forward(x: Tensor, weight: Tensor, bias: Tensor, groups: int, eps: float, silu: bool) -> tuple[Tensor, Tensor]:
+    """``ctmr_norm_forward`` of contiguous (N, ..., C) rows: the output and the (N, groups, 4) statistics
+    that ``norm_backward`` reads."""
+    _require_device(x, weight, bias)
+    n, c = int(x.shape[0]), int(x.shape[-1])
+    y = torch.empty_like(x)
+    saved = torch.empty((n, groups, 4), device=x.device, dtype=torch.float32)
+    if x.numel() == 0:
+        return y, saved.zero_()
+    s, elem, lib = x.numel() // (n * c), ELEMENTS[x.dtype], _lib.lib()
+    with _on(x):
+        nbytes = _lib.check(lib.ctmr_norm_workspace_bytes(n, s, c, groups, elem, 0), "ctmr_norm_workspace_bytes")
+        ws = _workspace(nbytes, x.device)
+        _lib.check(lib.ctmr_norm_forward(n, s, c, groups, eps, elem, x.data_ptr(), ELEMENTS[weight.dtype],
+                                         weight.data_ptr(), bias.data_ptr(), silu, y.data_ptr(), saved.data_ptr(),
+                                         _ptr(ws), nbytes, _stream(x.device)), "ctmr_norm_forward")
+    return y, saved
+
+
+@norm_forward.register_fake
+def _(x, weight, bias, groups, eps, silu):
+    return torch.empty_like(x), x.new_empty((x.shape[0], groups, 4), dtype=torch.float32)
+
+
+@_custom_op("ctmr::norm_backward")
+def norm_backward(x: Tensor, dy: Tensor, weight: Tensor, bias: Tensor, saved: Tensor, silu: bool, want_x: bool,
+                  want_params: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """``ctmr_norm_backward``: gradients of ``x``, ``weight`` and ``bias``; empty where not wanted."""
+    _require_device(x, dy, weight, bias, saved)
+    n, c, groups = int(x.shape[0]), int(x.shape[-1]), int(saved.shape[1])
+    none = (0,)
+    dx = torch.empty_like(x) if want_x else x.new_empty(none)
+    dw, db = (torch.empty_like(weight), torch.empty_like(bias)) if want_params else (weight.new_empty(none),
+                                                                                     bias.new_empty(none))
+    if x.numel() == 0:
+        return dx, dw.zero_(), db.zero_()
+    s, elem, lib = x.numel() // (n * c), ELEMENTS[x.dtype], _lib.lib()
+    with _on(x):
+        nbytes = _lib.check(lib.ctmr_norm_workspace_bytes(n, s, c, groups, elem, 1), "ctmr_norm_workspace_bytes")
+        ws = _workspace(nbytes, x.device)
+        _lib.check(lib.ctmr_norm_backward(n, s, c, groups, elem, x.data_ptr(), dy.data_ptr(), ELEMENTS[weight.dtype],
+                                          weight.data_ptr(), bias.data_ptr(), silu, saved.data_ptr(),
+                                          dx.data_ptr() if want_x else None, dw.data_ptr() if want_params else None,
+                                          db.data_ptr() if want_params else None, _ptr(ws), nbytes,
+                                          _stream(x.device)), "ctmr_norm_backward")
+    return dx, dw, db
+
+
+@norm_backward.register_fake
+def _(x, dy, weight, bias, saved, silu, want_x, want_params):
+    none = (0,)
+    return (torch.empty_like(x) if want_x else x.new_empty(none),
+            torch.empty_like(weight) if want_params else weight.new_empty(none),
+            torch.empty_like(bias) if want_params else bias.new_empty(none))
+
+
+def _heads_like(t: Tensor) -> Tensor:
+    """An empty (B, H, L, D) tensor that lies as (B, L, H, D) rows, the layout of a projection's output."""
+    b, h, l, d = t.shape
+    return t.new_empty((b, l, h, d)).transpose(1, 2)
+
+
+@functools.lru_cache(maxsize=64)
+def _turns(sections: tuple[int, ...], base: float):
+    """Turns of every pair at position 1 as a C array: ``base ** (-2 i / width) / (2 pi)``."""
+    turns = [base ** (-2.0 * i / w) / (2.0 * math.pi) for w in sections for i in range(w // 2)]
+    return (ctypes.c_double * len(turns))(*turns)
+
+
+@_custom_op("ctmr::rotary")
+def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, sections: Sequence[int], base: float,
+           inverse: bool) -> tuple[Tensor, Tensor]:
+    """``ctmr_rotary`` of (B, H, L, D) heads with a unit last stride and contiguous positions; the outputs
+    lie as (B, L, H, D), the second is empty without ``k``."""
+    _require_device(q, k, positions)
+    b, hq, l, d = (int(v) for v in q.shape)
+    out = _heads_like(q)
+    k_out = q.new_empty((0,)) if k is None else _heads_like(k)
+    if q.numel() == 0:
+        return out, k_out
+    widths = tuple(int(w) for w in sections)
+    desc = _lib.RotaryDesc(b, l, hq, 0 if k is None else int(k.shape[1]), d, len(widths), (ctypes.c_int32 * 4)(*widths),
+                           ELEMENTS[q.dtype], POSITION_TYPES[positions.dtype], inverse, 0,
+                           positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0,
+                           q.stride()[:3], (0, 0, 0) if k is None else k.stride()[:3], out.stride()[:3],
+                           (0, 0, 0) if k is None else k_out.stride()[:3])
+    with _on(q):
+        _lib.check(_lib.lib().ctmr_rotary(ctypes.byref(desc), q.data_ptr(), _ptr(k), positions.data_ptr(),
+                                          _turns(widths, base), out.data_ptr(),
+                                          None if k is None else k_out.data_ptr(), _stream(q.device)), "ctmr_rotary")
+    return out, k_out
+
+
+@rotary.register_fake
+def _(q, k, positions, sections, base, inverse):
+    return _heads_like(q), q.new_empty((0,)) if k is None else _heads_like(k)

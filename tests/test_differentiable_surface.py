@@ -1,0 +1,121 @@
+"""CPU tests of the differentiable operators: what they refuse, their host checks, registration and tracing."""
+
+from __future__ import annotations
+
+import ctypes
+import gc
+
+import pytest
+import torch
+
+
+def _norm(f, x=(2, 5, 8), w=8, b=8, xt=torch.float32, wt=torch.float32, bt=torch.float32, groups=2, eps=1e-6):
+    return f.group_norm(torch.zeros(x, dtype=xt), torch.zeros(w, dtype=wt), torch.zeros(b, dtype=bt), num_groups=groups,
+                        eps=eps)
+
+
+@pytest.mark.parametrize(
+    ("kw", "message"),
+    [({"x": (8,)}, "x must be"), ({"xt": torch.float64}, "float32, bfloat16 or float16"),
+     ({"groups": 3}, "not divisible"), ({"groups": 0}, "not divisible"), ({"w": 7}, "weight must be"),
+     ({"b": 9}, "bias must be"), ({"wt": torch.bfloat16}, "weight must be"), ({"eps": -1.0}, "eps"),
+     ({"eps": float("nan")}, "eps"), ({"xt": torch.bfloat16, "wt": torch.bfloat16}, "differ in type"),
+     ({}, "on the GPU")])
+def test_group_norm_refuses(ctmr, kw, message):
+    with pytest.raises(ValueError, match=message):
+        _norm(ctmr.differentiable, **kw)
+
+
+def _rotary(f, q=(2, 4, 6, 32), k=(2, 2, 6, 32), qt=torch.float32, kt=torch.float32, pos=(6, 2), pt=torch.int32,
+            sections=(8, 8), base=10000.0):
+    return f.rotary(torch.zeros(q, dtype=qt), None if k is None else torch.zeros(k, dtype=kt),
+                    torch.zeros(pos, dtype=pt), sections=sections, base=base)
+
+
+@pytest.mark.parametrize(
+    ("kw", "message"),
+    [({"q": (4, 6, 32)}, "q must be 4-D"), ({"qt": torch.int32}, "float32, bfloat16"), ({"kt": torch.float16}, "k is"),
+     ({"k": (2, 2, 7, 32)}, "differ in more"), ({"k": (1, 2, 6, 32)}, "differ in more"), ({"sections": ()}, "sections"),
+     ({"sections": (7, 8)}, "even"), ({"sections": (32, 2)}, "do not fit"), ({"sections": (2,) * 5}, "one to four"),
+     ({"sections": (0, 8)}, "even"), ({"base": 0.0}, "base"), ({"base": float("inf")}, "base"),
+     ({"pt": torch.float64}, "positions"), ({"pos": (6, 3)}, "positions"), ({"pos": (3, 6, 2)}, "positions"),
+     ({"q": (2, 4, 6, 514), "k": None}, "at most 512"), ({}, "on the GPU")])
+def test_rotary_refuses(ctmr, kw, message):
+    with pytest.raises(ValueError, match=message):
+        _rotary(ctmr.differentiable, **kw)
+
+
+def test_norm_host_checks(ctmr, native_loaded):
+    L, p = ctmr._lib, 4096
+    space = native_loaded.ctmr_norm_workspace_bytes
+    assert space(2, 64, 64, 8, 0, 0) == 0 and space(2, 64, 64, 8, 0, 1) == 2 * 64 * 16
+    assert space(1, 64, 64, 8, 0, 1) == 0 and space(1, 100000, 64, 8, 1, 0) > 0
+    assert space(0, 1, 8, 2, 0, 0) == L.E_INVALID and space(1, 1, 8, 3, 0, 0) == L.E_INVALID
+    assert space(1, 1, 8, 2, 3, 0) == L.E_INVALID and space(1, 1 << 41, 8, 2, 0, 0) == L.E_UNSUPPORTED
+    fwd = lambda **kw: native_loaded.ctmr_norm_forward(
+        kw.get("n", 1), kw.get("s", 16), 8, 2, 1e-6, kw.get("elem", 0), kw.get("x", p), kw.get("ptype", 0), p, p, 1,
+        kw.get("y", p), kw.get("saved", p), kw.get("ws", p), kw.get("bytes", 0), None)
+    for kw, code in (({"x": None}, L.E_INVALID), ({"y": None}, L.E_INVALID), ({"saved": None}, L.E_INVALID),
+                     ({"saved": p + 4}, L.E_INVALID), ({"elem": 5}, L.E_INVALID), ({"ptype": -1}, L.E_INVALID),
+                     ({"n": 70000}, L.E_UNSUPPORTED), ({"s": 100000}, L.E_WORKSPACE),
+                     ({"s": 100000, "ws": p + 8, "bytes": 1 << 30}, L.E_WORKSPACE),
+                     ({"s": 100000, "ws": None, "bytes": 1 << 30}, L.E_WORKSPACE)):
+        assert fwd(**kw) == code, kw
+    bwd = lambda **kw: native_loaded.ctmr_norm_backward(
+        1, kw.get("s", 16), 8, 2, 0, p, kw.get("dy", p), 0, p, p, 1, p, kw.get("dx", None), kw.get("dw", None),
+        kw.get("db", None), p, kw.get("bytes", 0), None)
+    assert bwd() == L.OK  # nothing wanted, nothing launched
+    assert bwd(dy=None) == L.E_INVALID and bwd(dw=p) == L.E_INVALID and bwd(s=100000, dx=p) == L.E_WORKSPACE
+
+
+def test_rotary_host_checks(ctmr, native_loaded):
+    L, p = ctmr._lib, 4096
+    turns = (ctypes.c_double * 256)()
+
+    def call(q=p, out=p, k=p, pos=p, turns=turns, **kw):
+        d = L.RotaryDesc(1, 4, 2, 1, 32, 2, (ctypes.c_int32 * 4)(8, 8), 0, 0, 0, 0, 0)
+        for name, value in kw.items():
+            setattr(d, name, (ctypes.c_int32 * 4)(*value) if name == "widths" else value)
+        return native_loaded.ctmr_rotary(ctypes.byref(d), q, k, pos, turns, out, p, None)
+
+    assert native_loaded.ctmr_rotary(None, p, p, p, turns, p, p, None) == L.E_INVALID
+    for kw in ({"q": None}, {"k": None}, {"pos": None}, {"turns": None}, {"out": None}, {"n": 0}, {"l": 0}, {"axes": 5},
+               {"axes": 0}, {"elem": 3}, {"position_type": 3}, {"head_dim": 31}, {"widths": (7, 8)}, {"widths": (8, 0)},
+               {"widths": (24, 10)}, {"q_heads": 0}, {"k_heads": -1}):
+        assert call(**kw) == L.E_INVALID, kw
+    assert call(n=70000) == L.E_UNSUPPORTED and call(head_dim=514) == L.E_UNSUPPORTED
+
+
+def test_a_leaf_of_a_living_eager_graph_is_refused_in_a_capture(ctmr, monkeypatch):
+    f = ctmr.differentiable
+    state = {"capturing": False}
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    leaf, other = torch.zeros(3, requires_grad=True), torch.zeros(3, requires_grad=True)
+    token = f._graph_token(leaf, None, leaf * 2)
+    assert f._graph_token(leaf.detach()) is None
+    state["capturing"] = True
+    assert f._graph_token(other) is None and f._graph_token(leaf * 2) is None
+    with pytest.raises(RuntimeError, match="outside this capture"):
+        f._graph_token(other, leaf)
+    with pytest.raises(RuntimeError, match="both"):
+        f._check_capture(False)
+    f._check_capture(True)
+    del token
+    gc.collect()
+    assert f._graph_token(leaf) is None
+
+
+def test_registered_operators_trace(ctmr):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x = torch.empty(2, 5, 8, device="cuda", dtype=torch.bfloat16)
+        w = torch.empty(8, device="cuda")
+        y, saved = torch.ops.ctmr.norm_forward(x, w, w, 2, 1e-6, True)
+        assert y.shape == x.shape and y.dtype == x.dtype and saved.shape == (2, 2, 4)
+        dx, dw, db = torch.ops.ctmr.norm_backward(x, y, w, w, saved, True, True, False)
+        assert dx.shape == x.shape and dw.shape == db.shape == (0,)
+        q = torch.empty(2, 4, 6, 32, device="cuda")
+        out, k_out = torch.ops.ctmr.rotary(q, None, torch.empty(6, 2, device="cuda", dtype=torch.int32), [8, 8], 1e4,
+                                           False)
+        assert out.shape == q.shape and out.transpose(1, 2).is_contiguous() and k_out.shape == (0,)
