@@ -476,6 +476,51 @@ typedef struct ctmr_rotary_desc {
 int ctmr_rotary(const ctmr_rotary_desc* desc, const void* q, const void* k, const void* positions,
                 const double* turns, void* q_out, void* k_out, void* stream);
 
+/* Document ids of query and key rows laid out for ctmr_masked_attention: (n, lq)
+ * and (n, lk) int32 ids, negative ones padding, in any order (rows of a document
+ * side by side let the kernels skip the others' tiles).  The plan (16-byte
+ * aligned) holds a copy of the ids and serves every call with these n, lq, lk. */
+int64_t ctmr_documents_bytes(int32_t n, int32_t lq, int32_t lk);
+int ctmr_documents(int32_t n, int32_t lq, int32_t lk, const int32_t* query_ids, const int32_t* key_ids, void* plan,
+                   size_t plan_bytes, void* stream);
+
+/* out = softmax(scores) v per head for q (n, q_heads, lq, head_dim) and k, v
+ * (n, k_heads, lk, head_dim), all of type elem, q_heads a multiple of k_heads
+ * (query head h reads key head h / (q_heads / k_heads)).  head_dim is a multiple
+ * of 8 up to 128; strides (batch, head, row) in values are multiples of 16 bytes,
+ * values of a head lie side by side.  Scores of row i and key j, p_i = i + lk - lq:
+ *   s = scale q_i . k_j;  softcap > 0: s = softcap tanh(s / softcap)
+ *   slopes (q_heads) or NULL: s -= slopes[h] |p_i - j|
+ * Key j is visible to row i if: with `prefixed`, j <= p_i or j < the prefix
+ * (prefixes[item], or the descriptor's value where that is NULL); with a plan
+ * (ctmr_documents), both have the same id and it is not negative.  A row that sees
+ * no key gives zeros.  What masked places hold has no effect, NaN included.
+ * lse (n, q_heads, lq) or NULL: log2 of each row's sum, +inf for an empty row.
+ * The kernel splits long keys over workgroups where there are few rows: workspace
+ * of ctmr_masked_attention_workspace_bytes, 16-byte aligned. */
+typedef struct ctmr_masked_attention_desc {
+  int32_t n, lq, lk, q_heads, k_heads, head_dim, elem;
+  int32_t prefixed, prefix;
+  float scale, softcap;
+  int32_t reserved;
+  int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3];
+} ctmr_masked_attention_desc;
+int64_t ctmr_masked_attention_workspace_bytes(const ctmr_masked_attention_desc* desc);
+int ctmr_masked_attention(const ctmr_masked_attention_desc* desc, const void* q, const void* k, const void* v,
+                          const float* slopes, const int32_t* prefixes, const void* plan, void* out, float* lse,
+                          void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients of q, k and v (any of dq, dk and dv may be NULL), given the call's out
+ * and lse and dout (strides as q's); out's strides are multiples of 16 bytes here.
+ * fp32 and bf16 (CTMR_E_UNSUPPORTED for fp16: ds would leave its range).  Gradients
+ * of shared key heads are summed over their query heads.  dq, dk and dv may not
+ * overlap the inputs. */
+int64_t ctmr_masked_attention_backward_workspace_bytes(const ctmr_masked_attention_desc* desc);
+int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* desc, const void* q, const void* k, const void* v,
+                                   const float* slopes, const int32_t* prefixes, const void* plan, const void* out,
+                                   const float* lse, const void* dout, const int64_t* dout_strides, void* dq,
+                                   const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                                   const int64_t* dv_strides, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

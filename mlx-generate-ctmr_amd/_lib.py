@@ -62,6 +62,17 @@ class RotaryDesc(ctypes.Structure):
     )
 
 
+class MaskedAttentionDesc(ctypes.Structure):
+    """``ctmr_masked_attention_desc``."""
+
+    _fields_ = (
+        [(name, ctypes.c_int32) for name in ("n", "lq", "lk", "q_heads", "k_heads", "head_dim", "elem", "prefixed",
+                                             "prefix")]
+        + [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("reserved", ctypes.c_int32)]
+        + [(name, ctypes.c_int64 * 3) for name in ("q_strides", "k_strides", "v_strides", "out_strides")]
+    )
+
+
 _c_int, _c_i32, _c_i64 = ctypes.c_int, ctypes.c_int32, ctypes.c_int64
 _vp, _sz, _f = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_float
 _desc_p = ctypes.POINTER(ConvDesc)
@@ -107,6 +118,13 @@ _PROTOTYPES = {
     "ctmr_norm_backward": (_c_int, [_c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _vp, _vp, _c_i32, _vp, _vp, _c_i32, _vp,
                                     _vp, _vp, _vp, _vp, _sz, _vp]),
     "ctmr_rotary": (_c_int, [ctypes.POINTER(RotaryDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ctmr_documents_bytes": (_c_i64, [_c_i32, _c_i32, _c_i32]),
+    "ctmr_documents": (_c_int, [_c_i32, _c_i32, _c_i32, _vp, _vp, _vp, _sz, _vp]),
+    "ctmr_masked_attention_workspace_bytes": (_c_i64, [ctypes.POINTER(MaskedAttentionDesc)]),
+    "ctmr_masked_attention": (_c_int, [ctypes.POINTER(MaskedAttentionDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                       _vp, _sz, _vp]),
+    "ctmr_masked_attention_backward_workspace_bytes": (_c_i64, [ctypes.POINTER(MaskedAttentionDesc)]),
+    "ctmr_masked_attention_backward": (_c_int, [ctypes.POINTER(MaskedAttentionDesc)] + [_vp] * 17 + [_sz, _vp]),
 }
 
 _lock = threading.Lock()

@@ -5,6 +5,8 @@ The reference is inference only; these are what fine-tuning its UNet and Control
 
 * ``group_norm``  channels-last group norm + SiLU
 * ``rotary``      rotary positions over one to four axes (depth, height, width) for q and k
+* ``attention``   attention with grouped heads, a tanh cap, a distance bias, documents and a prefix
+* ``Documents``   which tokens of a batch belong together (volumes of different sizes in one row, padding)
 """
 
 from __future__ import annotations
@@ -12,7 +14,7 @@ from __future__ import annotations
 import math
 import weakref
 from collections.abc import Sequence
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 from torch import Tensor
@@ -208,3 +210,126 @@ def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, *, sections: Seque
         return _Rotary.apply(q, k, positions, sections, base)
     out, k_out = ops.rotary(q, k, positions, sections, base, False)
     return out, (None if k is None else k_out)
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+class Documents:
+    """Which query rows and keys belong together, laid out once for every ``attention`` of a batch.
+
+    ``ids`` ``(B, Lq)`` int32 holds each query row's document, ``key_ids`` ``(B, Lk)`` each key's (the same rows
+    if left out).  A row sees the keys of its own document; negative ids are padding, which sees and is seen by
+    nothing.  Ids may come in any order, but only rows of a document that lie side by side let the kernels skip
+    the rest.  The ids are copied: changing the tensors afterwards changes nothing here.
+
+    Raises:
+        ValueError: on ids that are not (B, L) int32 tensors of one device and batch on the GPU, or empty."""
+
+    def __init__(self, ids: Tensor, key_ids: Optional[Tensor] = None):
+        key_ids = ids if key_ids is None else key_ids
+        for t, name in ((ids, "ids"), (key_ids, "key_ids")):
+            if not isinstance(t, Tensor) or t.dtype != torch.int32 or t.dim() != 2:
+                raise ValueError(f"{name} must be a (B, L) int32 tensor")
+            if t.numel() == 0:
+                raise ValueError(f"{name} is empty: {tuple(t.shape)}")
+        if ids.device != key_ids.device or ids.shape[0] != key_ids.shape[0]:
+            raise ValueError("ids and key_ids differ in device or batch")
+        _on_gpu(ids, "ids")
+        self.shape = (int(ids.shape[0]), int(ids.shape[1]), int(key_ids.shape[1]))
+        self.plan = ops.documents(ids.contiguous(), key_ids.contiguous())
+
+    @property
+    def device(self) -> torch.device:
+        return self.plan.device
+
+
+def _attention_heads(t: Tensor) -> Tensor:
+    """``t`` with a unit last stride, 16-byte aligned rows and a row stride that the kernels can address."""
+    size = t.element_size()
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0:
+        strides = ops._head_strides(t)
+        if all(s * size % 16 == 0 for s in strides) and strides[2] * size <= 1 << 24:
+            return t
+    return t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, prefixes, plan, scale, softcap, prefixed, prefix):
+        out, lse = ops.masked_attention(q, k, v, slopes, prefixes, plan, scale, softcap, prefixed, prefix, True)
+        ctx.save_for_backward(q, k, v, slopes, prefixes, plan, out, lse)
+        ctx.args = (scale, softcap, prefixed, prefix)
+        ctx.token, ctx.captured = _graph_token(q, k, v), torch.cuda.is_current_stream_capturing()
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        _check_capture(ctx.captured)
+        want_q, want_k, want_v = ctx.needs_input_grad[:3]
+        dq, dk, dv = ops.masked_attention_backward(*ctx.saved_tensors, _attention_heads(dout), *ctx.args, want_q,
+                                                   want_k or want_v)
+        return (dq if want_q else None, dk if want_k else None, dv if want_v else None, *(None,) * 7)
+
+
+def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float = 0.0, slopes: Optional[Tensor] = None,
+              prefix: Union[int, Tensor, None] = None, documents: Optional[Documents] = None) -> Tensor:
+    """Masked attention of ``(B, H, L, D)`` heads; differentiable in ``q``, ``k`` and ``v`` (fp32 and bf16).
+
+    ``q`` has ``Hq`` heads and ``Lq`` rows, ``k`` and ``v`` ``Hk`` heads and ``Lk`` keys, ``Hq`` a multiple of
+    ``Hk`` (query head ``h`` reads key head ``h // (Hq // Hk)``); ``D`` is a multiple of 8 up to 128.  With
+    ``p_i = i + Lk - Lq`` the place of row ``i`` among the keys:
+
+    * ``softcap`` > 0 caps the scores ``s = scale * q.k`` as ``softcap * tanh(s / softcap)``;
+    * ``slopes`` ``(Hq,)`` fp32 subtract ``slopes[h] * |p_i - j|`` (no gradient);
+    * ``prefix``, an int or a ``(B,)`` int32 tensor, hides key ``j`` from row ``i`` unless ``j <= p_i`` or ``j <
+      prefix`` (0: each row sees the keys up to its own place; None: every key);
+    * ``documents`` hides the keys of other documents and padding (``Documents``).
+
+    A row that sees no key gives zeros and gets no gradient.  What masked places hold has no effect, NaN included.
+    Statistics and sums are fp32; the softmax weights are rounded to the inputs' type for their product with
+    ``v``.  The output has ``q``'s type and lies as ``(B, Lq, Hq, D)`` in memory, so merging the heads is a view.
+
+    Raises:
+        ValueError: on other types, devices or shapes, a scale that is not positive and finite, a negative cap,
+            slopes that need a gradient, or fp16 tensors that need one (it would leave fp16's range)."""
+    _activation(q, "q", 4)
+    _like(k, q, "k", 4)
+    _like(v, q, "v", 4)
+    b, hq, lq, d = (int(s) for s in q.shape)
+    hk, lk = int(k.shape[1]), int(k.shape[2])
+    if k.shape != v.shape or int(k.shape[0]) != b or int(k.shape[3]) != d:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit each other")
+    if hk < 1 or hq < 1 or hq % hk:
+        raise ValueError(f"{hq} query heads are not a multiple of {hk} key heads")
+    if d < 8 or d % 8 or d > 128:
+        raise ValueError(f"head width must be a multiple of 8 up to 128; got {d}")
+    scale, softcap = float(scale), float(softcap)
+    if not (math.isfinite(scale) and scale > 0.0) or not (math.isfinite(softcap) and softcap >= 0.0):
+        raise ValueError(f"scale must be positive, softcap not negative, both finite; got {scale} and {softcap}")
+    if slopes is not None:
+        if not isinstance(slopes, Tensor) or slopes.dtype != torch.float32 or tuple(slopes.shape) != (hq,) or (
+                slopes.device != q.device):
+            raise ValueError(f"slopes must be a ({hq},) float32 tensor on {q.device}")
+        if slopes.requires_grad and torch.is_grad_enabled():
+            raise ValueError("slopes have no gradient; pass them detached")
+        slopes = slopes.contiguous()
+    prefixes, value = None, 0
+    if isinstance(prefix, Tensor):
+        if prefix.dtype != torch.int32 or tuple(prefix.shape) != (b,) or prefix.device != q.device:
+            raise ValueError(f"prefix must be an int or a ({b},) int32 tensor on {q.device}")
+        prefixes = prefix.contiguous()
+    elif prefix is not None:
+        value = max(0, min(int(prefix), lk))
+    if documents is not None and (documents.shape != (b, lq, lk) or documents.device != q.device):
+        raise ValueError(f"documents are for {documents.shape} rows on {documents.device}; got {(b, lq, lk)} on {q.device}")
+    needs = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    if needs and q.dtype == torch.float16:
+        raise ValueError("attention has no float16 gradient (it would leave the type's range); use bfloat16 or float32")
+    _on_gpu(q, "q")
+    q, k, v = _attention_heads(q), _attention_heads(k), _attention_heads(v)
+    plan = None if documents is None else documents.plan
+    if needs:
+        return _Attention.apply(q, k, v, slopes, prefixes, plan, scale, softcap, prefix is not None, value)
+    return ops.masked_attention(q, k, v, slopes, prefixes, plan, scale, softcap, prefix is not None, value, False)[0]

@@ -674,3 +674,99 @@ def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, sections: Sequence
 @rotary.register_fake
 def _(q, k, positions, sections, base, inverse):
     return _heads_like(q), q.new_empty((0,)) if k is None else _heads_like(k)
+
+
+@_custom_op("ctmr::documents")
+def documents(query_ids: Tensor, key_ids: Tensor) -> Tensor:
+    """``ctmr_documents``: the plan of contiguous (B, Lq) and (B, Lk) int32 ids, as raw bytes."""
+    _require_device(query_ids, key_ids)
+    n, lq, lk = int(query_ids.shape[0]), int(query_ids.shape[1]), int(key_ids.shape[1])
+    lib = _lib.lib()
+    nbytes = _lib.check(lib.ctmr_documents_bytes(n, lq, lk), "ctmr_documents_bytes")
+    plan = torch.empty(nbytes, device=query_ids.device, dtype=torch.uint8)
+    with _on(query_ids):
+        _lib.check(lib.ctmr_documents(n, lq, lk, query_ids.data_ptr(), key_ids.data_ptr(), plan.data_ptr(), nbytes,
+                                      _stream(plan.device)), "ctmr_documents")
+    return plan
+
+
+@documents.register_fake
+def _(query_ids, key_ids):
+    n, lq, lk = query_ids.shape[0], query_ids.shape[1], key_ids.shape[1]
+    return query_ids.new_empty(_lib.lib().ctmr_documents_bytes(int(n), int(lq), int(lk)), dtype=torch.uint8)
+
+
+def _head_strides(t: Tensor) -> tuple[int, int, int]:
+    """Strides of batch, head and row, 0 for an axis of one."""
+    shape, s = t.shape, t.stride()
+    return (s[0] if shape[0] > 1 else 0, s[1] if shape[1] > 1 else 0, s[2] if shape[2] > 1 else 0)
+
+
+def _attention_desc(q: Tensor, k: Tensor, v: Tensor, out: Tensor, scale: float, softcap: float,
+                    prefixed: bool, prefix: int) -> "_lib.MaskedAttentionDesc":
+    return _lib.MaskedAttentionDesc(int(q.shape[0]), int(q.shape[2]), int(k.shape[2]), int(q.shape[1]), int(k.shape[1]),
+                                    int(q.shape[3]), ELEMENTS[q.dtype], prefixed, prefix, scale, softcap, 0,
+                                    _head_strides(q), _head_strides(k), _head_strides(v), _head_strides(out))
+
+
+@_custom_op("ctmr::masked_attention")
+def masked_attention(q: Tensor, k: Tensor, v: Tensor, slopes: Optional[Tensor], prefixes: Optional[Tensor],
+                     plan: Optional[Tensor], scale: float, softcap: float, prefixed: bool, prefix: int,
+                     want_lse: bool) -> tuple[Tensor, Tensor]:
+    """``ctmr_masked_attention`` of (B, H, L, D) heads: the output, which lies as (B, L, H, D), and the rows'
+    (B, H, Lq) log2 sums, empty unless wanted."""
+    _require_device(q, k, v, slopes, prefixes, plan)
+    out = _heads_like(q)
+    lse = torch.empty(q.shape[:3] if want_lse else (0,), device=q.device, dtype=torch.float32)
+    if q.numel() == 0 or k.shape[2] == 0:
+        return out.zero_(), lse.fill_(math.inf)
+    desc, lib = _attention_desc(q, k, v, out, scale, softcap, prefixed, prefix), _lib.lib()
+    with _on(q):
+        nbytes = _lib.check(lib.ctmr_masked_attention_workspace_bytes(ctypes.byref(desc)),
+                            "ctmr_masked_attention_workspace_bytes")
+        ws = _workspace(nbytes, q.device)
+        _lib.check(lib.ctmr_masked_attention(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(slopes),
+                                             _ptr(prefixes), _ptr(plan), out.data_ptr(),
+                                             lse.data_ptr() if want_lse else None, _ptr(ws), nbytes,
+                                             _stream(q.device)), "ctmr_masked_attention")
+    return out, lse
+
+
+@masked_attention.register_fake
+def _(q, k, v, slopes, prefixes, plan, scale, softcap, prefixed, prefix, want_lse):
+    return _heads_like(q), q.new_empty(q.shape[:3] if want_lse else (0,), dtype=torch.float32)
+
+
+@_custom_op("ctmr::masked_attention_backward")
+def masked_attention_backward(q: Tensor, k: Tensor, v: Tensor, slopes: Optional[Tensor], prefixes: Optional[Tensor],
+                              plan: Optional[Tensor], out: Tensor, lse: Tensor, dout: Tensor, scale: float,
+                              softcap: float, prefixed: bool, prefix: int, want_q: bool,
+                              want_kv: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """``ctmr_masked_attention_backward``: gradients of ``q``, ``k`` and ``v``, which lie as (B, L, H, D); empty
+    where not wanted."""
+    _require_device(q, k, v, slopes, prefixes, plan, out, lse, dout)
+    none = (0,)
+    dq = _heads_like(q) if want_q else q.new_empty(none)
+    dk, dv = (_heads_like(k), _heads_like(v)) if want_kv else (k.new_empty(none), v.new_empty(none))
+    if q.numel() == 0 or k.shape[2] == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    desc, lib = _attention_desc(q, k, v, out, scale, softcap, prefixed, prefix), _lib.lib()
+    strides = lambda t, want=True: (ctypes.c_int64 * 3)(*_head_strides(t)) if want else None
+    with _on(q):
+        nbytes = _lib.check(lib.ctmr_masked_attention_backward_workspace_bytes(ctypes.byref(desc)),
+                            "ctmr_masked_attention_backward_workspace_bytes")
+        ws = _workspace(nbytes, q.device)
+        _lib.check(lib.ctmr_masked_attention_backward(
+            ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(slopes), _ptr(prefixes), _ptr(plan),
+            out.data_ptr(), lse.data_ptr(), dout.data_ptr(), strides(dout), dq.data_ptr() if want_q else None,
+            strides(dq, want_q), dk.data_ptr() if want_kv else None, strides(dk, want_kv),
+            dv.data_ptr() if want_kv else None, strides(dv, want_kv), _ptr(ws), nbytes, _stream(q.device)),
+            "ctmr_masked_attention_backward")
+    return dq, dk, dv
+
+
+@masked_attention_backward.register_fake
+def _(q, k, v, slopes, prefixes, plan, out, lse, dout, scale, softcap, prefixed, prefix, want_q, want_kv):
+    none = (0,)
+    return (_heads_like(q) if want_q else q.new_empty(none), _heads_like(k) if want_kv else k.new_empty(none),
+            _heads_like(v) if want_kv else v.new_empty(none))

@@ -119,3 +119,102 @@ def test_registered_operators_trace(ctmr):
         out, k_out = torch.ops.ctmr.rotary(q, None, torch.empty(6, 2, device="cuda", dtype=torch.int32), [8, 8], 1e4,
                                            False)
         assert out.shape == q.shape and out.transpose(1, 2).is_contiguous() and k_out.shape == (0,)
+
+
+def _attention(f, q=(2, 4, 6, 32), k=(2, 2, 7, 32), v=None, qt=torch.float32, kt=torch.float32, scale=1.0, **kw):
+    return f.attention(torch.zeros(q, dtype=qt), torch.zeros(k, dtype=kt), torch.zeros(v or k, dtype=kt), scale=scale, **kw)
+
+
+@pytest.mark.parametrize(
+    ("kw", "message"),
+    [({"q": (4, 6, 32)}, "q must be 4-D"), ({"qt": torch.float64}, "float32, bfloat16"),
+     ({"kt": torch.bfloat16}, "k is"), ({"k": (1, 2, 7, 32)}, "do not fit"), ({"k": (2, 2, 7, 16)}, "do not fit"),
+     ({"v": (2, 2, 8, 32)}, "do not fit"), ({"k": (2, 3, 7, 32)}, "not a multiple"),
+     ({"k": (2, 0, 7, 32)}, "not a multiple"), ({"q": (2, 4, 6, 36), "k": (2, 2, 7, 36)}, "multiple of 8"),
+     ({"q": (2, 4, 6, 136), "k": (2, 2, 7, 136)}, "up to 128"), ({"scale": 0.0}, "scale"), ({"scale": -1.0}, "scale"),
+     ({"scale": float("inf")}, "scale"), ({"softcap": -1.0}, "softcap"), ({"slopes": torch.zeros(3)}, "slopes"),
+     ({"slopes": torch.zeros(4, dtype=torch.float64)}, "slopes"), ({"slopes": [0.0] * 4}, "slopes"),
+     ({"slopes": torch.zeros(4, requires_grad=True)}, "no gradient"), ({"prefix": torch.zeros(3).int()}, "prefix"),
+     ({"prefix": torch.zeros(2)}, "prefix"), ({}, "on the GPU")])
+def test_attention_refuses(ctmr, kw, message):
+    with pytest.raises(ValueError, match=message):
+        _attention(ctmr.differentiable, **kw)
+
+
+@pytest.mark.parametrize(
+    ("ids", "key_ids", "message"),
+    [(torch.zeros(2, 3), None, "int32"), (torch.zeros(2, 3).long(), None, "int32"), (torch.zeros(3).int(), None, "int32"),
+     (torch.zeros(2, 0).int(), None, "empty"), (torch.zeros(2, 3).int(), torch.zeros(1, 3).int(), "differ"),
+     ([[0]], None, "int32"), (torch.zeros(2, 3).int(), None, "on the GPU")])
+def test_documents_refuse(ctmr, ids, key_ids, message):
+    with pytest.raises(ValueError, match=message):
+        ctmr.differentiable.Documents(ids, key_ids)
+
+
+def _attention_desc(L, **kw):
+    d = L.MaskedAttentionDesc(1, 200, 300, 4, 2, 32, 0, 0, 0, 1.0, 0.0, 0, (25600, 32, 128), (19200, 32, 64),
+                              (19200, 32, 64), (25600, 32, 128))
+    for name, value in kw.items():
+        setattr(d, name, (ctypes.c_int64 * 3)(*value) if name.endswith("strides") else value)
+    return d
+
+
+def test_attention_host_checks(ctmr, native_loaded):
+    L, p = ctmr._lib, 4096
+    space = lambda **kw: native_loaded.ctmr_masked_attention_workspace_bytes(ctypes.byref(_attention_desc(L, **kw)))
+    assert native_loaded.ctmr_masked_attention_workspace_bytes(None) == L.E_INVALID
+    for kw in ({"n": 0}, {"lq": 0}, {"lk": 0}, {"q_heads": 3}, {"k_heads": 0}, {"elem": 3}, {"scale": 0.0},
+               {"scale": float("nan")}, {"softcap": -1.0}, {"softcap": float("inf")}, {"q_strides": (25600, 32, 130)},
+               {"k_strides": (-4, 32, 64)}, {"v_strides": (19200, 33, 64)}):
+        assert space(**kw) == L.E_INVALID, kw
+    for kw in ({"head_dim": 36}, {"head_dim": 136}, {"lq": 1 << 29}, {"k_strides": (0, 0, 1 << 23)},
+               {"n": 1 << 20, "q_heads": 1 << 10, "k_heads": 1}):
+        assert space(**kw) == L.E_UNSUPPORTED, kw
+    # splits: 8 query blocks of 5 key tiles make one part, one token of 16384 keys the most of its 256 tiles
+    assert space() == 4 * 0
+    assert space(lq=1, lk=16384) == 64 * 4 * (32 + 2) * 4
+    assert space(lq=1, lk=16384, n=64) == 8 * 64 * 4 * (32 + 2) * 4
+
+    def call(q=p, plan=None, out=p, ws=p, nbytes=0, **kw):
+        return native_loaded.ctmr_masked_attention(ctypes.byref(_attention_desc(L, **kw)), q, p, p, None, None, plan, out,
+                                                   None, ws, nbytes, None)
+
+    assert call(q=None) == L.E_INVALID and call(out=None) == L.E_INVALID and call(q=p + 8) == L.E_INVALID
+    assert call(plan=p + 4) == L.E_INVALID and call(out_strides=(25600, 32, 130)) == L.E_INVALID
+    assert call(lq=1, lk=16384, nbytes=100) == L.E_WORKSPACE
+    assert call(lq=1, lk=16384, ws=p + 4, nbytes=1 << 30) == L.E_WORKSPACE
+
+    strides = (ctypes.c_int64 * 3)(25600, 32, 128)
+
+    def back(q=p, out=p, lse=p, dout=p, s=strides, dq=None, dq_s=strides, dk=None, ws=p, nbytes=1 << 20, **kw):
+        return native_loaded.ctmr_masked_attention_backward(
+            ctypes.byref(_attention_desc(L, **kw)), q, p, p, None, None, None, out, lse, dout, s, dq, dq_s, dk, strides,
+            None, None, ws, nbytes, None)
+
+    assert back() == L.OK  # nothing wanted, nothing launched
+    bad = (ctypes.c_int64 * 3)(25600, 32, 126)
+    for kw in ({"q": None}, {"out": None}, {"lse": None}, {"dout": None}, {"s": None}, {"dq": p, "dq_s": None},
+               {"dout": p + 8}, {"dq": p + 8}, {"s": bad}, {"dq": p, "dq_s": bad}, {"out_strides": (25600, 32, 130)}):
+        assert back(**kw) == L.E_INVALID, kw
+    assert back(elem=L.ELEM_F16) == L.E_UNSUPPORTED and back(nbytes=100, dq=p) == L.E_WORKSPACE
+    assert back(ws=None, dq=p) == L.E_WORKSPACE
+
+    docs = native_loaded.ctmr_documents_bytes
+    assert docs(2, 100, 65) == 2 * (128 * 4 + 128 * 4 + 2 * 16 + 2 * 16 + 2 * 8 + 2 * 8)
+    assert docs(0, 1, 1) == L.E_INVALID and docs(70000, 1, 1) == L.E_UNSUPPORTED
+    assert native_loaded.ctmr_documents(2, 100, 65, p, p, p, 10, None) == L.E_WORKSPACE
+    assert native_loaded.ctmr_documents(2, 100, 65, None, p, p, 1 << 20, None) == L.E_INVALID
+
+
+def test_attention_traces(ctmr):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        q, k = (torch.empty(2, h, 6, 32, device="cuda", dtype=torch.bfloat16) for h in (4, 2))
+        out, lse = torch.ops.ctmr.masked_attention(q, k, k, None, None, None, 1.0, 0.0, False, 0, True)
+        assert out.shape == q.shape and out.transpose(1, 2).is_contiguous() and lse.shape == (2, 4, 6)
+        dq, dk, dv = torch.ops.ctmr.masked_attention_backward(q, k, k, None, None, None, out, lse, out, 1.0, 0.0, False, 0,
+                                                              True, False)
+        assert dq.shape == q.shape and dk.shape == dv.shape == (0,)
+        plan = torch.ops.ctmr.documents(*(torch.empty(2, l, device="cuda", dtype=torch.int32) for l in (100, 65)))
+        assert plan.dtype == torch.uint8 and plan.numel() == ctmr._lib.lib().ctmr_documents_bytes(2, 100, 65)
