@@ -495,7 +495,9 @@ int ctmr_documents(int32_t n, int32_t lq, int32_t lk, const int32_t* query_ids, 
  * (prefixes[item], or the descriptor's value where that is NULL); with a plan
  * (ctmr_documents), both have the same id and it is not negative.  A row that sees
  * no key gives zeros.  What masked places hold has no effect, NaN included.
- * lse (n, q_heads, lq) or NULL: log2 of each row's sum, +inf for an empty row.
+ * rest or NULL: what the rounding of out left out, of type elem, with out's strides
+ * (16 bits; not written for fp32).  lse (n, q_heads, lq) or NULL: log2 of each
+ * row's sum, +inf for an empty row.  The gradients read both.
  * The kernel splits long keys over workgroups where there are few rows: workspace
  * of ctmr_masked_attention_workspace_bytes, 16-byte aligned. */
 typedef struct ctmr_masked_attention_desc {
@@ -507,17 +509,17 @@ typedef struct ctmr_masked_attention_desc {
 } ctmr_masked_attention_desc;
 int64_t ctmr_masked_attention_workspace_bytes(const ctmr_masked_attention_desc* desc);
 int ctmr_masked_attention(const ctmr_masked_attention_desc* desc, const void* q, const void* k, const void* v,
-                          const float* slopes, const int32_t* prefixes, const void* plan, void* out, float* lse,
-                          void* workspace, size_t workspace_bytes, void* stream);
-/* Gradients of q, k and v (any of dq, dk and dv may be NULL), given the call's out
- * and lse and dout (strides as q's); out's strides are multiples of 16 bytes here.
+                          const float* slopes, const int32_t* prefixes, const void* plan, void* out, void* rest,
+                          float* lse, void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients of q, k and v (any of dq, dk and dv may be NULL), given the call's out,
+ * rest (NULL: not kept, with out's rounding in the gradients) and lse and dout (strides as q's); out's strides are multiples of 16 bytes here.
  * fp32 and bf16 (CTMR_E_UNSUPPORTED for fp16: ds would leave its range).  Gradients
  * of shared key heads are summed over their query heads.  dq, dk and dv may not
  * overlap the inputs. */
 int64_t ctmr_masked_attention_backward_workspace_bytes(const ctmr_masked_attention_desc* desc);
 int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* desc, const void* q, const void* k, const void* v,
                                    const float* slopes, const int32_t* prefixes, const void* plan, const void* out,
-                                   const float* lse, const void* dout, const int64_t* dout_strides, void* dq,
+                                   const void* rest, const float* lse, const void* dout, const int64_t* dout_strides, void* dq,
                                    const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
                                    const int64_t* dv_strides, void* workspace, size_t workspace_bytes, void* stream);
 

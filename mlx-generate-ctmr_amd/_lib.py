@@ -121,10 +121,9 @@ _PROTOTYPES = {
     "ctmr_documents_bytes": (_c_i64, [_c_i32, _c_i32, _c_i32]),
     "ctmr_documents": (_c_int, [_c_i32, _c_i32, _c_i32, _vp, _vp, _vp, _sz, _vp]),
     "ctmr_masked_attention_workspace_bytes": (_c_i64, [ctypes.POINTER(MaskedAttentionDesc)]),
-    "ctmr_masked_attention": (_c_int, [ctypes.POINTER(MaskedAttentionDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
-                                       _vp, _sz, _vp]),
+    "ctmr_masked_attention": (_c_int, [ctypes.POINTER(MaskedAttentionDesc)] + [_vp] * 10 + [_sz, _vp]),
     "ctmr_masked_attention_backward_workspace_bytes": (_c_i64, [ctypes.POINTER(MaskedAttentionDesc)]),
-    "ctmr_masked_attention_backward": (_c_int, [ctypes.POINTER(MaskedAttentionDesc)] + [_vp] * 17 + [_sz, _vp]),
+    "ctmr_masked_attention_backward": (_c_int, [ctypes.POINTER(MaskedAttentionDesc)] + [_vp] * 18 + [_sz, _vp]),
 }
 
 _lock = threading.Lock()

@@ -37,7 +37,8 @@ struct RowMask {
 };
 
 // Raw products of NB 32-key blocks -> scores in units of log2 / c (c returned): with a cap or slopes the scores
-// themselves (c = 1), else the products (c = scale log2 e).  Masked keys become -inf.
+// themselves (c = 1), else the products (c = scale log2 e).  Masked keys become -inf; ids: of the keys from k0 on, or
+// null.
 template <typename T, int NB>
 __device__ __forceinline__ float score_blocks(const Args& a, f16v (&s)[NB], int k0, int pos, float slope,
                                               bool partial, const RowMask& m, const int* ids, int lane) {
@@ -67,9 +68,9 @@ __device__ __forceinline__ float score_blocks(const Args& a, f16v (&s)[NB], int 
     for (int u = 0; u < NB; ++u)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int j = k0 + 32 * u + 8 * g + 4 * half;
+        const int at = 32 * u + 8 * g + 4 * half, j = k0 + at;
         int4 id = {m.id, m.id, m.id, m.id};
-        if (ids) id = *reinterpret_cast<const int4*>(ids + j);
+        if (ids) id = *reinterpret_cast<const int4*>(ids + at);
         if (j >= m.limit || id.x != m.id) s[u][4 * g] = -INFINITY;
         if (j + 1 >= m.limit || id.y != m.id) s[u][4 * g + 1] = -INFINITY;
         if (j + 2 >= m.limit || id.z != m.id) s[u][4 * g + 2] = -INFINITY;
@@ -114,7 +115,7 @@ __device__ void add_odd_values(const Args& a, f16v (&o)[ND], const T* v, int k0,
   for (int j = 0; j < kTile; ++j) {
     if (((j < 32 ? lo >> j : hi >> (j - 32)) & 1u) == 0u) continue;
     const int key = k0 + j;
-    const bool seen = key < m.limit && (!ids || ids[key] == m.id);
+    const bool seen = key < m.limit && (!ids || ids[j] == m.id);
     if (!seen) continue;
     const T* row = v + (int64_t)key * a.vl;
 #pragma unroll
@@ -136,6 +137,19 @@ __device__ __forceinline__ void split_range(int split, int splits, int& first, i
   last = min(last, first + per);
 }
 
+// Four values of an output row, and what their rounding left out.
+template <typename T>
+__device__ __forceinline__ void store_output(const Args& a, int64_t at, const Vec<float, 4>& v) {
+  T* out = static_cast<T*>(a.out) + at;
+  store_rounded<T, 4>(out, v);
+  if constexpr (sizeof(T) == 2) {
+    if (a.rest) {
+      const Vec<T, 4> r = __builtin_convertvector(v, Vec<T, 4>);
+      store_rounded<T, 4>(static_cast<T*>(a.rest) + at, v - __builtin_convertvector(r, Vec<float, 4>));
+    }
+  }
+}
+
 // A lane's O^T results as a row of out, or of the split's sums.
 template <typename T, int ND>
 __device__ __forceinline__ void write_row(const Args& a, const f16v (&o)[ND], float m, float l, int b, int h, int i,
@@ -155,7 +169,7 @@ __device__ __forceinline__ void write_row(const Args& a, const f16v (&o)[ND], fl
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  T* out = static_cast<T*>(a.out) + b * a.ob + h * a.oh + (int64_t)i * a.ol;
+  const int64_t out = b * a.ob + h * a.oh + (int64_t)i * a.ol;
 #pragma unroll
   for (int k = 0; k < ND; ++k)
 #pragma unroll
@@ -165,7 +179,7 @@ __device__ __forceinline__ void write_row(const Args& a, const f16v (&o)[ND], fl
         Vec<float, 4> v;
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = o[k][4 * g + r] * inv;
-        store_rounded<T, 4>(out + d, v);
+        store_output<T>(a, out + d, v);
       }
     }
   if (a.lse && half == 0)
@@ -181,6 +195,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(Args a) {
   constexpr int KS = tile_stride<T, D>(ALONG), VS = tile_stride<T, D>(DOWN);
   __shared__ __attribute__((aligned(16))) T kt[2][kTile * KS];
   __shared__ __attribute__((aligned(16))) T vt[2][kTile * VS];
+  __shared__ __attribute__((aligned(16))) int key_ids[2][kTile];
   __shared__ unsigned odd[3][2];
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -189,7 +204,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(Args a) {
   place(blockIdx.x, a.n * a.hq, blocks, item, block);
   if (a.prefixed) block = blocks - 1 - block;  // the longest rows first
   const int b = item / a.hq, h = item % a.hq;
-  const int i0 = block * kRows, i1 = min(i0 + kRows, a.lq) - 1;
+  const int i0 = block * kRows;
   const int i = i0 + 32 * wave + (lane & 31);
   const int prefix = a.prefixed ? prefix_of(a, b) : 0;
   const bool docs = a.qdoc.ids != nullptr;
@@ -201,14 +216,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(Args a) {
   const T* k = static_cast<const T*>(a.k) + b * a.kb + (h / a.group) * a.kh;
   const T* v = static_cast<const T*>(a.v) + b * a.vb + (h / a.group) * a.vh;
 
-  int first, last;
-  key_tiles(a, b, i0, i1, prefix, first, last);
+  const Meeting meet = meeting<kWaves>(wave, i0, a.lq, [&](int row) { return key_tiles(a, b, row, prefix); });
+  int first = meet.all.x, last = meet.all.y;
   split_range(blockIdx.y, a.splits, first, last);
-  // Whether a tile holds a pair that is masked: the same for the whole workgroup.
-  const int whole = limit_of(a, i0, prefix);  // keys that every row may see
-  auto is_partial = [&](int tile) {
-    return (tile + 1) * kTile > whole || (docs && !same_document(a, b, i0 / kTile, 2, tile, 1));
-  };
 
   Frag<T> qf[NK];
 #pragma unroll
@@ -219,60 +229,63 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(Args a) {
   float m = kNone, l = 0.f;
 
   Stream<T, D, kTile, kThreads> ks, vs;
-  bool partial = false;
-  auto stage = [&](int tile, int buf, int slot) {
+  bool partial = false;  // of the tile in flight: some row of the workgroup has a masked key in it
+  int id = 0;
+  auto fetch = [&](int tile) {
+    ks.fetch(k, a.kl, tile * kTile, a.lk, a.d, t);
+    vs.fetch(v, a.vl, tile * kTile, a.lk, a.d, t);
+    partial = meet.partial(tile);
+    if (docs && t < kTile) id = ids[tile * kTile + t];
+  };
+  auto stage = [&](int buf, int slot) {
     ks.template store<false>(kt[buf], KS, nullptr, t);
     if (partial) vs.template store<true>(vt[buf], VS, odd[slot], t);
     else vs.template store<false>(vt[buf], VS, nullptr, t);
+    if (docs && t < kTile) key_ids[buf][t] = id;
   };
   if (t < 6) odd[t / 2][t % 2] = 0u;
   if (first < last) {
-    ks.fetch(k, a.kl, first * kTile, a.lk, a.d, t);
-    vs.fetch(v, a.vl, first * kTile, a.lk, a.d, t);
-    partial = is_partial(first);
+    fetch(first);
     __syncthreads();
-    stage(first, 0, 0);
+    stage(0, 0);
   }
   int slot = 0;
   for (int tile = first; tile < last; ++tile) {
     const int buf = (tile - first) & 1, k0 = tile * kTile;
     const bool now = partial, more = tile + 1 < last;
-    if (more) {
-      ks.fetch(k, a.kl, k0 + kTile, a.lk, a.d, t);
-      vs.fetch(v, a.vl, k0 + kTile, a.lk, a.d, t);
-    }
+    if (more) fetch(tile + 1);
     __syncthreads();
-    f16v s[2] = {f16v(0.f), f16v(0.f)};
+    if (!meet.skips(tile)) {
+      f16v s[2] = {f16v(0.f), f16v(0.f)};
 #pragma unroll
-    for (int n = 0; n < NK; ++n)
+      for (int n = 0; n < NK; ++n)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) s[u] = mma<T>(frag_along(kt[buf], KS, 32 * u, n, lane), qf[n], s[u]);
-    const float c = score_blocks<T, 2>(a, s, k0, pos, slope, now, mask, ids, lane);
-    float alpha;
-    if (softmax_blocks<T, 2>(s, c, m, l, alpha)) {
+        for (int u = 0; u < 2; ++u) s[u] = mma<T>(frag_along(kt[buf], KS, 32 * u, n, lane), qf[n], s[u]);
+      const int* tile_ids = docs ? key_ids[buf] : nullptr;
+      const float c = score_blocks<T, 2>(a, s, k0, pos, slope, meet.masked(tile), mask, tile_ids, lane);
+      float alpha;
+      if (softmax_blocks<T, 2>(s, c, m, l, alpha)) {
 #pragma unroll
-      for (int n = 0; n < ND; ++n) o[n] *= alpha;
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const Frag<T> p = result_frag<T>(s[u], w);
-#pragma unroll
-        for (int n = 0; n < ND; ++n) o[n] = mma<T>(frag_down(vt[buf], VS, 32 * u + 16 * w, n, lane), p, o[n]);
+        for (int n = 0; n < ND; ++n) o[n] *= alpha;
       }
-    if (now) {
-      const unsigned lo = odd[slot][0], hi = odd[slot][1];
-      if (lo | hi) add_odd_values<T, ND>(a, o, v, k0, lo, hi, mask, ids, lane);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const Frag<T> p = result_frag<T>(s[u], w);
+#pragma unroll
+          for (int n = 0; n < ND; ++n) o[n] = mma<T>(frag_down(vt[buf], VS, 32 * u + 16 * w, n, lane), p, o[n]);
+        }
+      if (now) {
+        const unsigned lo = odd[slot][0], hi = odd[slot][1];
+        if (lo | hi) add_odd_values<T, ND>(a, o, v, k0, lo, hi, mask, tile_ids, lane);
+      }
     }
     // Three slots: this tile's is read until the next barrier, the next tile's is set from here on, the one after
     // that was read before this tile's barrier.
     const int next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
     if (t < 2) odd[after][t] = 0u;
-    if (more) {
-      partial = is_partial(tile + 1);
-      stage(tile + 1, buf ^ 1, next);
-    }
+    if (more) stage(buf ^ 1, next);
     slot = next;
   }
   l = half_sum(l);
@@ -316,10 +329,9 @@ __global__ __launch_bounds__(kThreads, 1) void attention_few_kernel(Args a) {
   T* kt = reinterpret_cast<T*>(lds) + wave * kFewTile * (KS + VS);
   T* vt = kt + kFewTile * KS;
 
-  int first, last;
-  key_tiles(a, b, 0, a.lq - 1, prefix, first, last);  // of 64 keys
+  const int4 range = key_tiles(a, b, 0, prefix);  // lq <= kGrain; tiles of 64 keys
+  int first = range.x, last = range.y;
   split_range(blockIdx.y, a.splits, first, last);
-  const int whole = limit_of(a, 0, prefix);
   const int end = min(last * kTile, a.lk);
 
   Frag<T> qf[NK];
@@ -337,7 +349,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_few_kernel(Args a) {
     vs.fetch(v, a.vl, k0, a.lk, a.d, lane);
   }
   for (; k0 < end; k0 += kWaves * kFewTile) {
-    const bool partial = k0 + kFewTile > whole || (docs && !same_document(a, b, 0, 1, k0 / kTile, 1));
+    const bool partial = k0 / kTile < range.z || k0 / kTile >= range.w;
     if (lane == 0) odd[wave] = 0u;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     ks.template store<false>(kt, KS, nullptr, lane);
@@ -352,7 +364,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_few_kernel(Args a) {
     f16v s[1] = {f16v(0.f)};
 #pragma unroll
     for (int n = 0; n < NK; ++n) s[0] = mma<T>(frag_along(kt, KS, 0, n, lane), qf[n], s[0]);
-    const float c = score_blocks<T, 1>(a, s, k0, pos, slope, partial, mask, ids, lane);
+    const float c = score_blocks<T, 1>(a, s, k0, pos, slope, partial, mask, docs ? ids + k0 : nullptr, lane);
     float alpha;
     if (softmax_blocks<T, 1>(s, c, m, l, alpha)) {
 #pragma unroll
@@ -366,7 +378,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_few_kernel(Args a) {
     }
     if (partial) {
       const unsigned set = odd[wave];
-      if (set) add_odd_values<T, ND>(a, o, v, k0, set, 0u, mask, ids, lane);
+      if (set) add_odd_values<T, ND>(a, o, v, k0, set, 0u, mask, docs ? ids + k0 : nullptr, lane);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
@@ -431,7 +443,7 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(Args a) {
   const int64_t b = bh / a.hq;
   if (d < a.d) {
     const float inv = total == 0.f ? 0.f : 1.0f / total;
-    store_rounded<T, 4>(static_cast<T*>(a.out) + b * a.ob + h * a.oh + (int64_t)i * a.ol + d, sum * inv);
+    store_output<T>(a, b * a.ob + h * a.oh + (int64_t)i * a.ol + d, sum * inv);
   }
   if (a.lse && d == 0) a.lse[at] = total == 0.f ? INFINITY : top + log2f(total) - kLift<T>;
 }
@@ -443,8 +455,8 @@ struct DocArgs {
   const int* from[2];
   int* ids[2];
   DocTile* tiles[2];
-  int2* hull[2];
-  int rows[2], stride[2], count[2];
+  int4* hull[2];
+  int rows[2], stride[2], count[2], grains[2];
 };
 
 // One wave per tile: blockIdx = (tile, item, side).
@@ -465,24 +477,47 @@ __global__ __launch_bounds__(kTile) void document_tiles_kernel(DocArgs a) {
   if (lane == 0) a.tiles[side][(int64_t)b * a.count[side] + tile] = DocTile{least, most, least_id, 0};
 }
 
+// One wave per kGrain rows: blockIdx = (grain, item, side).
 __global__ __launch_bounds__(kTile) void document_hulls_kernel(DocArgs a) {
-  const int side = blockIdx.z, b = blockIdx.y, tile = blockIdx.x, lane = threadIdx.x;
-  if (tile >= a.count[side]) return;
-  const DocTile own = a.tiles[side][(int64_t)b * a.count[side] + tile];
-  int lo = INT_MAX, hi = 0;
-  for (int o = lane; o < a.count[1 - side]; o += kTile) {
-    const DocTile other = a.tiles[1 - side][(int64_t)b * a.count[1 - side] + o];
+  const int side = blockIdx.z, b = blockIdx.y, grain = blockIdx.x, lane = threadIdx.x;
+  if (grain >= a.grains[side]) return;
+  const int i = grain * kGrain + lane % kGrain;
+  const int id = i < a.rows[side] ? a.ids[side][(int64_t)b * a.stride[side] + i] : -1;
+  DocTile own;
+  own.least = i < a.rows[side] ? id : INT_MAX;
+  own.most = id;
+  own.least_id = id >= 0 ? id : INT_MAX;
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) {
+    own.least = min(own.least, __shfl_xor(own.least, m));
+    own.most = max(own.most, __shfl_xor(own.most, m));
+    own.least_id = min(own.least_id, __shfl_xor(own.least_id, m));
+  }
+  const DocTile* others = a.tiles[1 - side] + (int64_t)b * a.count[1 - side];
+  const int count = a.count[1 - side];
+  const bool one = own.least == own.most && own.least >= 0;
+  int lo = INT_MAX, hi = 0, whole = INT_MAX;
+  for (int o = lane; o < count; o += kTile) {
+    const DocTile other = others[o];
     if (own.least_id <= other.most && other.least_id <= own.most) {
       lo = min(lo, o);
       hi = max(hi, o + 1);
     }
+    if (one && other.least == own.least && other.most == own.least) whole = min(whole, o);
   }
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) {
     lo = min(lo, __shfl_xor(lo, m));
     hi = max(hi, __shfl_xor(hi, m));
+    whole = min(whole, __shfl_xor(whole, m));
   }
-  if (lane == 0) a.hull[side][(int64_t)b * a.count[side] + tile] = int2{lo, hi};
+  // the first run of tiles that hold nothing but this document
+  int end = whole == INT_MAX ? 0 : count;
+  for (int o = lane; o < end; o += kTile)
+    if (o > whole && (others[o].least != own.least || others[o].most != own.least)) end = min(end, o);
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) end = min(end, __shfl_xor(end, m));
+  if (lane == 0) a.hull[side][(int64_t)b * a.grains[side] + grain] = int4{lo, hi, whole, end};
 }
 
 // --------------------------------------------------------------------------
@@ -525,9 +560,10 @@ static Side side_of(int rows, const int* ids, const void* tiles, const void* hul
   Side s = {};
   s.ids = ids;
   s.tiles = static_cast<const DocTile*>(tiles);
-  s.hull = static_cast<const int2*>(hull);
+  s.hull = static_cast<const int4*>(hull);
   s.count = (int)ceil_div(rows, kTile);
   s.stride = s.count * kTile;
+  s.grains = (int)ceil_div(rows, kGrain);
   return s;
 }
 
@@ -544,8 +580,8 @@ static void plan_parts(int32_t n, int32_t lq, int32_t lk, char* base, Side& q, S
   const int* ki = (const int*)take(n * nk * kTile * 4);
   const void* qt = take(n * nq * (int64_t)sizeof(DocTile));
   const void* kt = take(n * nk * (int64_t)sizeof(DocTile));
-  const void* qh = take(n * nq * 8);
-  const void* kh = take(n * nk * 8);
+  const void* qh = take(n * ceil_div(lq, kGrain) * 16);
+  const void* kh = take(n * ceil_div(lk, kGrain) * 16);
   q = side_of(lq, qi, qt, qh);
   k = side_of(lk, ki, kt, kh);
   if (bytes) *bytes = at;
@@ -620,14 +656,15 @@ int ctmr_documents(int32_t n, int32_t lq, int32_t lk, const int32_t* query_ids, 
   for (int s = 0; s < 2; ++s) {
     a.ids[s] = const_cast<int*>(sides[s]->ids);
     a.tiles[s] = const_cast<DocTile*>(sides[s]->tiles);
-    a.hull[s] = const_cast<int2*>(sides[s]->hull);
+    a.hull[s] = const_cast<int4*>(sides[s]->hull);
     a.rows[s] = rows[s], a.stride[s] = sides[s]->stride, a.count[s] = sides[s]->count;
+    a.grains[s] = sides[s]->grains;
   }
   const dim3 grid(std::max(a.count[0], a.count[1]), n, 2);
   hipLaunchKernelGGL(document_tiles_kernel, grid, dim3(kTile), 0, (hipStream_t)stream, a);
   const int rc = check_launch("document_tiles");
   if (rc) return rc;
-  hipLaunchKernelGGL(document_hulls_kernel, grid, dim3(kTile), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(document_hulls_kernel, dim3(std::max(a.grains[0], a.grains[1]), n, 2), dim3(kTile), 0, (hipStream_t)stream, a);
   return check_launch("document_hulls");
 }
 
@@ -639,13 +676,14 @@ int64_t ctmr_masked_attention_workspace_bytes(const ctmr_masked_attention_desc* 
 }
 
 int ctmr_masked_attention(const ctmr_masked_attention_desc* d, const void* q, const void* k, const void* v,
-                          const float* slopes, const int32_t* prefixes, const void* plan, void* out, float* lse,
-                          void* workspace, size_t workspace_bytes, void* stream) {
+                          const float* slopes, const int32_t* prefixes, const void* plan, void* out, void* rest,
+                          float* lse, void* workspace, size_t workspace_bytes, void* stream) {
   const int64_t need = ctmr_masked_attention_workspace_bytes(d);
   if (need < 0) return (int)need;
   if (!q || !k || !v || !out) return fail(CTMR_E_INVALID, "null pointer");
-  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)plan) & 15) != 0)
-    return fail(CTMR_E_INVALID, "q, k, v, out and the document plan must start on 16-byte boundaries");
+  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)rest | (uintptr_t)plan) & 15) !=
+      0)
+    return fail(CTMR_E_INVALID, "q, k, v, out, rest and the document plan must start on 16-byte boundaries");
   if ((d->out_strides[0] | d->out_strides[1] | d->out_strides[2]) % 4 != 0)
     return fail(CTMR_E_INVALID, "strides of out must be multiples of 4 values");
   if (need > 0 && ((int64_t)workspace_bytes < need || !workspace || ((uintptr_t)workspace & 15) != 0)) {
@@ -654,7 +692,7 @@ int ctmr_masked_attention(const ctmr_masked_attention_desc* d, const void* q, co
     return CTMR_E_WORKSPACE;
   }
   Args a = make_args(d, q, k, v, slopes, prefixes, plan);
-  a.out = out, a.lse = lse, a.part = (float*)workspace, a.splits = split_count(d);
+  a.out = out, a.rest = rest, a.lse = lse, a.part = (float*)workspace, a.splits = split_count(d);
   a.ob = d->out_strides[0], a.oh = d->out_strides[1], a.ol = d->out_strides[2];
   const bool few = few_rows(d);
   hipStream_t st = (hipStream_t)stream;

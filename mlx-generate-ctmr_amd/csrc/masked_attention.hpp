@@ -173,17 +173,19 @@ struct Stream {
 struct DocTile {     // of kTile rows: ids of all its rows, and of those that are no padding
   int least, most, least_id, unused;
 };
+constexpr int kGrain = 32;  // rows of a hull: a wave's
 
 struct Side {        // documents of the query or key rows
   const int* ids;    // (n, rows rounded up to kTile), -1 past the end
   const DocTile* tiles;
-  const int2* hull;  // tiles of the other side [x, y) that may hold a match
-  int stride, count;  // ids and tiles of a batch item
+  const int4* hull;  // of kGrain rows, tiles of the other side: [x, y) may hold a match, all pairs with [z, w) are one
+  int stride, count, grains;  // ids, tiles and hulls of a batch item
 };
 
 struct Args {
   const void *q, *k, *v;
   void* out;
+  void* rest;             // what rounding took from out, as out lies, or null
   float* lse;             // (n, hq, lq) log2 of a row's sum, +inf for an empty row
   float* part;            // split keys: (splits, n, hq, lq, D) sums, then (.., 2) maximum and total
   const void* dout;
@@ -246,43 +248,59 @@ __device__ __forceinline__ void place(int id, int items, int tiles, int& item, i
   }
 }
 
-// Whether every row of the query tiles [t, t + count) and every key of the key tiles [u, u + keys) share one
-// document.
-__device__ __forceinline__ bool same_document(const Args& a, int b, int t, int count, int u, int keys) {
-  const DocTile first = a.kdoc.tiles[(int64_t)b * a.kdoc.count + u];
-  bool same = first.least == first.most && first.least >= 0;
-  for (int i = u + 1; i < min(u + keys, a.kdoc.count); ++i) {
-    const DocTile k = a.kdoc.tiles[(int64_t)b * a.kdoc.count + i];
-    same = same && k.least == first.least && k.most == first.least;
+// Tiles that kGrain rows of one side meet: [x, y) may hold visible pairs, in [z, w) every pair is visible.
+__device__ __forceinline__ int4 meet(const Side& s, int b, int grain, int4 r) {
+  if (s.ids) {
+    const int4 hull = s.hull[(int64_t)b * s.grains + grain];
+    r = {max(r.x, hull.x), min(r.y, hull.y), max(r.z, hull.z), min(r.w, hull.w)};
   }
-  for (int i = t; i < min(t + count, a.qdoc.count); ++i) {
-    const DocTile q = a.qdoc.tiles[(int64_t)b * a.qdoc.count + i];
-    same = same && q.least == first.least && q.most == first.least;
-  }
-  return same;
+  r.y = max(r.y, 0);
+  r.x = min(r.x, r.y);
+  return r;
 }
 
-// The hull on the other side of the tiles that hold rows r0 .. r1.
-__device__ __forceinline__ int2 hull_of(const Side& s, int b, int r0, int r1) {
-  int2 hull = {0x7fffffff, 0};
-  for (int t = r0 / kTile; t <= r1 / kTile; ++t) {
-    const int2 h = s.hull[(int64_t)b * s.count + t];
-    hull.x = min(hull.x, h.x);
-    hull.y = max(hull.y, h.y);
-  }
-  return hull;
+// Key tiles of the rows i .. i + kGrain - 1 of item b, those past lq aside.
+__device__ __forceinline__ int4 key_tiles(const Args& a, int b, int i, int prefix) {
+  const int last = limit_of(a, min(i + kGrain, a.lq) - 1, prefix), first = limit_of(a, i, prefix);
+  return meet(a.qdoc, b, i / kGrain, int4{0, (max(last, 0) + kTile - 1) / kTile, 0, max(first, 0) / kTile});
 }
 
-// Key tiles [first, last) that rows i0 .. i1 of item b may see.
-__device__ __forceinline__ void key_tiles(const Args& a, int b, int i0, int i1, int prefix, int& first, int& last) {
-  first = 0;
-  last = max(0, (limit_of(a, i1, prefix) + kTile - 1) / kTile);
-  if (a.qdoc.ids) {
-    const int2 hull = hull_of(a.qdoc, b, i0, i1);
-    first = max(first, hull.x);
-    last = min(last, hull.y);
+// Query tiles of the keys j .. j + kGrain - 1: from the first row whose limit passes j; every key is seen from the
+// row whose limit passes the last one.
+__device__ __forceinline__ int4 query_tiles(const Args& a, int b, int j, int prefix) {
+  const int end = min(j + kGrain, a.lk) - 1, off = a.lk - a.lq, tiles = (a.lq + kTile - 1) / kTile;
+  const int first = a.prefixed && prefix <= j ? max(0, j - off) / kTile : 0;
+  const int whole = a.prefixed && prefix <= end ? (max(0, end - off) + kTile - 1) / kTile : 0;
+  return meet(a.kdoc, b, j / kGrain, int4{first, tiles, whole, tiles});
+}
+
+// A workgroup's tiles from its waves' (those with rows): any may hold a pair, all are whole.
+struct Meeting {
+  int4 mine, all;
+  __device__ __forceinline__ bool partial(int tile) const { return tile < all.z || tile >= all.w; }
+  __device__ __forceinline__ bool skips(int tile) const { return tile < mine.x || tile >= mine.y; }
+  __device__ __forceinline__ bool masked(int tile) const { return tile < mine.z || tile >= mine.w; }
+};
+template <int WAVES, typename F>
+__device__ __forceinline__ Meeting meeting(int wave, int row0, int rows, F tiles_of) {
+  Meeting m;
+  m.mine = int4{0, 0, 0, 0};
+  m.all = int4{0x7fffffff, 0, 0, 0x7fffffff};
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const int row = row0 + kGrain * w;
+    if (row >= rows) break;
+    const int4 r = tiles_of(row);
+    if (r.x < r.y) {
+      m.all.x = min(m.all.x, r.x);
+      m.all.y = max(m.all.y, r.y);
+    }
+    m.all.z = max(m.all.z, r.z);
+    m.all.w = min(m.all.w, r.w);
+    if (w == wave) m.mine = r;
   }
-  last = max(first, last);
+  m.all.x = min(m.all.x, m.all.y);
+  return m;
 }
 
 int check_desc(const ctmr_masked_attention_desc* d);

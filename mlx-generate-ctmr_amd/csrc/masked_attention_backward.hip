@@ -4,6 +4,9 @@
 //   dv_j = sum_i p_ij g_i
 //   ds_ij = p_ij (g_i . v_j - delta_i) (1 - t_ij^2),  delta_i = g_i . out_i,
 //           t = tanh(scale q_i . k_j / cap), 0 without a cap
+// delta takes out before its rounding (out + rest, as the forward call left it): with
+// few visible keys g . v_j - delta_i is small beside both, and out's half steps would
+// be the largest error of dq and dk.
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
 // sums over i running over all query heads that share the key head.
 //
@@ -75,6 +78,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dq_kerne
   constexpr int KS = tile_stride<T, D>(BOTH), VS = tile_stride<T, D>(ALONG);
   __shared__ __attribute__((aligned(16))) T kt[kTile * KS];
   __shared__ __attribute__((aligned(16))) T vt[kTile * VS];
+  __shared__ __attribute__((aligned(16))) int key_ids[kTile];
   __shared__ unsigned odd[2];
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -83,7 +87,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dq_kerne
   place(blockIdx.x, a.n * a.hq, blocks, item, block);
   if (a.prefixed) block = blocks - 1 - block;
   const int b = item / a.hq, h = item % a.hq;
-  const int i0 = block * kOwn, i1 = min(i0 + kOwn, a.lq) - 1;
+  const int i0 = block * kOwn;
   const int i = i0 + 32 * wave + (lane & 31);
   const bool real = i < a.lq;
   const int prefix = a.prefixed ? prefix_of(a, b) : 0;
@@ -108,6 +112,14 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dq_kerne
     const Frag<T> of = frag_global(out, s, a.d, lane, real);
 #pragma unroll
     for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[s][e], (float)of[e], delta);
+    if constexpr (sizeof(T) == 2) {
+      if (a.rest) {
+        const T* rest = static_cast<const T*>(a.rest) + b * a.ob + h * a.oh + (int64_t)i * a.ol;
+        const Frag<T> rf = frag_global(rest, s, a.d, lane, real);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[s][e], (float)rf[e], delta);
+      }
+    }
   }
   delta = half_sum(delta);
   if (real && half == 0) a.delta[stat] = delta;
@@ -117,19 +129,22 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dq_kerne
 #pragma unroll
   for (int n = 0; n < ND; ++n) dq[n] = f16v(0.f);
 
-  int first, last;
-  key_tiles(a, b, i0, i1, prefix, first, last);
-  const int whole = limit_of(a, i0, prefix);
+  const Meeting meet = meeting<kWaves>(wave, i0, a.lq, [&](int row) { return key_tiles(a, b, row, prefix); });
+  const int first = meet.all.x, last = meet.all.y;
   Stream<T, D, kTile, kThreads> ks, vs;
-  if (first < last) {
-    ks.fetch(k, a.kl, first * kTile, a.lk, a.d, t);
-    vs.fetch(v, a.vl, first * kTile, a.lk, a.d, t);
-  }
+  int other_id = 0;
+  auto fetch = [&](int tile) {
+    ks.fetch(k, a.kl, tile * kTile, a.lk, a.d, t);
+    vs.fetch(v, a.vl, tile * kTile, a.lk, a.d, t);
+    if (docs && t < kTile) other_id = ids[tile * kTile + t];
+  };
+  if (first < last) fetch(first);
   for (int tile = first; tile < last; ++tile) {
     const int k0 = tile * kTile;
-    const bool partial = k0 + kTile > whole || (docs && !same_document(a, b, i0 / kTile, 2, tile, 1));
+    const bool partial = meet.partial(tile);
     __syncthreads();  // the last tile is read
     if (t < 2) odd[t] = 0u;
+    if (docs && t < kTile) key_ids[t] = other_id;
     if (partial) {
       __syncthreads();
       ks.template store<true>(kt, KS, odd, t);
@@ -138,10 +153,9 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dq_kerne
     }
     vs.template store<false>(vt, VS, nullptr, t);
     __syncthreads();
-    if (tile + 1 < last) {
-      ks.fetch(k, a.kl, k0 + kTile, a.lk, a.d, t);
-      vs.fetch(v, a.vl, k0 + kTile, a.lk, a.d, t);
-    }
+    if (tile + 1 < last) fetch(tile + 1);
+    if (meet.skips(tile)) continue;
+    const bool masked = meet.masked(tile) || (partial && (odd[0] | odd[1]) != 0u);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f16v s = f16v(0.f), ds = f16v(0.f), slope_of = f16v(1.f);
@@ -155,12 +169,12 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dq_kerne
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (ds[r] - delta);
       if (a.cap > 0.f) ds *= slope_of;
-      if (partial) {
+      if (masked) {
         const unsigned set = odd[u];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           int4 other = {id, id, id, id};
-          if (docs) other = *reinterpret_cast<const int4*>(ids + at + 8 * w);
+          if (docs) other = *reinterpret_cast<const int4*>(key_ids + 32 * u + 4 * half + 8 * w);
           const int key_id[4] = {other.x, other.y, other.z, other.w};
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -190,14 +204,15 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dkv_kern
   __shared__ __attribute__((aligned(16))) T qt[kTile * S];
   __shared__ __attribute__((aligned(16))) T gt[kTile * S];
   __shared__ __attribute__((aligned(16))) float stats[2][kTile];  // lse, delta
-  __shared__ unsigned odd[2][2];                                  // of dout, of q
+  __shared__ __attribute__((aligned(16))) int query_ids[kTile];
+  __shared__ unsigned odd[2][2];  // of dout, of q
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int blocks = (a.lk + kOwn - 1) / kOwn;
   int item, block;
   place(blockIdx.x, a.n * a.hk, blocks, item, block);  // with a prefix the first keys have the most rows
   const int b = item / a.hk, hk = item % a.hk;
-  const int j0 = block * kOwn, j1 = min(j0 + kOwn, a.lk) - 1;
+  const int j0 = block * kOwn;
   const int j = j0 + 32 * wave + (lane & 31);
   const bool real = j < a.lk;
   const int prefix = a.prefixed ? prefix_of(a, b) : 0;
@@ -220,17 +235,12 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dkv_kern
 #pragma unroll
   for (int n = 0; n < ND; ++n) dk[n] = dv[n] = f16v(0.f);
 
-  // Query tiles that may see a key of the block: rows from the first whose limit passes j0.
-  int first = 0, last = (a.lq + kTile - 1) / kTile;
-  if (a.prefixed && prefix <= j0) first = max(0, j0 - off) / kTile;
-  if (docs) {
-    const int2 hull = hull_of(a.kdoc, b, j0, j1);
-    first = max(first, hull.x);
-    last = min(last, hull.y);
-  }
-  const int tiles = max(0, last - first), steps = tiles * a.group;
+  const Meeting meet = meeting<kWaves>(wave, j0, a.lk, [&](int row) { return query_tiles(a, b, row, prefix); });
+  const int first = meet.all.x, last = meet.all.y;
+  const int tiles = last - first, steps = tiles * a.group;
   Stream<T, D, kTile, kThreads> qs, gs;
   float stat = 0.f;
+  int other_id = 0;
   auto fetch = [&](int step) {
     const int h = hk * a.group + step / tiles, tile = first + step % tiles;
     qs.fetch(static_cast<const T*>(a.q) + b * a.qb + h * a.qh, a.ql, tile * kTile, a.lq, a.d, t);
@@ -239,16 +249,18 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dkv_kern
     if (t < 2 * kTile) {
       const float* from = t < kTile ? a.lse : a.delta;
       stat = i < a.lq ? from[((int64_t)b * a.hq + h) * a.lq + i] : t < kTile ? INFINITY : 0.f;
+      if (docs) other_id = ids[i];
     }
   };
   if (steps > 0) fetch(0);
   for (int step = 0; step < steps; ++step) {
     const int h = hk * a.group + step / tiles, tile = first + step % tiles, i0 = tile * kTile;
-    const bool partial = limit_of(a, i0, prefix) <= j1 || (docs && !same_document(a, b, tile, 1, j0 / kTile, 2));
+    const bool partial = meet.partial(tile);
     const float slope = a.slopes ? a.slopes[h] : 0.f;
     __syncthreads();
     if (t < 4) odd[t >> 1][t & 1] = 0u;
     if (t < 2 * kTile) stats[t / kTile][t % kTile] = stat;
+    if (docs && t < kTile) query_ids[t] = other_id;
     if (partial) {
       __syncthreads();
       qs.template store<true>(qt, S, odd[1], t);
@@ -259,6 +271,8 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dkv_kern
     }
     __syncthreads();
     if (step + 1 < steps) fetch(step + 1);
+    if (meet.skips(tile)) continue;
+    const bool masked = meet.masked(tile);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f16v s = f16v(0.f), ds = f16v(0.f), slope_of = f16v(1.f);
@@ -281,11 +295,11 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dkv_kern
       }
       if (a.cap > 0.f) ds *= slope_of;
       unsigned hidden = 0u;
-      if (partial) {
+      if (masked) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           int4 other = {id, id, id, id};
-          if (docs) other = *reinterpret_cast<const int4*>(ids + at + 8 * w);
+          if (docs) other = *reinterpret_cast<const int4*>(query_ids + 32 * u + 4 * half + 8 * w);
           const int query_id[4] = {other.x, other.y, other.z, other.w};
 #pragma unroll
           for (int r = 0; r < 4; ++r)
@@ -361,7 +375,7 @@ int64_t ctmr_masked_attention_backward_workspace_bytes(const ctmr_masked_attenti
 
 int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const void* q, const void* k, const void* v,
                                    const float* slopes, const int32_t* prefixes, const void* plan, const void* out,
-                                   const float* lse, const void* dout, const int64_t* dout_strides, void* dq,
+                                   const void* rest, const float* lse, const void* dout, const int64_t* dout_strides, void* dq,
                                    const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
                                    const int64_t* dv_strides, void* workspace, size_t workspace_bytes, void* stream) {
   const int64_t need = ctmr_masked_attention_backward_workspace_bytes(d);
@@ -370,7 +384,7 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const vo
   if (!q || !k || !v || !out || !lse || !dout || !dout_strides || (dq && !dq_strides) || (dk && !dk_strides) ||
       (dv && !dv_strides))
     return fail(CTMR_E_INVALID, "null pointer");
-  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq |
+  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)rest | (uintptr_t)dout | (uintptr_t)dq |
         (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)plan) & 15) != 0)
     return fail(CTMR_E_INVALID, "tensors and the document plan must start on 16-byte boundaries");
   const int bytes = elem_bytes(d->elem);
@@ -389,7 +403,7 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const vo
   }
   if (!dq && !dk && !dv) return CTMR_OK;
   Args a = make_args(d, q, k, v, slopes, prefixes, plan);
-  a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse), a.dout = dout;
+  a.out = const_cast<void*>(out), a.rest = const_cast<void*>(rest), a.lse = const_cast<float*>(lse), a.dout = dout;
   a.dq = dq, a.dk = dk, a.dv = dv, a.delta = (float*)workspace;
   a.ob = d->out_strides[0], a.oh = d->out_strides[1], a.ol = d->out_strides[2];
   a.gb = dout_strides[0], a.gh = dout_strides[1], a.gl = dout_strides[2];

@@ -257,8 +257,8 @@ def _attention_heads(t: Tensor) -> Tensor:
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, prefixes, plan, scale, softcap, prefixed, prefix):
-        out, lse = ops.masked_attention(q, k, v, slopes, prefixes, plan, scale, softcap, prefixed, prefix, True)
-        ctx.save_for_backward(q, k, v, slopes, prefixes, plan, out, lse)
+        out, rest, lse = ops.masked_attention(q, k, v, slopes, prefixes, plan, scale, softcap, prefixed, prefix, True)
+        ctx.save_for_backward(q, k, v, slopes, prefixes, plan, out, rest, lse)
         ctx.args = (scale, softcap, prefixed, prefix)
         ctx.token, ctx.captured = _graph_token(q, k, v), torch.cuda.is_current_stream_capturing()
         return out

@@ -573,8 +573,19 @@ def _on(t: Tensor):
     return _SAME_DEVICE if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
 
+def _raw_stream(device: torch.device) -> int:
+    """``_stream`` without building a stream object (2 us of a small call's host time)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _workspace(nbytes: int, device: torch.device) -> Optional[Tensor]:
     return torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_bytes(n: int, s: int, c: int, groups: int, elem: int, backward: int) -> int:
+    return _lib.check(_lib.lib().ctmr_norm_workspace_bytes(n, s, c, groups, elem, backward),
+                      "ctmr_norm_workspace_bytes")
 
 
 @_custom_op("ctmr::norm_forward")
@@ -589,11 +600,11 @@ def norm_forward(x: Tensor, weight: Tensor, bias: Tensor, groups: int, eps: floa
         return y, saved.zero_()
     s, elem, lib = x.numel() // (n * c), ELEMENTS[x.dtype], _lib.lib()
     with _on(x):
-        nbytes = _lib.check(lib.ctmr_norm_workspace_bytes(n, s, c, groups, elem, 0), "ctmr_norm_workspace_bytes")
+        nbytes = _norm_bytes(n, s, c, groups, elem, 0)
         ws = _workspace(nbytes, x.device)
         _lib.check(lib.ctmr_norm_forward(n, s, c, groups, eps, elem, x.data_ptr(), ELEMENTS[weight.dtype],
                                          weight.data_ptr(), bias.data_ptr(), silu, y.data_ptr(), saved.data_ptr(),
-                                         _ptr(ws), nbytes, _stream(x.device)), "ctmr_norm_forward")
+                                         _ptr(ws), nbytes, _raw_stream(x.device)), "ctmr_norm_forward")
     return y, saved
 
 
@@ -616,13 +627,13 @@ def norm_backward(x: Tensor, dy: Tensor, weight: Tensor, bias: Tensor, saved: Te
         return dx, dw.zero_(), db.zero_()
     s, elem, lib = x.numel() // (n * c), ELEMENTS[x.dtype], _lib.lib()
     with _on(x):
-        nbytes = _lib.check(lib.ctmr_norm_workspace_bytes(n, s, c, groups, elem, 1), "ctmr_norm_workspace_bytes")
+        nbytes = _norm_bytes(n, s, c, groups, elem, 1)
         ws = _workspace(nbytes, x.device)
         _lib.check(lib.ctmr_norm_backward(n, s, c, groups, elem, x.data_ptr(), dy.data_ptr(), ELEMENTS[weight.dtype],
                                           weight.data_ptr(), bias.data_ptr(), silu, saved.data_ptr(),
                                           dx.data_ptr() if want_x else None, dw.data_ptr() if want_params else None,
                                           db.data_ptr() if want_params else None, _ptr(ws), nbytes,
-                                          _stream(x.device)), "ctmr_norm_backward")
+                                          _raw_stream(x.device)), "ctmr_norm_backward")
     return dx, dw, db
 
 
@@ -640,11 +651,16 @@ def _heads_like(t: Tensor) -> Tensor:
     return t.new_empty((b, l, h, d)).transpose(1, 2)
 
 
-@functools.lru_cache(maxsize=64)
-def _turns(sections: tuple[int, ...], base: float):
-    """Turns of every pair at position 1 as a C array: ``base ** (-2 i / width) / (2 pi)``."""
-    turns = [base ** (-2.0 * i / w) / (2.0 * math.pi) for w in sections for i in range(w // 2)]
-    return (ctypes.c_double * len(turns))(*turns)
+@functools.lru_cache(maxsize=256)
+def _rotary_desc(shape: tuple[int, ...], k_heads: int, widths: tuple[int, ...], base: float, elem: int, position_type: int,
+                 inverse: bool, position_stride: int, q_strides: tuple[int, ...], k_strides: tuple[int, ...]):
+    """The descriptor, and the turns of every pair at position 1, ``base ** (-2 i / width) / (2 pi)``; the
+    outputs lie as (B, L, H, D)."""
+    b, hq, l, d = shape
+    desc = _lib.RotaryDesc(b, l, hq, k_heads, d, len(widths), widths, elem, position_type, inverse, 0, position_stride,
+                           q_strides[:3], k_strides[:3], (l * hq * d, d, hq * d), (l * k_heads * d, d, k_heads * d))
+    turns = [base ** (-2.0 * i / w) / (2.0 * math.pi) for w in widths for i in range(w // 2)]
+    return desc, (ctypes.c_double * len(turns))(*turns)
 
 
 @_custom_op("ctmr::rotary")
@@ -653,21 +669,18 @@ def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, sections: Sequence
     """``ctmr_rotary`` of (B, H, L, D) heads with a unit last stride and contiguous positions; the outputs
     lie as (B, L, H, D), the second is empty without ``k``."""
     _require_device(q, k, positions)
-    b, hq, l, d = (int(v) for v in q.shape)
     out = _heads_like(q)
     k_out = q.new_empty((0,)) if k is None else _heads_like(k)
     if q.numel() == 0:
         return out, k_out
-    widths = tuple(int(w) for w in sections)
-    desc = _lib.RotaryDesc(b, l, hq, 0 if k is None else int(k.shape[1]), d, len(widths), (ctypes.c_int32 * 4)(*widths),
-                           ELEMENTS[q.dtype], POSITION_TYPES[positions.dtype], inverse, 0,
-                           positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0,
-                           q.stride()[:3], (0, 0, 0) if k is None else k.stride()[:3], out.stride()[:3],
-                           (0, 0, 0) if k is None else k_out.stride()[:3])
+    desc, turns = _rotary_desc(tuple(q.shape), 0 if k is None else int(k.shape[1]), tuple(sections), base,
+                               ELEMENTS[q.dtype], POSITION_TYPES[positions.dtype], inverse,
+                               positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0,
+                               q.stride(), (0, 0, 0) if k is None else k.stride())
     with _on(q):
-        _lib.check(_lib.lib().ctmr_rotary(ctypes.byref(desc), q.data_ptr(), _ptr(k), positions.data_ptr(),
-                                          _turns(widths, base), out.data_ptr(),
-                                          None if k is None else k_out.data_ptr(), _stream(q.device)), "ctmr_rotary")
+        _lib.check(_lib.lib().ctmr_rotary(ctypes.byref(desc), q.data_ptr(), _ptr(k), positions.data_ptr(), turns,
+                                          out.data_ptr(), None if k is None else k_out.data_ptr(),
+                                          _raw_stream(q.device)), "ctmr_rotary")
     return out, k_out
 
 
@@ -686,7 +699,7 @@ def documents(query_ids: Tensor, key_ids: Tensor) -> Tensor:
     plan = torch.empty(nbytes, device=query_ids.device, dtype=torch.uint8)
     with _on(query_ids):
         _lib.check(lib.ctmr_documents(n, lq, lk, query_ids.data_ptr(), key_ids.data_ptr(), plan.data_ptr(), nbytes,
-                                      _stream(plan.device)), "ctmr_documents")
+                                      _raw_stream(plan.device)), "ctmr_documents")
     return plan
 
 
@@ -702,71 +715,81 @@ def _head_strides(t: Tensor) -> tuple[int, int, int]:
     return (s[0] if shape[0] > 1 else 0, s[1] if shape[1] > 1 else 0, s[2] if shape[2] > 1 else 0)
 
 
-def _attention_desc(q: Tensor, k: Tensor, v: Tensor, out: Tensor, scale: float, softcap: float,
-                    prefixed: bool, prefix: int) -> "_lib.MaskedAttentionDesc":
-    return _lib.MaskedAttentionDesc(int(q.shape[0]), int(q.shape[2]), int(k.shape[2]), int(q.shape[1]), int(k.shape[1]),
-                                    int(q.shape[3]), ELEMENTS[q.dtype], prefixed, prefix, scale, softcap, 0,
-                                    _head_strides(q), _head_strides(k), _head_strides(v), _head_strides(out))
+@functools.lru_cache(maxsize=256)
+def _attention_desc(q_shape, k_shape, elem: int, q_strides, k_strides, v_strides, scale: float, softcap: float,
+                    prefixed: bool, prefix: int):
+    """The descriptor and the forward and backward workspaces' bytes; the output lies as (B, L, H, D)."""
+    b, hq, lq, d = q_shape
+    desc = _lib.MaskedAttentionDesc(b, lq, k_shape[2], hq, k_shape[1], d, elem, prefixed, prefix, scale, softcap, 0,
+                                    q_strides, k_strides, v_strides, (lq * hq * d, d, hq * d))
+    ref, lib = ctypes.byref(desc), _lib.lib()
+    return (desc, _lib.check(lib.ctmr_masked_attention_workspace_bytes(ref), "ctmr_masked_attention_workspace_bytes"),
+            _lib.check(lib.ctmr_masked_attention_backward_workspace_bytes(ref),
+                       "ctmr_masked_attention_backward_workspace_bytes"))
+
+
+def _attention_desc_of(q: Tensor, k: Tensor, v: Tensor, scale: float, softcap: float, prefixed: bool, prefix: int):
+    return _attention_desc(tuple(q.shape), tuple(k.shape), ELEMENTS[q.dtype], _head_strides(q), _head_strides(k),
+                           _head_strides(v), scale, softcap, prefixed, prefix)
 
 
 @_custom_op("ctmr::masked_attention")
 def masked_attention(q: Tensor, k: Tensor, v: Tensor, slopes: Optional[Tensor], prefixes: Optional[Tensor],
                      plan: Optional[Tensor], scale: float, softcap: float, prefixed: bool, prefix: int,
-                     want_lse: bool) -> tuple[Tensor, Tensor]:
-    """``ctmr_masked_attention`` of (B, H, L, D) heads: the output, which lies as (B, L, H, D), and the rows'
-    (B, H, Lq) log2 sums, empty unless wanted."""
+                     want_grad: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """``ctmr_masked_attention`` of (B, H, L, D) heads: the output, which lies as (B, L, H, D), and what the
+    gradients need, empty unless wanted: what rounding took from a 16-bit output, and the rows' (B, H, Lq) log2
+    sums."""
     _require_device(q, k, v, slopes, prefixes, plan)
     out = _heads_like(q)
-    lse = torch.empty(q.shape[:3] if want_lse else (0,), device=q.device, dtype=torch.float32)
+    rest = _heads_like(q) if want_grad and q.element_size() == 2 else q.new_empty((0,))
+    lse = torch.empty(q.shape[:3] if want_grad else (0,), device=q.device, dtype=torch.float32)
     if q.numel() == 0 or k.shape[2] == 0:
-        return out.zero_(), lse.fill_(math.inf)
-    desc, lib = _attention_desc(q, k, v, out, scale, softcap, prefixed, prefix), _lib.lib()
+        return out.zero_(), rest.zero_(), lse.fill_(math.inf)
+    desc, nbytes, _ = _attention_desc_of(q, k, v, scale, softcap, prefixed, prefix)
     with _on(q):
-        nbytes = _lib.check(lib.ctmr_masked_attention_workspace_bytes(ctypes.byref(desc)),
-                            "ctmr_masked_attention_workspace_bytes")
         ws = _workspace(nbytes, q.device)
-        _lib.check(lib.ctmr_masked_attention(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(slopes),
-                                             _ptr(prefixes), _ptr(plan), out.data_ptr(),
-                                             lse.data_ptr() if want_lse else None, _ptr(ws), nbytes,
-                                             _stream(q.device)), "ctmr_masked_attention")
-    return out, lse
+        _lib.check(_lib.lib().ctmr_masked_attention(
+            ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(slopes), _ptr(prefixes), _ptr(plan),
+            out.data_ptr(), rest.data_ptr() if rest.numel() else None, lse.data_ptr() if want_grad else None, _ptr(ws),
+            nbytes, _raw_stream(q.device)), "ctmr_masked_attention")
+    return out, rest, lse
 
 
 @masked_attention.register_fake
-def _(q, k, v, slopes, prefixes, plan, scale, softcap, prefixed, prefix, want_lse):
-    return _heads_like(q), q.new_empty(q.shape[:3] if want_lse else (0,), dtype=torch.float32)
+def _(q, k, v, slopes, prefixes, plan, scale, softcap, prefixed, prefix, want_grad):
+    return (_heads_like(q), _heads_like(q) if want_grad and q.element_size() == 2 else q.new_empty((0,)),
+            q.new_empty(q.shape[:3] if want_grad else (0,), dtype=torch.float32))
 
 
 @_custom_op("ctmr::masked_attention_backward")
 def masked_attention_backward(q: Tensor, k: Tensor, v: Tensor, slopes: Optional[Tensor], prefixes: Optional[Tensor],
-                              plan: Optional[Tensor], out: Tensor, lse: Tensor, dout: Tensor, scale: float,
-                              softcap: float, prefixed: bool, prefix: int, want_q: bool,
+                              plan: Optional[Tensor], out: Tensor, rest: Tensor, lse: Tensor, dout: Tensor,
+                              scale: float, softcap: float, prefixed: bool, prefix: int, want_q: bool,
                               want_kv: bool) -> tuple[Tensor, Tensor, Tensor]:
     """``ctmr_masked_attention_backward``: gradients of ``q``, ``k`` and ``v``, which lie as (B, L, H, D); empty
     where not wanted."""
-    _require_device(q, k, v, slopes, prefixes, plan, out, lse, dout)
+    _require_device(q, k, v, slopes, prefixes, plan, out, rest, lse, dout)
     none = (0,)
     dq = _heads_like(q) if want_q else q.new_empty(none)
     dk, dv = (_heads_like(k), _heads_like(v)) if want_kv else (k.new_empty(none), v.new_empty(none))
     if q.numel() == 0 or k.shape[2] == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    desc, lib = _attention_desc(q, k, v, out, scale, softcap, prefixed, prefix), _lib.lib()
+    desc, _, nbytes = _attention_desc_of(q, k, v, scale, softcap, prefixed, prefix)
     strides = lambda t, want=True: (ctypes.c_int64 * 3)(*_head_strides(t)) if want else None
     with _on(q):
-        nbytes = _lib.check(lib.ctmr_masked_attention_backward_workspace_bytes(ctypes.byref(desc)),
-                            "ctmr_masked_attention_backward_workspace_bytes")
         ws = _workspace(nbytes, q.device)
-        _lib.check(lib.ctmr_masked_attention_backward(
+        _lib.check(_lib.lib().ctmr_masked_attention_backward(
             ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(slopes), _ptr(prefixes), _ptr(plan),
-            out.data_ptr(), lse.data_ptr(), dout.data_ptr(), strides(dout), dq.data_ptr() if want_q else None,
-            strides(dq, want_q), dk.data_ptr() if want_kv else None, strides(dk, want_kv),
-            dv.data_ptr() if want_kv else None, strides(dv, want_kv), _ptr(ws), nbytes, _stream(q.device)),
+            out.data_ptr(), rest.data_ptr() if rest.numel() else None, lse.data_ptr(), dout.data_ptr(), strides(dout),
+            dq.data_ptr() if want_q else None, strides(dq, want_q), dk.data_ptr() if want_kv else None, strides(dk, want_kv),
+            dv.data_ptr() if want_kv else None, strides(dv, want_kv), _ptr(ws), nbytes, _raw_stream(q.device)),
             "ctmr_masked_attention_backward")
     return dq, dk, dv
 
 
 @masked_attention_backward.register_fake
-def _(q, k, v, slopes, prefixes, plan, out, lse, dout, scale, softcap, prefixed, prefix, want_q, want_kv):
+def _(q, k, v, slopes, prefixes, plan, out, rest, lse, dout, scale, softcap, prefixed, prefix, want_q, want_kv):
     none = (0,)
     return (_heads_like(q) if want_q else q.new_empty(none), _heads_like(k) if want_kv else k.new_empty(none),
             _heads_like(v) if want_kv else v.new_empty(none))

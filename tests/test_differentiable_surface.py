@@ -177,7 +177,7 @@ def test_attention_host_checks(ctmr, native_loaded):
 
     def call(q=p, plan=None, out=p, ws=p, nbytes=0, **kw):
         return native_loaded.ctmr_masked_attention(ctypes.byref(_attention_desc(L, **kw)), q, p, p, None, None, plan, out,
-                                                   None, ws, nbytes, None)
+                                                   None, None, ws, nbytes, None)
 
     assert call(q=None) == L.E_INVALID and call(out=None) == L.E_INVALID and call(q=p + 8) == L.E_INVALID
     assert call(plan=p + 4) == L.E_INVALID and call(out_strides=(25600, 32, 130)) == L.E_INVALID
@@ -188,7 +188,7 @@ def test_attention_host_checks(ctmr, native_loaded):
 
     def back(q=p, out=p, lse=p, dout=p, s=strides, dq=None, dq_s=strides, dk=None, ws=p, nbytes=1 << 20, **kw):
         return native_loaded.ctmr_masked_attention_backward(
-            ctypes.byref(_attention_desc(L, **kw)), q, p, p, None, None, None, out, lse, dout, s, dq, dq_s, dk, strides,
+            ctypes.byref(_attention_desc(L, **kw)), q, p, p, None, None, None, out, None, lse, dout, s, dq, dq_s, dk, strides,
             None, None, ws, nbytes, None)
 
     assert back() == L.OK  # nothing wanted, nothing launched
@@ -200,7 +200,7 @@ def test_attention_host_checks(ctmr, native_loaded):
     assert back(ws=None, dq=p) == L.E_WORKSPACE
 
     docs = native_loaded.ctmr_documents_bytes
-    assert docs(2, 100, 65) == 2 * (128 * 4 + 128 * 4 + 2 * 16 + 2 * 16 + 2 * 8 + 2 * 8)
+    assert docs(2, 100, 65) == 2 * (128 * 4 + 128 * 4 + 2 * 16 + 2 * 16 + 4 * 16 + 3 * 16)
     assert docs(0, 1, 1) == L.E_INVALID and docs(70000, 1, 1) == L.E_UNSUPPORTED
     assert native_loaded.ctmr_documents(2, 100, 65, p, p, p, 10, None) == L.E_WORKSPACE
     assert native_loaded.ctmr_documents(2, 100, 65, None, p, p, 1 << 20, None) == L.E_INVALID
@@ -211,10 +211,11 @@ def test_attention_traces(ctmr):
 
     with FakeTensorMode():
         q, k = (torch.empty(2, h, 6, 32, device="cuda", dtype=torch.bfloat16) for h in (4, 2))
-        out, lse = torch.ops.ctmr.masked_attention(q, k, k, None, None, None, 1.0, 0.0, False, 0, True)
+        out, rest, lse = torch.ops.ctmr.masked_attention(q, k, k, None, None, None, 1.0, 0.0, False, 0, True)
         assert out.shape == q.shape and out.transpose(1, 2).is_contiguous() and lse.shape == (2, 4, 6)
-        dq, dk, dv = torch.ops.ctmr.masked_attention_backward(q, k, k, None, None, None, out, lse, out, 1.0, 0.0, False, 0,
-                                                              True, False)
+        assert rest.shape == out.shape and rest.stride() == out.stride()
+        dq, dk, dv = torch.ops.ctmr.masked_attention_backward(q, k, k, None, None, None, out, rest, lse, out, 1.0, 0.0,
+                                                              False, 0, True, False)
         assert dq.shape == q.shape and dk.shape == dv.shape == (0,)
         plan = torch.ops.ctmr.documents(*(torch.empty(2, l, device="cuda", dtype=torch.int32) for l in (100, 65)))
         assert plan.dtype == torch.uint8 and plan.numel() == ctmr._lib.lib().ctmr_documents_bytes(2, 100, 65)
