@@ -488,7 +488,8 @@ int ctmr_documents(int32_t n, int32_t lq, int32_t lk, const int32_t* query_ids, 
  * (n, k_heads, lk, head_dim), all of type elem, q_heads a multiple of k_heads
  * (query head h reads key head h / (q_heads / k_heads)).  head_dim is a multiple
  * of 8 up to 128; strides (batch, head, row) in values are multiples of 16 bytes,
- * values of a head lie side by side.  Scores of row i and key j, p_i = i + lk - lq:
+ * values of a head lie side by side and rows do not overlap (those of batch items
+ * and heads may).  Scores of row i and key j, p_i = i + lk - lq:
  *   s = scale q_i . k_j;  softcap > 0: s = softcap tanh(s / softcap)
  *   slopes (q_heads) or NULL: s -= slopes[h] |p_i - j|
  * Key j is visible to row i if: with `prefixed`, j <= p_i or j < the prefix

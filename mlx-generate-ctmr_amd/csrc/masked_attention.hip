@@ -24,7 +24,8 @@ namespace attn {
 namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
-constexpr int kRows = 32 * kWaves;  // query rows of a workgroup of the tiled form
+constexpr int kRows = kBlockRows;  // query rows of a workgroup of the tiled form
+static_assert(kRows == 32 * kWaves && kRows == 4 * kGrain, "32 rows a wave");
 constexpr float kLazy = 8.0f;
 // fp16 weights are raised by 2^6 (both in O and l): below 2^8 * 2^6 they stay in range, and weights down to
 // 2^-20 of the reference keep all their bits.
@@ -40,8 +41,8 @@ struct RowMask {
 // themselves (c = 1), else the products (c = scale log2 e).  Masked keys become -inf; ids: of the keys from k0 on, or
 // null.
 template <typename T, int NB>
-__device__ __forceinline__ float score_blocks(const Args& a, f16v (&s)[NB], int k0, int pos, float slope,
-                                              bool partial, const RowMask& m, const int* ids, int lane) {
+__device__ __forceinline__ float score_blocks(const Scoring& a, f16v (&s)[NB], int k0, int pos, bool partial,
+                                              const RowMask& m, const int* ids, int lane) {
   const int half = lane >> 5;
   float c = a.scale * kLog2e;
   if (a.cap > 0.f) {
@@ -49,11 +50,11 @@ __device__ __forceinline__ float score_blocks(const Args& a, f16v (&s)[NB], int 
 #pragma unroll
     for (int u = 0; u < NB; ++u)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[u][r] = out * tanh_of<T>(s[u][r] * in);
+      for (int r = 0; r < 16; ++r) s[u][r] = out * tanh_of<T>(s[u][r], in);
     c = 1.0f;
   }
-  if (a.slopes) {
-    const float per = slope * kLog2e;
+  if (a.sloped) {
+    const float per = a.slope * kLog2e;
 #pragma unroll
     for (int u = 0; u < NB; ++u)
 #pragma unroll
@@ -63,27 +64,34 @@ __device__ __forceinline__ float score_blocks(const Args& a, f16v (&s)[NB], int 
       }
     c = 1.0f;
   }
-  if (partial) {
+  // Two selects of two instructions each, and only where they decide something: a key past the end has no document.
+  if (partial && ids) {
 #pragma unroll
     for (int u = 0; u < NB; ++u)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int at = 32 * u + 8 * g + 4 * half, j = k0 + at;
-        int4 id = {m.id, m.id, m.id, m.id};
-        if (ids) id = *reinterpret_cast<const int4*>(ids + at);
-        if (j >= m.limit || id.x != m.id) s[u][4 * g] = -INFINITY;
-        if (j + 1 >= m.limit || id.y != m.id) s[u][4 * g + 1] = -INFINITY;
-        if (j + 2 >= m.limit || id.z != m.id) s[u][4 * g + 2] = -INFINITY;
-        if (j + 3 >= m.limit || id.w != m.id) s[u][4 * g + 3] = -INFINITY;
+        const int4 id = *reinterpret_cast<const int4*>(ids + 32 * u + 8 * g + 4 * half);
+        s[u][4 * g] = id.x != m.id ? -INFINITY : s[u][4 * g];
+        s[u][4 * g + 1] = id.y != m.id ? -INFINITY : s[u][4 * g + 1];
+        s[u][4 * g + 2] = id.z != m.id ? -INFINITY : s[u][4 * g + 2];
+        s[u][4 * g + 3] = id.w != m.id ? -INFINITY : s[u][4 * g + 3];
       }
+  }
+  if (partial && (a.prefixed || !ids)) {
+    const int limit = m.limit - k0 - 4 * half;
+#pragma unroll
+    for (int u = 0; u < NB; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[u][r] = 32 * u + 8 * (r >> 2) + (r & 3) >= limit ? -INFINITY : s[u][r];
   }
   return c;
 }
 
-// One step of the running softmax: scores (units log2 / c) -> P; m and l move, returns whether any row's outputs
-// must be scaled by alpha first.
+// One step of the running softmax: scores (units log2 / c) -> P as operands; m and l move, returns whether any row's
+// outputs must be scaled by alpha first.  l sums P before its rounding: the gradients' P is exact to lse.
 template <typename T, int NB>
-__device__ __forceinline__ bool softmax_blocks(f16v (&s)[NB], float c, float& m, float& l, float& alpha) {
+__device__ __forceinline__ bool softmax_blocks(f16v (&s)[NB], Frag<T> (&p)[NB][2], float c, float& m, float& l,
+                                               float& alpha) {
   float top = s[0][0];
 #pragma unroll
   for (int u = 0; u < NB; ++u)
@@ -95,16 +103,18 @@ __device__ __forceinline__ bool softmax_blocks(f16v (&s)[NB], float c, float& m,
   alpha = move ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
   m = mn;
   const float shift = kLift<T> - mn;
-  float sum = 0.f;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int u = 0; u < NB; ++u)
+  for (int u = 0; u < NB; ++u) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float p = __builtin_amdgcn_exp2f(fmaf(s[u][r], c, shift));
-      s[u][r] = p;
-      sum += p;
+      s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c, shift));
+      sum[r & 3] += s[u][r];
     }
-  l = l * alpha + sum;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) p[u][w] = result_frag<T>(s[u], w);
+  }
+  l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
   return __any(move);
 }
 
@@ -190,57 +200,67 @@ __device__ __forceinline__ void write_row(const Args& a, const f16v (&o)[ND], fl
 // wave, and streams K and V through LDS in 64-key tiles, double-buffered: the loads
 // of the next tile are in flight while the current one is multiplied.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void attention_kernel(Args a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void attention_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
-  constexpr int KS = tile_stride<T, D>(ALONG), VS = tile_stride<T, D>(DOWN);
-  __shared__ __attribute__((aligned(16))) T kt[2][kTile * KS];
-  __shared__ __attribute__((aligned(16))) T vt[2][kTile * VS];
+  typedef Tile<T, D> Lds;
+  __shared__ __attribute__((aligned(16))) char kt[2][kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char vt[2][kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) int key_ids[2][kTile];
   __shared__ unsigned odd[3][2];
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int blocks = (a.lq + kRows - 1) / kRows;
+  const bool docs = a.qdoc.ids != nullptr;
   int item, block;
-  place(blockIdx.x, a.n * a.hq, blocks, item, block);
+  Part part;
+  place(blockIdx.x, a.n * a.hq, blocks, docs ? 2 : 1, item, block, part.part);
   if (a.prefixed) block = blocks - 1 - block;  // the longest rows first
   const int b = item / a.hq, h = item % a.hq;
+  if (part.part == 1 && !is_mixed(a.qdoc, b, block)) return;
   const int i0 = block * kRows;
   const int i = i0 + 32 * wave + (lane & 31);
   const int prefix = a.prefixed ? prefix_of(a, b) : 0;
-  const bool docs = a.qdoc.ids != nullptr;
   const int* ids = docs ? a.kdoc.ids + (int64_t)b * a.kdoc.stride : nullptr;
-  const RowMask mask = {i < a.lq ? limit_of(a, i, prefix) : 0, docs && i < a.lq ? row_id(a, b, i) : -2};
+  part.first_id = docs ? id_of(a, b, i0) : 0;
+  const int own = docs && i < a.lq ? id_of(a, b, i) : 0;
+  const bool mine = i < a.lq && (!docs || part.has(own));  // rows of the other part are left to it
+  const RowMask mask = {mine ? limit_of(a, i, prefix) : 0, own < 0 || !mine ? -2 : own};
   const int pos = i + a.lk - a.lq;
-  const float slope = a.slopes ? a.slopes[h] : 0.f;
+  const Scoring scoring = scoring_of(a, h);
   const T* q = static_cast<const T*>(a.q) + b * a.qb + h * a.qh + (int64_t)i * a.ql;
   const T* k = static_cast<const T*>(a.k) + b * a.kb + (h / a.group) * a.kh;
   const T* v = static_cast<const T*>(a.v) + b * a.vb + (h / a.group) * a.vh;
 
-  const Meeting meet = meeting<kWaves>(wave, i0, a.lq, [&](int row) { return key_tiles(a, b, row, prefix); });
+  const Meeting meet = meeting<kWaves>(wave, i0, a.lq, [&](int row) { return key_tiles(a, b, row, prefix, &part); });
   int first = meet.all.x, last = meet.all.y;
   split_range(blockIdx.y, a.splits, first, last);
 
   Frag<T> qf[NK];
 #pragma unroll
-  for (int s = 0; s < NK; ++s) qf[s] = frag_global(q, s, a.d, lane, i < a.lq);
+  for (int s = 0; s < NK; ++s) qf[s] = frag_global(q, s, a.d, lane, mine);
   f16v o[ND];
 #pragma unroll
   for (int n = 0; n < ND; ++n) o[n] = f16v(0.f);
   float m = kNone, l = 0.f;
 
+  Rows<T, kTile> krows, vrows;
+  krows.begin(k, a.kl, first * kTile, a.lk, a.d);
+  vrows.begin(v, a.vl, first * kTile, a.lk, a.d);
   Stream<T, D, kTile, kThreads> ks, vs;
   bool partial = false;  // of the tile in flight: some row of the workgroup has a masked key in it
   int id = 0;
   auto fetch = [&](int tile) {
-    ks.fetch(k, a.kl, tile * kTile, a.lk, a.d, t);
-    vs.fetch(v, a.vl, tile * kTile, a.lk, a.d, t);
+    ks.fetch(krows, t);
+    vs.fetch(vrows, t);
+    krows.next();
+    vrows.next();
     partial = meet.partial(tile);
     if (docs && t < kTile) id = ids[tile * kTile + t];
   };
   auto stage = [&](int buf, int slot) {
-    ks.template store<false>(kt[buf], KS, nullptr, t);
-    if (partial) vs.template store<true>(vt[buf], VS, odd[slot], t);
-    else vs.template store<false>(vt[buf], VS, nullptr, t);
+    ks.template store<false>(kt[buf], nullptr, t);
+    if (partial) vs.template store<true>(vt[buf], odd[slot], t);
+    else vs.template store<false>(vt[buf], nullptr, t);
     if (docs && t < kTile) key_ids[buf][t] = id;
   };
   if (t < 6) odd[t / 2][t % 2] = 0u;
@@ -260,22 +280,29 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(Args a) {
 #pragma unroll
       for (int n = 0; n < NK; ++n)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) s[u] = mma<T>(frag_along(kt[buf], KS, 32 * u, n, lane), qf[n], s[u]);
+        for (int u = 0; u < 2; ++u) s[u] = mma<T>(Lds::along(kt[buf], 32 * u, n, lane), qf[n], s[u]);
+      // V's first operands are read before the softmax, which covers the latency, as far as registers go.
+      constexpr int kEarly = sizeof(T) == 4 ? 0 : D == 128 ? 0 : 2;  // contraction steps
+      Frag<T> vf[2][ND];
+#pragma unroll
+      for (int w = 0; w < kEarly; ++w)
+#pragma unroll
+        for (int n = 0; n < ND; ++n) vf[w][n] = Lds::down(vt[buf], 16 * w, n, lane);
       const int* tile_ids = docs ? key_ids[buf] : nullptr;
-      const float c = score_blocks<T, 2>(a, s, k0, pos, slope, meet.masked(tile), mask, tile_ids, lane);
+      const float c = score_blocks<T, 2>(scoring, s, k0, pos, meet.masked(tile), mask, tile_ids, lane);
       float alpha;
-      if (softmax_blocks<T, 2>(s, c, m, l, alpha)) {
+      Frag<T> p[2][2];
+      if (softmax_blocks<T, 2>(s, p, c, m, l, alpha)) {
 #pragma unroll
         for (int n = 0; n < ND; ++n) o[n] *= alpha;
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const Frag<T> p = result_frag<T>(s[u], w);
+        for (int w = 0; w < 2; ++w)
 #pragma unroll
-          for (int n = 0; n < ND; ++n) o[n] = mma<T>(frag_down(vt[buf], VS, 32 * u + 16 * w, n, lane), p, o[n]);
-        }
+          for (int n = 0; n < ND; ++n)
+            o[n] = mma<T>(u == 0 && w < kEarly ? vf[w][n] : Lds::down(vt[buf], 32 * u + 16 * w, n, lane), p[u][w], o[n]);
       if (now) {
         const unsigned lo = odd[slot][0], hi = odd[slot][1];
         if (lo | hi) add_odd_values<T, ND>(a, o, v, k0, lo, hi, mask, tile_ids, lane);
@@ -289,7 +316,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(Args a) {
     slot = next;
   }
   l = half_sum(l);
-  if (i < a.lq) write_row<T, ND>(a, o, m, l, b, h, i, blockIdx.y, lane);
+  if (mine) write_row<T, ND>(a, o, m, l, b, h, i, blockIdx.y, lane);
 }
 
 // The form for few rows: the group * lq <= 32 query rows of a key head are one
@@ -300,7 +327,7 @@ constexpr int kFewTile = 32;
 
 template <typename T, int D>
 constexpr int few_lds() {  // bytes; the join takes four 32 x D blocks of fp32 and (m, l) of each
-  constexpr int tiles = kWaves * kFewTile * (tile_stride<T, D>(ALONG) + tile_stride<T, D>(DOWN)) * (int)sizeof(T);
+  constexpr int tiles = kWaves * kFewTile * 2 * Tile<T, D>::kRow;
   constexpr int join = kWaves * 32 * (D + 4) * 4;
   return tiles > join ? tiles : join;
 }
@@ -308,7 +335,7 @@ constexpr int few_lds() {  // bytes; the join takes four 32 x D blocks of fp32 a
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 1) void attention_few_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
-  constexpr int KS = tile_stride<T, D>(ALONG), VS = tile_stride<T, D>(DOWN);
+  typedef Tile<T, D> Lds;
   __shared__ __attribute__((aligned(16))) char lds[few_lds<T, D>()];
   __shared__ unsigned odd[kWaves];
   __shared__ float2 state[kWaves][32];
@@ -320,16 +347,17 @@ __global__ __launch_bounds__(kThreads, 1) void attention_few_kernel(Args a) {
   const int prefix = a.prefixed ? prefix_of(a, b) : 0;
   const bool docs = a.qdoc.ids != nullptr;
   const int* ids = docs ? a.kdoc.ids + (int64_t)b * a.kdoc.stride : nullptr;
-  const RowMask mask = {limit_of(a, i, prefix), docs ? row_id(a, b, i) : -2};
+  const int own = docs ? id_of(a, b, i) : 0;
+  const RowMask mask = {limit_of(a, i, prefix), own < 0 ? -2 : own};
   const int pos = i + a.lk - a.lq;
-  const float slope = a.slopes ? a.slopes[h] : 0.f;
+  const Scoring scoring = scoring_of(a, h);
   const T* q = static_cast<const T*>(a.q) + b * a.qb + h * a.qh + (int64_t)i * a.ql;
   const T* k = static_cast<const T*>(a.k) + b * a.kb + hk * a.kh;
   const T* v = static_cast<const T*>(a.v) + b * a.vb + hk * a.vh;
-  T* kt = reinterpret_cast<T*>(lds) + wave * kFewTile * (KS + VS);
-  T* vt = kt + kFewTile * KS;
+  char* kt = lds + wave * kFewTile * 2 * Lds::kRow;
+  char* vt = kt + kFewTile * Lds::kRow;
 
-  const int4 range = key_tiles(a, b, 0, prefix);  // lq <= kGrain; tiles of 64 keys
+  const int4 range = key_tiles(a, b, 0, prefix, nullptr);  // lq <= kGrain; tiles of 64 keys
   int first = range.x, last = range.y;
   split_range(blockIdx.y, a.splits, first, last);
   const int end = min(last * kTile, a.lk);
@@ -343,39 +371,39 @@ __global__ __launch_bounds__(kThreads, 1) void attention_few_kernel(Args a) {
   float m = kNone, l = 0.f;
 
   Stream<T, D, kFewTile, 64> ks, vs;
+  Rows<T, kFewTile> krows, vrows;
   int k0 = first * kTile + wave * kFewTile;
-  if (k0 < end) {
-    ks.fetch(k, a.kl, k0, a.lk, a.d, lane);
-    vs.fetch(v, a.vl, k0, a.lk, a.d, lane);
-  }
+  auto fetch = [&](int at) {
+    krows.begin(k, a.kl, at, a.lk, a.d);
+    vrows.begin(v, a.vl, at, a.lk, a.d);
+    ks.fetch(krows, lane);
+    vs.fetch(vrows, lane);
+  };
+  if (k0 < end) fetch(k0);
   for (; k0 < end; k0 += kWaves * kFewTile) {
     const bool partial = k0 / kTile < range.z || k0 / kTile >= range.w;
     if (lane == 0) odd[wave] = 0u;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    ks.template store<false>(kt, KS, nullptr, lane);
-    if (partial) vs.template store<true>(vt, VS, &odd[wave], lane);
-    else vs.template store<false>(vt, VS, nullptr, lane);
+    ks.template store<false>(kt, nullptr, lane);
+    if (partial) vs.template store<true>(vt, &odd[wave], lane);
+    else vs.template store<false>(vt, nullptr, lane);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const int next = k0 + kWaves * kFewTile;
-    if (next < end) {
-      ks.fetch(k, a.kl, next, a.lk, a.d, lane);
-      vs.fetch(v, a.vl, next, a.lk, a.d, lane);
-    }
+    if (next < end) fetch(next);
     f16v s[1] = {f16v(0.f)};
 #pragma unroll
-    for (int n = 0; n < NK; ++n) s[0] = mma<T>(frag_along(kt, KS, 0, n, lane), qf[n], s[0]);
-    const float c = score_blocks<T, 1>(a, s, k0, pos, slope, partial, mask, docs ? ids + k0 : nullptr, lane);
+    for (int n = 0; n < NK; ++n) s[0] = mma<T>(Lds::along(kt, 0, n, lane), qf[n], s[0]);
+    const float c = score_blocks<T, 1>(scoring, s, k0, pos, partial, mask, docs ? ids + k0 : nullptr, lane);
     float alpha;
-    if (softmax_blocks<T, 1>(s, c, m, l, alpha)) {
+    Frag<T> p[1][2];
+    if (softmax_blocks<T, 1>(s, p, c, m, l, alpha)) {
 #pragma unroll
       for (int n = 0; n < ND; ++n) o[n] *= alpha;
     }
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const Frag<T> p = result_frag<T>(s[0], w);
+    for (int w = 0; w < 2; ++w)
 #pragma unroll
-      for (int n = 0; n < ND; ++n) o[n] = mma<T>(frag_down(vt, VS, 16 * w, n, lane), p, o[n]);
-    }
+      for (int n = 0; n < ND; ++n) o[n] = mma<T>(Lds::down(vt, 16 * w, n, lane), p[0][w], o[n]);
     if (partial) {
       const unsigned set = odd[wave];
       if (set) add_odd_values<T, ND>(a, o, v, k0, set, 0u, mask, docs ? ids + k0 : nullptr, lane);
@@ -456,6 +484,7 @@ struct DocArgs {
   int* ids[2];
   DocTile* tiles[2];
   int4* hull[2];
+  int* mixed[2];
   int rows[2], stride[2], count[2], grains[2];
 };
 
@@ -477,47 +506,73 @@ __global__ __launch_bounds__(kTile) void document_tiles_kernel(DocArgs a) {
   if (lane == 0) a.tiles[side][(int64_t)b * a.count[side] + tile] = DocTile{least, most, least_id, 0};
 }
 
+// Tiles of a side [x, y) that may hold ids least .. most, and the first run [z, w) of tiles that hold only the one
+// id, for least = most >= 0.
+__device__ __forceinline__ int4 document_run(const DocArgs& a, int side, int b, int lane, int least, int most) {
+  const DocTile* tiles = a.tiles[side] + (int64_t)b * a.count[side];
+  const int count = a.count[side];
+  const bool one = least == most;
+  int4 run = {INT_MAX, 0, INT_MAX, 0};
+  if (most < 0 || least > most) return run;
+  for (int o = lane; o < count; o += kTile) {
+    const DocTile tile = tiles[o];
+    if (least <= tile.most && tile.least_id <= most) {
+      run.x = min(run.x, o);
+      run.y = max(run.y, o + 1);
+    }
+    if (one && tile.least == least && tile.most == least) run.z = min(run.z, o);
+  }
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) {
+    run.x = min(run.x, __shfl_xor(run.x, m));
+    run.y = max(run.y, __shfl_xor(run.y, m));
+    run.z = min(run.z, __shfl_xor(run.z, m));
+  }
+  int end = run.z == INT_MAX ? 0 : count;
+  for (int o = lane; o < end; o += kTile)
+    if (o > run.z && (tiles[o].least != least || tiles[o].most != least)) end = min(end, o);
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) end = min(end, __shfl_xor(end, m));
+  run.w = end;
+  return run;
+}
+
 // One wave per kGrain rows: blockIdx = (grain, item, side).
 __global__ __launch_bounds__(kTile) void document_hulls_kernel(DocArgs a) {
   const int side = blockIdx.z, b = blockIdx.y, grain = blockIdx.x, lane = threadIdx.x;
   if (grain >= a.grains[side]) return;
+  if (grain % 4 == 0) {
+    const int* ids = a.ids[side] + (int64_t)b * a.stride[side];
+    bool other = false;
+#pragma unroll
+    for (int r = lane; r < kBlockRows; r += kTile) {
+      const int row = grain * kGrain + r;
+      other |= row < a.rows[side] && ids[row] != ids[grain * kGrain];
+    }
+    other = __any(other);
+    if (lane == 0) a.mixed[side][(int64_t)b * ((a.grains[side] + 3) / 4) + grain / 4] = other;
+  }
   const int i = grain * kGrain + lane % kGrain;
   const int id = i < a.rows[side] ? a.ids[side][(int64_t)b * a.stride[side] + i] : -1;
-  DocTile own;
-  own.least = i < a.rows[side] ? id : INT_MAX;
-  own.most = id;
-  own.least_id = id >= 0 ? id : INT_MAX;
+  // The first row's document, and the range of the other rows' ids, padding aside: which tiles may hold them, and
+  // the first run of tiles that hold nothing else.
+  const int first = __shfl(id, 0);
+  int least = id >= 0 && id != first ? id : INT_MAX, most = id != first ? id : -1;
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) {
-    own.least = min(own.least, __shfl_xor(own.least, m));
-    own.most = max(own.most, __shfl_xor(own.most, m));
-    own.least_id = min(own.least_id, __shfl_xor(own.least_id, m));
+    least = min(least, __shfl_xor(least, m));
+    most = max(most, __shfl_xor(most, m));
   }
-  const DocTile* others = a.tiles[1 - side] + (int64_t)b * a.count[1 - side];
-  const int count = a.count[1 - side];
-  const bool one = own.least == own.most && own.least >= 0;
-  int lo = INT_MAX, hi = 0, whole = INT_MAX;
-  for (int o = lane; o < count; o += kTile) {
-    const DocTile other = others[o];
-    if (own.least_id <= other.most && other.least_id <= own.most) {
-      lo = min(lo, o);
-      hi = max(hi, o + 1);
-    }
-    if (one && other.least == own.least && other.most == own.least) whole = min(whole, o);
+  const bool padded = __any(i < a.rows[side] && id < 0 && first >= 0);
+  const int4 own = document_run(a, 1 - side, b, lane, first, first);
+  const int4 rest = document_run(a, 1 - side, b, lane, least, most);
+  if (lane == 0) {
+    int4* hull = a.hull[side] + 3 * ((int64_t)b * a.grains[side] + grain);
+    hull[0] = own;
+    hull[1] = rest;
+    // padding among the rows is as good as another document that no tile holds
+    hull[2] = least <= most ? int4{padded ? -1 : least, most, 0, 0} : padded ? int4{-1, -1, 0, 0} : int4{1, 0, 0, 0};
   }
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) {
-    lo = min(lo, __shfl_xor(lo, m));
-    hi = max(hi, __shfl_xor(hi, m));
-    whole = min(whole, __shfl_xor(whole, m));
-  }
-  // the first run of tiles that hold nothing but this document
-  int end = whole == INT_MAX ? 0 : count;
-  for (int o = lane; o < end; o += kTile)
-    if (o > whole && (others[o].least != own.least || others[o].most != own.least)) end = min(end, o);
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) end = min(end, __shfl_xor(end, m));
-  if (lane == 0) a.hull[side][(int64_t)b * a.grains[side] + grain] = int4{lo, hi, whole, end};
 }
 
 // --------------------------------------------------------------------------
@@ -542,7 +597,7 @@ int launch(const Args& a, bool few, hipStream_t st) {
   if (few)
     hipLaunchKernelGGL((attention_few_kernel<T, D>), dim3(a.n * a.hk, a.splits), dim3(kThreads), 0, st, a);
   else
-    hipLaunchKernelGGL((attention_kernel<T, D>), dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kRows), a.splits),
+    hipLaunchKernelGGL((attention_kernel<T, D>), dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kRows) * (a.qdoc.ids ? 2u : 1u), a.splits),
                        dim3(kThreads), 0, st, a);
   const int rc = check_launch("masked_attention");
   if (rc || a.splits == 1) return rc;
@@ -556,11 +611,12 @@ int launch(const Args& a, bool few, hipStream_t st) {
 
 int padded(int head_dim) { return head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : 128; }
 
-static Side side_of(int rows, const int* ids, const void* tiles, const void* hull) {
+static Side side_of(int rows, const int* ids, const void* tiles, const void* hull, const int* mixed) {
   Side s = {};
   s.ids = ids;
   s.tiles = static_cast<const DocTile*>(tiles);
   s.hull = static_cast<const int4*>(hull);
+  s.mixed = mixed;
   s.count = (int)ceil_div(rows, kTile);
   s.stride = s.count * kTile;
   s.grains = (int)ceil_div(rows, kGrain);
@@ -580,10 +636,12 @@ static void plan_parts(int32_t n, int32_t lq, int32_t lk, char* base, Side& q, S
   const int* ki = (const int*)take(n * nk * kTile * 4);
   const void* qt = take(n * nq * (int64_t)sizeof(DocTile));
   const void* kt = take(n * nk * (int64_t)sizeof(DocTile));
-  const void* qh = take(n * ceil_div(lq, kGrain) * 16);
-  const void* kh = take(n * ceil_div(lk, kGrain) * 16);
-  q = side_of(lq, qi, qt, qh);
-  k = side_of(lk, ki, kt, kh);
+  const void* qh = take(n * ceil_div(lq, kGrain) * 48);
+  const void* kh = take(n * ceil_div(lk, kGrain) * 48);
+  const int* qm = (const int*)take(n * ceil_div(lq, kBlockRows) * 4);
+  const int* km = (const int*)take(n * ceil_div(lk, kBlockRows) * 4);
+  q = side_of(lq, qi, qt, qh, qm);
+  k = side_of(lk, ki, kt, kh, km);
   if (bytes) *bytes = at;
 }
 
@@ -600,14 +658,22 @@ int check_desc(const ctmr_masked_attention_desc* d) {
   if (d->lq > (1 << 28) || d->lk > (1 << 28) ||
       (int64_t)d->n * d->q_heads * ceil_div(std::max(d->lq, d->lk), kTile) > (1ll << 30))
     return fail(CTMR_E_UNSUPPORTED, "too many rows");
+  int rc = check_strides(d, d->q_strides, d->lq);
+  if (!rc) rc = check_strides(d, d->k_strides, d->lk);
+  return rc ? rc : check_strides(d, d->v_strides, d->lk);
+}
+
+// Rows may not overlap: the kernels take what lies past the last one as out of range.
+int check_strides(const ctmr_masked_attention_desc* d, const int64_t* s, int rows) {
   const int bytes = elem_bytes(d->elem);
-  for (const int64_t* s : {d->q_strides, d->k_strides, d->v_strides}) {
-    if (s[0] < 0 || s[1] < 0 || s[2] < 0 || (s[0] | s[1] | s[2]) * bytes % 16 != 0)
-      return fail(CTMR_E_INVALID, "strides must be multiples of 16 bytes and not negative");
-    if (s[2] * bytes > (1ll << 31) / kTile - 4096) return fail(CTMR_E_UNSUPPORTED, "row stride too large");
-  }
+  if (s[0] < 0 || s[1] < 0 || s[2] < 0 || (s[0] | s[1] | s[2]) * bytes % 16 != 0)
+    return fail(CTMR_E_INVALID, "strides must be multiples of 16 bytes and not negative");
+  if (rows > 1 && s[2] < d->head_dim) return fail(CTMR_E_INVALID, "rows overlap");
+  if (s[2] * bytes > (1ll << 30) / kTile - 4096) return fail(CTMR_E_UNSUPPORTED, "row stride too large");
   return CTMR_OK;
 }
+
+int64_t row_stride(const int64_t* s, int rows, int head_dim) { return rows > 1 ? s[2] : head_dim; }
 
 Args make_args(const ctmr_masked_attention_desc* d, const void* q, const void* k, const void* v, const float* slopes,
                const int32_t* prefixes, const void* plan) {
@@ -615,9 +681,9 @@ Args make_args(const ctmr_masked_attention_desc* d, const void* q, const void* k
   a.q = q, a.k = k, a.v = v, a.slopes = slopes, a.prefixes = prefixes;
   a.n = d->n, a.lq = d->lq, a.lk = d->lk, a.hq = d->q_heads, a.hk = d->k_heads, a.group = d->q_heads / d->k_heads;
   a.d = d->head_dim, a.prefixed = d->prefixed != 0, a.prefix = d->prefix, a.scale = d->scale, a.cap = d->softcap;
-  a.qb = d->q_strides[0], a.qh = d->q_strides[1], a.ql = d->q_strides[2];
-  a.kb = d->k_strides[0], a.kh = d->k_strides[1], a.kl = d->k_strides[2];
-  a.vb = d->v_strides[0], a.vh = d->v_strides[1], a.vl = d->v_strides[2];
+  a.qb = d->q_strides[0], a.qh = d->q_strides[1], a.ql = row_stride(d->q_strides, d->lq, d->head_dim);
+  a.kb = d->k_strides[0], a.kh = d->k_strides[1], a.kl = row_stride(d->k_strides, d->lk, d->head_dim);
+  a.vb = d->v_strides[0], a.vh = d->v_strides[1], a.vl = row_stride(d->v_strides, d->lk, d->head_dim);
   a.splits = 1;
   if (plan) plan_parts(d->n, d->lq, d->lk, (char*)plan, a.qdoc, a.kdoc, nullptr);
   return a;
@@ -657,6 +723,7 @@ int ctmr_documents(int32_t n, int32_t lq, int32_t lk, const int32_t* query_ids, 
     a.ids[s] = const_cast<int*>(sides[s]->ids);
     a.tiles[s] = const_cast<DocTile*>(sides[s]->tiles);
     a.hull[s] = const_cast<int4*>(sides[s]->hull);
+    a.mixed[s] = const_cast<int*>(sides[s]->mixed);
     a.rows[s] = rows[s], a.stride[s] = sides[s]->stride, a.count[s] = sides[s]->count;
     a.grains[s] = sides[s]->grains;
   }

@@ -57,49 +57,67 @@ __device__ __forceinline__ Frag<T> result_frag(const f16v& s, int step) {
   return __builtin_convertvector(v, Frag<T>);
 }
 
-// Values and bytes between rows of a tile in LDS.  ALONG: read along its rows only,
-// 16 bytes a lane from 32 rows (16 bytes of padding spread them over the banks);
-// DOWN: down its columns only, four rows of 64 bytes at a time (rows 64 bytes
-// apart modulo 256); BOTH: 32 bytes of padding, a conflict of two either way.
-enum Reads { ALONG, DOWN, BOTH };
+// A value that is the same for the wave, in a scalar register of its own: the kernel's arguments come in blocks of
+// up to 16 registers, and a loop that needs one value of each spills them.
+template <typename V>
+__device__ __forceinline__ V apart(V v) {
+  asm("" : "+s"(v));
+  return v;
+}
+
+// A tile of D-value rows in LDS, in pieces of 16 bytes.  The pieces of a row are
+// permuted by the row (an exclusive or of the low bits), so that both kinds of reads
+// meet 32 banks without conflicts and without padding: along, eight lanes read one
+// piece of eight rows; down, sixteen lanes read two neighbouring pieces of four rows.
+// (Rows padded by 16 or 32 bytes instead cost a conflict of two in one of them:
+// 11 % of the cycles of the key gradients' kernel.)
 template <typename T, int D>
-constexpr int tile_stride(Reads r) {
-  if (sizeof(T) == 4) return D + 4;
-  if (r == ALONG) return D + 8;
-  if (r == BOTH) return D + 16;
-  return D == 32 ? 32 : D + 32;
-}
+struct Tile {
+  static constexpr int kRow = D * (int)sizeof(T);  // bytes
+  static constexpr int kPieces = kRow / 16;        // 4, 8, 16 or 32
 
-// A operand of 32 rows from `row`, contraction over the values 16 step .. + 15 of a row.
-template <typename T>
-__device__ __forceinline__ Frag<T> frag_along(const T* tile, int stride, int row, int step, int lane) {
-  const T* p = tile + (row + (lane & 31)) * stride + 16 * step + 8 * (lane >> 5);
-  return *reinterpret_cast<const Frag<T>*>(p);
-}
-
-// A operand whose rows are the values 32 block .. + 31, contraction over the tile's rows `row` .. + 15 in the
-// results' order.
-template <typename T>
-__device__ __forceinline__ Frag<T> frag_down(const T* tile, int stride, int row, int block, int lane) {
-  const int half = lane >> 5;
-  if constexpr (sizeof(T) == 4) {
-    const T* p = tile + (row + 4 * half) * stride + 32 * block + (lane & 31);
-    Frag<T> f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = p[(e + (e & 4)) * stride];
-    return f;
-  } else {
-    // A transposing read: of 16 lanes, lane m gives the address of four values of row m / 4 and gets column m
-    // of the four rows.
-    typedef Vec<short, 4> s4;
-    typedef __attribute__((address_space(3))) s4 lds_s4;
-    const T* p = tile + (row + 4 * half + ((lane & 15) >> 2)) * stride + 32 * block + 16 * ((lane >> 4) & 1) +
-                 4 * (lane & 3);
-    const s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p);
-    const s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 8 * stride));
-    return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
+  static __device__ __forceinline__ int mix(int row) {
+    return kPieces == 4 ? ((row & 2) | ((row >> 2) & 1)) : (((row & 3) << 1) | ((row >> 2) & 1));
   }
-}
+  static __device__ __forceinline__ int at(int row, int piece) { return row * kRow + ((piece ^ mix(row)) << 4); }
+
+  // A operand of the 32 rows from `row` (a multiple of 8), contraction over the values 16 step .. + 15 of a row.
+  static __device__ __forceinline__ Frag<T> along(const char* tile, int row, int step, int lane) {
+    const char* p = tile + row * kRow;
+    const int r = lane & 31, half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<const Frag<T>*>(p + at(r, 2 * step + half));
+    } else {
+      const f4 u = *reinterpret_cast<const f4*>(p + at(r, 4 * step + 2 * half));
+      const f4 w = *reinterpret_cast<const f4*>(p + at(r, 4 * step + 2 * half + 1));
+      return __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+
+  // A operand whose rows are the values 32 block .. + 31, contraction over the tile's rows `row` .. + 15 (a
+  // multiple of 8) in the results' order.
+  static __device__ __forceinline__ Frag<T> down(const char* tile, int row, int block, int lane) {
+    const char* p = tile + row * kRow;
+    const int half = lane >> 5;
+    if constexpr (sizeof(T) == 4) {
+      Frag<T> f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        f[e] = *reinterpret_cast<const T*>(p + at(4 * half + e + (e & 4), 8 * block + ((lane & 31) >> 2)) + 4 * (lane & 3));
+      return f;
+    } else {
+      // A transposing read: of 16 lanes, lane m gives the address of four values of row m / 4 and gets column m
+      // of the four rows.
+      typedef Vec<short, 4> s4;
+      typedef __attribute__((address_space(3))) s4 lds_s4;
+      const char* from = p + at(4 * half + ((lane & 15) >> 2), 4 * block + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) +
+                         8 * (lane & 1);
+      const s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)from);
+      const s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(from + 8 * kRow));
+      return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
 
 // B operand of a wave's 32 rows straight from memory: this lane's row, zeros where `valid` is false or past d values.
 template <typename T>
@@ -113,35 +131,56 @@ __device__ __forceinline__ Frag<T> frag_global(const T* row, int step, int d, in
 // --------------------------------------------------------------------------
 // streaming a tile: memory -> registers -> LDS, 16 bytes a thread and piece
 // --------------------------------------------------------------------------
+// The rows of one head from some row on, walked ROWS at a time; the same for all threads.  The host keeps kTile *
+// stride bytes below 2^30.
+template <typename T, int ROWS>
+struct Rows {
+  const char* base;
+  int64_t step;     // bytes of ROWS rows
+  int left;       // rows
+  int row, last;  // bytes of a row's stride and of its values
+
+  __device__ __forceinline__ void begin(const T* rows, int64_t stride, int first, int count, int d) {
+    row = apart((int)(stride * (int)sizeof(T)));
+    last = apart(d * (int)sizeof(T));
+    step = (int64_t)ROWS * row;
+    base = reinterpret_cast<const char*>(rows + (int64_t)first * stride);
+    left = count - first;
+  }
+  __device__ __forceinline__ void next() {
+    base += step;
+    left -= ROWS;
+  }
+  // Loads past the last row give zeros.
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer() const {
+    const int bytes = max((min(left, ROWS) - 1) * row + last, 0);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes, 0x00020000);
+  }
+};
+
 template <typename T, int D, int ROWS, int THREADS>
 struct Stream {
-  static constexpr int kPer = 16 / (int)sizeof(T);            // values of a piece
-  static constexpr int kPieces = ROWS * D / kPer / THREADS;   // of a thread
-  static_assert(ROWS * D % (kPer * THREADS) == 0, "whole pieces");
+  typedef Tile<T, D> Lds;
+  static constexpr int kPieces = ROWS * Lds::kPieces / THREADS;  // of a thread
+  static_assert(ROWS * Lds::kPieces % THREADS == 0, "whole pieces");
   u4 piece[kPieces];
 
-  static __device__ __forceinline__ int row_of(int i, int t) { return (i * THREADS + t) / (D / kPer); }
-  static __device__ __forceinline__ int col_of(int i, int t) { return (i * THREADS + t) % (D / kPer) * kPer; }
+  static __device__ __forceinline__ int row_of(int i, int t) { return (i * THREADS + t) / Lds::kPieces; }
+  static __device__ __forceinline__ int piece_of(int t) { return t % Lds::kPieces; }  // THREADS is a multiple
 
-  // Rows first .. first + ROWS - 1 of `rows` (strides in values, d values each); zeros past either end.  The
-  // buffer's range ends with the last row; a column past d has an offset past every range.  The host keeps
-  // kTile * stride bytes below 2^31.
-  __device__ __forceinline__ void fetch(const T* base, int64_t stride, int first, int rows, int d, int t) {
-    const int left = min(rows - first, ROWS);
-    const int bytes = left > 0 ? (int)(((int64_t)(left - 1) * stride + d) * (int)sizeof(T)) : 0;
-    const __amdgpu_buffer_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)first * stride), (short)0, bytes, 0x00020000);
+  // Columns past the head's values have an offset past every range, 2^30 + 2^29 and more.
+  __device__ __forceinline__ void fetch(const Rows<T, ROWS>& rows, int t) {
+    const __amdgpu_buffer_rsrc_t r = rows.buffer();
+    unsigned off = row_of(0, t) * rows.row + piece_of(t) * 16;
+    off = piece_of(t) * 16 < rows.last ? off : 0x60000000u;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int row = row_of(i, t), col = col_of(i, t);
-      const int off = col < d ? (int)((row * stride + col) * (int)sizeof(T)) : 0x7ffffff0;
-      piece[i] = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
-    }
+    for (int i = 0; i < kPieces; ++i)
+      piece[i] = __builtin_amdgcn_raw_buffer_load_b128(r, (int)(off + i * (THREADS / Lds::kPieces) * rows.row), 0, 0);
   }
 
   // CLEAN: values that are not finite become zeros and their rows' bits are set in odd[ROWS / 32].
   template <bool CLEAN>
-  __device__ __forceinline__ void store(T* tile, int stride, unsigned* odd, int t) {
+  __device__ __forceinline__ void store(char* tile, unsigned* odd, int t) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int row = row_of(i, t);
@@ -162,7 +201,7 @@ struct Stream {
         }
         if (found) atomicOr(&odd[row >> 5], 1u << (row & 31));
       }
-      *reinterpret_cast<u4*>(tile + row * stride + col_of(i, t)) = piece[i];
+      *reinterpret_cast<u4*>(tile + Lds::at(row, piece_of(t))) = piece[i];
     }
   }
 };
@@ -174,11 +213,16 @@ struct DocTile {     // of kTile rows: ids of all its rows, and of those that ar
   int least, most, least_id, unused;
 };
 constexpr int kGrain = 32;  // rows of a hull: a wave's
+constexpr int kBlockRows = 128;  // rows of a workgroup of four waves
 
 struct Side {        // documents of the query or key rows
   const int* ids;    // (n, rows rounded up to kTile), -1 past the end
   const DocTile* tiles;
-  const int4* hull;  // of kGrain rows, tiles of the other side: [x, y) may hold a match, all pairs with [z, w) are one
+  // Three for kGrain rows: tiles of the other side, [x, y) that may hold a match of the first row's document and
+  // [z, w) that hold nothing else; the same of the other rows' documents ([z, w) empty if they are of several);
+  // the least and the largest id of these, x > y if there are none.
+  const int4* hull;
+  const int* mixed;  // whether kBlockRows rows are of more than one document
   int stride, count, grains;  // ids, tiles and hulls of a batch item
 };
 
@@ -201,6 +245,15 @@ struct Args {
   float scale, cap;
 };
 
+// What scores of one head are made of, apart.
+struct Scoring {
+  float scale, cap, slope;
+  bool sloped, prefixed;
+};
+__device__ __forceinline__ Scoring scoring_of(const Args& a, int h) {
+  return {apart(a.scale), apart(a.cap), a.slopes ? a.slopes[h] : 0.f, a.slopes != nullptr, a.prefixed != 0};
+}
+
 __device__ __forceinline__ int prefix_of(const Args& a, int b) { return a.prefixes ? a.prefixes[b] : a.prefix; }
 
 // First key that row i can no longer see, documents aside.
@@ -208,19 +261,19 @@ __device__ __forceinline__ int limit_of(const Args& a, int i, int prefix) {
   return a.prefixed ? min(a.lk, max(i + a.lk - a.lq + 1, prefix)) : a.lk;
 }
 
-// What a row compares key ids with: its own id, -2 where it is padding.
-__device__ __forceinline__ int row_id(const Args& a, int b, int i) {
-  const int id = a.qdoc.ids[(int64_t)b * a.qdoc.stride + i];
-  return id < 0 ? -2 : id;
+// Document of a query row; negative is padding, which compares as -2 with ids that are -1 at least.
+__device__ __forceinline__ int id_of(const Args& a, int b, int i) {
+  return a.qdoc.ids[(int64_t)b * a.qdoc.stride + i];
 }
 
-// tanh to about 2e-7 absolute: enough for 16-bit operands, whose scores it moves by under 2^-17 at a cap of 50.
+// tanh(x / in_scale) of x, in_scale given as 1 / in_scale; of 16-bit operands to about 2e-7 absolute, which moves
+// their scores by under 2^-17 at a cap of 50.
 template <typename T>
-__device__ __forceinline__ float tanh_of(float x) {
+__device__ __forceinline__ float tanh_of(float x, float per) {
   if constexpr (sizeof(T) == 4) {
-    return tanhf(x);
+    return tanhf(x * per);
   } else {
-    const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * x);
+    const float e = __builtin_amdgcn_exp2f(x * (per * (2.0f * kLog2e)));
     return fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
   }
 }
@@ -234,25 +287,55 @@ __device__ __forceinline__ float half_sum(float v) {
   return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
-// Item and tile of a workgroup: blocks go round the eight XCDs, each of which has
-// its own L2, so all tiles of a (batch item, head) that stream the same rows go to
-// one of them where the items divide by eight.
-__device__ __forceinline__ void place(int id, int items, int tiles, int& item, int& tile) {
-  if (items % 8 == 0) {
-    const int rest = id >> 3;
-    item = rest / tiles * 8 + (id & 7);
-    tile = rest % tiles;
-  } else {
-    item = id / tiles;
-    tile = id % tiles;
+// Item, tile and part of a workgroup: blocks go round the eight XCDs, each of which
+// has its own L2, so all tiles of a (batch item, head) that stream the same rows go
+// to one of them where the items divide by eight.
+//
+// With documents two workgroups share a block of rows (parts 2): part 0 takes the
+// rows of the first row's document, part 1 the others.  A block that two long
+// documents meet in would else walk both, twice as long as any other: of 6144
+// tokens in documents of 2048, 1573, 2048 and 400, 16 heads of 32, that one block a
+// head made 145 us of what is 55 us with the borders on block borders.
+__device__ __forceinline__ void place(int id, int items, int tiles, int parts, int& item, int& tile, int& part) {
+  const bool spread = items % 8 == 0;
+  int rest = spread ? id >> 3 : id;
+  part = 0;
+  if (parts == 2) {  // the second parts first: most have no rows and leave at once
+    const int each = spread ? items / 8 * tiles : items * tiles;
+    part = rest < each ? 1 : 0;
+    rest -= part ? 0 : each;
   }
+  item = spread ? rest / tiles * 8 + (id & 7) : rest / tiles;
+  tile = rest % tiles;
 }
 
-// Tiles that kGrain rows of one side meet: [x, y) may hold visible pairs, in [z, w) every pair is visible.
-__device__ __forceinline__ int4 meet(const Side& s, int b, int grain, int4 r) {
+// The rows of a workgroup's part: those whose id is (part 0) or is not (part 1) `first_id`.
+struct Part {
+  int part, first_id;
+  __device__ __forceinline__ bool has(int id) const { return (id == first_id) == (part == 0); }
+};
+
+// Whether a block of rows has a second part.
+__device__ __forceinline__ bool is_mixed(const Side& s, int b, int block) {
+  return s.mixed[(int64_t)b * ((s.grains + 3) / 4) + block] != 0;
+}
+
+// Tiles that kGrain rows of one side meet: [x, y) may hold visible pairs, in [z, w) every pair is visible.  With
+// documents and a part only the part's rows count.
+__device__ __forceinline__ int4 meet(const Side& s, int b, int grain, int4 r, const Part* part) {
   if (s.ids) {
-    const int4 hull = s.hull[(int64_t)b * s.grains + grain];
-    r = {max(r.x, hull.x), min(r.y, hull.y), max(r.z, hull.z), min(r.w, hull.w)};
+    const int4* hull = s.hull + 3 * ((int64_t)b * s.grains + grain);
+    const int4 ids = hull[2];
+    const bool first = !part || part->has(s.ids[(int64_t)b * s.stride + grain * kGrain]);
+    const bool others = ids.x <= ids.y &&
+                        (!part || part->part == 1 || (ids.x <= part->first_id && part->first_id <= ids.y));
+    int4 u = {0x7fffffff, 0, 0x7fffffff, 0};
+    if (first) u = hull[0];
+    if (others) {
+      const int4 o = hull[1];
+      u = {min(u.x, o.x), max(u.y, o.y), first ? 0x7fffffff : o.z, first ? 0 : o.w};
+    }
+    r = {max(r.x, u.x), min(r.y, u.y), max(r.z, u.z), min(r.w, u.w)};
   }
   r.y = max(r.y, 0);
   r.x = min(r.x, r.y);
@@ -260,21 +343,21 @@ __device__ __forceinline__ int4 meet(const Side& s, int b, int grain, int4 r) {
 }
 
 // Key tiles of the rows i .. i + kGrain - 1 of item b, those past lq aside.
-__device__ __forceinline__ int4 key_tiles(const Args& a, int b, int i, int prefix) {
+__device__ __forceinline__ int4 key_tiles(const Args& a, int b, int i, int prefix, const Part* part) {
   const int last = limit_of(a, min(i + kGrain, a.lq) - 1, prefix), first = limit_of(a, i, prefix);
-  return meet(a.qdoc, b, i / kGrain, int4{0, (max(last, 0) + kTile - 1) / kTile, 0, max(first, 0) / kTile});
+  return meet(a.qdoc, b, i / kGrain, int4{0, (max(last, 0) + kTile - 1) / kTile, 0, max(first, 0) / kTile}, part);
 }
 
 // Query tiles of the keys j .. j + kGrain - 1: from the first row whose limit passes j; every key is seen from the
 // row whose limit passes the last one.
-__device__ __forceinline__ int4 query_tiles(const Args& a, int b, int j, int prefix) {
+__device__ __forceinline__ int4 query_tiles(const Args& a, int b, int j, int prefix, const Part* part) {
   const int end = min(j + kGrain, a.lk) - 1, off = a.lk - a.lq, tiles = (a.lq + kTile - 1) / kTile;
   const int first = a.prefixed && prefix <= j ? max(0, j - off) / kTile : 0;
   const int whole = a.prefixed && prefix <= end ? (max(0, end - off) + kTile - 1) / kTile : 0;
-  return meet(a.kdoc, b, j / kGrain, int4{first, tiles, whole, tiles});
+  return meet(a.kdoc, b, j / kGrain, int4{first, tiles, whole, tiles}, part);
 }
 
-// A workgroup's tiles from its waves' (those with rows): any may hold a pair, all are whole.
+// A workgroup's tiles from its waves' (those that meet any): any wave may hold a pair, all waves' are whole.
 struct Meeting {
   int4 mine, all;
   __device__ __forceinline__ bool partial(int tile) const { return tile < all.z || tile >= all.w; }
@@ -294,9 +377,9 @@ __device__ __forceinline__ Meeting meeting(int wave, int row0, int rows, F tiles
     if (r.x < r.y) {
       m.all.x = min(m.all.x, r.x);
       m.all.y = max(m.all.y, r.y);
+      m.all.z = max(m.all.z, r.z);
+      m.all.w = min(m.all.w, r.w);
     }
-    m.all.z = max(m.all.z, r.z);
-    m.all.w = min(m.all.w, r.w);
     if (w == wave) m.mine = r;
   }
   m.all.x = min(m.all.x, m.all.y);
@@ -304,6 +387,8 @@ __device__ __forceinline__ Meeting meeting(int wave, int row0, int rows, F tiles
 }
 
 int check_desc(const ctmr_masked_attention_desc* d);
+int check_strides(const ctmr_masked_attention_desc* d, const int64_t* strides, int rows);
+int64_t row_stride(const int64_t* strides, int rows, int head_dim);  // of one row: any that does not overlap
 int padded(int head_dim);
 Args make_args(const ctmr_masked_attention_desc* d, const void* q, const void* k, const void* v, const float* slopes,
                const int32_t* prefixes, const void* plan);

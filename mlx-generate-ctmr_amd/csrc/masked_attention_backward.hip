@@ -29,25 +29,26 @@ namespace attn {
 namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
-constexpr int kOwn = 32 * kWaves;  // rows that a workgroup keeps in registers
+constexpr int kOwn = kBlockRows;  // rows that a workgroup keeps in registers
+static_assert(kOwn == 32 * kWaves && kOwn == 4 * kGrain, "32 rows a wave");
 
 // Products of a 32 x 32 block -> log2 scores in units of 1 / c (c returned) and, with a cap, 1 - t^2 in `slope_of`.
 // Row r of a lane is `at` + 8 (r / 4) + r % 4; `x` is where the distance to it is zero.
 template <typename T>
-__device__ __forceinline__ float scores(const Args& a, f16v& s, f16v& slope_of, int at, int x, float slope) {
+__device__ __forceinline__ float scores(const Scoring& a, f16v& s, f16v& slope_of, int at, int x) {
   float c = a.scale * kLog2e;
   if (a.cap > 0.f) {
     const float in = a.scale / a.cap, out = a.cap * kLog2e;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float t = tanh_of<T>(s[r] * in);
+      const float t = tanh_of<T>(s[r], in);
       s[r] = out * t;
       slope_of[r] = fmaf(-t, t, 1.0f);
     }
     c = 1.0f;
   }
-  if (a.slopes) {
-    const float per = slope * kLog2e;
+  if (a.sloped) {
+    const float per = a.slope * kLog2e;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = fmaf(-per, fabsf((float)(at + 8 * (r >> 2) + (r & 3) - x)), s[r] * c);
     c = 1.0f;
@@ -73,29 +74,33 @@ __device__ __forceinline__ void write_gradient(T* out, const f16v (&g)[ND], floa
 
 // dq and delta: 128 query rows of a head, key tiles streaming.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dq_kernel(Args a) {
+__global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attention_dq_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
-  constexpr int KS = tile_stride<T, D>(BOTH), VS = tile_stride<T, D>(ALONG);
-  __shared__ __attribute__((aligned(16))) T kt[kTile * KS];
-  __shared__ __attribute__((aligned(16))) T vt[kTile * VS];
+  typedef Tile<T, D> Lds;
+  __shared__ __attribute__((aligned(16))) char kt[kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char vt[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) int key_ids[kTile];
   __shared__ unsigned odd[2];
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int blocks = (a.lq + kOwn - 1) / kOwn;
+  const bool docs = a.qdoc.ids != nullptr;
   int item, block;
-  place(blockIdx.x, a.n * a.hq, blocks, item, block);
+  Part part;
+  place(blockIdx.x, a.n * a.hq, blocks, docs ? 2 : 1, item, block, part.part);
   if (a.prefixed) block = blocks - 1 - block;
   const int b = item / a.hq, h = item % a.hq;
+  if (part.part == 1 && !is_mixed(a.qdoc, b, block)) return;
   const int i0 = block * kOwn;
   const int i = i0 + 32 * wave + (lane & 31);
-  const bool real = i < a.lq;
   const int prefix = a.prefixed ? prefix_of(a, b) : 0;
-  const bool docs = a.qdoc.ids != nullptr;
   const int* ids = docs ? a.kdoc.ids + (int64_t)b * a.kdoc.stride : nullptr;
-  const int limit = real ? limit_of(a, i, prefix) : 0, id = docs && real ? row_id(a, b, i) : -2;
+  part.first_id = docs ? id_of(a, b, i0) : 0;
+  const int own = docs && i < a.lq ? id_of(a, b, i) : 0;
+  const bool real = i < a.lq && (!docs || part.has(own));  // rows of the other part are left to it
+  const int limit = real ? limit_of(a, i, prefix) : 0, id = own < 0 || !real ? -2 : own;
   const int pos = i + a.lk - a.lq;
-  const float slope = a.slopes ? a.slopes[h] : 0.f;
+  const Scoring scoring = scoring_of(a, h);
   const int64_t stat = ((int64_t)b * a.hq + h) * a.lq + i;
   const T* q = static_cast<const T*>(a.q) + b * a.qb + h * a.qh + (int64_t)i * a.ql;
   const T* g = static_cast<const T*>(a.dout) + b * a.gb + h * a.gh + (int64_t)i * a.gl;
@@ -129,13 +134,18 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dq_kerne
 #pragma unroll
   for (int n = 0; n < ND; ++n) dq[n] = f16v(0.f);
 
-  const Meeting meet = meeting<kWaves>(wave, i0, a.lq, [&](int row) { return key_tiles(a, b, row, prefix); });
+  const Meeting meet = meeting<kWaves>(wave, i0, a.lq, [&](int row) { return key_tiles(a, b, row, prefix, &part); });
   const int first = meet.all.x, last = meet.all.y;
+  Rows<T, kTile> krows, vrows;
+  krows.begin(k, a.kl, first * kTile, a.lk, a.d);
+  vrows.begin(v, a.vl, first * kTile, a.lk, a.d);
   Stream<T, D, kTile, kThreads> ks, vs;
   int other_id = 0;
   auto fetch = [&](int tile) {
-    ks.fetch(k, a.kl, tile * kTile, a.lk, a.d, t);
-    vs.fetch(v, a.vl, tile * kTile, a.lk, a.d, t);
+    ks.fetch(krows, t);
+    vs.fetch(vrows, t);
+    krows.next();
+    vrows.next();
     if (docs && t < kTile) other_id = ids[tile * kTile + t];
   };
   if (first < last) fetch(first);
@@ -147,11 +157,11 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dq_kerne
     if (docs && t < kTile) key_ids[t] = other_id;
     if (partial) {
       __syncthreads();
-      ks.template store<true>(kt, KS, odd, t);
+      ks.template store<true>(kt, odd, t);
     } else {
-      ks.template store<false>(kt, KS, nullptr, t);
+      ks.template store<false>(kt, nullptr, t);
     }
-    vs.template store<false>(vt, VS, nullptr, t);
+    vs.template store<false>(vt, nullptr, t);
     __syncthreads();
     if (tile + 1 < last) fetch(tile + 1);
     if (meet.skips(tile)) continue;
@@ -161,34 +171,38 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dq_kerne
       f16v s = f16v(0.f), ds = f16v(0.f), slope_of = f16v(1.f);
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
-        s = mma<T>(frag_along(kt, KS, 32 * u, n, lane), qf[n], s);
-        ds = mma<T>(frag_along(vt, VS, 32 * u, n, lane), gf[n], ds);
+        s = mma<T>(Lds::along(kt, 32 * u, n, lane), qf[n], s);
+        ds = mma<T>(Lds::along(vt, 32 * u, n, lane), gf[n], ds);
       }
       const int at = k0 + 32 * u + 4 * half;
-      const float c = scores<T>(a, s, slope_of, at, pos, slope);
+      const float c = scores<T>(scoring, s, slope_of, at, pos);
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (ds[r] - delta);
-      if (a.cap > 0.f) ds *= slope_of;
+      if (scoring.cap > 0.f) ds *= slope_of;
       if (masked) {
-        const unsigned set = odd[u];
+        // a visible key whose values were zeroed in LDS because they are not finite: no gradient is
+        const unsigned set = partial ? odd[u] >> (4 * half) : 0u;
+        if (set)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          int4 other = {id, id, id, id};
-          if (docs) other = *reinterpret_cast<const int4*>(key_ids + 32 * u + 4 * half + 8 * w);
-          const int key_id[4] = {other.x, other.y, other.z, other.w};
+          for (int r = 0; r < 16; ++r) ds[r] = (set >> (8 * (r >> 2) + (r & 3))) & 1u ? NAN : ds[r];
+        if (docs)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            // a visible key whose values were zeroed in LDS because they are not finite: no gradient is
-            if ((set >> (8 * w + 4 * half + r)) & 1u) ds[4 * w + r] = NAN;
-            if (at + 8 * w + r >= limit || key_id[r] != id) ds[4 * w + r] = 0.f;
+          for (int w = 0; w < 4; ++w) {
+            const int4 other = *reinterpret_cast<const int4*>(key_ids + 32 * u + 4 * half + 8 * w);
+            ds[4 * w] = other.x != id ? 0.f : ds[4 * w];
+            ds[4 * w + 1] = other.y != id ? 0.f : ds[4 * w + 1];
+            ds[4 * w + 2] = other.z != id ? 0.f : ds[4 * w + 2];
+            ds[4 * w + 3] = other.w != id ? 0.f : ds[4 * w + 3];
           }
-        }
+        if (scoring.prefixed || !docs)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) ds[r] = 8 * (r >> 2) + (r & 3) >= limit - at ? 0.f : ds[r];
       }
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const Frag<T> f = result_frag<T>(ds, w);
 #pragma unroll
-        for (int n = 0; n < ND; ++n) dq[n] = mma<T>(frag_down(kt, KS, 32 * u + 16 * w, n, lane), f, dq[n]);
+        for (int n = 0; n < ND; ++n) dq[n] = mma<T>(Lds::down(kt, 32 * u + 16 * w, n, lane), f, dq[n]);
       }
     }
   }
@@ -198,29 +212,32 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dq_kerne
 
 // dk and dv: 128 keys of a key head, the query tiles of its heads streaming.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dkv_kernel(Args a) {
+__global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attention_dkv_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
-  constexpr int S = tile_stride<T, D>(BOTH);
-  __shared__ __attribute__((aligned(16))) T qt[kTile * S];
-  __shared__ __attribute__((aligned(16))) T gt[kTile * S];
+  typedef Tile<T, D> Lds;
+  __shared__ __attribute__((aligned(16))) char qt[kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char gt[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) float stats[2][kTile];  // lse, delta
   __shared__ __attribute__((aligned(16))) int query_ids[kTile];
   __shared__ unsigned odd[2][2];  // of dout, of q
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int blocks = (a.lk + kOwn - 1) / kOwn;
+  const bool docs = a.qdoc.ids != nullptr;
   int item, block;
-  place(blockIdx.x, a.n * a.hk, blocks, item, block);  // with a prefix the first keys have the most rows
+  Part part;
+  place(blockIdx.x, a.n * a.hk, blocks, docs ? 2 : 1, item, block, part.part);  // a prefix: the first have most rows
   const int b = item / a.hk, hk = item % a.hk;
+  if (part.part == 1 && !is_mixed(a.kdoc, b, block)) return;
   const int j0 = block * kOwn;
   const int j = j0 + 32 * wave + (lane & 31);
-  const bool real = j < a.lk;
   const int prefix = a.prefixed ? prefix_of(a, b) : 0;
-  const bool docs = a.qdoc.ids != nullptr;
   const int* ids = docs ? a.qdoc.ids + (int64_t)b * a.qdoc.stride : nullptr;
-  // padding keys match no row: rows' negative ids are -1
-  const int own_id = docs && real ? a.kdoc.ids[(int64_t)b * a.kdoc.stride + j] : 0;
-  const int id = own_id < 0 ? -2 : own_id;
+  const int* own_ids = docs ? a.kdoc.ids + (int64_t)b * a.kdoc.stride : nullptr;
+  part.first_id = docs ? own_ids[j0] : 0;
+  const int own = docs && j < a.lk ? own_ids[j] : 0;
+  const bool real = j < a.lk && (!docs || part.has(own));  // keys of the other part are left to it
+  const int id = own < 0 || !real ? -2 : own;  // -2 matches no row
   const int off = a.lk - a.lq;
   const T* k = static_cast<const T*>(a.k) + b * a.kb + hk * a.kh + (int64_t)j * a.kl;
   const T* v = static_cast<const T*>(a.v) + b * a.vb + hk * a.vh + (int64_t)j * a.vl;
@@ -235,16 +252,29 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dkv_kern
 #pragma unroll
   for (int n = 0; n < ND; ++n) dk[n] = dv[n] = f16v(0.f);
 
-  const Meeting meet = meeting<kWaves>(wave, j0, a.lk, [&](int row) { return query_tiles(a, b, row, prefix); });
+  const Meeting meet = meeting<kWaves>(wave, j0, a.lk, [&](int row) { return query_tiles(a, b, row, prefix, &part); });
   const int first = meet.all.x, last = meet.all.y;
   const int tiles = last - first, steps = tiles * a.group;
   Stream<T, D, kTile, kThreads> qs, gs;
   float stat = 0.f;
   int other_id = 0;
-  auto fetch = [&](int step) {
-    const int h = hk * a.group + step / tiles, tile = first + step % tiles;
-    qs.fetch(static_cast<const T*>(a.q) + b * a.qb + h * a.qh, a.ql, tile * kTile, a.lq, a.d, t);
-    gs.fetch(static_cast<const T*>(a.dout) + b * a.gb + h * a.gh, a.gl, tile * kTile, a.lq, a.d, t);
+  Rows<T, kTile> qrows, grows;
+  int fetched = hk * a.group;  // head and tile of the next fetch
+  int at_tile = first;
+  auto fetch = [&]() {
+    const int h = fetched, tile = at_tile;
+    if (tile == first) {
+      qrows.begin(static_cast<const T*>(a.q) + b * a.qb + h * a.qh, a.ql, tile * kTile, a.lq, a.d);
+      grows.begin(static_cast<const T*>(a.dout) + b * a.gb + h * a.gh, a.gl, tile * kTile, a.lq, a.d);
+    }
+    qs.fetch(qrows, t);
+    gs.fetch(grows, t);
+    qrows.next();
+    grows.next();
+    if (++at_tile == last) {
+      at_tile = first;
+      ++fetched;
+    }
     const int i = tile * kTile + (t & (kTile - 1));
     if (t < 2 * kTile) {
       const float* from = t < kTile ? a.lse : a.delta;
@@ -252,25 +282,31 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dkv_kern
       if (docs) other_id = ids[i];
     }
   };
-  if (steps > 0) fetch(0);
+  Scoring scoring = scoring_of(a, hk * a.group);
+  if (steps > 0) fetch();
+  int h = hk * a.group, tile = first - 1;
   for (int step = 0; step < steps; ++step) {
-    const int h = hk * a.group + step / tiles, tile = first + step % tiles, i0 = tile * kTile;
+    if (++tile == last) {
+      tile = first;
+      ++h;
+    }
+    const int i0 = tile * kTile;
     const bool partial = meet.partial(tile);
-    const float slope = a.slopes ? a.slopes[h] : 0.f;
+    if (a.slopes) scoring.slope = a.slopes[h];
     __syncthreads();
     if (t < 4) odd[t >> 1][t & 1] = 0u;
     if (t < 2 * kTile) stats[t / kTile][t % kTile] = stat;
     if (docs && t < kTile) query_ids[t] = other_id;
     if (partial) {
       __syncthreads();
-      qs.template store<true>(qt, S, odd[1], t);
-      gs.template store<true>(gt, S, odd[0], t);
+      qs.template store<true>(qt, odd[1], t);
+      gs.template store<true>(gt, odd[0], t);
     } else {
-      qs.template store<false>(qt, S, nullptr, t);
-      gs.template store<false>(gt, S, nullptr, t);
+      qs.template store<false>(qt, nullptr, t);
+      gs.template store<false>(gt, nullptr, t);
     }
     __syncthreads();
-    if (step + 1 < steps) fetch(step + 1);
+    if (step + 1 < steps) fetch();
     if (meet.skips(tile)) continue;
     const bool masked = meet.masked(tile);
 #pragma unroll
@@ -278,11 +314,11 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dkv_kern
       f16v s = f16v(0.f), ds = f16v(0.f), slope_of = f16v(1.f);
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
-        s = mma<T>(frag_along(qt, S, 32 * u, n, lane), kf[n], s);
-        ds = mma<T>(frag_along(gt, S, 32 * u, n, lane), vf[n], ds);
+        s = mma<T>(Lds::along(qt, 32 * u, n, lane), kf[n], s);
+        ds = mma<T>(Lds::along(gt, 32 * u, n, lane), vf[n], ds);
       }
       const int at = i0 + 32 * u + 4 * half;
-      const float c = scores<T>(a, s, slope_of, at, j - off, slope);
+      const float c = scores<T>(scoring, s, slope_of, at, j - off);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const f4 lse = *reinterpret_cast<const f4*>(&stats[0][32 * u + 8 * w + 4 * half]);
@@ -293,41 +329,41 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dkv_kern
           ds[4 * w + r] = s[4 * w + r] * (ds[4 * w + r] - delta[r]);
         }
       }
-      if (a.cap > 0.f) ds *= slope_of;
-      unsigned hidden = 0u;
+      if (scoring.cap > 0.f) ds *= slope_of;
       if (masked) {
+        auto hide = [&](int r, bool so) {
+          s[r] = so ? 0.f : s[r];
+          ds[r] = so ? 0.f : ds[r];
+        };
+        if (docs)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          int4 other = {id, id, id, id};
-          if (docs) other = *reinterpret_cast<const int4*>(query_ids + 32 * u + 4 * half + 8 * w);
-          const int query_id[4] = {other.x, other.y, other.z, other.w};
+          for (int w = 0; w < 4; ++w) {
+            const int4 other = *reinterpret_cast<const int4*>(query_ids + 32 * u + 4 * half + 8 * w);
+            hide(4 * w, other.x != id);
+            hide(4 * w + 1, other.y != id);
+            hide(4 * w + 2, other.z != id);
+            hide(4 * w + 3, other.w != id);
+          }
+        if (scoring.prefixed && j >= prefix)  // else every row sees the key
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (j >= limit_of(a, at + 8 * w + r, prefix) || query_id[r] != id) {
-              s[4 * w + r] = ds[4 * w + r] = 0.f;
-              hidden |= 1u << (4 * w + r);
-            }
-        }
+          for (int r = 0; r < 16; ++r) hide(r, 8 * (r >> 2) + (r & 3) < j - off - at);
       }
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const Frag<T> p = result_frag<T>(s, w), f = result_frag<T>(ds, w);
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
-          dv[n] = mma<T>(frag_down(gt, S, 32 * u + 16 * w, n, lane), p, dv[n]);
-          dk[n] = mma<T>(frag_down(qt, S, 32 * u + 16 * w, n, lane), f, dk[n]);
+          dv[n] = mma<T>(Lds::down(gt, 32 * u + 16 * w, n, lane), p, dv[n]);
+          dk[n] = mma<T>(Lds::down(qt, 32 * u + 16 * w, n, lane), f, dk[n]);
         }
       }
       if (partial && odd[0][u]) {
-        // Values of dout that were zeroed in LDS, for the keys that their rows see.  A lane knows 16 of the 32
-        // rows; the other half of the wave, which has the same keys, knows the rest.
-        const unsigned others = (unsigned)__shfl_xor((int)hidden, 32);
+        // Values of dout that were zeroed in LDS, for the keys that their rows see.
         const T* gh = static_cast<const T*>(a.dout) + b * a.gb + h * a.gh;
         for (int r = 0; r < 32; ++r) {
           if (((odd[0][u] >> r) & 1u) == 0u) continue;
-          const int bit = 4 * (r >> 3) + (r & 3);
-          const unsigned seen_by = ((r >> 2) & 1) == half ? hidden : others;
-          if (((seen_by >> bit) & 1u) != 0u) continue;
+          const int i = i0 + 32 * u + r;
+          if (j >= limit_of(a, i, prefix) || (docs && query_ids[32 * u + r] != id)) continue;
           const T* row = gh + (int64_t)(i0 + 32 * u + r) * a.gl;
 #pragma unroll
           for (int n = 0; n < ND; ++n)
@@ -350,11 +386,12 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_dkv_kern
 
 template <typename T, int D>
 int launch(const Args& a, hipStream_t st) {
-  hipLaunchKernelGGL((attention_dq_kernel<T, D>), dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kOwn)), dim3(kThreads), 0,
+  const unsigned parts = a.qdoc.ids ? 2u : 1u;
+  hipLaunchKernelGGL((attention_dq_kernel<T, D>), dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kOwn) * parts), dim3(kThreads), 0,
                      st, a);
   const int rc = check_launch("attention_dq");
   if (rc || (!a.dk && !a.dv)) return rc;
-  hipLaunchKernelGGL((attention_dkv_kernel<T, D>), dim3(a.n * a.hk * (unsigned)ceil_div(a.lk, kOwn)), dim3(kThreads),
+  hipLaunchKernelGGL((attention_dkv_kernel<T, D>), dim3(a.n * a.hk * (unsigned)ceil_div(a.lk, kOwn) * parts), dim3(kThreads),
                      0, st, a);
   return check_launch("attention_dkv");
 }
@@ -387,11 +424,9 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const vo
   if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)rest | (uintptr_t)dout | (uintptr_t)dq |
         (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)plan) & 15) != 0)
     return fail(CTMR_E_INVALID, "tensors and the document plan must start on 16-byte boundaries");
-  const int bytes = elem_bytes(d->elem);
   for (const int64_t* s : {dout_strides, d->out_strides}) {
-    if (s[0] < 0 || s[1] < 0 || s[2] < 0 || (s[0] | s[1] | s[2]) * bytes % 16 != 0)
-      return fail(CTMR_E_INVALID, "strides must be multiples of 16 bytes and not negative");
-    if (s[2] * bytes > (1ll << 31) / kTile - 4096) return fail(CTMR_E_UNSUPPORTED, "row stride too large");
+    const int rc = check_strides(d, s, d->lq);
+    if (rc) return rc;
   }
   for (const int64_t* s : {dq ? dq_strides : nullptr, dk ? dk_strides : nullptr, dv ? dv_strides : nullptr})
     if (s && (s[0] | s[1] | s[2]) % 4 != 0)
@@ -406,7 +441,7 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const vo
   a.out = const_cast<void*>(out), a.rest = const_cast<void*>(rest), a.lse = const_cast<float*>(lse), a.dout = dout;
   a.dq = dq, a.dk = dk, a.dv = dv, a.delta = (float*)workspace;
   a.ob = d->out_strides[0], a.oh = d->out_strides[1], a.ol = d->out_strides[2];
-  a.gb = dout_strides[0], a.gh = dout_strides[1], a.gl = dout_strides[2];
+  a.gb = dout_strides[0], a.gh = dout_strides[1], a.gl = row_stride(dout_strides, d->lq, d->head_dim);
   if (dq) a.dqb = dq_strides[0], a.dqh = dq_strides[1], a.dql = dq_strides[2];
   if (dk) a.dkb = dk_strides[0], a.dkh = dk_strides[1], a.dkl = dk_strides[2];
   if (dv) a.dvb = dv_strides[0], a.dvh = dv_strides[1], a.dvl = dv_strides[2];

@@ -245,11 +245,12 @@ class Documents:
 
 
 def _attention_heads(t: Tensor) -> Tensor:
-    """``t`` with a unit last stride, 16-byte aligned rows and a row stride that the kernels can address."""
+    """``t`` with a unit last stride and 16-byte aligned rows that do not overlap, in a stride the kernels can address."""
     size = t.element_size()
     if t.stride(3) == 1 and t.data_ptr() % 16 == 0:
         strides = ops._head_strides(t)
-        if all(s * size % 16 == 0 for s in strides) and strides[2] * size <= 1 << 24:
+        if (all(s * size % 16 == 0 for s in strides) and strides[2] * size <= 1 << 23
+                and (t.shape[2] <= 1 or strides[2] >= t.shape[3])):
             return t
     return t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
 

@@ -181,6 +181,8 @@ def test_strides(ctmr, dev, dtype):
     _compare(ctmr, q, k, v, dout)
     wide = k[:1].expand(n, h, l, d)
     _compare(ctmr, q, wide, wide, dout)
+    same = k[:, :, :1].expand(n, h, l, d)  # one row for every key
+    _compare(ctmr, q, same, v, dout[:, :, 5:6].expand(n, h, l, d))
     flat = torch.zeros(q.numel() + 1, device=dev, dtype=dtype)
     odd = flat[1:].view(n, h, l, d)
     odd.copy_(q)
@@ -236,6 +238,20 @@ def test_visible_nan_and_infinity_show(ctmr, dev, dtype, lq):
         dv = _run(f, q, k, clean.new_zeros(v.shape), dout, **kw)[3]
         col = dv[0, 0, :, 2]
         assert bool((col[key_ids[0] == 0] == math.inf).all()) and bool(col[key_ids[0] != 0].isfinite().all())
+
+
+def test_infinity_in_a_single_row(ctmr, dev):
+    """What a tile holds past its only row is nothing, not the row again."""
+    f = ctmr.differentiable
+    for dtype in TYPES:
+        q, k, v, dout = (t.clone() for t in _inputs(dev, 1, 1, 1, 1, 1, 32, dtype))
+        v[..., 3] = math.inf
+        out = f.attention(q, k, v, scale=0.1)
+        assert torch.equal(out, v)
+        if dtype != torch.float16:
+            v.zero_()
+            dout[..., 4] = -math.inf
+            assert torch.equal(_run(f, q, k, v, dout, scale=0.1)[3], dout)
 
 
 @pytest.mark.parametrize("kw", [{}, {"softcap": 2.0}, {"prefix": 20}, {"slopes": True}, {"ids": True}], ids=str)

@@ -165,9 +165,10 @@ def test_attention_host_checks(ctmr, native_loaded):
     assert native_loaded.ctmr_masked_attention_workspace_bytes(None) == L.E_INVALID
     for kw in ({"n": 0}, {"lq": 0}, {"lk": 0}, {"q_heads": 3}, {"k_heads": 0}, {"elem": 3}, {"scale": 0.0},
                {"scale": float("nan")}, {"softcap": -1.0}, {"softcap": float("inf")}, {"q_strides": (25600, 32, 130)},
-               {"k_strides": (-4, 32, 64)}, {"v_strides": (19200, 33, 64)}):
+               {"k_strides": (-4, 32, 64)}, {"v_strides": (19200, 33, 64)},
+               {"k_strides": (19200, 32, 24)}, {"q_strides": (0, 0, 0)}):
         assert space(**kw) == L.E_INVALID, kw
-    for kw in ({"head_dim": 36}, {"head_dim": 136}, {"lq": 1 << 29}, {"k_strides": (0, 0, 1 << 23)},
+    for kw in ({"head_dim": 36}, {"head_dim": 136}, {"lq": 1 << 29}, {"k_strides": (0, 0, 1 << 22)},
                {"n": 1 << 20, "q_heads": 1 << 10, "k_heads": 1}):
         assert space(**kw) == L.E_UNSUPPORTED, kw
     # splits: 8 query blocks of 5 key tiles make one part, one token of 16384 keys the most of its 256 tiles
@@ -200,7 +201,7 @@ def test_attention_host_checks(ctmr, native_loaded):
     assert back(ws=None, dq=p) == L.E_WORKSPACE
 
     docs = native_loaded.ctmr_documents_bytes
-    assert docs(2, 100, 65) == 2 * (128 * 4 + 128 * 4 + 2 * 16 + 2 * 16 + 4 * 16 + 3 * 16)
+    assert docs(2, 100, 65) == 2 * (128 * 4 + 128 * 4 + 2 * 16 + 2 * 16 + 4 * 48 + 3 * 48 + 4 + 4)
     assert docs(0, 1, 1) == L.E_INVALID and docs(70000, 1, 1) == L.E_UNSUPPORTED
     assert native_loaded.ctmr_documents(2, 100, 65, p, p, p, 10, None) == L.E_WORKSPACE
     assert native_loaded.ctmr_documents(2, 100, 65, None, p, p, 1 << 20, None) == L.E_INVALID
