@@ -37,8 +37,8 @@ struct RowMask {
   int limit, id;
 };
 
-// Raw products of NB 32-key blocks -> scores in units of log2 / c (c returned): with a cap or slopes the scores
-// themselves (c = 1), else the products (c = scale log2 e).  Masked keys become -inf; ids: of the keys from k0 on, or
+// Raw products of NB 32-key blocks -> scores in units of 1 / c (c returned): the products, or with a cap tanh, less
+// the distance in these units.  Masked keys become -inf; ids: of the keys from k0 on, or
 // null.
 template <typename T, int NB>
 __device__ __forceinline__ float score_blocks(const Scoring& a, f16v (&s)[NB], int k0, int pos, bool partial,
@@ -46,23 +46,20 @@ __device__ __forceinline__ float score_blocks(const Scoring& a, f16v (&s)[NB], i
   const int half = lane >> 5;
   float c = a.scale * kLog2e;
   if (a.cap > 0.f) {
-    const float in = a.scale / a.cap, out = a.cap * kLog2e;
+    const float in = a.scale / a.cap;
 #pragma unroll
     for (int u = 0; u < NB; ++u)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[u][r] = out * tanh_of<T>(s[u][r], in);
-    c = 1.0f;
+      for (int r = 0; r < 16; ++r) s[u][r] = tanh_of<T>(s[u][r], in);
+    c = a.cap * kLog2e;
   }
   if (a.sloped) {
-    const float per = a.slope * kLog2e;
+    const float per = -a.slope * kLog2e / c, from = (float)(k0 + 4 * half - pos);
 #pragma unroll
     for (int u = 0; u < NB; ++u)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = k0 + 32 * u + 8 * (r >> 2) + 4 * half + (r & 3);
-        s[u][r] = fmaf(-per, fabsf((float)(pos - j)), s[u][r] * c);
-      }
-    c = 1.0f;
+      for (int r = 0; r < 16; ++r)
+        s[u][r] = fmaf(per, fabsf(from + (float)(32 * u + 8 * (r >> 2) + (r & 3))), s[u][r]);
   }
   // Two selects of two instructions each, and only where they decide something: a key past the end has no document.
   if (partial && ids) {
@@ -276,18 +273,19 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
     if (more) fetch(tile + 1);
     __syncthreads();
     if (!meet.skips(tile)) {
+      const int at = fresh<D == 128>(lane);
       f16v s[2] = {f16v(0.f), f16v(0.f)};
 #pragma unroll
       for (int n = 0; n < NK; ++n)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) s[u] = mma<T>(Lds::along(kt[buf], 32 * u, n, lane), qf[n], s[u]);
+        for (int u = 0; u < 2; ++u) s[u] = mma<T>(Lds::along(kt[buf], 32 * u, n, at), qf[n], s[u]);
       // V's first operands are read before the softmax, which covers the latency, as far as registers go.
       constexpr int kEarly = sizeof(T) == 4 ? 0 : D == 128 ? 0 : 2;  // contraction steps
       Frag<T> vf[2][ND];
 #pragma unroll
       for (int w = 0; w < kEarly; ++w)
 #pragma unroll
-        for (int n = 0; n < ND; ++n) vf[w][n] = Lds::down(vt[buf], 16 * w, n, lane);
+        for (int n = 0; n < ND; ++n) vf[w][n] = Lds::down(vt[buf], 16 * w, n, at);
       const int* tile_ids = docs ? key_ids[buf] : nullptr;
       const float c = score_blocks<T, 2>(scoring, s, k0, pos, meet.masked(tile), mask, tile_ids, lane);
       float alpha;
@@ -302,7 +300,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
         for (int w = 0; w < 2; ++w)
 #pragma unroll
           for (int n = 0; n < ND; ++n)
-            o[n] = mma<T>(u == 0 && w < kEarly ? vf[w][n] : Lds::down(vt[buf], 32 * u + 16 * w, n, lane), p[u][w], o[n]);
+            o[n] = mma<T>(u == 0 && w < kEarly ? vf[w][n] : Lds::down(vt[buf], 32 * u + 16 * w, n, at), p[u][w], o[n]);
       if (now) {
         const unsigned lo = odd[slot][0], hi = odd[slot][1];
         if (lo | hi) add_odd_values<T, ND>(a, o, v, k0, lo, hi, mask, tile_ids, lane);
@@ -333,7 +331,7 @@ constexpr int few_lds() {  // bytes; the join takes four 32 x D blocks of fp32 a
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 1) void attention_few_kernel(Args a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 64 ? 2 : 1) void attention_few_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
   __shared__ __attribute__((aligned(16))) char lds[few_lds<T, D>()];
@@ -447,31 +445,46 @@ __global__ __launch_bounds__(kThreads, 1) void attention_few_kernel(Args a) {
   if ((lane & 31) < rows) write_row<T, ND>(a, o, top, total, b, h, i, blockIdx.y, lane);
 }
 
-// Joins the splits of a row: 4 values a thread, splits in order.
+// Joins the splits of a row, one workgroup a row: D / 4 threads hold the values of a split, four each, and the
+// others every kThreads / (D / 4)-th split; then in order.  (A thread that walked all splits took 19 us for 128 rows
+// of 32 splits, one load after the other.)
+constexpr int kMostSplits = 64;
+
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void attention_join_kernel(Args a) {
-  const int64_t rows = (int64_t)a.n * a.hq * a.lq;
-  const int64_t at = (int64_t)blockIdx.x * (kThreads * 4 / D) + threadIdx.x / (D / 4);
-  const int d = threadIdx.x % (D / 4) * 4;
-  if (at >= rows) return;
+  constexpr int kLanes = D / 4, kGroups = kThreads / kLanes;
+  __shared__ float weight[kMostSplits];
+  __shared__ f4 sums[kGroups][kLanes];
+  const int64_t rows = (int64_t)a.n * a.hq * a.lq, at = blockIdx.x;
+  const int lane = threadIdx.x & 63, d = threadIdx.x % kLanes * 4, group = threadIdx.x / kLanes;
   const float2* state = reinterpret_cast<const float2*>(a.part + rows * a.splits * D);
-  float top = kNone;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, state[s * rows + at].x);
-  float total = 0.f;
-  Vec<float, 4> sum = Vec<float, 4>(0.f);
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 sw = state[s * rows + at];
-    const float w = __builtin_amdgcn_exp2f(sw.x - top);
-    total += sw.y * w;
-    sum += *reinterpret_cast<const Vec<float, 4>*>(a.part + (s * rows + at) * D + d) * w;
-  }
+  const float2 mine = lane < a.splits ? state[lane * rows + at] : float2{kNone, 0.f};
+  float top = mine.x;
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
+  const float w = __builtin_amdgcn_exp2f(mine.x - top);
+  float total = mine.y * w;
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) total += __shfl_xor(total, m);
+  if (threadIdx.x < kMostSplits) weight[threadIdx.x] = w;
+  __syncthreads();
+  f4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = group; s < a.splits; s += kGroups)
+    sum += *reinterpret_cast<const f4*>(a.part + (s * rows + at) * D + d) * weight[s];
+  sums[group][d / 4] = sum;
+  __syncthreads();
+  if (group != 0) return;
+  Vec<float, 4> out = Vec<float, 4>(0.f);
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) out += sums[g][d / 4];
   const int i = (int)(at % a.lq);
   const int64_t bh = at / a.lq;
   const int h = (int)(bh % a.hq);
   const int64_t b = bh / a.hq;
   if (d < a.d) {
     const float inv = total == 0.f ? 0.f : 1.0f / total;
-    store_output<T>(a, b * a.ob + h * a.oh + (int64_t)i * a.ol + d, sum * inv);
+    store_output<T>(a, b * a.ob + h * a.oh + (int64_t)i * a.ol + d, out * inv);
   }
   if (a.lse && d == 0) a.lse[at] = total == 0.f ? INFINITY : top + log2f(total) - kLift<T>;
 }
@@ -580,16 +593,16 @@ __global__ __launch_bounds__(kTile) void document_hulls_kernel(DocArgs a) {
 // --------------------------------------------------------------------------
 bool few_rows(const ctmr_masked_attention_desc* d) { return (int64_t)(d->q_heads / d->k_heads) * d->lq <= 32; }
 
-// Parts of the keys where the rows alone do not fill the chip: about 512 workgroups
-// (1024 of the few-row form, whose workgroups are bound by the latency of their
-// loads), of at least four 64-key tiles each.  From the shape only, so that a shape's
-// sums have one order.
+// Parts of the keys where the rows alone do not fill the chip: about 512 workgroups, or 256 of the few-row form, of
+// at least four 64-key tiles each.  From the shape only, so that a shape's sums have one order.  Few rows, bf16, 4 x 8
+// key heads of 128 values, 16384 keys (268 MB): 49.7 us with 256 workgroups (one a CU at a time; 5.4 TB/s), 56 with
+// 384, 51 with 512, 58 with 1024.
 int split_count(const ctmr_masked_attention_desc* d) {
   const bool few = few_rows(d);
   const int64_t blocks = (int64_t)d->n * (few ? d->k_heads : d->q_heads * ceil_div(d->lq, kRows));
   const int64_t tiles = ceil_div(d->lk, kTile);
-  const int64_t want = std::max<int64_t>(1, (few ? 1024 : 512) / blocks);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / 4, 64}));
+  const int64_t want = std::max<int64_t>(1, (few ? 256 : 512) / blocks);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / 4, kMostSplits}));
 }
 
 template <typename T, int D>
@@ -602,8 +615,7 @@ int launch(const Args& a, bool few, hipStream_t st) {
   const int rc = check_launch("masked_attention");
   if (rc || a.splits == 1) return rc;
   const int64_t rows = (int64_t)a.n * a.hq * a.lq;
-  hipLaunchKernelGGL((attention_join_kernel<T, D>), dim3((unsigned)ceil_div(rows, kThreads * 4 / D)), dim3(kThreads), 0,
-                     st, a);
+  hipLaunchKernelGGL((attention_join_kernel<T, D>), dim3((unsigned)rows), dim3(kThreads), 0, st, a);
   return check_launch("masked_attention_join");
 }
 

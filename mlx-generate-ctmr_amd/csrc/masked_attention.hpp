@@ -65,23 +65,33 @@ __device__ __forceinline__ V apart(V v) {
   return v;
 }
 
+// The lane, unknown to the compiler: the permuted addresses of a tile's reads are then computed where they are used
+// (one exclusive or each) instead of held in registers over the loop, for kernels that have none to spare.
+template <bool HIDE>
+__device__ __forceinline__ int fresh(int lane) {
+  if constexpr (HIDE) asm volatile("" : "+v"(lane));
+  return lane;
+}
+
 // A tile of D-value rows in LDS, in pieces of 16 bytes.  The pieces of a row are
-// permuted by the row (an exclusive or of the low bits), so that both kinds of reads
-// meet 32 banks without conflicts and without padding: along, eight lanes read one
-// piece of eight rows; down, sixteen lanes read two neighbouring pieces of four rows.
-// (Rows padded by 16 or 32 bytes instead cost a conflict of two in one of them:
-// 11 % of the cycles of the key gradients' kernel.)
+// permuted by the row (an exclusive or) so that no read meets a bank twice in the 256
+// bytes that LDS moves a cycle, without padding: along, sixteen lanes read one piece of
+// sixteen rows; down, 32 lanes read 64 bytes of four rows, or in fp32 64 lanes read 128
+// bytes of rows r and r + 4 (rows of 128 bytes keep a conflict of two there).
 template <typename T, int D>
 struct Tile {
   static constexpr int kRow = D * (int)sizeof(T);  // bytes
   static constexpr int kPieces = kRow / 16;        // 4, 8, 16 or 32
 
-  static __device__ __forceinline__ int mix(int row) {
-    return kPieces == 4 ? ((row & 2) | ((row >> 2) & 1)) : (((row & 3) << 1) | ((row >> 2) & 1));
+  static __device__ __forceinline__ int mix(int r) {
+    if constexpr (kPieces == 4) return (r >> 2) & 3;
+    if constexpr (kPieces == 8) return ((r << 1) & 4) | ((r >> 2) & 3);
+    if constexpr (sizeof(T) == 4) return ((r << 1) & 8) | ((r << 1) & 6) | ((r >> 3) & 1);
+    return ((r & 3) << 2) | ((r >> 2) & 3);
   }
   static __device__ __forceinline__ int at(int row, int piece) { return row * kRow + ((piece ^ mix(row)) << 4); }
 
-  // A operand of the 32 rows from `row` (a multiple of 8), contraction over the values 16 step .. + 15 of a row.
+  // A operand of the 32 rows from `row` (a multiple of 16), contraction over the values 16 step .. + 15 of a row.
   static __device__ __forceinline__ Frag<T> along(const char* tile, int row, int step, int lane) {
     const char* p = tile + row * kRow;
     const int r = lane & 31, half = lane >> 5;
@@ -95,7 +105,7 @@ struct Tile {
   }
 
   // A operand whose rows are the values 32 block .. + 31, contraction over the tile's rows `row` .. + 15 (a
-  // multiple of 8) in the results' order.
+  // multiple of 16) in the results' order.
   static __device__ __forceinline__ Frag<T> down(const char* tile, int row, int block, int lane) {
     const char* p = tile + row * kRow;
     const int half = lane >> 5;
@@ -110,10 +120,9 @@ struct Tile {
       // of the four rows.
       typedef Vec<short, 4> s4;
       typedef __attribute__((address_space(3))) s4 lds_s4;
-      const char* from = p + at(4 * half + ((lane & 15) >> 2), 4 * block + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) +
-                         8 * (lane & 1);
-      const s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)from);
-      const s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(from + 8 * kRow));
+      const int r = 4 * half + ((lane & 15) >> 2), piece = 4 * block + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+      const s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + at(r, piece) + 8 * (lane & 1)));
+      const s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + at(r + 8, piece) + 8 * (lane & 1)));
       return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }

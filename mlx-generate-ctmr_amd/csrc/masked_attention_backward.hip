@@ -38,20 +38,18 @@ template <typename T>
 __device__ __forceinline__ float scores(const Scoring& a, f16v& s, f16v& slope_of, int at, int x) {
   float c = a.scale * kLog2e;
   if (a.cap > 0.f) {
-    const float in = a.scale / a.cap, out = a.cap * kLog2e;
+    const float in = a.scale / a.cap;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float t = tanh_of<T>(s[r], in);
-      s[r] = out * t;
-      slope_of[r] = fmaf(-t, t, 1.0f);
+      s[r] = tanh_of<T>(s[r], in);
+      slope_of[r] = fmaf(-s[r], s[r], 1.0f);
     }
-    c = 1.0f;
+    c = a.cap * kLog2e;
   }
   if (a.sloped) {
-    const float per = a.slope * kLog2e;
+    const float per = -a.slope * kLog2e / c, from = (float)(at - x);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = fmaf(-per, fabsf((float)(at + 8 * (r >> 2) + (r & 3) - x)), s[r] * c);
-    c = 1.0f;
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(per, fabsf(from + (float)(8 * (r >> 2) + (r & 3))), s[r]);
   }
   return c;
 }
@@ -165,14 +163,15 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
     __syncthreads();
     if (tile + 1 < last) fetch(tile + 1);
     if (meet.skips(tile)) continue;
+    const int la = fresh<D == 128 && sizeof(T) == 2>(lane);
     const bool masked = meet.masked(tile) || (partial && (odd[0] | odd[1]) != 0u);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f16v s = f16v(0.f), ds = f16v(0.f), slope_of = f16v(1.f);
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
-        s = mma<T>(Lds::along(kt, 32 * u, n, lane), qf[n], s);
-        ds = mma<T>(Lds::along(vt, 32 * u, n, lane), gf[n], ds);
+        s = mma<T>(Lds::along(kt, 32 * u, n, la), qf[n], s);
+        ds = mma<T>(Lds::along(vt, 32 * u, n, la), gf[n], ds);
       }
       const int at = k0 + 32 * u + 4 * half;
       const float c = scores<T>(scoring, s, slope_of, at, pos);
@@ -202,7 +201,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
       for (int w = 0; w < 2; ++w) {
         const Frag<T> f = result_frag<T>(ds, w);
 #pragma unroll
-        for (int n = 0; n < ND; ++n) dq[n] = mma<T>(Lds::down(kt, 32 * u + 16 * w, n, lane), f, dq[n]);
+        for (int n = 0; n < ND; ++n) dq[n] = mma<T>(Lds::down(kt, 32 * u + 16 * w, n, la), f, dq[n]);
       }
     }
   }

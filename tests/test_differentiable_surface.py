@@ -174,7 +174,7 @@ def test_attention_host_checks(ctmr, native_loaded):
     # splits: 8 query blocks of 5 key tiles make one part, one token of 16384 keys the most of its 256 tiles
     assert space() == 4 * 0
     assert space(lq=1, lk=16384) == 64 * 4 * (32 + 2) * 4
-    assert space(lq=1, lk=16384, n=64) == 8 * 64 * 4 * (32 + 2) * 4
+    assert space(lq=1, lk=16384, n=64) == 2 * 64 * 4 * (32 + 2) * 4
 
     def call(q=p, plan=None, out=p, ws=p, nbytes=0, **kw):
         return native_loaded.ctmr_masked_attention(ctypes.byref(_attention_desc(L, **kw)), q, p, p, None, None, plan, out,
