@@ -22,7 +22,7 @@
 //    workgroup between the sums and the element-wise pass: one launch (two
 //    backward with several items, whose dgamma are added in order by the second).
 //  * large: partial sums per (item, chunk of voxels, channel), a fixed-order
-//    reduction per group, the element-wise pass: three launches.
+//    reduction per group, the element-wise pass: three launches each way.
 // No atomics: every sum has an order given by the shape.
 #include "elements.hpp"
 
@@ -77,16 +77,13 @@ __device__ __forceinline__ float through_silu(float dy, float z) {
   return dy * (sig * fmaf(z, 1.0f - sig, 1.0f));
 }
 
-// Sums v[2V] of the `rows` threads of each of `cols` columns (thread = row * cols
-// + col, others idle), in LDS; the threads of row 0 hold the result.  The tree's
-// shape depends on rows only.
+// Sums W values of the `rows` threads of each of `cols` columns (thread = row * cols
+// + col, others idle) that lie in LDS, value k of a thread at k * rows * cols +
+// thread; the threads of row 0 get the result.  The tree's shape depends on rows only.
 template <int W>
-__device__ __forceinline__ void reduce_rows(double (&v)[W], double* lds, int col, int row, int rows, int cols,
-                                            bool active) {
+__device__ __forceinline__ void sum_rows(double (&v)[W], double* lds, int col, int row, int rows, int cols,
+                                         bool active) {
   const int stride = cols * rows;
-  if (active)
-#pragma unroll
-    for (int k = 0; k < W; ++k) lds[k * stride + row * cols + col] = v[k];
   int left = rows;
   while (left > 1) {
     const int half = (left + 1) >> 1;
@@ -102,9 +99,24 @@ __device__ __forceinline__ void reduce_rows(double (&v)[W], double* lds, int col
     for (int k = 0; k < W; ++k) v[k] = lds[k * stride + col];
 }
 
-// Per-channel sums of a chunk: x and x^2, or backward dz and dz xhat.
+template <int W>
+__device__ __forceinline__ void reduce_rows(double (&v)[W], double* lds, int col, int row, int rows, int cols,
+                                            bool active) {
+  if (active)
+#pragma unroll
+    for (int k = 0; k < W; ++k) lds[k * cols * rows + row * cols + col] = v[k];
+  sum_rows<W>(v, lds, col, row, rows, cols, active);
+}
+
+// Per-channel sums of a chunk: x and x^2, or backward dz and dz xhat.  A thread sums kBatch rows in fp32 before they
+// join its fp64 sums: with three fp64 operations a value the backward sums took 99 us for 80x128x128 voxels of 64
+// channels in bf16, bound by them, not by memory.  Forward the fp32 sums are of x - x0, x0 the thread's first value of
+// the channel, so that they lose nothing to a mean far above the spread.
+constexpr int kBatch = 32;
+
+// The fp64 sums wait in LDS, where they are added up at the end.
 template <typename T, int V, bool BACKWARD>
-__global__ __launch_bounds__(kThreads) void gn_sums_kernel(NormArgs a) {
+__global__ __launch_bounds__(kThreads, BACKWARD ? 4 : 5) void gn_sums_kernel(NormArgs a) {
   __shared__ double lds[2 * V * kThreads];
   const int b = blockIdx.y;
   const int col0 = blockIdx.z * kThreads;
@@ -112,25 +124,45 @@ __global__ __launch_bounds__(kThreads) void gn_sums_kernel(NormArgs a) {
   const int col = threadIdx.x % cols, row = threadIdx.x / cols;
   const bool active = row < rows;
   const int c0 = (col0 + col) * V;
-  double acc[2 * V];
-#pragma unroll
-  for (int k = 0; k < 2 * V; ++k) acc[k] = 0.0;
+  const int slots = rows * cols;
+  double* acc = lds + threadIdx.x;
   if (active) {
-    const int64_t first = (int64_t)blockIdx.x * a.chunk, last = min(first + a.chunk, a.s);
-    const T* x = static_cast<const T*>(a.x) + (int64_t)b * a.s * a.c + c0;
+#pragma unroll
+    for (int k = 0; k < 2 * V; ++k) acc[k * slots] = 0.0;
+    const int64_t first = (int64_t)blockIdx.x * a.chunk + row, last = min((int64_t)(blockIdx.x + 1) * a.chunk, a.s);
+    const int64_t step = (int64_t)rows * a.c;
+    const T* x = static_cast<const T*>(a.x) + ((int64_t)b * a.s + first) * a.c + c0;
+    int left = first < last ? (int)((last - first + rows - 1) / rows) : 0;
+    const int count = left;
     if constexpr (!BACKWARD) {
-#pragma unroll 4
-      for (int64_t r = first + row; r < last; r += rows) {
-        const Vec<float, V> v = load_as_float<T, V>(x + r * a.c);
+      Vec<float, V> x0 = Vec<float, V>(0.f);
+      if (left > 0) x0 = load_as_float<T, V>(x);
+      while (left > 0) {
+        Vec<float, V> p = Vec<float, V>(0.f), q = Vec<float, V>(0.f);
+        const int batch = min(left, kBatch);
+#pragma unroll 8
+        for (int r = 0; r < batch; ++r) {
+          const Vec<float, V> d = load_as_float<T, V>(x) - x0;
+          x += step;
+          p += d;
+#pragma unroll
+          for (int k = 0; k < V; ++k) q[k] = fmaf(d[k], d[k], q[k]);
+        }
+        left -= batch;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const double d = (double)v[k];
-          acc[k] += d;
-          acc[V + k] = fma(d, d, acc[V + k]);
+          acc[k * slots] += (double)p[k];
+          acc[(V + k) * slots] += (double)q[k];
         }
       }
+#pragma unroll
+      for (int k = 0; k < V; ++k) {  // sums of x and x^2 again
+        const double base = (double)x0[k], sum = acc[k * slots], all = fma((double)count, base, sum);
+        acc[k * slots] = all;
+        acc[(V + k) * slots] += base * (sum + all);
+      }
     } else {
-      const T* dy = static_cast<const T*>(a.dy) + (int64_t)b * a.s * a.c + c0;
+      const T* dy = static_cast<const T*>(a.dy) + ((int64_t)b * a.s + first) * a.c + c0;
       Mean m[V];
       float gamma[V], beta[V];
 #pragma unroll
@@ -139,26 +171,39 @@ __global__ __launch_bounds__(kThreads) void gn_sums_kernel(NormArgs a) {
         gamma[k] = load_param(a.gamma, a.ptype, c0 + k);
         beta[k] = load_param(a.beta, a.ptype, c0 + k);
       }
-#pragma unroll 2
-      for (int64_t r = first + row; r < last; r += rows) {
-        const Vec<float, V> v = load_as_float<T, V>(x + r * a.c), g = load_as_float<T, V>(dy + r * a.c);
+      while (left > 0) {
+        Vec<float, V> p = Vec<float, V>(0.f), q = Vec<float, V>(0.f);
+        const int batch = min(left, kBatch);
+#pragma unroll(16 / V < 4 ? 16 / V : 4)
+        for (int r = 0; r < batch; ++r) {
+          const Vec<float, V> v = load_as_float<T, V>(x), g = load_as_float<T, V>(dy);
+          x += step;
+          dy += step;
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const float xh = xhat_of(v[k], m[k]);
+            const float dz = a.silu ? through_silu(g[k], fmaf(gamma[k], xh, beta[k])) : g[k];
+            p[k] += dz;
+            q[k] = fmaf(dz, xh, q[k]);
+          }
+        }
+        left -= batch;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float xh = xhat_of(v[k], m[k]);
-          const float dz = a.silu ? through_silu(g[k], fmaf(gamma[k], xh, beta[k])) : g[k];
-          acc[k] += (double)dz;
-          acc[V + k] = fma((double)dz, (double)xh, acc[V + k]);
+          acc[k * slots] += (double)p[k];
+          acc[(V + k) * slots] += (double)q[k];
         }
       }
     }
   }
-  reduce_rows<2 * V>(acc, lds, col, row, rows, cols, active);
+  double sums[2 * V];
+  sum_rows<2 * V>(sums, lds, col, row, rows, cols, active);
   if (active && row == 0) {
     double* out = a.part + (((int64_t)b * a.chunks + blockIdx.x) * a.c + c0) * 2;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      out[2 * k] = acc[k];
-      out[2 * k + 1] = acc[V + k];
+      out[2 * k] = sums[k];
+      out[2 * k + 1] = sums[V + k];
     }
   }
 }
@@ -184,72 +229,81 @@ __device__ __forceinline__ void block_sum2(double& p, double& q, double* lds, in
 }
 
 // (mean, rstd) of a group from its channels' partials: blockIdx = (group, item).
-__global__ __launch_bounds__(kThreads) void gn_mean_kernel(NormArgs a) {
-  __shared__ double lds[2 * kThreads / 64];
+constexpr int kWide = 256;
+__global__ __launch_bounds__(kWide) void gn_mean_kernel(NormArgs a) {
+  __shared__ double lds[2 * kWide / 64];
   const int g = blockIdx.x, b = blockIdx.y;
   double p = 0.0, q = 0.0;
   const double* part = a.part + ((int64_t)b * a.chunks * a.c + (int64_t)g * a.cpg) * 2;
-  for (int i = threadIdx.x; i < a.chunks * a.cpg; i += kThreads) {
-    const double* v = part + ((int64_t)(i / a.cpg) * a.c + i % a.cpg) * 2;
-    p += v[0];
-    q += v[1];
+#pragma unroll 4
+  for (int i = threadIdx.x; i < a.chunks * a.cpg; i += kWide) {
+    const double2 v = *reinterpret_cast<const double2*>(part + ((int64_t)(i / a.cpg) * a.c + i % a.cpg) * 2);
+    p += v.x;
+    q += v.y;
   }
-  block_sum2(p, q, lds, kThreads);
+  block_sum2(p, q, lds, kWide);
   if (threadIdx.x == 0) a.saved[b * a.groups + g] = finish(p, q, (double)a.s * a.cpg, a.eps);
 }
 
-// Sums over chunks of one channel and item: blockIdx = (channel, item).
-__global__ __launch_bounds__(64) void gn_channel_kernel(NormArgs a) {
-  const int c = blockIdx.x, b = blockIdx.y;
-  double p = 0.0, q = 0.0;
-  const double* part = a.part + ((int64_t)b * a.chunks * a.c + c) * 2;
-  for (int i = threadIdx.x; i < a.chunks; i += 64) {
-    p += part[(int64_t)i * a.c * 2];
-    q += part[(int64_t)i * a.c * 2 + 1];
-  }
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) {
-    p += __shfl_xor(p, m);
-    q += __shfl_xor(q, m);
-  }
-  if (threadIdx.x == 0) {
-    a.sums[((int64_t)b * a.c + c) * 2] = p;
-    a.sums[((int64_t)b * a.c + c) * 2 + 1] = q;
-  }
-}
-
-// The coefficients A and B of a group and item from `sums`; serial over cpg.
-__device__ __forceinline__ void coefficients(const NormArgs& a, int b, int g, float& ca, float& cb) {
-  double p = 0.0, q = 0.0;
-  for (int k = 0; k < a.cpg; ++k) {
-    const int c = g * a.cpg + k;
-    const double gamma = load_param(a.gamma, a.ptype, c);
-    p += gamma * a.sums[((int64_t)b * a.c + c) * 2];
-    q += gamma * a.sums[((int64_t)b * a.c + c) * 2 + 1];
-  }
+// One workgroup a group: for each item the sums of its channels over the chunks, which give A and B; over the items
+// (in order) dgamma and dbeta.
+__global__ __launch_bounds__(kWide) void gn_params_kernel(NormArgs a) {
+  __shared__ double lds[2 * kWide];
+  const int g = blockIdx.x;
+  const int cols = min(a.cpg, kWide), rows = kWide / cols;
+  const int col = threadIdx.x % cols, row = threadIdx.x / cols;
+  const bool active = row < rows;
   const double count = (double)a.s * a.cpg;
-  ca = (float)(p / count);
-  cb = (float)(q / count);
+  for (int c0 = 0; c0 < a.cpg; c0 += cols) {  // more channels than threads: block by block
+    const int c = g * a.cpg + c0 + col;
+    const bool real = active && c0 + col < a.cpg;
+    double beta = 0.0, gamma = 0.0;
+    const double weight = real ? (double)load_param(a.gamma, a.ptype, c) : 0.0;
+    for (int b = 0; b < a.n; ++b) {
+      double v[2] = {0.0, 0.0};
+      if (real) {
+        const double* part = a.part + ((int64_t)b * a.chunks * a.c + c) * 2;
+#pragma unroll 4
+        for (int i = row; i < a.chunks; i += rows) {
+          const double2 d = *reinterpret_cast<const double2*>(part + (int64_t)i * a.c * 2);
+          v[0] += d.x;
+          v[1] += d.y;
+        }
+      }
+      __syncthreads();  // the last item's sums are read
+      reduce_rows<2>(v, lds, col, row, rows, cols, active);
+      const bool first = active && row == 0;
+      beta += first ? v[0] : 0.0;
+      gamma += first ? v[1] : 0.0;
+      double p = first ? weight * v[0] : 0.0, q = first ? weight * v[1] : 0.0;
+      __syncthreads();
+      block_sum2(p, q, lds, kWide);
+      if (threadIdx.x == 0) {
+        float* coef = a.coef + 2 * ((int64_t)b * a.groups + g);
+        coef[0] = (c0 ? coef[0] : 0.f) + (float)(p / count);
+        coef[1] = (c0 ? coef[1] : 0.f) + (float)(q / count);
+      }
+    }
+    if (real && row == 0 && a.dgamma) {
+      store_param(a.dbeta, a.ptype, c, (float)beta);
+      store_param(a.dgamma, a.ptype, c, (float)gamma);
+    }
+  }
 }
 
-// dgamma and dbeta (items added in order) and, where wanted, A and B.
-__global__ __launch_bounds__(kThreads) void gn_params_kernel(NormArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i < a.c && a.dgamma) {
-    double p = 0.0, q = 0.0;
-    for (int b = 0; b < a.n; ++b) {
-      p += a.sums[((int64_t)b * a.c + i) * 2];
-      q += a.sums[((int64_t)b * a.c + i) * 2 + 1];
-    }
-    store_param(a.dbeta, a.ptype, i, (float)p);
-    store_param(a.dgamma, a.ptype, i, (float)q);
+// The small form's dgamma and dbeta: items added in order.
+__global__ __launch_bounds__(kThreads) void gn_small_params_kernel(NormArgs a) {
+  const int i = blockIdx.x * kThreads + threadIdx.x;
+  if (i >= a.c) return;
+  double p = 0.0, q = 0.0;
+#pragma unroll 4
+  for (int b = 0; b < a.n; ++b) {
+    const double2 v = *reinterpret_cast<const double2*>(a.sums + ((int64_t)b * a.c + i) * 2);
+    p += v.x;
+    q += v.y;
   }
-  if (a.coef && i < (int64_t)a.n * a.groups) {
-    float ca, cb;
-    coefficients(a, (int)(i / a.groups), (int)(i % a.groups), ca, cb);
-    a.coef[2 * i] = ca;
-    a.coef[2 * i + 1] = cb;
-  }
+  store_param(a.dbeta, a.ptype, i, (float)p);
+  store_param(a.dgamma, a.ptype, i, (float)q);
 }
 
 // The element-wise pass.  The chunks run from the last to the first: what the
@@ -456,8 +510,10 @@ bool small_form(int64_t s, int cpg, int elem) {
   return s <= rows * (kSmallBytes / elem_bytes(elem));
 }
 
-// Voxels of a chunk: about 1024 chunks over all items, at least 32 KB of values
-// each, so that a chunk's 16 bytes a channel of partials stay a few percent of it.
+// Voxels of a chunk: about 1024 chunks over all items, four workgroups a CU, at least 32 KB of values each, so that a
+// chunk's 16 bytes a channel of partials stay a few percent of it.  With 2048, 80x128x128 voxels of 64 channels, bf16,
+// took 115 us forward where 1024 take 103, and 182 backward where 1024 take 193; 45x90x117 of 128, fp16, 88 for 74 and
+// 143 for 129.
 int64_t chunk_voxels(int n, int64_t s, int c, int bytes) {
   const int64_t fill = ceil_div(s * n, 1024);
   const int64_t least = std::max<int64_t>(ceil_div(32768, (int64_t)c * bytes), 64);
@@ -474,7 +530,7 @@ int norm_check(int32_t n, int64_t s, int32_t c, int32_t groups, int32_t elem, in
 }
 
 struct NormSpace {  // byte offsets in the workspace
-  int64_t part = 0, sums = 0, coef = 0, total = 0;
+  int64_t part = 0, coef = 0, total = 0;
 };
 
 NormSpace norm_space(int32_t n, int64_t s, int32_t c, int32_t groups, int32_t elem, bool backward) {
@@ -484,8 +540,7 @@ NormSpace norm_space(int32_t n, int64_t s, int32_t c, int32_t groups, int32_t el
     return w;
   }
   const int64_t chunks = ceil_div(s, chunk_voxels(n, s, c, elem_bytes(elem)));
-  w.sums = (int64_t)n * chunks * c * 16;
-  w.coef = w.sums + (backward ? (int64_t)n * c * 16 : 0);
+  w.coef = (int64_t)n * chunks * c * 16;
   w.total = w.coef + (backward ? (int64_t)n * groups * 8 : 0);
   return w;
 }
@@ -502,25 +557,20 @@ template <typename T, int V, bool BACKWARD>
 int launch(NormArgs a, bool small, hipStream_t st) {
   if (small) {
     hipLaunchKernelGGL((gn_small_kernel<T, V, BACKWARD>), dim3(a.groups, a.n), dim3(kSmallThreads), 0, st, a);
-    int rc = check_launch("gn_small");
+    const int rc = check_launch("gn_small");
     if (rc || !BACKWARD || !a.sums || !a.dgamma) return rc;
-    hipLaunchKernelGGL(gn_params_kernel, dim3((unsigned)ceil_div(a.c, kThreads)), dim3(kThreads), 0, st, a);
-    return check_launch("gn_params");
+    hipLaunchKernelGGL(gn_small_params_kernel, dim3((unsigned)ceil_div(a.c, kThreads)), dim3(kThreads), 0, st, a);
+    return check_launch("gn_small_params");
   }
   a.cols = a.c / V;
   const dim3 grid(a.chunks, a.n, (unsigned)ceil_div(a.cols, kThreads));
   hipLaunchKernelGGL((gn_sums_kernel<T, V, BACKWARD>), grid, dim3(kThreads), 0, st, a);
   int rc = check_launch("gn_sums");
   if (rc) return rc;
-  if constexpr (!BACKWARD) {
-    hipLaunchKernelGGL(gn_mean_kernel, dim3(a.groups, a.n), dim3(kThreads), 0, st, a);
-  } else {
-    hipLaunchKernelGGL(gn_channel_kernel, dim3(a.c, a.n), dim3(64), 0, st, a);
-    rc = check_launch("gn_channel");
-    if (rc) return rc;
-    const int64_t items = std::max<int64_t>(a.c, (int64_t)a.n * a.groups);
-    hipLaunchKernelGGL(gn_params_kernel, dim3((unsigned)ceil_div(items, kThreads)), dim3(kThreads), 0, st, a);
-  }
+  if constexpr (!BACKWARD)
+    hipLaunchKernelGGL(gn_mean_kernel, dim3(a.groups, a.n), dim3(kWide), 0, st, a);
+  else
+    hipLaunchKernelGGL(gn_params_kernel, dim3(a.groups), dim3(kWide), 0, st, a);
   rc = check_launch("gn_reduce");
   if (rc || !a.y) return rc;
   hipLaunchKernelGGL((gn_apply_kernel<T, V, BACKWARD>), grid, dim3(kThreads), 0, st, a);
@@ -628,7 +678,6 @@ int ctmr_norm_backward(int32_t n, int64_t s, int32_t c, int32_t groups, int32_t 
     a.sums = n > 1 ? (double*)base : nullptr;
   } else {
     a.part = (double*)(base + w.part);
-    a.sums = (double*)(base + w.sums);
     a.coef = (float*)(base + w.coef);
   }
   return dispatch<true>(a, elem, (hipStream_t)stream);

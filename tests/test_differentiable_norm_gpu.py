@@ -59,8 +59,11 @@ def _check(y, grads, x, w, b, dy, groups, eps, silu):
     group_mean = lambda t: t.reshape(n, -1, groups, c // groups).mean((1, 3), keepdim=True).expand(
         n, t.numel() // n // c, groups, c // groups).reshape(x.shape)
     exh = 4 * U * xhat.abs()
-    ea = group_mean(wd.abs() * edz)
-    eb = group_mean(wd.abs() * (edz * xhat.abs() + dz_abs * exh))
+    # sums over voxels: up to 32 terms are added in fp32 before they join an fp64 sum, at most 31 roundings of partial
+    # sums that the terms' sizes bound, and one of each product
+    batch = 32 * U
+    ea = group_mean(wd.abs() * (edz + batch * dz_abs))
+    eb = group_mean(wd.abs() * (edz * xhat.abs() + dz_abs * exh + batch * dz_abs * xhat.abs()))
     a, bb = group_mean((wd.abs() * dz_abs)), group_mean(wd.abs() * dz_abs * xhat.abs())
     tol = half * rx.abs() + rstd * (wd.abs() * edz + ea + eb * xhat.abs() + bb * exh
                                     + 6 * U * (wd.abs() * dz_abs + a + bb * xhat.abs()))
@@ -68,8 +71,8 @@ def _check(y, grads, x, w, b, dy, groups, eps, silu):
         tol = tol + 2.0 ** -25
     assert bool(((grads[0].double() - rx).abs() <= tol).all())
     half = torch.finfo(w.dtype).eps / 2
-    assert bool(((grads[2].double() - rb).abs() <= edz.sum(over) + half * rb.abs() + U).all())
-    assert bool(((grads[1].double() - rw).abs() <= (edz * xhat.abs() + dz_abs * exh).sum(over) + half * rw.abs() + U).all())
+    assert bool(((grads[2].double() - rb).abs() <= (edz + batch * dz_abs).sum(over) + half * rb.abs() + U).all())
+    assert bool(((grads[1].double() - rw).abs() <= (edz * xhat.abs() + dz_abs * exh + batch * dz_abs * xhat.abs()).sum(over) + half * rw.abs() + U).all())
 
 
 # (shape, groups): one voxel; ragged; channel counts that 8, 4 and 2 do not divide; one channel a group; one group;
