@@ -7,16 +7,20 @@ The reference is inference only; these are what fine-tuning its UNet and Control
 * ``rotary``      rotary positions over one to four axes (depth, height, width) for q and k
 * ``attention``   attention with grouped heads, a tanh cap, a distance bias, documents and a prefix
 * ``Documents``   which tokens of a batch belong together (volumes of different sizes in one row, padding)
+* ``PackedVolumes``  the documents and voxel positions of several volumes in one row
+* ``self_attention_tokens``  projections, rotary positions and attention of tokens
+  (``maisi.spatial_attention_volumes`` is the networks' block over it)
 """
 
 from __future__ import annotations
 
 import math
 import weakref
-from collections.abc import Sequence
+from collections.abc import Mapping, Sequence
 from typing import Optional, Union
 
 import torch
+import torch.nn.functional as F
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
@@ -44,7 +48,8 @@ def _graph_token(*tensors: Optional[Tensor]) -> Optional[_EagerGraph]:
 
     Raises:
         RuntimeError: in a capture, if a leaf belongs to a living graph recorded outside it."""
-    leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
+    given = [t if t._base is None else t._base for t in tensors if t is not None and t.requires_grad]  # views: their leaf
+    leaves = [t for t in given if t.requires_grad and t.is_leaf]
     if not leaves:
         return None
     if not torch.cuda.is_current_stream_capturing():
@@ -334,3 +339,64 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
     if needs:
         return _Attention.apply(q, k, v, slopes, prefixes, plan, scale, softcap, prefix is not None, value)
     return ops.masked_attention(q, k, v, slopes, prefixes, plan, scale, softcap, prefix is not None, value, False)[0]
+
+
+# ---------------------------------------------------------------------------
+# the networks' attention over these operators
+# ---------------------------------------------------------------------------
+class PackedVolumes:
+    """Volumes of different sizes as one row of tokens, voxel after voxel in (depth, height, width) order.
+
+    ``shapes`` are the volumes' (D, H, W).  ``positions`` ``(L, 3)`` int32 are the voxels' places for ``rotary``,
+    ``documents`` keeps the volumes apart in ``attention`` (None for a single volume, which needs no mask) and
+    ``lengths`` are the volumes' voxel counts.  Laid out once for every block that works on the batch.
+
+    Raises:
+        ValueError: on no volumes, or a shape that is not three positive sizes."""
+
+    def __init__(self, shapes: Sequence[Sequence[int]], device: Union[torch.device, str, int] = "cuda"):
+        self.shapes = tuple(tuple(int(s) for s in shape) for shape in shapes)
+        if not self.shapes or any(len(s) != 3 or min(s) < 1 for s in self.shapes):
+            raise ValueError(f"shapes must be one or more (D, H, W) of positive sizes; got {self.shapes}")
+        self.lengths = tuple(d * h * w for d, h, w in self.shapes)
+        grids = [torch.stack(torch.meshgrid(*(torch.arange(s, dtype=torch.int32) for s in shape), indexing="ij"),
+                             dim=-1).reshape(-1, 3) for shape in self.shapes]
+        self.positions = torch.cat(grids).to(device)
+        self.documents = None
+        if len(self.shapes) > 1:
+            ids = torch.repeat_interleave(torch.arange(len(self.shapes), dtype=torch.int32), torch.tensor(self.lengths))
+            self.documents = Documents(ids[None].to(self.positions.device))
+
+
+def self_attention_tokens(tokens: Tensor, weights: Mapping[str, Tensor], *, heads: int, scale: float, include_fc: bool,
+                          documents: Optional[Documents] = None, positions: Optional[Tensor] = None,
+                          sections: Optional[Sequence[int]] = None, base: float = 10000.0, prefix: str = "attn",
+                          qkv_bias: bool = True) -> Tensor:
+    """Q/K/V projections, rotary positions, self-attention and optional ``out_proj`` on ``(B, L, C)`` tokens;
+    differentiable in the tokens and the weights (fp32 and bf16; fp16 without gradients).
+
+    Takes the weights of ``fast_fp32.self_attention_tokens`` in the tokens' type.  ``documents`` keeps tokens apart;
+    ``positions`` with ``sections`` (see ``rotary``) turns q and k, and is left out for attention without positions.
+
+    Raises:
+        ValueError: on tokens that are not (B, L, C), heads that do not divide C, positions without sections or the
+            reverse, and what ``rotary`` and ``attention`` refuse."""
+    _activation(tokens, "tokens", 3)
+    n, length, c = (int(s) for s in tokens.shape)
+    heads = int(heads)
+    if heads < 1 or c < 1 or c % heads:
+        raise ValueError(f"{c} channels are not divisible by {heads} heads")
+    if (positions is None) != (sections is None):
+        raise ValueError("positions and sections go together")
+    names = [f"{prefix}.to_{m}" for m in ("q", "k", "v")]
+    w = torch.cat([_like(weights[f"{m}.weight"], tokens, f"{m}.weight", 2) for m in names])
+    b = torch.cat([_like(weights[f"{m}.bias"], tokens, f"{m}.bias", 1) for m in names]) if qkv_bias else None
+    # (B, L, 3, H, D): q, k and v are strided views of the one product
+    q, k, v = F.linear(tokens, w, b).reshape(n, length, 3, heads, c // heads).permute(2, 0, 3, 1, 4).unbind(0)
+    if positions is not None:
+        q, k = rotary(q, k, positions, sections=sections, base=base)
+    merged = attention(q, k, v, scale=scale, documents=documents).transpose(1, 2).reshape(n, length, c)
+    if include_fc:
+        merged = F.linear(merged, _like(weights[f"{prefix}.out_proj.weight"], tokens, f"{prefix}.out_proj.weight", 2),
+                          _like(weights[f"{prefix}.out_proj.bias"], tokens, f"{prefix}.out_proj.bias", 1))
+    return merged

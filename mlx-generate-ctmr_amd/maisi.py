@@ -33,6 +33,7 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor
 
+from . import differentiable as df
 from . import fast_fp32 as ff
 
 Z_SCALE = 4
@@ -112,6 +113,42 @@ def spatial_attention(x: Tensor, weights: Mapping[str, Tensor], *, num_groups: i
     merged = ff.self_attention_tokens(hidden.reshape(n, d * h * w, c), weights, heads=heads, scale=scale,
                                       include_fc=include_fc)
     return ff.add_with_stats(x, merged.reshape(n, d, h, w, c))
+
+
+def spatial_attention_volumes(volumes: Sequence[Tensor], weights: Mapping[str, Tensor], *, num_groups: int, eps: float,
+                              num_head_channels: int, include_fc: bool, packed: Optional[df.PackedVolumes] = None,
+                              sections: Optional[Sequence[int]] = None, base: float = 10000.0) -> list[Tensor]:
+    """``spatial_attention`` of several DHWC volumes at once, each over its own voxels, differentiable in the volumes
+    and the weights (fp32 and bf16; fp16 without gradients): what fine-tuning on volumes of different sizes runs.
+
+    Each volume has group statistics of its own; the tokens of all lie in one row, whose documents the attention
+    keeps apart, so no volume is padded to another's size.  ``packed`` is the batch's ``PackedVolumes`` where more
+    than one block uses it.  ``sections`` turns q and k by the voxels' (depth, height, width) (``differentiable.rotary``).
+
+    Raises:
+        ValueError: on no volumes, volumes that are not (D, H, W, C) of one C, type and device, channels that
+            ``num_head_channels`` does not divide, a ``packed`` of other shapes, and what the operators refuse."""
+    volumes = list(volumes)
+    if not volumes or any(not isinstance(v, Tensor) or v.dim() != 4 for v in volumes):
+        raise ValueError("volumes must be one or more (D, H, W, C) tensors")
+    c, like = int(volumes[0].shape[-1]), volumes[0]
+    if any(int(v.shape[-1]) != c or v.dtype != like.dtype or v.device != like.device for v in volumes):
+        raise ValueError("volumes differ in channels, type or device")
+    if num_head_channels < 1 or c % num_head_channels != 0:
+        raise ValueError("num_channels must be divisible by num_head_channels")
+    shapes = tuple(tuple(int(s) for s in v.shape[:3]) for v in volumes)
+    if packed is None:
+        packed = df.PackedVolumes(shapes, like.device)
+    elif packed.shapes != shapes or packed.positions.device != like.device:
+        raise ValueError(f"packed is for volumes {packed.shapes} on {packed.positions.device}; got {shapes} on "
+                         f"{like.device}")
+    rows = [df.group_norm(v[None], weights["norm.weight"], weights["norm.bias"], num_groups=num_groups, eps=eps)
+            .reshape(1, -1, c) for v in volumes]
+    merged = df.self_attention_tokens(rows[0] if len(rows) == 1 else torch.cat(rows, dim=1), weights,
+                                      heads=c // num_head_channels, scale=float(num_head_channels) ** -0.5,
+                                      include_fc=include_fc, documents=packed.documents, sections=sections, base=base,
+                                      positions=None if sections is None else packed.positions)
+    return [v + part.reshape(v.shape) for v, part in zip(volumes, merged.split(packed.lengths, dim=1))]
 
 
 # ---------------------------------------------------------------------------

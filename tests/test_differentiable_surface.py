@@ -100,6 +100,8 @@ def test_a_leaf_of_a_living_eager_graph_is_refused_in_a_capture(ctmr, monkeypatc
     with pytest.raises(RuntimeError, match="both"):
         f._check_capture(False)
     f._check_capture(True)
+    with pytest.raises(RuntimeError, match="outside this capture"):
+        f._graph_token(leaf[None])
     del token
     gc.collect()
     assert f._graph_token(leaf) is None
@@ -220,3 +222,45 @@ def test_attention_traces(ctmr):
         assert dq.shape == q.shape and dk.shape == dv.shape == (0,)
         plan = torch.ops.ctmr.documents(*(torch.empty(2, l, device="cuda", dtype=torch.int32) for l in (100, 65)))
         assert plan.dtype == torch.uint8 and plan.numel() == ctmr._lib.lib().ctmr_documents_bytes(2, 100, 65)
+
+
+def _block_weights(c=64, dtype=torch.float32):
+    w = {f"attn.{n}.weight": torch.zeros(c, c, dtype=dtype) for n in ("to_q", "to_k", "to_v", "out_proj")}
+    w |= {f"attn.{n}.bias": torch.zeros(c, dtype=dtype) for n in ("to_q", "to_k", "to_v", "out_proj")}
+    return w | {"norm.weight": torch.ones(c), "norm.bias": torch.zeros(c)}
+
+
+def test_packed_volumes(ctmr):
+    f = ctmr.differentiable
+    one = f.PackedVolumes([(2, 3, 1)], "cpu")
+    assert one.documents is None and one.lengths == (6,) and one.positions.dtype == torch.int32
+    assert one.positions.tolist() == [[0, 0, 0], [0, 1, 0], [0, 2, 0], [1, 0, 0], [1, 1, 0], [1, 2, 0]]
+    for shapes in ((), [(1, 2)], [(2, 0, 1)]):
+        with pytest.raises(ValueError, match="shapes must be"):
+            f.PackedVolumes(shapes, "cpu")
+    with pytest.raises(ValueError, match="on the GPU"):
+        f.PackedVolumes([(1, 1, 2), (1, 1, 1)], "cpu")
+
+
+@pytest.mark.parametrize(
+    ("kw", "message"),
+    [({"tokens": torch.zeros(5, 64)}, "tokens must be 3-D"), ({"heads": 3}, "not divisible"), ({"heads": 0}, "not divisible"),
+     ({"positions": torch.zeros(5, 3)}, "go together"), ({"sections": (8, 12, 12)}, "go together"),
+     ({"weights": _block_weights(dtype=torch.bfloat16)}, "to_q.weight is"), ({}, "on the GPU")])
+def test_self_attention_tokens_refuses(ctmr, kw, message):
+    kw = {"tokens": torch.zeros(1, 5, 64), "weights": _block_weights(), "heads": 2, "scale": 1.0, "include_fc": True} | kw
+    with pytest.raises(ValueError, match=message):
+        ctmr.differentiable.self_attention_tokens(kw.pop("tokens"), kw.pop("weights"), **kw)
+
+
+@pytest.mark.parametrize(
+    ("volumes", "kw", "message"),
+    [([], {}, "one or more"), ([(2, 3, 64)], {}, "one or more"), ([(1, 2, 3, 64), (1, 2, 3, 32)], {}, "differ in channels"),
+     ([(1, 2, 3, 64)], {"num_head_channels": 24}, "divisible"), ([(1, 2, 3, 64)], {"num_head_channels": 0}, "divisible"),
+     ([(1, 2, 3, 64)], {"packed": (1, 3, 2)}, "packed is for"), ([(1, 2, 3, 64)], {}, "on the GPU")])
+def test_spatial_attention_volumes_refuses(ctmr, volumes, kw, message):
+    if "packed" in kw:
+        kw = kw | {"packed": ctmr.differentiable.PackedVolumes([kw["packed"]], "cpu")}
+    kw = {"num_groups": 16, "eps": 1e-6, "num_head_channels": 32, "include_fc": True} | kw
+    with pytest.raises(ValueError, match=message):
+        ctmr.maisi.spatial_attention_volumes([torch.zeros(s) for s in volumes], _block_weights(), **kw)
