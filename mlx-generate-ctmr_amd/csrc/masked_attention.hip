@@ -445,9 +445,58 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 64 ? 2 : 1) void a
   if ((lane & 31) < rows) write_row<T, ND>(a, o, top, total, b, h, i, blockIdx.y, lane);
 }
 
-// Joins the splits of a row, one workgroup a row: D / 4 threads hold the values of a split, four each, and the
-// others every kThreads / (D / 4)-th split; then in order.  (A thread that walked all splits took 19 us for 128 rows
-// of 32 splits, one load after the other.)
+// Four joined values of row `at` and, by the thread of its first ones, lse.
+template <typename T>
+__device__ __forceinline__ void write_joined(const Args& a, int64_t at, int d, const Vec<float, 4>& out, float top,
+                                             float total) {
+  const int i = (int)(at % a.lq);
+  const int64_t bh = at / a.lq;
+  const int h = (int)(bh % a.hq);
+  const int64_t b = bh / a.hq;
+  if (d < a.d) {
+    const float inv = total == 0.f ? 0.f : 1.0f / total;
+    store_output<T>(a, b * a.ob + h * a.oh + (int64_t)i * a.ol + d, out * inv);
+  }
+  if (a.lse && d == 0) a.lse[at] = total == 0.f ? INFINITY : top + log2f(total) - kLift<T>;
+}
+
+// Joins up to kFewSplits splits: four values of a row a thread, all its loads at once.
+constexpr int kFewSplits = 8;
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void attention_join_few_kernel(Args a) {
+  const int64_t rows = (int64_t)a.n * a.hq * a.lq;
+  const int64_t at = (int64_t)blockIdx.x * (kThreads / (D / 4)) + threadIdx.x / (D / 4);
+  const int d = threadIdx.x % (D / 4) * 4;
+  if (at >= rows) return;
+  const float2* state = reinterpret_cast<const float2*>(a.part + rows * a.splits * D);
+  float2 part[kFewSplits];
+  f4 value[kFewSplits];
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    part[s] = float2{kNone, 0.f};
+    value[s] = f4{0.f, 0.f, 0.f, 0.f};
+    if (s < a.splits) {
+      part[s] = state[s * rows + at];
+      value[s] = *reinterpret_cast<const f4*>(a.part + (s * rows + at) * D + d);
+    }
+  }
+  float top = kNone, total = 0.f;
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) top = fmaxf(top, part[s].x);
+  Vec<float, 4> out = Vec<float, 4>(0.f);
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    const float w = __builtin_amdgcn_exp2f(part[s].x - top);
+    total = fmaf(part[s].y, w, total);
+    out += value[s] * w;
+  }
+  write_joined<T>(a, at, d, out, top, total);
+}
+
+// Joins more, one workgroup a row: D / 4 threads hold the values of a split, four each, and the others every
+// kThreads / (D / 4)-th split; then in order.  (A thread that walked all splits took 19 us for 128 rows of 32 splits,
+// one load after the other; a workgroup a row for 32768 rows of two splits 74 us.)
 constexpr int kMostSplits = 64;
 
 template <typename T, int D>
@@ -478,15 +527,7 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(Args a) {
   Vec<float, 4> out = Vec<float, 4>(0.f);
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) out += sums[g][d / 4];
-  const int i = (int)(at % a.lq);
-  const int64_t bh = at / a.lq;
-  const int h = (int)(bh % a.hq);
-  const int64_t b = bh / a.hq;
-  if (d < a.d) {
-    const float inv = total == 0.f ? 0.f : 1.0f / total;
-    store_output<T>(a, b * a.ob + h * a.oh + (int64_t)i * a.ol + d, out * inv);
-  }
-  if (a.lse && d == 0) a.lse[at] = total == 0.f ? INFINITY : top + log2f(total) - kLift<T>;
+  write_joined<T>(a, at, d, out, top, total);
 }
 
 // --------------------------------------------------------------------------
@@ -594,7 +635,7 @@ __global__ __launch_bounds__(kTile) void document_hulls_kernel(DocArgs a) {
 bool few_rows(const ctmr_masked_attention_desc* d) { return (int64_t)(d->q_heads / d->k_heads) * d->lq <= 32; }
 
 // Parts of the keys where the rows alone do not fill the chip: about 512 workgroups, or 256 of the few-row form, of
-// at least four 64-key tiles each.  From the shape only, so that a shape's sums have one order.  Few rows, bf16, 4 x 8
+// at least four 64-key tiles each (two in fp32).  From the shape only, so that a shape's sums have one order.  Few rows, bf16, 4 x 8
 // key heads of 128 values, 16384 keys (268 MB): 49.7 us with 256 workgroups (one a CU at a time; 5.4 TB/s), 56 with
 // 384, 51 with 512, 58 with 1024.
 int split_count(const ctmr_masked_attention_desc* d) {
@@ -602,7 +643,7 @@ int split_count(const ctmr_masked_attention_desc* d) {
   const int64_t blocks = (int64_t)d->n * (few ? d->k_heads : d->q_heads * ceil_div(d->lq, kRows));
   const int64_t tiles = ceil_div(d->lk, kTile);
   const int64_t want = std::max<int64_t>(1, (few ? 256 : 512) / blocks);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / 4, kMostSplits}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / (d->elem == CTMR_ELEM_F32 ? 2 : 4), kMostSplits}));
 }
 
 template <typename T, int D>
@@ -615,7 +656,11 @@ int launch(const Args& a, bool few, hipStream_t st) {
   const int rc = check_launch("masked_attention");
   if (rc || a.splits == 1) return rc;
   const int64_t rows = (int64_t)a.n * a.hq * a.lq;
-  hipLaunchKernelGGL((attention_join_kernel<T, D>), dim3((unsigned)rows), dim3(kThreads), 0, st, a);
+  if (a.splits <= kFewSplits)
+    hipLaunchKernelGGL((attention_join_few_kernel<T, D>), dim3((unsigned)ceil_div(rows, kThreads / (D / 4))), dim3(kThreads),
+                       0, st, a);
+  else
+    hipLaunchKernelGGL((attention_join_kernel<T, D>), dim3((unsigned)rows), dim3(kThreads), 0, st, a);
   return check_launch("masked_attention_join");
 }
 

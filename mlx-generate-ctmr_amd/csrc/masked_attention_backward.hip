@@ -14,8 +14,9 @@
 // the other in registers: queries stay and keys stream for dq (and delta, which it
 // leaves for the other), keys stay and queries stream for dk and dv.  That is seven
 // products for the five of the formulas (scores and g . v twice), but no atomics:
-// each sum has one order, and the gradients are bit-identical run to run.  p and ds
-// are rounded to the operands' type for their products, half a step of it on each
+// each sum has one order, and the gradients are bit-identical run to run.  Where the
+// blocks of 128 rows do not fill the chip, each block's stream is cut into parts whose
+// fp32 sums a third kernel adds in order.  p and ds are rounded to the operands' type for their products, half a step of it on each
 // term of an fp32 sum.
 //
 // fp16 is refused: without a scale that follows the data ds leaves its range.
@@ -32,17 +33,18 @@ constexpr int kThreads = 256, kWaves = 4;
 constexpr int kOwn = kBlockRows;  // rows that a workgroup keeps in registers
 static_assert(kOwn == 32 * kWaves && kOwn == 4 * kGrain, "32 rows a wave");
 
-// Products of a 32 x 32 block -> log2 scores in units of 1 / c (c returned) and, with a cap, 1 - t^2 in `slope_of`.
-// Row r of a lane is `at` + 8 (r / 4) + r % 4; `x` is where the distance to it is zero.
-template <typename T>
-__device__ __forceinline__ float scores(const Scoring& a, f16v& s, f16v& slope_of, int at, int x) {
+// Products of a 32 x 32 block -> log2 scores in units of 1 / c (c returned).  Row r of a lane is `at` + 8 (r / 4) + r
+// % 4; `x` is where the distance to it is zero.  With CAP g . v - delta, in `ds`, is multiplied by 1 - t^2.  (As a
+// branch on the cap the factor was 48 instructions of 145 a block for every call: the compiler selects what it skips.)
+template <typename T, bool CAP>
+__device__ __forceinline__ float scores(const Scoring& a, f16v& s, f16v& ds, int at, int x) {
   float c = a.scale * kLog2e;
-  if (a.cap > 0.f) {
+  if constexpr (CAP) {
     const float in = a.scale / a.cap;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       s[r] = tanh_of<T>(s[r], in);
-      slope_of[r] = fmaf(-s[r], s[r], 1.0f);
+      ds[r] *= fmaf(-s[r], s[r], 1.0f);
     }
     c = a.cap * kLog2e;
   }
@@ -70,8 +72,14 @@ __device__ __forceinline__ void write_gradient(T* out, const f16v (&g)[ND], floa
     }
 }
 
+// The first of `count` steps of part `split` of `splits`, and the one past its last.
+__device__ __forceinline__ int2 split_steps(int count, int split, int splits) {
+  const int per = (count + splits - 1) / splits, first = min(count, split * per);
+  return {first, min(count, first + per)};
+}
+
 // dq and delta: 128 query rows of a head, key tiles streaming.
-template <typename T, int D>
+template <typename T, int D, bool CAP>
 __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attention_dq_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
@@ -125,7 +133,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
     }
   }
   delta = half_sum(delta);
-  if (real && half == 0) a.delta[stat] = delta;
+  if (real && half == 0 && blockIdx.y == 0) a.delta[stat] = delta;
   if (!a.dq) return;
   const float lse = real ? a.lse[stat] : INFINITY;
   f16v dq[ND];
@@ -133,7 +141,8 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
   for (int n = 0; n < ND; ++n) dq[n] = f16v(0.f);
 
   const Meeting meet = meeting<kWaves>(wave, i0, a.lq, [&](int row) { return key_tiles(a, b, row, prefix, &part); });
-  const int first = meet.all.x, last = meet.all.y;
+  const int2 mine = split_steps(meet.all.y - meet.all.x, blockIdx.y, a.splits);
+  const int first = meet.all.x + mine.x, last = meet.all.x + mine.y;
   Rows<T, kTile> krows, vrows;
   krows.begin(k, a.kl, first * kTile, a.lk, a.d);
   vrows.begin(v, a.vl, first * kTile, a.lk, a.d);
@@ -167,17 +176,16 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
     const bool masked = meet.masked(tile) || (partial && (odd[0] | odd[1]) != 0u);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      f16v s = f16v(0.f), ds = f16v(0.f), slope_of = f16v(1.f);
+      f16v s = f16v(0.f), ds = f16v(-delta);
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
         s = mma<T>(Lds::along(kt, 32 * u, n, la), qf[n], s);
         ds = mma<T>(Lds::along(vt, 32 * u, n, la), gf[n], ds);
       }
       const int at = k0 + 32 * u + 4 * half;
-      const float c = scores<T>(scoring, s, slope_of, at, pos);
+      const float c = scores<T, CAP>(scoring, s, ds, at, pos);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (ds[r] - delta);
-      if (scoring.cap > 0.f) ds *= slope_of;
+      for (int r = 0; r < 16; ++r) ds[r] *= __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse));
       if (masked) {
         // a visible key whose values were zeroed in LDS because they are not finite: no gradient is
         const unsigned set = partial ? odd[u] >> (4 * half) : 0u;
@@ -205,18 +213,21 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
       }
     }
   }
-  if (real)
+  if (!real) return;
+  if (a.splits > 1)
+    write_gradient<float, ND>(a.part + ((int64_t)blockIdx.y * a.n * a.hq * a.lq + stat) * D, dq, 1.0f, D, lane);
+  else
     write_gradient<T, ND>(static_cast<T*>(a.dq) + b * a.dqb + h * a.dqh + (int64_t)i * a.dql, dq, a.scale, a.d, lane);
 }
 
 // dk and dv: 128 keys of a key head, the query tiles of its heads streaming.
-template <typename T, int D>
+template <typename T, int D, bool CAP>
 __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attention_dkv_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
   __shared__ __attribute__((aligned(16))) char qt[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) char gt[kTile * Lds::kRow];
-  __shared__ __attribute__((aligned(16))) float stats[2][kTile];  // lse, delta
+  __shared__ __attribute__((aligned(16))) float stats[2][kTile];  // lse, -delta
   __shared__ __attribute__((aligned(16))) int query_ids[kTile];
   __shared__ unsigned odd[2][2];  // of dout, of q
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
@@ -253,16 +264,19 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
 
   const Meeting meet = meeting<kWaves>(wave, j0, a.lk, [&](int row) { return query_tiles(a, b, row, prefix, &part); });
   const int first = meet.all.x, last = meet.all.y;
-  const int tiles = last - first, steps = tiles * a.group;
+  const int tiles = last - first;
+  const int2 mine = split_steps(tiles * a.group, blockIdx.y, a.splits);
   Stream<T, D, kTile, kThreads> qs, gs;
   float stat = 0.f;
   int other_id = 0;
   Rows<T, kTile> qrows, grows;
-  int fetched = hk * a.group;  // head and tile of the next fetch
-  int at_tile = first;
+  int h = hk * a.group + (tiles > 0 ? mine.x / tiles : 0), tile = first + (tiles > 0 ? mine.x % tiles : 0) - 1;
+  int fetched = h, at_tile = tile + 1;  // head and tile of the next fetch
+  bool begun = false;
   auto fetch = [&]() {
     const int h = fetched, tile = at_tile;
-    if (tile == first) {
+    if (tile == first || !begun) {
+      begun = true;
       qrows.begin(static_cast<const T*>(a.q) + b * a.qb + h * a.qh, a.ql, tile * kTile, a.lq, a.d);
       grows.begin(static_cast<const T*>(a.dout) + b * a.gb + h * a.gh, a.gl, tile * kTile, a.lq, a.d);
     }
@@ -282,9 +296,8 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
     }
   };
   Scoring scoring = scoring_of(a, hk * a.group);
-  if (steps > 0) fetch();
-  int h = hk * a.group, tile = first - 1;
-  for (int step = 0; step < steps; ++step) {
+  if (mine.x < mine.y) fetch();
+  for (int step = mine.x; step < mine.y; ++step) {
     if (++tile == last) {
       tile = first;
       ++h;
@@ -294,7 +307,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
     if (a.slopes) scoring.slope = a.slopes[h];
     __syncthreads();
     if (t < 4) odd[t >> 1][t & 1] = 0u;
-    if (t < 2 * kTile) stats[t / kTile][t % kTile] = stat;
+    if (t < 2 * kTile) stats[t / kTile][t % kTile] = t < kTile ? stat : -stat;
     if (docs && t < kTile) query_ids[t] = other_id;
     if (partial) {
       __syncthreads();
@@ -305,30 +318,34 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
       gs.template store<false>(gt, nullptr, t);
     }
     __syncthreads();
-    if (step + 1 < steps) fetch();
+    if (step + 1 < mine.y) fetch();
     if (meet.skips(tile)) continue;
     const bool masked = meet.masked(tile);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      f16v s = f16v(0.f), ds = f16v(0.f), slope_of = f16v(1.f);
+      f16v s = f16v(0.f), ds;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const f4 delta = *reinterpret_cast<const f4*>(&stats[1][32 * u + 8 * w + 4 * half]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ds[4 * w + r] = delta[r];
+      }
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
         s = mma<T>(Lds::along(qt, 32 * u, n, lane), kf[n], s);
         ds = mma<T>(Lds::along(gt, 32 * u, n, lane), vf[n], ds);
       }
       const int at = i0 + 32 * u + 4 * half;
-      const float c = scores<T>(scoring, s, slope_of, at, j - off);
+      const float c = scores<T, CAP>(scoring, s, ds, at, j - off);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const f4 lse = *reinterpret_cast<const f4*>(&stats[0][32 * u + 8 * w + 4 * half]);
-        const f4 delta = *reinterpret_cast<const f4*>(&stats[1][32 * u + 8 * w + 4 * half]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           s[4 * w + r] = __builtin_amdgcn_exp2f(fmaf(s[4 * w + r], c, -lse[r]));
-          ds[4 * w + r] = s[4 * w + r] * (ds[4 * w + r] - delta[r]);
+          ds[4 * w + r] *= s[4 * w + r];
         }
       }
-      if (scoring.cap > 0.f) ds *= slope_of;
       if (masked) {
         auto hide = [&](int r, bool so) {
           s[r] = so ? 0.f : s[r];
@@ -377,22 +394,96 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
     }
   }
   if (!real) return;
+  if (a.splits > 1) {
+    const int64_t rows = (int64_t)a.n * a.hk * a.lk;
+    float* part = a.part + (2 * blockIdx.y * rows + ((int64_t)b * a.hk + hk) * a.lk + j) * D;
+    if (a.dk) write_gradient<float, ND>(part, dk, 1.0f, D, lane);
+    if (a.dv) write_gradient<float, ND>(part + rows * D, dv, 1.0f, D, lane);
+    return;
+  }
   if (a.dk)
     write_gradient<T, ND>(static_cast<T*>(a.dk) + b * a.dkb + hk * a.dkh + (int64_t)j * a.dkl, dk, a.scale, a.d, lane);
   if (a.dv)
     write_gradient<T, ND>(static_cast<T*>(a.dv) + b * a.dvb + hk * a.dvh + (int64_t)j * a.dvl, dv, 1.0f, a.d, lane);
 }
 
+// Adds the parts of gradients in order: four values a thread.  blockIdx.y: which of up to two gradients.
+struct SumArgs {
+  const float* part;  // (splits, gradients, rows, D)
+  void* out[2];       // null: left out
+  int64_t sb[2], sh[2], sl[2];
+  float scale[2];
+  int rows, heads, length, d, splits, gradients;
+};
+
 template <typename T, int D>
-int launch(const Args& a, hipStream_t st) {
+__global__ __launch_bounds__(kThreads) void attention_sum_kernel(SumArgs a) {
+  const int which = blockIdx.y;
+  const int at = blockIdx.x * kThreads + threadIdx.x, row = at / (D / 4), e = at % (D / 4) * 4;
+  if (row >= a.rows || e >= a.d || !a.out[which]) return;
+  const float* part = a.part + ((int64_t)which * a.rows + row) * D + e;
+  f4 sum = *reinterpret_cast<const f4*>(part);
+#pragma unroll 4
+  for (int s = 1; s < a.splits; ++s) sum += *reinterpret_cast<const f4*>(part + (int64_t)s * a.gradients * a.rows * D);
+  const int i = row % a.length, bh = row / a.length;
+  T* out = static_cast<T*>(a.out[which]) + bh / a.heads * a.sb[which] + bh % a.heads * a.sh[which] + i * a.sl[which];
+  Vec<float, 4> v;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = sum[r] * a.scale[which];
+  store_rounded<T, 4>(out + e, v);
+}
+
+// Parts of each block's stream where the blocks alone do not fill the chip: as many workgroups as it holds at a time
+// (one a CU where a row has 256 bytes or more, else two), of at least `least` steps.  From the shape only, so that a
+// shape's sums have one order.  1500 rows of 8 heads on 2 key heads of 96 values, fp32: 471 us, 2288 in one part; 2000
+// rows of 16 heads on 4 of 128, bf16: 223, 535 in one part; 256 rows of 2 x 16 heads of 32, bf16, whose 64 blocks have
+// 4 steps each: 26 as one part, 31 as two.
+constexpr int kMostParts = 64;
+int part_count(int64_t blocks, int64_t steps, int elem, int head_dim) {
+  const int64_t slots = padded(head_dim) * elem_bytes(elem) >= 256 ? 256 : 512;
+  const int64_t least = elem != CTMR_ELEM_F32 ? 4 : padded(head_dim) >= 64 ? 1 : 2;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({slots / blocks, steps / least, kMostParts}));
+}
+int query_parts(const ctmr_masked_attention_desc* d) {
+  return part_count((int64_t)d->n * d->q_heads * ceil_div(d->lq, kOwn), ceil_div(d->lk, kTile), d->elem, d->head_dim);
+}
+int key_parts(const ctmr_masked_attention_desc* d) {
+  return part_count((int64_t)d->n * d->k_heads * ceil_div(d->lk, kOwn),
+                    ceil_div(d->lq, kTile) * (d->q_heads / d->k_heads), d->elem, d->head_dim);
+}
+
+// Bytes of delta in the workspace; the parts follow, dq's and then, in the same place, dk's and dv's.
+int64_t delta_bytes(const ctmr_masked_attention_desc* d) {
+  return ceil_div((int64_t)d->n * d->q_heads * d->lq * 4, 16) * 16;
+}
+
+template <typename T, int D, bool CAP>
+int launch(Args a, int qparts, int kparts, hipStream_t st) {
   const unsigned parts = a.qdoc.ids ? 2u : 1u;
-  hipLaunchKernelGGL((attention_dq_kernel<T, D>), dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kOwn) * parts), dim3(kThreads), 0,
-                     st, a);
-  const int rc = check_launch("attention_dq");
-  if (rc || (!a.dk && !a.dv)) return rc;
-  hipLaunchKernelGGL((attention_dkv_kernel<T, D>), dim3(a.n * a.hk * (unsigned)ceil_div(a.lk, kOwn) * parts), dim3(kThreads),
-                     0, st, a);
-  return check_launch("attention_dkv");
+  a.splits = a.dq ? qparts : 1;
+  hipLaunchKernelGGL((attention_dq_kernel<T, D, CAP>), dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kOwn) * parts, a.splits),
+                     dim3(kThreads), 0, st, a);
+  int rc = check_launch("attention_dq");
+  if (rc) return rc;
+  if (a.splits > 1) {
+    SumArgs s = {a.part, {a.dq, nullptr}, {a.dqb, 0}, {a.dqh, 0}, {a.dql, 0}, {a.scale, 0.f},
+                 a.n * a.hq * a.lq, a.hq, a.lq, a.d, a.splits, 1};
+    hipLaunchKernelGGL((attention_sum_kernel<T, D>), dim3((unsigned)ceil_div((int64_t)s.rows * (D / 4), kThreads)),
+                       dim3(kThreads), 0, st, s);
+    rc = check_launch("attention_sum");
+    if (rc) return rc;
+  }
+  if (!a.dk && !a.dv) return rc;
+  a.splits = kparts;
+  hipLaunchKernelGGL((attention_dkv_kernel<T, D, CAP>), dim3(a.n * a.hk * (unsigned)ceil_div(a.lk, kOwn) * parts, a.splits),
+                     dim3(kThreads), 0, st, a);
+  rc = check_launch("attention_dkv");
+  if (rc || a.splits == 1) return rc;
+  SumArgs s = {a.part, {a.dk, a.dv}, {a.dkb, a.dvb}, {a.dkh, a.dvh}, {a.dkl, a.dvl}, {a.scale, 1.0f},
+               a.n * a.hk * a.lk, a.hk, a.lk, a.d, a.splits, 2};
+  hipLaunchKernelGGL((attention_sum_kernel<T, D>), dim3((unsigned)ceil_div((int64_t)s.rows * (D / 4), kThreads), 2),
+                     dim3(kThreads), 0, st, s);
+  return check_launch("attention_sum");
 }
 
 }  // namespace
@@ -406,7 +497,11 @@ extern "C" {
 
 int64_t ctmr_masked_attention_backward_workspace_bytes(const ctmr_masked_attention_desc* d) {
   const int rc = check_desc(d);
-  return rc ? rc : (int64_t)d->n * d->q_heads * d->lq * 4;
+  if (rc) return rc;
+  const int64_t q = query_parts(d), k = key_parts(d);
+  const int64_t qbytes = q > 1 ? q * d->n * d->q_heads * d->lq * padded(d->head_dim) * 4 : 0;
+  const int64_t kbytes = k > 1 ? 2 * k * d->n * d->k_heads * d->lk * padded(d->head_dim) * 4 : 0;
+  return delta_bytes(d) + std::max(qbytes, kbytes);
 }
 
 int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const void* q, const void* k, const void* v,
@@ -439,20 +534,26 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const vo
   Args a = make_args(d, q, k, v, slopes, prefixes, plan);
   a.out = const_cast<void*>(out), a.rest = const_cast<void*>(rest), a.lse = const_cast<float*>(lse), a.dout = dout;
   a.dq = dq, a.dk = dk, a.dv = dv, a.delta = (float*)workspace;
+  a.part = (float*)((char*)workspace + delta_bytes(d));
   a.ob = d->out_strides[0], a.oh = d->out_strides[1], a.ol = d->out_strides[2];
   a.gb = dout_strides[0], a.gh = dout_strides[1], a.gl = row_stride(dout_strides, d->lq, d->head_dim);
   if (dq) a.dqb = dq_strides[0], a.dqh = dq_strides[1], a.dql = dq_strides[2];
   if (dk) a.dkb = dk_strides[0], a.dkh = dk_strides[1], a.dkl = dk_strides[2];
   if (dv) a.dvb = dv_strides[0], a.dvh = dv_strides[1], a.dvl = dv_strides[2];
+  const int qparts = query_parts(d), kparts = key_parts(d);
   hipStream_t st = (hipStream_t)stream;
-#define CTMR_ATTENTION_CASE(T)              \
+  const bool cap = d->softcap > 0.f;
+#define CTMR_ATTENTION_CASE(T, D) \
+  return cap ? launch<T, D, true>(a, qparts, kparts, st) : launch<T, D, false>(a, qparts, kparts, st);
+#define CTMR_ATTENTION_TYPE(T)              \
   switch (padded(d->head_dim)) {            \
-    case 32: return launch<T, 32>(a, st);   \
-    case 64: return launch<T, 64>(a, st);   \
-    default: return launch<T, 128>(a, st);  \
+    case 32: CTMR_ATTENTION_CASE(T, 32)     \
+    case 64: CTMR_ATTENTION_CASE(T, 64)     \
+    default: CTMR_ATTENTION_CASE(T, 128)    \
   }
-  if (d->elem == CTMR_ELEM_F32) CTMR_ATTENTION_CASE(float)
-  CTMR_ATTENTION_CASE(__bf16)
+  if (d->elem == CTMR_ELEM_F32) CTMR_ATTENTION_TYPE(float)
+  CTMR_ATTENTION_TYPE(__bf16)
+#undef CTMR_ATTENTION_TYPE
 #undef CTMR_ATTENTION_CASE
 }
 
