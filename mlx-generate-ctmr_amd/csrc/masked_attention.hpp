@@ -167,6 +167,20 @@ struct Rows {
   }
 };
 
+// Every thread's loads into LDS are there, and the reads before it are done.
+__device__ __forceinline__ void arrive() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  __syncthreads();
+}
+
+// A wave's 64 floats from place `first` of `count` straight into LDS, zeros past the end.  Complete after arrive().
+__device__ __forceinline__ void load_floats(float* to, const float* from, int first, int count, int lane) {
+  typedef __attribute__((address_space(3))) void lds_void;
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(from + first), (short)0, max(min(count - first, 64), 0) * 4, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)to, 4, lane * 4, 0, 0, 0);
+}
+
 template <typename T, int D, int ROWS, int THREADS>
 struct Stream {
   typedef Tile<T, D> Lds;
@@ -176,6 +190,25 @@ struct Stream {
 
   static __device__ __forceinline__ int row_of(int i, int t) { return (i * THREADS + t) / Lds::kPieces; }
   static __device__ __forceinline__ int piece_of(int t) { return t % Lds::kPieces; }  // THREADS is a multiple
+
+  // Whether 16 bytes hold finite values only; those that are not become zeros.
+  static __device__ __forceinline__ bool finite(u4& v) {
+    bool all = true;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      unsigned u = v[w];
+      if constexpr (sizeof(T) == 4) {
+        if ((u & 0x7f800000u) == 0x7f800000u) u = 0u;
+      } else {
+        constexpr unsigned kExp = std::is_same_v<T, __bf16> ? 0x7f80u : 0x7c00u;
+        if ((u & kExp) == kExp) u &= 0xffff0000u;
+        if ((u & (kExp << 16)) == (kExp << 16)) u &= 0x0000ffffu;
+      }
+      all &= u == v[w];
+      v[w] = u;
+    }
+    return all;
+  }
 
   // Columns past the head's values have an offset past every range, 2^30 + 2^29 and more.
   __device__ __forceinline__ void fetch(const Rows<T, ROWS>& rows, int t) {
@@ -187,6 +220,33 @@ struct Stream {
       piece[i] = __builtin_amdgcn_raw_buffer_load_b128(r, (int)(off + i * (THREADS / Lds::kPieces) * rows.row), 0, 0);
   }
 
+  // Straight into LDS: a wave's lanes write 16 bytes each side by side, so the permutation is done on the memory's side.
+  // Complete after arrive().
+  static __device__ __forceinline__ void load(char* tile, const Rows<T, ROWS>& rows, int t) {
+    typedef __attribute__((address_space(3))) void lds_void;
+    const __amdgpu_buffer_rsrc_t r = rows.buffer();
+    char* wave = tile + __builtin_amdgcn_readfirstlane(t & ~63) * 16;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int row = row_of(i, t), piece = piece_of(t) ^ Lds::mix(row);
+      const unsigned off = piece * 16 < rows.last ? row * rows.row + piece * 16 : 0x60000000u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(wave + i * THREADS * 16), 16, (int)off, 0, 0, 0);
+    }
+  }
+
+  // Of a tile in LDS: values that are not finite become zeros and their rows' bits are set in odd[ROWS / 32].
+  static __device__ __forceinline__ void clean(char* tile, unsigned* odd, int t) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      u4* at = reinterpret_cast<u4*>(tile + (i * THREADS + t) * 16);
+      u4 v = *at;
+      if (finite(v)) continue;
+      *at = v;
+      const int row = row_of(i, t);
+      atomicOr(&odd[row >> 5], 1u << (row & 31));
+    }
+  }
+
   // CLEAN: values that are not finite become zeros and their rows' bits are set in odd[ROWS / 32].
   template <bool CLEAN>
   __device__ __forceinline__ void store(char* tile, unsigned* odd, int t) {
@@ -194,21 +254,7 @@ struct Stream {
     for (int i = 0; i < kPieces; ++i) {
       const int row = row_of(i, t);
       if constexpr (CLEAN) {
-        bool found = false;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          unsigned u = piece[i][w];
-          if constexpr (sizeof(T) == 4) {
-            if ((u & 0x7f800000u) == 0x7f800000u) u = 0u;
-          } else {
-            constexpr unsigned kExp = std::is_same_v<T, __bf16> ? 0x7f80u : 0x7c00u;
-            if ((u & kExp) == kExp) u &= 0xffff0000u;
-            if ((u & (kExp << 16)) == (kExp << 16)) u &= 0x0000ffffu;
-          }
-          found |= u != piece[i][w];
-          piece[i][w] = u;
-        }
-        if (found) atomicOr(&odd[row >> 5], 1u << (row & 31));
+        if (!finite(piece[i])) atomicOr(&odd[row >> 5], 1u << (row & 31));
       }
       *reinterpret_cast<u4*>(tile + Lds::at(row, piece_of(t))) = piece[i];
     }
@@ -243,7 +289,7 @@ struct Args {
   float* part;            // split keys: (splits, n, hq, lq, D) sums, then (.., 2) maximum and total
   const void* dout;
   void *dq, *dk, *dv;
-  float* delta;           // (n, hq, lq) sum_d dout out
+  float* delta;           // (n, hq, lq) -sum_d dout out
   const float* slopes;    // (hq)
   const int* prefixes;    // (n), or null with `prefix`
   Side qdoc, kdoc;        // ids null: no documents

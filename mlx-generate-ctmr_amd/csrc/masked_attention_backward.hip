@@ -78,14 +78,21 @@ __device__ __forceinline__ int2 split_steps(int count, int split, int splits) {
   return {first, min(count, first + per)};
 }
 
+// Waves a SIMD that the registers are kept for.
+template <typename T, int D>
+constexpr int dq_waves() {
+  return D * sizeof(T) >= 512 ? 1 : D * sizeof(T) == 128 ? 3 : 2;
+}
+
 // dq and delta: 128 query rows of a head, key tiles streaming.
 template <typename T, int D, bool CAP>
-__global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attention_dq_kernel(Args a) {
+__global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
-  __shared__ __attribute__((aligned(16))) char kt[kTile * Lds::kRow];
-  __shared__ __attribute__((aligned(16))) char vt[kTile * Lds::kRow];
-  __shared__ __attribute__((aligned(16))) int key_ids[kTile];
+  __shared__ __attribute__((aligned(16))) char kt0[kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char vt0[kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char kt1[kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char vt1[kTile * Lds::kRow];
   __shared__ unsigned odd[2];
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -133,7 +140,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
     }
   }
   delta = half_sum(delta);
-  if (real && half == 0 && blockIdx.y == 0) a.delta[stat] = delta;
+  if (real && half == 0 && blockIdx.y == 0) a.delta[stat] = -delta;
   if (!a.dq) return;
   const float lse = real ? a.lse[stat] : INFINITY;
   f16v dq[ND];
@@ -146,32 +153,26 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
   Rows<T, kTile> krows, vrows;
   krows.begin(k, a.kl, first * kTile, a.lk, a.d);
   vrows.begin(v, a.vl, first * kTile, a.lk, a.d);
-  Stream<T, D, kTile, kThreads> ks, vs;
-  int other_id = 0;
-  auto fetch = [&](int tile) {
-    ks.fetch(krows, t);
-    vs.fetch(vrows, t);
+  typedef Stream<T, D, kTile, kThreads> Load;
+  auto fetch = [&](char* kt, char* vt) {
+    Load::load(kt, krows, t);
+    Load::load(vt, vrows, t);
     krows.next();
     vrows.next();
-    if (docs && t < kTile) other_id = ids[tile * kTile + t];
   };
-  if (first < last) fetch(first);
-  for (int tile = first; tile < last; ++tile) {
+  // One tile, while the next one is on its way into the other pair of arrays.
+  auto step = [&](int tile, char* kt, char* vt, char* next_kt, char* next_vt) {
     const int k0 = tile * kTile;
     const bool partial = meet.partial(tile);
-    __syncthreads();  // the last tile is read
-    if (t < 2) odd[t] = 0u;
-    if (docs && t < kTile) key_ids[t] = other_id;
+    arrive();
+    if (tile + 1 < last) fetch(next_kt, next_vt);
     if (partial) {
+      if (t < 2) odd[t] = 0u;
       __syncthreads();
-      ks.template store<true>(kt, odd, t);
-    } else {
-      ks.template store<false>(kt, nullptr, t);
+      Load::clean(kt, odd, t);
+      __syncthreads();
     }
-    vs.template store<false>(vt, nullptr, t);
-    __syncthreads();
-    if (tile + 1 < last) fetch(tile + 1);
-    if (meet.skips(tile)) continue;
+    if (meet.skips(tile)) return;
     const int la = fresh<D == 128 && sizeof(T) == 2>(lane);
     const bool masked = meet.masked(tile) || (partial && (odd[0] | odd[1]) != 0u);
 #pragma unroll
@@ -195,7 +196,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
         if (docs)
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const int4 other = *reinterpret_cast<const int4*>(key_ids + 32 * u + 4 * half + 8 * w);
+            const int4 other = *reinterpret_cast<const int4*>(ids + k0 + 32 * u + 4 * half + 8 * w);
             ds[4 * w] = other.x != id ? 0.f : ds[4 * w];
             ds[4 * w + 1] = other.y != id ? 0.f : ds[4 * w + 1];
             ds[4 * w + 2] = other.z != id ? 0.f : ds[4 * w + 2];
@@ -212,6 +213,11 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
         for (int n = 0; n < ND; ++n) dq[n] = mma<T>(Lds::down(kt, 32 * u + 16 * w, n, la), f, dq[n]);
       }
     }
+  };
+  if (first < last) fetch(kt0, vt0);
+  for (int tile = first; tile < last; tile += 2) {
+    step(tile, kt0, vt0, kt1, vt1);
+    if (tile + 1 < last) step(tile + 1, kt1, vt1, kt0, vt0);
   }
   if (!real) return;
   if (a.splits > 1)
@@ -220,15 +226,22 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
     write_gradient<T, ND>(static_cast<T*>(a.dq) + b * a.dqb + h * a.dqh + (int64_t)i * a.dql, dq, a.scale, a.d, lane);
 }
 
+template <typename T, int D>
+constexpr int dkv_waves() {
+  return D * sizeof(T) >= 256 ? 1 : 2;
+}
+
 // dk and dv: 128 keys of a key head, the query tiles of its heads streaming.
 template <typename T, int D, bool CAP>
-__global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attention_dkv_kernel(Args a) {
+__global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
-  __shared__ __attribute__((aligned(16))) char qt[kTile * Lds::kRow];
-  __shared__ __attribute__((aligned(16))) char gt[kTile * Lds::kRow];
-  __shared__ __attribute__((aligned(16))) float stats[2][kTile];  // lse, -delta
-  __shared__ __attribute__((aligned(16))) int query_ids[kTile];
+  __shared__ __attribute__((aligned(16))) char qt0[kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char gt0[kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char qt1[kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char gt1[kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) float stats0[2 * kTile];  // lse, -delta
+  __shared__ __attribute__((aligned(16))) float stats1[2 * kTile];
   __shared__ unsigned odd[2][2];  // of dout, of q
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -266,38 +279,32 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
   const int first = meet.all.x, last = meet.all.y;
   const int tiles = last - first;
   const int2 mine = split_steps(tiles * a.group, blockIdx.y, a.splits);
-  Stream<T, D, kTile, kThreads> qs, gs;
-  float stat = 0.f;
-  int other_id = 0;
+  typedef Stream<T, D, kTile, kThreads> Load;
   Rows<T, kTile> qrows, grows;
   int h = hk * a.group + (tiles > 0 ? mine.x / tiles : 0), tile = first + (tiles > 0 ? mine.x % tiles : 0) - 1;
   int fetched = h, at_tile = tile + 1;  // head and tile of the next fetch
   bool begun = false;
-  auto fetch = [&]() {
-    const int h = fetched, tile = at_tile;
-    if (tile == first || !begun) {
+  auto fetch = [&](char* qt, char* gt, float* stats) {
+    if (at_tile == first || !begun) {
       begun = true;
-      qrows.begin(static_cast<const T*>(a.q) + b * a.qb + h * a.qh, a.ql, tile * kTile, a.lq, a.d);
-      grows.begin(static_cast<const T*>(a.dout) + b * a.gb + h * a.gh, a.gl, tile * kTile, a.lq, a.d);
+      qrows.begin(static_cast<const T*>(a.q) + b * a.qb + fetched * a.qh, a.ql, at_tile * kTile, a.lq, a.d);
+      grows.begin(static_cast<const T*>(a.dout) + b * a.gb + fetched * a.gh, a.gl, at_tile * kTile, a.lq, a.d);
     }
-    qs.fetch(qrows, t);
-    gs.fetch(grows, t);
+    Load::load(qt, qrows, t);
+    Load::load(gt, grows, t);
     qrows.next();
     grows.next();
+    // Rows past the end have zeros everywhere, so their p, whatever it is, adds nothing.
+    if (wave < 2) load_floats(stats + wave * kTile, (wave == 0 ? a.lse : a.delta) + ((int64_t)b * a.hq + fetched) * a.lq,
+                              at_tile * kTile, a.lq, lane);
     if (++at_tile == last) {
       at_tile = first;
       ++fetched;
     }
-    const int i = tile * kTile + (t & (kTile - 1));
-    if (t < 2 * kTile) {
-      const float* from = t < kTile ? a.lse : a.delta;
-      stat = i < a.lq ? from[((int64_t)b * a.hq + h) * a.lq + i] : t < kTile ? INFINITY : 0.f;
-      if (docs) other_id = ids[i];
-    }
   };
   Scoring scoring = scoring_of(a, hk * a.group);
-  if (mine.x < mine.y) fetch();
-  for (int step = mine.x; step < mine.y; ++step) {
+  // One tile, while the next one is on its way into the other arrays.
+  auto step = [&](bool more, char* qt, char* gt, float* stats, char* next_qt, char* next_gt, float* next_stats) {
     if (++tile == last) {
       tile = first;
       ++h;
@@ -305,28 +312,23 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
     const int i0 = tile * kTile;
     const bool partial = meet.partial(tile);
     if (a.slopes) scoring.slope = a.slopes[h];
-    __syncthreads();
-    if (t < 4) odd[t >> 1][t & 1] = 0u;
-    if (t < 2 * kTile) stats[t / kTile][t % kTile] = t < kTile ? stat : -stat;
-    if (docs && t < kTile) query_ids[t] = other_id;
+    arrive();
+    if (more) fetch(next_qt, next_gt, next_stats);
     if (partial) {
+      if (t < 4) odd[t >> 1][t & 1] = 0u;
       __syncthreads();
-      qs.template store<true>(qt, odd[1], t);
-      gs.template store<true>(gt, odd[0], t);
-    } else {
-      qs.template store<false>(qt, nullptr, t);
-      gs.template store<false>(gt, nullptr, t);
+      Load::clean(qt, odd[1], t);
+      Load::clean(gt, odd[0], t);
+      __syncthreads();
     }
-    __syncthreads();
-    if (step + 1 < mine.y) fetch();
-    if (meet.skips(tile)) continue;
+    if (meet.skips(tile)) return;
     const bool masked = meet.masked(tile);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f16v s = f16v(0.f), ds;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const f4 delta = *reinterpret_cast<const f4*>(&stats[1][32 * u + 8 * w + 4 * half]);
+        const f4 delta = *reinterpret_cast<const f4*>(stats + kTile + 32 * u + 8 * w + 4 * half);
 #pragma unroll
         for (int r = 0; r < 4; ++r) ds[4 * w + r] = delta[r];
       }
@@ -339,7 +341,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
       const float c = scores<T, CAP>(scoring, s, ds, at, j - off);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const f4 lse = *reinterpret_cast<const f4*>(&stats[0][32 * u + 8 * w + 4 * half]);
+        const f4 lse = *reinterpret_cast<const f4*>(stats + 32 * u + 8 * w + 4 * half);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           s[4 * w + r] = __builtin_amdgcn_exp2f(fmaf(s[4 * w + r], c, -lse[r]));
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
         if (docs)
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const int4 other = *reinterpret_cast<const int4*>(query_ids + 32 * u + 4 * half + 8 * w);
+            const int4 other = *reinterpret_cast<const int4*>(ids + i0 + 32 * u + 4 * half + 8 * w);
             hide(4 * w, other.x != id);
             hide(4 * w + 1, other.y != id);
             hide(4 * w + 2, other.z != id);
@@ -379,8 +381,8 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
         for (int r = 0; r < 32; ++r) {
           if (((odd[0][u] >> r) & 1u) == 0u) continue;
           const int i = i0 + 32 * u + r;
-          if (j >= limit_of(a, i, prefix) || (docs && query_ids[32 * u + r] != id)) continue;
-          const T* row = gh + (int64_t)(i0 + 32 * u + r) * a.gl;
+          if (j >= limit_of(a, i, prefix) || (docs && ids[i] != id)) continue;
+          const T* row = gh + (int64_t)i * a.gl;
 #pragma unroll
           for (int n = 0; n < ND; ++n)
 #pragma unroll
@@ -392,6 +394,11 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) >= 256 ? 1 : 2) void attent
         }
       }
     }
+  };
+  if (mine.x < mine.y) fetch(qt0, gt0, stats0);
+  for (int s = mine.x; s < mine.y; s += 2) {
+    step(s + 1 < mine.y, qt0, gt0, stats0, qt1, gt1, stats1);
+    if (s + 1 < mine.y) step(s + 2 < mine.y, qt1, gt1, stats1, qt0, gt0, stats0);
   }
   if (!real) return;
   if (a.splits > 1) {
