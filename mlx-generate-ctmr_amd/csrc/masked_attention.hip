@@ -119,6 +119,7 @@ __device__ __forceinline__ bool softmax_blocks(f16v (&s)[NB], Frag<T> (&p)[NB][2
 template <typename T, int ND>
 __device__ void add_odd_values(const Args& a, f16v (&o)[ND], const T* v, int k0, unsigned lo, unsigned hi,
                                const RowMask& m, const int* ids, int lane) {
+  const int half = fresh<true>(lane) >> 5;  // else the offsets below stay in registers over the caller's loop
   for (int j = 0; j < kTile; ++j) {
     if (((j < 32 ? lo >> j : hi >> (j - 32)) & 1u) == 0u) continue;
     const int key = k0 + j;
@@ -129,7 +130,7 @@ __device__ void add_odd_values(const Args& a, f16v (&o)[ND], const T* v, int k0,
     for (int b = 0; b < ND; ++b)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int d = 32 * b + 8 * g + 4 * (lane >> 5);  // results past the head's values are not stored
+        const int d = 32 * b + 8 * g + 4 * half;  // results past the head's values are not stored
         const Vec<float, 4> value = load_as_float<T, 4>(row + min(d, a.d - 4));
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[b][4 * g + r] += fabsf(value[r]) < INFINITY ? 0.f : value[r];
@@ -194,16 +195,17 @@ __device__ __forceinline__ void write_row(const Args& a, const f16v (&o)[ND], fl
 }
 
 // The tiled form: a workgroup of four waves takes 128 query rows of a head, 32 a
-// wave, and streams K and V through LDS in 64-key tiles, double-buffered: the loads
-// of the next tile are in flight while the current one is multiplied.
+// wave, and streams K and V through LDS in 64-key tiles: the next tile is loaded
+// straight into a second pair of arrays while the current one is multiplied.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void attention_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
-  __shared__ __attribute__((aligned(16))) char kt[2][kTile * Lds::kRow];
-  __shared__ __attribute__((aligned(16))) char vt[2][kTile * Lds::kRow];
-  __shared__ __attribute__((aligned(16))) int key_ids[2][kTile];
-  __shared__ unsigned odd[3][2];
+  __shared__ __attribute__((aligned(16))) char kt0[kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char vt0[kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char kt1[kTile * Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char vt1[kTile * Lds::kRow];
+  __shared__ unsigned odd[2];
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int blocks = (a.lq + kRows - 1) / kRows;
@@ -243,75 +245,63 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
   Rows<T, kTile> krows, vrows;
   krows.begin(k, a.kl, first * kTile, a.lk, a.d);
   vrows.begin(v, a.vl, first * kTile, a.lk, a.d);
-  Stream<T, D, kTile, kThreads> ks, vs;
-  bool partial = false;  // of the tile in flight: some row of the workgroup has a masked key in it
-  int id = 0;
-  auto fetch = [&](int tile) {
-    ks.fetch(krows, t);
-    vs.fetch(vrows, t);
+  typedef Stream<T, D, kTile, kThreads> Load;
+  auto fetch = [&](char* kt, char* vt) {
+    Load::load(kt, krows, t);
+    Load::load(vt, vrows, t);
     krows.next();
     vrows.next();
-    partial = meet.partial(tile);
-    if (docs && t < kTile) id = ids[tile * kTile + t];
   };
-  auto stage = [&](int buf, int slot) {
-    ks.template store<false>(kt[buf], nullptr, t);
-    if (partial) vs.template store<true>(vt[buf], odd[slot], t);
-    else vs.template store<false>(vt[buf], nullptr, t);
-    if (docs && t < kTile) key_ids[buf][t] = id;
-  };
-  if (t < 6) odd[t / 2][t % 2] = 0u;
-  if (first < last) {
-    fetch(first);
-    __syncthreads();
-    stage(0, 0);
-  }
-  int slot = 0;
-  for (int tile = first; tile < last; ++tile) {
-    const int buf = (tile - first) & 1, k0 = tile * kTile;
-    const bool now = partial, more = tile + 1 < last;
-    if (more) fetch(tile + 1);
-    __syncthreads();
-    if (!meet.skips(tile)) {
-      const int at = fresh<D == 128>(lane);
-      f16v s[2] = {f16v(0.f), f16v(0.f)};
-#pragma unroll
-      for (int n = 0; n < NK; ++n)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) s[u] = mma<T>(Lds::along(kt[buf], 32 * u, n, at), qf[n], s[u]);
-      // V's first operands are read before the softmax, which covers the latency, as far as registers go.
-      constexpr int kEarly = sizeof(T) == 4 ? 0 : D == 128 ? 0 : 2;  // contraction steps
-      Frag<T> vf[2][ND];
-#pragma unroll
-      for (int w = 0; w < kEarly; ++w)
-#pragma unroll
-        for (int n = 0; n < ND; ++n) vf[w][n] = Lds::down(vt[buf], 16 * w, n, at);
-      const int* tile_ids = docs ? key_ids[buf] : nullptr;
-      const float c = score_blocks<T, 2>(scoring, s, k0, pos, meet.masked(tile), mask, tile_ids, lane);
-      float alpha;
-      Frag<T> p[2][2];
-      if (softmax_blocks<T, 2>(s, p, c, m, l, alpha)) {
-#pragma unroll
-        for (int n = 0; n < ND; ++n) o[n] *= alpha;
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-#pragma unroll
-          for (int n = 0; n < ND; ++n)
-            o[n] = mma<T>(u == 0 && w < kEarly ? vf[w][n] : Lds::down(vt[buf], 32 * u + 16 * w, n, at), p[u][w], o[n]);
-      if (now) {
-        const unsigned lo = odd[slot][0], hi = odd[slot][1];
-        if (lo | hi) add_odd_values<T, ND>(a, o, v, k0, lo, hi, mask, tile_ids, lane);
-      }
+  // One tile, while the next one is on its way into the other pair of arrays.
+  auto step = [&](int tile, char* kt, char* vt, char* next_kt, char* next_vt) {
+    const int k0 = tile * kTile;
+    const bool partial = meet.partial(tile);  // some row of the workgroup has a masked key in it
+    arrive();
+    if (tile + 1 < last) fetch(next_kt, next_vt);
+    if (partial) {
+      if (t < 2) odd[t] = 0u;
+      __syncthreads();
+      Load::clean(vt, odd, t);
+      __syncthreads();
     }
-    // Three slots: this tile's is read until the next barrier, the next tile's is set from here on, the one after
-    // that was read before this tile's barrier.
-    const int next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
-    if (t < 2) odd[after][t] = 0u;
-    if (more) stage(buf ^ 1, next);
-    slot = next;
+    if (meet.skips(tile)) return;
+    const int at = fresh<D == 128>(lane);
+    f16v s[2] = {f16v(0.f), f16v(0.f)};
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) s[u] = mma<T>(Lds::along(kt, 32 * u, n, at), qf[n], s[u]);
+    // V's first operands are read before the softmax, which covers the latency, as far as registers go.
+    constexpr int kEarly = sizeof(T) == 4 ? 0 : D == 128 ? 0 : 2;  // contraction steps
+    Frag<T> vf[2][ND];
+#pragma unroll
+    for (int w = 0; w < kEarly; ++w)
+#pragma unroll
+      for (int n = 0; n < ND; ++n) vf[w][n] = Lds::down(vt, 16 * w, n, at);
+    const int* tile_ids = docs ? ids + k0 : nullptr;
+    const float c = score_blocks<T, 2>(scoring, s, k0, pos, meet.masked(tile), mask, tile_ids, lane);
+    float alpha;
+    Frag<T> p[2][2];
+    if (softmax_blocks<T, 2>(s, p, c, m, l, alpha)) {
+#pragma unroll
+      for (int n = 0; n < ND; ++n) o[n] *= alpha;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+          o[n] = mma<T>(u == 0 && w < kEarly ? vf[w][n] : Lds::down(vt, 32 * u + 16 * w, n, at), p[u][w], o[n]);
+    if (partial) {
+      const unsigned lo = odd[0], hi = odd[1];
+      if (lo | hi) add_odd_values<T, ND>(a, o, v, k0, lo, hi, mask, tile_ids, lane);
+    }
+  };
+  if (first < last) fetch(kt0, vt0);
+  for (int tile = first; tile < last; tile += 2) {
+    step(tile, kt0, vt0, kt1, vt1);
+    if (tile + 1 < last) step(tile + 1, kt1, vt1, kt0, vt0);
   }
   l = half_sum(l);
   if (mine) write_row<T, ND>(a, o, m, l, b, h, i, blockIdx.y, lane);

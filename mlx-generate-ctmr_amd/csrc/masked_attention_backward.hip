@@ -78,7 +78,8 @@ __device__ __forceinline__ int2 split_steps(int count, int split, int splits) {
   return {first, min(count, first + per)};
 }
 
-// Waves a SIMD that the registers are kept for.
+// Waves a SIMD that the registers are kept for.  (64-wide 16-bit heads with three for dk and dv spill 20 registers: 577
+// us for 2 x 16 heads of 4096 rows, 505 with two.)
 template <typename T, int D>
 constexpr int dq_waves() {
   return D * sizeof(T) >= 512 ? 1 : D * sizeof(T) == 128 ? 3 : 2;
@@ -322,6 +323,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
       __syncthreads();
     }
     if (meet.skips(tile)) return;
+    const int la = fresh<D == 128>(lane);
     const bool masked = meet.masked(tile);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -334,8 +336,8 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
       }
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
-        s = mma<T>(Lds::along(qt, 32 * u, n, lane), kf[n], s);
-        ds = mma<T>(Lds::along(gt, 32 * u, n, lane), vf[n], ds);
+        s = mma<T>(Lds::along(qt, 32 * u, n, la), kf[n], s);
+        ds = mma<T>(Lds::along(gt, 32 * u, n, la), vf[n], ds);
       }
       const int at = i0 + 32 * u + 4 * half;
       const float c = scores<T, CAP>(scoring, s, ds, at, j - off);
@@ -371,12 +373,13 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
         const Frag<T> p = result_frag<T>(s, w), f = result_frag<T>(ds, w);
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
-          dv[n] = mma<T>(Lds::down(gt, 32 * u + 16 * w, n, lane), p, dv[n]);
-          dk[n] = mma<T>(Lds::down(qt, 32 * u + 16 * w, n, lane), f, dk[n]);
+          dv[n] = mma<T>(Lds::down(gt, 32 * u + 16 * w, n, la), p, dv[n]);
+          dk[n] = mma<T>(Lds::down(qt, 32 * u + 16 * w, n, la), f, dk[n]);
         }
       }
       if (partial && odd[0][u]) {
         // Values of dout that were zeroed in LDS, for the keys that their rows see.
+        const int odd_half = fresh<true>(lane) >> 5;  // else the offsets below stay in registers over the loop
         const T* gh = static_cast<const T*>(a.dout) + b * a.gb + h * a.gh;
         for (int r = 0; r < 32; ++r) {
           if (((odd[0][u] >> r) & 1u) == 0u) continue;
@@ -387,7 +390,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
           for (int n = 0; n < ND; ++n)
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              const Vec<float, 4> value = load_as_float<T, 4>(row + min(32 * n + 8 * w + 4 * half, a.d - 4));
+              const Vec<float, 4> value = load_as_float<T, 4>(row + min(32 * n + 8 * w + 4 * odd_half, a.d - 4));
 #pragma unroll
               for (int e = 0; e < 4; ++e) dv[n][4 * w + e] += fabsf(value[e]) < INFINITY ? 0.f : value[e];
             }
