@@ -334,10 +334,45 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
 #pragma unroll
         for (int r = 0; r < 4; ++r) ds[4 * w + r] = delta[r];
       }
+      // With one wave a SIMD nothing else covers the latency of the reads: they are issued a group ahead of their
+      // products, the first operands of the gradients before the scores are worked on.  (Left to itself the compiler
+      // reads one operand, waits for it and multiplies.)
+      constexpr bool kAhead = sizeof(T) == 2 && D == 128;
+      Frag<T> along[2][NK], down[2][ND][2];
+      auto read_along = [&](int n) {
+        along[0][n] = Lds::along(qt, 32 * u, n, la);
+        along[1][n] = Lds::along(gt, 32 * u, n, la);
+      };
+      auto read_down = [&](int w) {
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+          down[0][n][w] = Lds::down(gt, 32 * u + 16 * w, n, la);
+          down[1][n][w] = Lds::down(qt, 32 * u + 16 * w, n, la);
+        }
+      };
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int n = 0; n < NK / 2; ++n) read_along(n);
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
-        s = mma<T>(Lds::along(qt, 32 * u, n, la), kf[n], s);
-        ds = mma<T>(Lds::along(gt, 32 * u, n, la), vf[n], ds);
+        if constexpr (kAhead) {
+          if (n == 0) {
+#pragma unroll
+            for (int e = NK / 2; e < NK; ++e) read_along(e);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (n == NK / 2) {
+            __builtin_amdgcn_sched_barrier(0);
+            read_down(0);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        } else {
+          read_along(n);
+        }
+        s = mma<T>(along[0][n], kf[n], s);
+        ds = mma<T>(along[1][n], vf[n], ds);
       }
       const int at = i0 + 32 * u + 4 * half;
       const float c = scores<T, CAP>(scoring, s, ds, at, j - off);
@@ -368,13 +403,18 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
 #pragma unroll
           for (int r = 0; r < 16; ++r) hide(r, 8 * (r >> 2) + (r & 3) < j - off - at);
       }
+      if constexpr (kAhead) {
+        read_down(1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const Frag<T> p = result_frag<T>(s, w), f = result_frag<T>(ds, w);
+        if constexpr (!kAhead) read_down(w);
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
-          dv[n] = mma<T>(Lds::down(gt, 32 * u + 16 * w, n, la), p, dv[n]);
-          dk[n] = mma<T>(Lds::down(qt, 32 * u + 16 * w, n, la), f, dk[n]);
+          dv[n] = mma<T>(down[0][n][w], p, dv[n]);
+          dk[n] = mma<T>(down[1][n][w], f, dk[n]);
         }
       }
       if (partial && odd[0][u]) {
