@@ -334,10 +334,10 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
 #pragma unroll
         for (int r = 0; r < 4; ++r) ds[4 * w + r] = delta[r];
       }
-      // With one wave a SIMD nothing else covers the latency of the reads: they are issued a group ahead of their
+      // With one or two waves a SIMD little else covers the latency of the reads: they are issued a group ahead of their
       // products, the first operands of the gradients before the scores are worked on.  (Left to itself the compiler
       // reads one operand, waits for it and multiplies.)
-      constexpr bool kAhead = sizeof(T) == 2 && D == 128;
+      constexpr bool kAhead = sizeof(T) == 2 && D >= 64;
       Frag<T> along[2][NK], down[2][ND][2];
       auto read_along = [&](int n) {
         along[0][n] = Lds::along(qt, 32 * u, n, la);
