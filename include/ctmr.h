@@ -498,7 +498,8 @@ int ctmr_documents(int32_t n, int32_t lq, int32_t lk, const int32_t* query_ids, 
  * no key gives zeros.  What masked places hold has no effect, NaN included.
  * rest or NULL: what the rounding of out left out, of type elem, with out's strides
  * (16 bits; not written for fp32).  lse (n, q_heads, lq) or NULL: log2 of each
- * row's sum, +inf for an empty row.  The gradients read both.
+ * row's sum (of 16-bit types with a cap: of the scores less the cap), +inf for an
+ * empty row.  The gradients read both.
  * The kernel splits long keys over workgroups where there are few rows: workspace
  * of ctmr_masked_attention_workspace_bytes, 16-byte aligned. */
 typedef struct ctmr_masked_attention_desc {
@@ -513,7 +514,8 @@ int ctmr_masked_attention(const ctmr_masked_attention_desc* desc, const void* q,
                           const float* slopes, const int32_t* prefixes, const void* plan, void* out, void* rest,
                           float* lse, void* workspace, size_t workspace_bytes, void* stream);
 /* Gradients of q, k and v (any of dq, dk and dv may be NULL), given the call's out,
- * rest (NULL: not kept, with out's rounding in the gradients) and lse and dout (strides as q's); out's strides are multiples of 16 bytes here.
+ * rest (NULL: not kept, with out's rounding in the gradients) and lse and dout
+ * (strides as q's); out's strides are multiples of 16 bytes here.
  * fp32 and bf16 (CTMR_E_UNSUPPORTED for fp16: ds would leave its range).  Gradients
  * of shared key heads are summed over their query heads.  dq, dk and dv may not
  * overlap the inputs. */

@@ -37,7 +37,7 @@ struct RowMask {
   int limit, id;
 };
 
-// Raw products of NB 32-key blocks -> scores in units of 1 / c (c returned): the products, or with a cap tanh, less
+// Raw products of NB 32-key blocks -> scores in units of 1 / c (c returned): the products, or with a cap cap_scores, less
 // the distance in these units.  Masked keys become -inf; ids: of the keys from k0 on, or
 // null.
 template <typename T, int NB>
@@ -48,10 +48,8 @@ __device__ __forceinline__ float score_blocks(const Scoring& a, f16v (&s)[NB], i
   if (a.cap > 0.f) {
     const float in = a.scale / a.cap;
 #pragma unroll
-    for (int u = 0; u < NB; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[u][r] = tanh_of<T>(s[u][r], in);
-    c = a.cap * kLog2e;
+    for (int u = 0; u < NB; ++u) cap_scores<T>(s[u], in);
+    c = a.cap * (kLog2e * kCapUnits<T>);
   }
   if (a.sloped) {
     const float per = -a.slope * kLog2e / c, from = (float)(k0 + 4 * half - pos);

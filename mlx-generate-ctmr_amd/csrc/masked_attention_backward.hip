@@ -33,20 +33,23 @@ constexpr int kThreads = 256, kWaves = 4;
 constexpr int kOwn = kBlockRows;  // rows that a workgroup keeps in registers
 static_assert(kOwn == 32 * kWaves && kOwn == 4 * kGrain, "32 rows a wave");
 
+// What dq and dk are multiplied by at the end.
+template <typename T, bool CAP>
+__host__ __device__ __forceinline__ float ds_scale(const Args& a) {
+  return a.scale * (CAP ? kCapSlope<T> : 1.0f);
+}
+
 // Products of a 32 x 32 block -> log2 scores in units of 1 / c (c returned).  Row r of a lane is `at` + 8 (r / 4) + r
-// % 4; `x` is where the distance to it is zero.  With CAP g . v - delta, in `ds`, is multiplied by 1 - t^2.  (As a
-// branch on the cap the factor was 48 instructions of 145 a block for every call: the compiler selects what it skips.)
+// % 4; `x` is where the distance to it is zero.  With CAP g . v - delta, in `ds`, is multiplied by 1 - t^2
+// (in units of kCapSlope).  (As a branch on the cap the factor was 48 instructions of 145 a block for every call: the compiler selects what it skips.)
 template <typename T, bool CAP>
 __device__ __forceinline__ float scores(const Scoring& a, f16v& s, f16v& ds, int at, int x) {
   float c = a.scale * kLog2e;
   if constexpr (CAP) {
-    const float in = a.scale / a.cap;
+    cap_scores<T>(s, a.scale / a.cap);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = tanh_of<T>(s[r], in);
-      ds[r] *= fmaf(-s[r], s[r], 1.0f);
-    }
-    c = a.cap * kLog2e;
+    for (int r = 0; r < 16; ++r) ds[r] *= cap_slope<T>(s[r]);
+    c = a.cap * (kLog2e * kCapUnits<T>);
   }
   if (a.sloped) {
     const float per = -a.slope * kLog2e / c, from = (float)(at - x);
@@ -224,7 +227,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
   if (a.splits > 1)
     write_gradient<float, ND>(a.part + ((int64_t)blockIdx.y * a.n * a.hq * a.lq + stat) * D, dq, 1.0f, D, lane);
   else
-    write_gradient<T, ND>(static_cast<T*>(a.dq) + b * a.dqb + h * a.dqh + (int64_t)i * a.dql, dq, a.scale, a.d, lane);
+    write_gradient<T, ND>(static_cast<T*>(a.dq) + b * a.dqb + h * a.dqh + (int64_t)i * a.dql, dq, ds_scale<T, CAP>(a), a.d, lane);
 }
 
 template <typename T, int D>
@@ -452,7 +455,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
     return;
   }
   if (a.dk)
-    write_gradient<T, ND>(static_cast<T*>(a.dk) + b * a.dkb + hk * a.dkh + (int64_t)j * a.dkl, dk, a.scale, a.d, lane);
+    write_gradient<T, ND>(static_cast<T*>(a.dk) + b * a.dkb + hk * a.dkh + (int64_t)j * a.dkl, dk, ds_scale<T, CAP>(a), a.d, lane);
   if (a.dv)
     write_gradient<T, ND>(static_cast<T*>(a.dv) + b * a.dvb + hk * a.dvh + (int64_t)j * a.dvl, dv, 1.0f, a.d, lane);
 }
@@ -516,7 +519,7 @@ int launch(Args a, int qparts, int kparts, hipStream_t st) {
   int rc = check_launch("attention_dq");
   if (rc) return rc;
   if (a.splits > 1) {
-    SumArgs s = {a.part, {a.dq, nullptr}, {a.dqb, 0}, {a.dqh, 0}, {a.dql, 0}, {a.scale, 0.f},
+    SumArgs s = {a.part, {a.dq, nullptr}, {a.dqb, 0}, {a.dqh, 0}, {a.dql, 0}, {ds_scale<T, CAP>(a), 0.f},
                  a.n * a.hq * a.lq, a.hq, a.lq, a.d, a.splits, 1};
     hipLaunchKernelGGL((attention_sum_kernel<T, D>), dim3((unsigned)ceil_div((int64_t)s.rows * (D / 4), kThreads)),
                        dim3(kThreads), 0, st, s);
@@ -529,7 +532,7 @@ int launch(Args a, int qparts, int kparts, hipStream_t st) {
                      dim3(kThreads), 0, st, a);
   rc = check_launch("attention_dkv");
   if (rc || a.splits == 1) return rc;
-  SumArgs s = {a.part, {a.dk, a.dv}, {a.dkb, a.dvb}, {a.dkh, a.dvh}, {a.dkl, a.dvl}, {a.scale, 1.0f},
+  SumArgs s = {a.part, {a.dk, a.dv}, {a.dkb, a.dvb}, {a.dkh, a.dvh}, {a.dkl, a.dvl}, {ds_scale<T, CAP>(a), 1.0f},
                a.n * a.hk * a.lk, a.hk, a.lk, a.d, a.splits, 2};
   hipLaunchKernelGGL((attention_sum_kernel<T, D>), dim3((unsigned)ceil_div((int64_t)s.rows * (D / 4), kThreads), 2),
                      dim3(kThreads), 0, st, s);
