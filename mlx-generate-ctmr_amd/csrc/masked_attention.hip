@@ -623,15 +623,16 @@ __global__ __launch_bounds__(kTile) void document_hulls_kernel(DocArgs a) {
 bool few_rows(const ctmr_masked_attention_desc* d) { return (int64_t)(d->q_heads / d->k_heads) * d->lq <= 32; }
 
 // Parts of the keys where the rows alone do not fill the chip: about 512 workgroups, or 256 of the few-row form, of
-// at least four 64-key tiles each (two in fp32).  From the shape only, so that a shape's sums have one order.  Few rows, bf16, 4 x 8
+// at least four 64-key tiles each (two of fp32 heads of 64 and more).  From the shape only, so that a shape's sums have one order.  Few rows, bf16, 4 x 8
 // key heads of 128 values, 16384 keys (268 MB): 49.7 us with 256 workgroups (one a CU at a time; 5.4 TB/s), 56 with
 // 384, 51 with 512, 58 with 1024.
 int split_count(const ctmr_masked_attention_desc* d) {
   const bool few = few_rows(d);
   const int64_t blocks = (int64_t)d->n * (few ? d->k_heads : d->q_heads * ceil_div(d->lq, kRows));
   const int64_t tiles = ceil_div(d->lk, kTile);
+  const int64_t least = d->elem == CTMR_ELEM_F32 && padded(d->head_dim) >= 64 ? 2 : 4;
   const int64_t want = std::max<int64_t>(1, (few ? 256 : 512) / blocks);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / (d->elem == CTMR_ELEM_F32 ? 2 : 4), kMostSplits}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / least, kMostSplits}));
 }
 
 template <typename T, int D>
@@ -700,8 +701,10 @@ int check_desc(const ctmr_masked_attention_desc* d) {
     return fail(CTMR_E_UNSUPPORTED, "head_dim must be a multiple of 8 up to 128");
   if (!(d->scale > 0.f) || !(d->scale < INFINITY) || !(d->softcap >= 0.f) || !(d->softcap < INFINITY))
     return fail(CTMR_E_INVALID, "scale must be positive, softcap not negative, both finite");
+  if (d->softcap > 0.f && !(d->scale / d->softcap < 1e30f))
+    return fail(CTMR_E_INVALID, "softcap too small for the scale");
   if (d->lq > (1 << 28) || d->lk > (1 << 28) ||
-      (int64_t)d->n * d->q_heads * ceil_div(std::max(d->lq, d->lk), kTile) > (1ll << 30))
+      (int64_t)d->n * d->q_heads * ceil_div(std::max(d->lq, d->lk), kTile) > (1ll << 23))  // 2^32 threads
     return fail(CTMR_E_UNSUPPORTED, "too many rows");
   int rc = check_strides(d, d->q_strides, d->lq);
   if (!rc) rc = check_strides(d, d->k_strides, d->lk);

@@ -167,6 +167,7 @@ extern "C" int ctmr_rotary(const ctmr_rotary_desc* d, const void* q, const void*
   int tokens = std::max(1, std::min(16, kTable / a.pairs));
   while (tokens > 1 && ceil_div(a.l, tokens) * a.n < 2048) tokens >>= 1;
   a.tokens = tokens;
+  if (ceil_div(a.l, tokens) > (1 << 23)) return fail(CTMR_E_UNSUPPORTED, "too many tokens");  // 2^32 threads
   const dim3 grid((unsigned)ceil_div(a.l, tokens), a.n);
   hipStream_t st = (hipStream_t)stream;
 #define CTMR_ROTARY_CASE(T, W) \

@@ -66,6 +66,14 @@ def _graph_token(*tensors: Optional[Tensor]) -> Optional[_EagerGraph]:
     return None
 
 
+def _hold(out: Tensor, token: Optional[_EagerGraph]) -> Tensor:
+    """``out``, whose graph keeps ``token`` while it lives: for calls whose leaves reach autograd through other
+    operators than these."""
+    if token is not None and out.grad_fn is not None:
+        out.grad_fn.metadata["ctmr.leaves"] = token
+    return out
+
+
 def _check_capture(captured: bool) -> None:
     """Refuses a backward pass in another capture state than its forward pass."""
     if torch.cuda.is_current_stream_capturing() != captured:
@@ -190,7 +198,9 @@ def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, *, sections: Seque
         ValueError: on other types, devices or shapes, sections that are odd, not positive, wider than the head
             or not one for each axis, or a base that is not positive and finite."""
     _activation(q, "q", 4)
-    b, _, l, d = (int(v) for v in q.shape)
+    b, hq, l, d = (int(v) for v in q.shape)
+    if hq < 1:
+        raise ValueError("q has no heads")
     if k is not None:
         _like(k, q, "k", 4)
         if int(k.shape[0]) != b or int(k.shape[2]) != l or int(k.shape[3]) != d:
@@ -314,6 +324,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
     scale, softcap = float(scale), float(softcap)
     if not (math.isfinite(scale) and scale > 0.0) or not (math.isfinite(softcap) and softcap >= 0.0):
         raise ValueError(f"scale must be positive, softcap not negative, both finite; got {scale} and {softcap}")
+    if softcap > 0.0 and not scale / softcap < 1e30:
+        raise ValueError(f"softcap {softcap} is too small for a scale of {scale}")
     if slopes is not None:
         if not isinstance(slopes, Tensor) or slopes.dtype != torch.float32 or tuple(slopes.shape) != (hq,) or (
                 slopes.device != q.device):
@@ -389,6 +401,9 @@ def self_attention_tokens(tokens: Tensor, weights: Mapping[str, Tensor], *, head
     if (positions is None) != (sections is None):
         raise ValueError("positions and sections go together")
     names = [f"{prefix}.to_{m}" for m in ("q", "k", "v")]
+    used = [weights[f"{m}.{part}"] for m in [*names, *([f"{prefix}.out_proj"] if include_fc else [])]
+            for part in (("weight", "bias") if qkv_bias or m.endswith("out_proj") else ("weight",))]
+    token = _graph_token(tokens, *used) if torch.is_grad_enabled() and tokens.is_cuda else None
     w = torch.cat([_like(weights[f"{m}.weight"], tokens, f"{m}.weight", 2) for m in names])
     b = torch.cat([_like(weights[f"{m}.bias"], tokens, f"{m}.bias", 1) for m in names]) if qkv_bias else None
     # (B, L, 3, H, D): q, k and v are strided views of the one product
@@ -399,4 +414,4 @@ def self_attention_tokens(tokens: Tensor, weights: Mapping[str, Tensor], *, head
     if include_fc:
         merged = F.linear(merged, _like(weights[f"{prefix}.out_proj.weight"], tokens, f"{prefix}.out_proj.weight", 2),
                           _like(weights[f"{prefix}.out_proj.bias"], tokens, f"{prefix}.out_proj.bias", 1))
-    return merged
+    return _hold(merged, token)

@@ -264,3 +264,35 @@ def test_spatial_attention_volumes_refuses(ctmr, volumes, kw, message):
     kw = {"num_groups": 16, "eps": 1e-6, "num_head_channels": 32, "include_fc": True} | kw
     with pytest.raises(ValueError, match=message):
         ctmr.maisi.spatial_attention_volumes([torch.zeros(s) for s in volumes], _block_weights(), **kw)
+
+
+def test_leaves_behind_other_operators_are_held(ctmr, monkeypatch):
+    f = ctmr.differentiable
+    state = {"capturing": False}
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    weight = torch.zeros(3, requires_grad=True)
+    out = f._hold(weight * 2, f._graph_token(weight))
+    later = out + 1
+    del out  # the graph lives on in what was made of it
+    gc.collect()
+    state["capturing"] = True
+    with pytest.raises(RuntimeError, match="outside this capture"):
+        f._graph_token(weight)
+    del later
+    gc.collect()
+    assert f._graph_token(weight) is None
+
+
+def test_calls_that_no_launch_can_take_are_refused(ctmr, native_loaded):
+    L, p, f = ctmr._lib, 4096, ctmr.differentiable
+    space = lambda **kw: native_loaded.ctmr_masked_attention_workspace_bytes(ctypes.byref(_attention_desc(L, **kw)))
+    # 2^23 blocks of 64 rows are the most: their workgroups, two parts each, stay below 2^32 threads
+    assert space(n=1 << 19, lq=64, lk=64, q_heads=16, k_heads=16) >= 0
+    assert space(n=1 << 19, lq=65, lk=64, q_heads=16, k_heads=16) == L.E_UNSUPPORTED
+    assert space(softcap=1e-38, scale=1.0) == L.E_INVALID and space(softcap=1e-20, scale=1.0) >= 0
+    with pytest.raises(ValueError, match="too small"):
+        _attention(f, softcap=1e-38)
+    with pytest.raises(ValueError, match="no heads"):
+        _rotary(f, q=(2, 0, 6, 32))
+    d = L.RotaryDesc(1, (1 << 31) - 1, 1, 0, 512, 1, (ctypes.c_int32 * 4)(512), 0, 0, 0, 0, 0)
+    assert native_loaded.ctmr_rotary(ctypes.byref(d), p, None, p, (ctypes.c_double * 256)(), p, None, None) == L.E_UNSUPPORTED
