@@ -296,3 +296,10 @@ def test_calls_that_no_launch_can_take_are_refused(ctmr, native_loaded):
         _rotary(f, q=(2, 0, 6, 32))
     d = L.RotaryDesc(1, (1 << 31) - 1, 1, 0, 512, 1, (ctypes.c_int32 * 4)(512), 0, 0, 0, 0, 0)
     assert native_loaded.ctmr_rotary(ctypes.byref(d), p, None, p, (ctypes.c_double * 256)(), p, None, None) == L.E_UNSUPPORTED
+
+
+def test_volumes_are_not_laid_out_inside_a_capture(ctmr, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before a graph is captured"):
+        ctmr.differentiable.PackedVolumes([(1, 2, 3)], "cpu")
