@@ -648,7 +648,7 @@ def _(x, dy, weight, bias, saved, silu, want_x, want_params):
 def _heads_like(t: Tensor) -> Tensor:
     """An empty (B, H, L, D) tensor that lies as (B, L, H, D) rows, the layout of a projection's output."""
     b, h, l, d = t.shape
-    return t.new_empty((b, l, h, d)).transpose(1, 2)
+    return t.new_empty_strided((b, h, l, d), (l * h * d, d, h * d, 1))
 
 
 @functools.lru_cache(maxsize=256)
