@@ -268,7 +268,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
       __syncthreads();
     }
     if (meet.skips(tile)) return;
-    const int at = fresh<D == 128>(lane);
+    const int at = fresh<D == 128 && sizeof(T) == 4>(lane);
     f16v s[2] = {f16v(0.f), f16v(0.f)};
 #pragma unroll
     for (int n = 0; n < NK; ++n)

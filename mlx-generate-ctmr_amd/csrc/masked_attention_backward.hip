@@ -184,7 +184,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
       __syncthreads();
     }
     if (meet.skips(tile)) return;
-    const int la = fresh<D == 128 && sizeof(T) == 2>(lane);
+    const int la = fresh<D == 128 && sizeof(T) == 2 && CAP>(lane);
     const bool masked = meet.masked(tile) || (partial && (odd[0] | odd[1]) != 0u);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
