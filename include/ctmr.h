@@ -516,9 +516,8 @@ int ctmr_masked_attention(const ctmr_masked_attention_desc* desc, const void* q,
 /* Gradients of q, k and v (any of dq, dk and dv may be NULL), given the call's out,
  * rest (NULL: not kept, with out's rounding in the gradients) and lse and dout
  * (strides as q's); out's strides are multiples of 16 bytes here.
- * fp32 and bf16 (CTMR_E_UNSUPPORTED for fp16: ds would leave its range).  Gradients
- * of shared key heads are summed over their query heads.  dq, dk and dv may not
- * overlap the inputs. */
+ * Gradients of shared key heads are summed over their query heads.  dq, dk and dv
+ * may not overlap the inputs. */
 int64_t ctmr_masked_attention_backward_workspace_bytes(const ctmr_masked_attention_desc* desc);
 int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* desc, const void* q, const void* k, const void* v,
                                    const float* slopes, const int32_t* prefixes, const void* plan, const void* out,

@@ -293,6 +293,7 @@ struct Args {
   const void* dout;
   void *dq, *dk, *dv;
   float* delta;           // (n, hq, lq) -sum_d dout out
+  unsigned* most;         // fp16 gradients: (n, hk, 2) bits of the largest |dout| and |v|, as fp32
   const float* slopes;    // (hq)
   const int* prefixes;    // (n), or null with `prefix`
   Side qdoc, kdoc;        // ids null: no documents
@@ -426,12 +427,12 @@ __device__ __forceinline__ int4 key_tiles(const Args& a, int b, int i, int prefi
 }
 
 // Query tiles of the keys j .. j + kGrain - 1: from the first row whose limit passes j; every key is seen from the
-// row whose limit passes the last one.
+// row whose limit passes the last one, up to the last whole tile.
 __device__ __forceinline__ int4 query_tiles(const Args& a, int b, int j, int prefix, const Part* part) {
   const int end = min(j + kGrain, a.lk) - 1, off = a.lk - a.lq, tiles = (a.lq + kTile - 1) / kTile;
   const int first = a.prefixed && prefix <= j ? max(0, j - off) / kTile : 0;
   const int whole = a.prefixed && prefix <= end ? (max(0, end - off) + kTile - 1) / kTile : 0;
-  return meet(a.kdoc, b, j / kGrain, int4{first, tiles, whole, tiles}, part);
+  return meet(a.kdoc, b, j / kGrain, int4{first, tiles, whole, a.lq / kTile}, part);
 }
 
 // A workgroup's tiles from its waves' (those that meet any): any wave may hold a pair, all waves' are whole.

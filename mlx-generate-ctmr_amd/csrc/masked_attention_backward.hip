@@ -1,4 +1,4 @@
-// Gradients of the masked attention (masked_attention.hip), for fp32 and bf16.
+// Gradients of the masked attention (masked_attention.hip), for fp32, bf16 and fp16.
 //
 // With p_ij = 2^(s2_ij - lse_i) recomputed from q, k and lse, g = dout:
 //   dv_j = sum_i p_ij g_i
@@ -24,7 +24,10 @@
 // of the five products, 950 of the seven), of 128 1013; fp32, 2 x 8 heads of 2048 rows
 // of 32: 252 (119 of the seven, where a library product of 8192^3 reaches 153).
 //
-// fp16 is refused: without a scale that follows the data ds leaves its range.
+// fp16's range is far smaller than what ds spans: |ds| < 2 d max |dout| max |v|, and
+// these two maxima of a key head (a pass over dout and v of its own) give the power of
+// two that takes ds just below 2^15; p is raised by 2^15. Both come out of the sums
+// again at the end, exactly, so weights and ds down to 2^-39 of their largest count.
 #include "masked_attention.hpp"
 
 #include <algorithm>
@@ -42,6 +45,19 @@ static_assert(kOwn == 32 * kWaves && kOwn == 4 * kGrain, "32 rows a wave");
 template <typename T, bool CAP>
 __host__ __device__ __forceinline__ float ds_scale(const Args& a) {
   return a.scale * (CAP ? kCapSlope<T> : 1.0f);
+}
+
+template <typename T>
+constexpr bool kHalf = std::is_same_v<T, _Float16>;
+constexpr float kRaise = 15.0f;  // of p, in log2
+
+// log2 of what ds of a key head is multiplied by: 0 but in fp16.
+template <typename T>
+__device__ __forceinline__ int ds_raise(const Args& a, int b, int hk) {
+  if constexpr (!kHalf<T>) return 0;
+  const unsigned* most = a.most + 2 * ((int64_t)b * a.hk + hk);
+  const float bound = 2.0f * (float)a.d * __uint_as_float(most[0]) * __uint_as_float(most[1]);
+  return bound > 0.f ? 15 - __builtin_amdgcn_frexp_expf(bound) : 0;
 }
 
 // Products of a 32 x 32 block -> log2 scores in units of 1 / c (c returned).  Row r of a lane is `at` + 8 (r / 4) + r
@@ -153,7 +169,8 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
   delta = half_sum(delta);
   if (real && half == 0 && blockIdx.y == 0) a.delta[stat] = -delta;
   if (!a.dq) return;
-  const float lse = real ? a.lse[stat] : INFINITY;
+  const int raise = ds_raise<T>(a, b, h / a.group);
+  const float lse = (real ? a.lse[stat] : INFINITY) - (float)raise;
   f16v dq[ND];
 #pragma unroll
   for (int n = 0; n < ND; ++n) dq[n] = f16v(0.f);
@@ -231,11 +248,12 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
     if (tile + 1 < last) step(tile + 1, kt1, vt1, kt0, vt0);
   }
   if (!real) return;
+  const float lower = __builtin_ldexpf(1.0f, -raise);
   if (a.splits > 1)
-    write_gradient<float, ND>(a.part + ((int64_t)blockIdx.y * a.n * a.hq * a.lq + stat) * D, dq, 1.0f, D, lane);
+    write_gradient<float, ND>(a.part + ((int64_t)blockIdx.y * a.n * a.hq * a.lq + stat) * D, dq, lower, D, lane);
   else
-    write_gradient<T, ND>(static_cast<T*>(a.dq) + b * a.dqb + h * a.dqh + (int64_t)i * a.dql, dq, ds_scale<T, CAP>(a),
-                          a.d, lane);
+    write_gradient<T, ND>(static_cast<T*>(a.dq) + b * a.dqb + h * a.dqh + (int64_t)i * a.dql, dq,
+                          ds_scale<T, CAP>(a) * lower, a.d, lane);
 }
 
 template <typename T, int D>
@@ -306,7 +324,6 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
     Load::load(gt, grows, t);
     qrows.next();
     grows.next();
-    // Rows past the end have zeros everywhere, so their p, whatever it is, adds nothing.
     const int64_t row = ((int64_t)b * a.hq + fetched) * a.lq;
     if (wave < 2) load_floats(stats + wave * kTile, (wave == 0 ? a.lse : a.delta) + row, at_tile * kTile, a.lq, lane);
     if (++at_tile == last) {
@@ -315,6 +332,8 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
     }
   };
   Scoring scoring = scoring_of(a, hk * a.group);
+  const int raise = ds_raise<T>(a, b, hk);
+  const float raised = __builtin_ldexpf(1.0f, raise - (int)kRaise);  // of ds, whose p is raised already
   // One tile, while the next one is on its way into the other arrays.
   auto step = [&](bool more, char* qt, char* gt, float* stats, char* next_qt, char* next_gt, float* next_stats) {
     if (++tile == last) {
@@ -392,8 +411,9 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
         const f4 lse = *reinterpret_cast<const f4*>(stats + 32 * u + 8 * w + 4 * half);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          s[4 * w + r] = __builtin_amdgcn_exp2f(fmaf(s[4 * w + r], c, -lse[r]));
+          s[4 * w + r] = __builtin_amdgcn_exp2f(fmaf(s[4 * w + r], c, kHalf<T> ? kRaise - lse[r] : -lse[r]));
           ds[4 * w + r] *= s[4 * w + r];
+          if constexpr (kHalf<T>) ds[4 * w + r] *= raised;
         }
       }
       if (masked) {
@@ -410,6 +430,9 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
             hide(4 * w + 2, other.z != id);
             hide(4 * w + 3, other.w != id);
           }
+        if (i0 + kTile > a.lq)  // rows past the end, whose zeros give a p that may be infinite
+#pragma unroll
+          for (int r = 0; r < 16; ++r) hide(r, 8 * (r >> 2) + (r & 3) >= a.lq - at);
         if (scoring.prefixed && j >= prefix)  // else every row sees the key
 #pragma unroll
           for (int r = 0; r < 16; ++r) hide(r, 8 * (r >> 2) + (r & 3) < j - off - at);
@@ -455,18 +478,57 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
     if (s + 1 < mine.y) step(s + 2 < mine.y, qt1, gt1, stats1, qt0, gt0, stats0);
   }
   if (!real) return;
+  const float lower = __builtin_ldexpf(1.0f, -raise), lower_p = kHalf<T> ? __builtin_ldexpf(1.0f, -(int)kRaise) : 1.0f;
   if (a.splits > 1) {
     const int64_t rows = (int64_t)a.n * a.hk * a.lk;
     float* part = a.part + (2 * blockIdx.y * rows + ((int64_t)b * a.hk + hk) * a.lk + j) * D;
-    if (a.dk) write_gradient<float, ND>(part, dk, 1.0f, D, lane);
-    if (a.dv) write_gradient<float, ND>(part + rows * D, dv, 1.0f, D, lane);
+    if (a.dk) write_gradient<float, ND>(part, dk, lower, D, lane);
+    if (a.dv) write_gradient<float, ND>(part + rows * D, dv, lower_p, D, lane);
     return;
   }
   if (a.dk)
-    write_gradient<T, ND>(static_cast<T*>(a.dk) + b * a.dkb + hk * a.dkh + (int64_t)j * a.dkl, dk, ds_scale<T, CAP>(a),
-                          a.d, lane);
+    write_gradient<T, ND>(static_cast<T*>(a.dk) + b * a.dkb + hk * a.dkh + (int64_t)j * a.dkl, dk,
+                          ds_scale<T, CAP>(a) * lower, a.d, lane);
   if (a.dv)
-    write_gradient<T, ND>(static_cast<T*>(a.dv) + b * a.dvb + hk * a.dvh + (int64_t)j * a.dvl, dv, 1.0f, a.d, lane);
+    write_gradient<T, ND>(static_cast<T*>(a.dv) + b * a.dvb + hk * a.dvh + (int64_t)j * a.dvl, dv, lower_p, a.d, lane);
+}
+
+// The largest finite |v| and |dout| of each key head, rows that see nothing and padding aside.  blockIdx.y: dout or v;
+// blockIdx.x: part of a key head.  The maximum does not depend on the order.
+__global__ __launch_bounds__(kThreads) void attention_most_zero_kernel(unsigned* most, int count) {
+  const int i = blockIdx.x * kThreads + threadIdx.x;
+  if (i < count) most[i] = 0u;
+}
+
+__global__ __launch_bounds__(kThreads) void attention_most_kernel(Args a, int parts) {
+  const int item = blockIdx.x / parts, b = item / a.hk, hk = item % a.hk;
+  const bool values = blockIdx.y == 1;
+  const int rows = values ? a.lk : a.lq, pieces = a.d / 8;
+  const int prefix = a.prefixed ? prefix_of(a, b) : 0;
+  const int* ids = a.qdoc.ids ? (values ? a.kdoc.ids + (int64_t)b * a.kdoc.stride : a.qdoc.ids + (int64_t)b * a.qdoc.stride)
+                              : nullptr;
+  const int64_t count = (int64_t)rows * pieces * (values ? 1 : a.group);
+  unsigned top = 0u;
+  for (int64_t at = (int64_t)(blockIdx.x % parts) * kThreads + threadIdx.x; at < count; at += (int64_t)parts * kThreads) {
+    const int piece = (int)(at % pieces);
+    const int64_t line = at / pieces;
+    const int i = (int)(line % rows), h = hk * a.group + (int)(line / rows);
+    if ((ids && ids[i] < 0) || (!values && limit_of(a, i, prefix) <= 0)) continue;
+    const _Float16* row = values ? static_cast<const _Float16*>(a.v) + b * a.vb + hk * a.vh + (int64_t)i * a.vl
+                                 : static_cast<const _Float16*>(a.dout) + b * a.gb + h * a.gh + (int64_t)i * a.gl;
+    const u4 v = *reinterpret_cast<const u4*>(row + 8 * piece);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const unsigned lo = v[w] & 0x7fffu, hi = (v[w] >> 16) & 0x7fffu;
+      top = max(top, lo < 0x7c00u ? lo : 0u);
+      top = max(top, hi < 0x7c00u ? hi : 0u);
+    }
+  }
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, m));
+  if (threadIdx.x % 64 == 0 && top)
+    atomicMax(a.most + 2 * (int64_t)item + (values ? 1 : 0),
+              __float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)top)));
 }
 
 // Adds the parts of gradients in order: four values a thread.  blockIdx.y: which of up to two gradients.
@@ -514,14 +576,31 @@ int key_parts(const ctmr_masked_attention_desc* d) {
                     ceil_div(d->lq, kTile) * (d->q_heads / d->k_heads), d->elem, d->head_dim);
 }
 
-// Bytes of delta in the workspace; the parts follow, dq's and then, in the same place, dk's and dv's.
+// Bytes of delta, and of fp16's maxima, in the workspace; the parts follow, dq's and then, in the same place, dk's and dv's.
 int64_t delta_bytes(const ctmr_masked_attention_desc* d) {
   return ceil_div((int64_t)d->n * d->q_heads * d->lq * 4, 16) * 16;
+}
+
+int64_t most_bytes(const ctmr_masked_attention_desc* d) {
+  return d->elem == CTMR_ELEM_F16 ? ceil_div((int64_t)d->n * d->k_heads * 8, 16) * 16 : 0;
 }
 
 template <typename T, int D, bool CAP>
 int launch(Args a, int qparts, int kparts, hipStream_t st) {
   const unsigned parts = a.qdoc.ids ? 2u : 1u;
+  if constexpr (kHalf<T>) {
+    const int heads = a.n * a.hk;
+    hipLaunchKernelGGL(attention_most_zero_kernel, dim3((unsigned)ceil_div(2 * (int64_t)heads, kThreads)), dim3(kThreads), 0,
+                       st, a.most, 2 * heads);
+    int rc = check_launch("attention_most_zero");
+    if (rc) return rc;
+    // about 1024 workgroups, of 16 KB at least
+    const int64_t pieces = (int64_t)std::max<int64_t>(a.lk, (int64_t)a.lq * a.group) * (a.d / 8);
+    const int cut = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / heads, ceil_div(pieces, 4 * kThreads)));
+    hipLaunchKernelGGL(attention_most_kernel, dim3(heads * (unsigned)cut, 2), dim3(kThreads), 0, st, a, cut);
+    rc = check_launch("attention_most");
+    if (rc) return rc;
+  }
   a.splits = a.dq ? qparts : 1;
   const unsigned q_blocks = a.n * a.hq * (unsigned)ceil_div(a.lq, kOwn) * parts;
   hipLaunchKernelGGL((attention_dq_kernel<T, D, CAP>), dim3(q_blocks, a.splits), dim3(kThreads), 0, st, a);
@@ -563,7 +642,7 @@ int64_t ctmr_masked_attention_backward_workspace_bytes(const ctmr_masked_attenti
   const int64_t q = query_parts(d), k = key_parts(d);
   const int64_t qbytes = q > 1 ? q * d->n * d->q_heads * d->lq * padded(d->head_dim) * 4 : 0;
   const int64_t kbytes = k > 1 ? 2 * k * d->n * d->k_heads * d->lk * padded(d->head_dim) * 4 : 0;
-  return delta_bytes(d) + std::max(qbytes, kbytes);
+  return delta_bytes(d) + most_bytes(d) + std::max(qbytes, kbytes);
 }
 
 int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const void* q, const void* k, const void* v,
@@ -573,7 +652,6 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const vo
                                    const int64_t* dv_strides, void* workspace, size_t workspace_bytes, void* stream) {
   const int64_t need = ctmr_masked_attention_backward_workspace_bytes(d);
   if (need < 0) return (int)need;
-  if (d->elem == CTMR_ELEM_F16) return fail(CTMR_E_UNSUPPORTED, "attention has no fp16 gradient");
   if (!q || !k || !v || !out || !lse || !dout || !dout_strides || (dq && !dq_strides) || (dk && !dk_strides) ||
       (dv && !dv_strides))
     return fail(CTMR_E_INVALID, "null pointer");
@@ -596,7 +674,8 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const vo
   Args a = make_args(d, q, k, v, slopes, prefixes, plan);
   a.out = const_cast<void*>(out), a.rest = const_cast<void*>(rest), a.lse = const_cast<float*>(lse), a.dout = dout;
   a.dq = dq, a.dk = dk, a.dv = dv, a.delta = (float*)workspace;
-  a.part = (float*)((char*)workspace + delta_bytes(d));
+  a.most = (unsigned*)((char*)workspace + delta_bytes(d));
+  a.part = (float*)((char*)workspace + delta_bytes(d) + most_bytes(d));
   a.ob = d->out_strides[0], a.oh = d->out_strides[1], a.ol = d->out_strides[2];
   a.gb = dout_strides[0], a.gh = dout_strides[1], a.gl = row_stride(dout_strides, d->lq, d->head_dim);
   if (dq) a.dqb = dq_strides[0], a.dqh = dq_strides[1], a.dql = dq_strides[2];
@@ -614,7 +693,8 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const vo
     default: CTMR_ATTENTION_CASE(T, 128)    \
   }
   if (d->elem == CTMR_ELEM_F32) CTMR_ATTENTION_TYPE(float)
-  CTMR_ATTENTION_TYPE(__bf16)
+  if (d->elem == CTMR_ELEM_BF16) CTMR_ATTENTION_TYPE(__bf16)
+  CTMR_ATTENTION_TYPE(_Float16)
 #undef CTMR_ATTENTION_TYPE
 #undef CTMR_ATTENTION_CASE
 }

@@ -291,7 +291,7 @@ class _Attention(torch.autograd.Function):
 
 def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float = 0.0, slopes: Optional[Tensor] = None,
               prefix: Union[int, Tensor, None] = None, documents: Optional[Documents] = None) -> Tensor:
-    """Masked attention of ``(B, H, L, D)`` heads; differentiable in ``q``, ``k`` and ``v`` (fp32 and bf16).
+    """Masked attention of ``(B, H, L, D)`` heads; differentiable in ``q``, ``k`` and ``v``.
 
     ``q`` has ``Hq`` heads and ``Lq`` rows, ``k`` and ``v`` ``Hk`` heads and ``Lk`` keys, ``Hq`` a multiple of
     ``Hk`` (query head ``h`` reads key head ``h // (Hq // Hk)``); ``D`` is a multiple of 8 up to 128.  With
@@ -304,12 +304,13 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
     * ``documents`` hides the keys of other documents and padding (``Documents``).
 
     A row that sees no key gives zeros and gets no gradient.  What masked places hold has no effect, NaN included.
-    Statistics and sums are fp32; the softmax weights are rounded to the inputs' type for their product with
-    ``v``.  The output has ``q``'s type and lies as ``(B, Lq, Hq, D)`` in memory, so merging the heads is a view.
+    Statistics and sums are fp32; the softmax weights, and in the gradients those of the scores, are rounded to the
+    inputs' type for their products (in fp16 raised by powers of two that keep them in its range).  The output has
+    ``q``'s type and lies as ``(B, Lq, Hq, D)`` in memory, so merging the heads is a view.
 
     Raises:
-        ValueError: on other types, devices or shapes, a scale that is not positive and finite, a negative cap,
-            slopes that need a gradient, or fp16 tensors that need one (it would leave fp16's range)."""
+        ValueError: on other types, devices or shapes, a scale that is not positive and finite, a cap that is
+            negative or too small beside it, or slopes that need a gradient."""
     _activation(q, "q", 4)
     _like(k, q, "k", 4)
     _like(v, q, "v", 4)
@@ -344,8 +345,6 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
         raise ValueError(f"documents are for {documents.shape} rows on {documents.device}; got {(b, lq, lk)} on "
                          f"{q.device}")
     needs = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-    if needs and q.dtype == torch.float16:
-        raise ValueError("attention has no float16 gradient (it would leave the type's range); use bfloat16 or float32")
     _on_gpu(q, "q")
     q, k, v = _attention_heads(q), _attention_heads(k), _attention_heads(v)
     plan = None if documents is None else documents.plan
@@ -389,7 +388,7 @@ def self_attention_tokens(tokens: Tensor, weights: Mapping[str, Tensor], *, head
                           sections: Optional[Sequence[int]] = None, base: float = 10000.0, prefix: str = "attn",
                           qkv_bias: bool = True) -> Tensor:
     """Q/K/V projections, rotary positions, self-attention and optional ``out_proj`` on ``(B, L, C)`` tokens;
-    differentiable in the tokens and the weights (fp32 and bf16; fp16 without gradients).
+    differentiable in the tokens and the weights.
 
     Takes the weights of ``fast_fp32.self_attention_tokens`` in the tokens' type.  ``documents`` keeps tokens apart;
     ``positions`` with ``sections`` (see ``rotary``) turns q and k, and is left out for attention without positions.

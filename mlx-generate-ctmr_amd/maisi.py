@@ -119,7 +119,7 @@ def spatial_attention_volumes(volumes: Sequence[Tensor], weights: Mapping[str, T
                               num_head_channels: int, include_fc: bool, packed: Optional[df.PackedVolumes] = None,
                               sections: Optional[Sequence[int]] = None, base: float = 10000.0) -> list[Tensor]:
     """``spatial_attention`` of several DHWC volumes at once, each over its own voxels, differentiable in the volumes
-    and the weights (fp32 and bf16; fp16 without gradients): what fine-tuning on volumes of different sizes runs.
+    and the weights: what fine-tuning on volumes of different sizes runs.
 
     Each volume has group statistics of its own; the tokens of all lie in one row, whose documents the attention
     keeps apart, so no volume is padded to another's size.  ``packed`` is the batch's ``PackedVolumes`` where more

@@ -75,14 +75,18 @@ def attention(q, k, v, *, scale, softcap=0.0, slopes=None, mask=None, dout=None)
     if factor is not None:
         e_inner = e_inner + (dp - delta).abs() * (2 * es / softcap + 8e-7)
     eds = ep * inner.abs() + p * e_inner + u * ds.abs()
+    if tiny:
+        # ds is raised to below 2^15 by a bound of twice d max |g| max |v|, p by 2^15: half a step of the least
+        # values, 2^-25, is 2^-39 of the bound (a power of two above it aside), and 2^-40 of p
+        eds = eds + mask * (2.0 ** -39 * 2 * d * float(g.abs().max()) * float(v.abs().max()))
     dq = scale * (ds @ k)
-    edq = scale * ((eds + 6 * math.sqrt(lk) * U * ds.abs()) @ k.abs()) + u * dq.abs()
+    edq = scale * ((eds + 6 * math.sqrt(lk) * U * ds.abs()) @ k.abs()) + u * dq.abs() + tiny
     shared = lambda t: t.reshape(b, hk, group, lk, d).sum(2)
     rows = 6 * math.sqrt(lq * group) * U
     dk = shared(scale * (ds.transpose(2, 3) @ q))
-    edk = shared(scale * ((eds + rows * ds.abs()).transpose(2, 3) @ q.abs())) + u * dk.abs()
+    edk = shared(scale * ((eds + rows * ds.abs()).transpose(2, 3) @ q.abs())) + u * dk.abs() + tiny
     dv = shared(p.transpose(2, 3) @ g)
-    edv = shared((ep + u * p + rows * p).transpose(2, 3) @ g.abs()) + u * dv.abs()
+    edv = shared((ep + u * p + rows * p + tiny * 2.0 ** -15 * mask).transpose(2, 3) @ g.abs()) + u * dv.abs() + tiny
     return result + [(dq, edq), (dk, edk), (dv, edv)]
 
 

@@ -349,10 +349,8 @@ def test_empty(ctmr, dev):
             assert g.shape == t.shape and bool((g == 0).all())
 
 
-def test_refuses_fp16_gradients_and_foreign_documents(ctmr, dev):
+def test_refuses_foreign_documents(ctmr, dev):
     f = ctmr.differentiable
     q, k, v, _ = _inputs(dev, 1, 2, 2, 8, 8, 16, torch.float16)
-    with pytest.raises(ValueError, match="float16 gradient"):
-        f.attention(q.detach().requires_grad_(), k, v, scale=1.0)
     with pytest.raises(ValueError, match="documents are for"):
         f.attention(q, k, v, scale=1.0, documents=f.Documents(torch.zeros(1, 9, dtype=torch.int32, device=dev)))

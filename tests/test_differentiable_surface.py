@@ -199,7 +199,7 @@ def test_attention_host_checks(ctmr, native_loaded):
     for kw in ({"q": None}, {"out": None}, {"lse": None}, {"dout": None}, {"s": None}, {"dq": p, "dq_s": None},
                {"dout": p + 8}, {"dq": p + 8}, {"s": bad}, {"dq": p, "dq_s": bad}, {"out_strides": (25600, 32, 130)}):
         assert back(**kw) == L.E_INVALID, kw
-    assert back(elem=L.ELEM_F16) == L.E_UNSUPPORTED and back(nbytes=100, dq=p) == L.E_WORKSPACE
+    assert back(elem=L.ELEM_F16) == L.OK and back(nbytes=100, dq=p) == L.E_WORKSPACE
     assert back(ws=None, dq=p) == L.E_WORKSPACE
 
     docs = native_loaded.ctmr_documents_bytes
