@@ -17,7 +17,7 @@
 // Bound by the softmax's vector operations (five a score: fma, exp, a sum, half a
 // maximum, half a conversion) with heads of 32 and 64, by them and the matrix products
 // in turn with 128: bf16, 2 x 16 heads of 4096 rows, every key: heads of 32 124 us
-// (556 TFLOP/s), of 64 179 (769), of 128 302 (911); fp32, 2 x 8 heads of 2048 rows of
+// (556 TFLOP/s), of 64 179 (769), of 128 290 (948); fp32, 2 x 8 heads of 2048 rows of
 // 32: 84 us, 102 TFLOP/s of the products alone, which run at 153 at best.
 #include "masked_attention.hpp"
 

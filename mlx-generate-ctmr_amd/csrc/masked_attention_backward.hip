@@ -21,8 +21,9 @@
 //
 // Bound by the matrix products and, at their side, the exponentials: 2 x 16 heads of
 // 4096 rows, every key, bf16, both kernels: heads of 32 327 us, of 64 505 (680 TFLOP/s
-// of the five products, 950 of the seven), of 128 1013; fp32, 2 x 8 heads of 2048 rows
-// of 32: 252 (119 of the seven, where a library product of 8192^3 reaches 153).
+// of the five products, 950 of the seven), of 128 990; fp16 370, 582, 1124 (two more
+// operations a score in dk and dv); fp32, 2 x 8 heads of 2048 rows of 32: 252 (119 of
+// the seven, where a library product of 8192^3 reaches 153).
 //
 // fp16's range is far smaller than what ds spans: |ds| < 2 d max |dout| max |v|, and
 // these two maxima of a key head (a pass over dout and v of its own) give the power of
