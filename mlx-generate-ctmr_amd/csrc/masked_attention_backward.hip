@@ -560,9 +560,9 @@ __global__ __launch_bounds__(kThreads) void attention_sum_kernel(SumArgs a) {
 
 // Parts of each block's stream where the blocks alone do not fill the chip: as many workgroups as it holds at a time
 // (one a CU where a row has 256 bytes or more, else two), of at least `least` steps.  From the shape only, so that a
-// shape's sums have one order.  1500 rows of 8 heads on 2 key heads of 96 values, fp32: 471 us, 2288 in one part; 2000
-// rows of 16 heads on 4 of 128, bf16: 223, 535 in one part; 256 rows of 2 x 16 heads of 32, bf16, whose 64 blocks have
-// 4 steps each: 26 as one part, 31 as two.
+// shape's sums have one order.  2000 rows of 16 heads on 4 key heads of 128, bf16: 183 us, 382 in one part; 1500 rows
+// of 8 heads on 2 of 64: 74, 174 in one part; 256 rows of 2 x 16 heads of 32, whose 64 blocks have 4 steps each: 24 as
+// one part, 30 as two.
 constexpr int kMostParts = 64;
 int part_count(int64_t blocks, int64_t steps, int elem, int head_dim) {
   const int64_t slots = padded(head_dim) * elem_bytes(elem) >= 256 ? 256 : 512;
