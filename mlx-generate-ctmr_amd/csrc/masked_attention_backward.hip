@@ -494,8 +494,8 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
     write_gradient<T, ND>(static_cast<T*>(a.dv) + b * a.dvb + hk * a.dvh + (int64_t)j * a.dvl, dv, lower_p, a.d, lane);
 }
 
-// The largest finite |v| and |dout| of each key head, rows that see nothing and padding aside.  blockIdx.y: dout or v;
-// blockIdx.x: part of a key head.  The maximum does not depend on the order.
+// The largest finite |v| and |dout| of each key head, padding and rows that see nothing (lse is infinite) aside.
+// blockIdx.y: dout or v; blockIdx.x: part of a key head.  The maximum does not depend on the order.
 __global__ __launch_bounds__(kThreads) void attention_most_zero_kernel(unsigned* most, int count) {
   const int i = blockIdx.x * kThreads + threadIdx.x;
   if (i < count) most[i] = 0u;
@@ -505,16 +505,14 @@ __global__ __launch_bounds__(kThreads) void attention_most_kernel(Args a, int pa
   const int item = blockIdx.x / parts, b = item / a.hk, hk = item % a.hk;
   const bool values = blockIdx.y == 1;
   const int rows = values ? a.lk : a.lq, pieces = a.d / 8;
-  const int prefix = a.prefixed ? prefix_of(a, b) : 0;
-  const int* ids = a.qdoc.ids ? (values ? a.kdoc.ids + (int64_t)b * a.kdoc.stride : a.qdoc.ids + (int64_t)b * a.qdoc.stride)
-                              : nullptr;
+  const int* ids = values && a.kdoc.ids ? a.kdoc.ids + (int64_t)b * a.kdoc.stride : nullptr;
   const int64_t count = (int64_t)rows * pieces * (values ? 1 : a.group);
   unsigned top = 0u;
   for (int64_t at = (int64_t)(blockIdx.x % parts) * kThreads + threadIdx.x; at < count; at += (int64_t)parts * kThreads) {
     const int piece = (int)(at % pieces);
     const int64_t line = at / pieces;
     const int i = (int)(line % rows), h = hk * a.group + (int)(line / rows);
-    if ((ids && ids[i] < 0) || (!values && limit_of(a, i, prefix) <= 0)) continue;
+    if (ids ? ids[i] < 0 : !values && a.lse[((int64_t)b * a.hq + h) * a.lq + i] == INFINITY) continue;
     const _Float16* row = values ? static_cast<const _Float16*>(a.v) + b * a.vb + hk * a.vh + (int64_t)i * a.vl
                                  : static_cast<const _Float16*>(a.dout) + b * a.gb + h * a.gh + (int64_t)i * a.gl;
     const u4 v = *reinterpret_cast<const u4*>(row + 8 * piece);

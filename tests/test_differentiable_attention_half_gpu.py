@@ -78,6 +78,25 @@ def test_rows_that_see_nothing_do_not_lower_the_gradients(ctmr, dev):
     assert all(torch.equal(a, b) for a, b in zip(clean, again))
 
 
+def test_documents_without_keys_do_not_lower_the_gradients(ctmr, dev):
+    f = ctmr.differentiable
+    q, k, v, dout = (t.contiguous() for t in _inputs(dev, 2, 2, 1, 70, 900, 32, torch.float16, seed=6))
+    dout = (dout.float() * 2.0 ** -10).half()
+    ids, key_ids = (torch.zeros(2, l, dtype=torch.int32, device=dev) for l in (70, 900))
+    ids[:, 40:] = 7  # no key is of it
+    documents, mask = f.Documents(ids, key_ids), oracle.visible(2, 70, 900, dev, ids, key_ids)
+    results = []
+    for value in (None, 65504.0):
+        if value is not None:
+            dout[:, :, 40:] = value
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = f.attention(*leaves, scale=0.2, documents=documents)
+        results.append([out.detach(), *torch.autograd.grad(out, leaves, dout)])
+        for t, w in zip(results[-1], oracle.attention(q, k, v, scale=0.2, mask=mask, dout=dout)):
+            oracle.check(t, w)
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 def test_visible_infinity_and_nan_show(ctmr, dev):
     for value in (math.inf, math.nan):
         q, k, v, dout = (t.contiguous() for t in _inputs(dev, 1, 1, 1, 70, 70, 32, torch.float16, seed=4))
