@@ -613,12 +613,13 @@ __global__ __launch_bounds__(kTile) void document_hulls_kernel(DocArgs a) {
   }
   const bool padded = __any(i < a.rows[side] && id < 0 && first >= 0);
   const int4 own = document_run(a, 1 - side, b, lane, first, first);
-  const int4 rest = document_run(a, 1 - side, b, lane, least, most);
+  int4 rest = document_run(a, 1 - side, b, lane, least, most);
+  if (padded) rest.z = INT_MAX, rest.w = 0;  // the padding goes with the other documents and sees none of their tiles
   if (lane == 0) {
     int4* hull = a.hull[side] + 3 * ((int64_t)b * a.grains[side] + grain);
     hull[0] = own;
     hull[1] = rest;
-    // padding among the rows is as good as another document that no tile holds
+    // padding among the rows is as good as another document that no tile holds, so no tile is whole for the rest
     hull[2] = least <= most ? int4{padded ? -1 : least, most, 0, 0} : padded ? int4{-1, -1, 0, 0} : int4{1, 0, 0, 0};
   }
 }

@@ -276,8 +276,8 @@ struct Side {        // documents of the query or key rows
   const int* ids;    // (n, rows rounded up to kTile), -1 past the end
   const DocTile* tiles;
   // Three for kGrain rows: tiles of the other side, [x, y) that may hold a match of the first row's document and
-  // [z, w) that hold nothing else; the same of the other rows' documents ([z, w) empty if they are of several);
-  // the least and the largest id of these, x > y if there are none.
+  // [z, w) that hold nothing else; the same of the other rows' documents ([z, w) empty if they are of several, or
+  // padding is among them); the least and the largest id of these (-1: padding), x > y if there are none.
   const int4* hull;
   const int* mixed;  // whether kBlockRows rows are of more than one document
   int stride, count, grains;  // ids, tiles and hulls of a batch item
