@@ -293,7 +293,6 @@ struct Args {
   const void* dout;
   void *dq, *dk, *dv;
   float* delta;           // (n, hq, lq) -sum_d dout out
-  unsigned* most;         // fp16 gradients: (n, hk, 2) bits of the largest |dout| and |v|, as fp32
   const float* slopes;    // (hq)
   const int* prefixes;    // (n), or null with `prefix`
   Side qdoc, kdoc;        // ids null: no documents

@@ -21,14 +21,16 @@
 //
 // Bound by the matrix products and, at their side, the exponentials: 2 x 16 heads of
 // 4096 rows, every key, bf16, both kernels: heads of 32 327 us, of 64 505 (680 TFLOP/s
-// of the five products, 950 of the seven), of 128 990; fp16 370, 582, 1124 (two more
-// operations a score in dk and dv); fp32, 2 x 8 heads of 2048 rows of 32: 252 (119 of
-// the seven, where a library product of 8192^3 reaches 153).
+// of the five products, 950 of the seven), of 128 990; fp16 378, 568, 1147 (the powers of
+// two below: two operations a score in dk and dv, half a one in dq); fp32, 2 x 8 heads of
+// 2048 rows of 32: 252 (119 of the seven, where a library product of 8192^3 reaches 153).
 //
-// fp16's range is far smaller than what ds spans: |ds| < 2 d max |dout| max |v|, and
-// these two maxima of a key head (a pass over dout and v of its own) give the power of
-// two that takes ds just below 2^15; p is raised by 2^15. Both come out of the sums
-// again at the end, exactly, so weights and ds down to 2^-39 of their largest count.
+// fp16's range is far smaller than what ds spans, so every row of dq and every key of
+// dk (a lane's column) has a power of two of its own that ds is multiplied by: the sums
+// start with 2^40 and move down, like a running maximum, when a ds passes 2^15.  Values
+// of ds down to 2^-38 of the largest that the row or key has met count, whatever other
+// rows, heads and documents hold.  p is raised by 2^15.  All comes out of the sums again
+// at the end, exactly.
 #include "masked_attention.hpp"
 
 #include <algorithm>
@@ -51,14 +53,34 @@ __host__ __device__ __forceinline__ float ds_scale(const Args& a) {
 template <typename T>
 constexpr bool kHalf = std::is_same_v<T, _Float16>;
 constexpr float kRaise = 15.0f;  // of p, in log2
-
-// log2 of what ds of a key head is multiplied by: 0 but in fp16.
+// log2 of what fp16's ds are multiplied by at first: those that need more (below 2^-54, where they lose bits) are nothing
+// in a gradient, |ds k| < 2^-38, and the largest, below 2^40, stay far from fp32's end.
 template <typename T>
-__device__ __forceinline__ int ds_raise(const Args& a, int b, int hk) {
-  if constexpr (!kHalf<T>) return 0;
-  const unsigned* most = a.most + 2 * ((int64_t)b * a.hk + hk);
-  const float bound = 2.0f * (float)a.d * __uint_as_float(most[0]) * __uint_as_float(most[1]);
-  return bound > 0.f ? 15 - __builtin_amdgcn_frexp_expf(bound) : 0;
+constexpr float kDsRaise = kHalf<T> ? 40.0f : 0.0f;
+
+// Keeps a lane's ds, multiplied by 2^raise, in fp16's range, its sums with them: a ds past 2^15 takes the largest to
+// [2^13, 2^14).  What is not finite moves nothing.  The lanes of a column, l and l + 32, move together.
+// ACC: the sums live in accumulation registers, and are taken out of them nowhere but here (left to itself the compiler
+// moves dk's 64 to and fro in each block: 2 x 16 heads of 4096 rows of 128, dk and dv 787 us for 740).
+template <bool ACC, int ND>
+__device__ __forceinline__ void keep_in_range(f16v& ds, f16v (&sums)[ND], float& raise) {
+  float top = fabsf(ds[0]);
+#pragma unroll
+  for (int r = 1; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
+  top = half_max(top);
+  const bool over = top > 32768.0f && top < INFINITY;
+  if (__any(over)) {
+    const int down = over ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
+    const float factor = __builtin_ldexpf(1.0f, -down);
+    ds *= factor;
+#pragma unroll
+    for (int n = 0; n < ND; ++n) {
+      if constexpr (ACC) asm("" : "+a"(sums[n]));
+      sums[n] *= factor;
+      if constexpr (ACC) asm("" : "+a"(sums[n]));
+    }
+    raise -= (float)down;
+  }
 }
 
 // Products of a 32 x 32 block -> log2 scores in units of 1 / c (c returned).  Row r of a lane is `at` + 8 (r / 4) + r
@@ -80,6 +102,16 @@ __device__ __forceinline__ float scores(const Scoring& a, f16v& s, f16v& ds, int
     for (int r = 0; r < 16; ++r) s[r] = fmaf(per, fabsf(from + (float)(8 * (r >> 2) + (r & 3))), s[r]);
   }
   return c;
+}
+
+// Takes fp16's 2^raise out of the sums.
+template <typename T, int ND>
+__device__ __forceinline__ void lower(f16v (&sums)[ND], float raise) {
+  if constexpr (kHalf<T>) {
+    const float factor = __builtin_ldexpf(1.0f, -(int)raise);
+#pragma unroll
+    for (int n = 0; n < ND; ++n) sums[n] *= factor;
+  }
 }
 
 template <typename T, int ND>
@@ -170,8 +202,8 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
   delta = half_sum(delta);
   if (real && half == 0 && blockIdx.y == 0) a.delta[stat] = -delta;
   if (!a.dq) return;
-  const int raise = ds_raise<T>(a, b, h / a.group);
-  const float lse = (real ? a.lse[stat] : INFINITY) - (float)raise;
+  const float lse = real ? a.lse[stat] : INFINITY;
+  float raise = kDsRaise<T>;
   f16v dq[ND];
 #pragma unroll
   for (int n = 0; n < ND; ++n) dq[n] = f16v(0.f);
@@ -215,7 +247,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
       const int at = k0 + 32 * u + 4 * half;
       const float c = scores<T, CAP>(scoring, s, ds, at, pos);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] *= __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse));
+      for (int r = 0; r < 16; ++r) ds[r] *= __builtin_amdgcn_exp2f(fmaf(s[r], c, kHalf<T> ? raise - lse : -lse));
       if (masked) {
         // a visible key whose values were zeroed in LDS because they are not finite: no gradient is
         const unsigned set = partial ? odd[u] >> (4 * half) : 0u;
@@ -235,6 +267,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
 #pragma unroll
           for (int r = 0; r < 16; ++r) ds[r] = 8 * (r >> 2) + (r & 3) >= limit - at ? 0.f : ds[r];
       }
+      if constexpr (kHalf<T>) keep_in_range<false, ND>(ds, dq, raise);
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const Frag<T> f = result_frag<T>(ds, w);
@@ -249,12 +282,12 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
     if (tile + 1 < last) step(tile + 1, kt1, vt1, kt0, vt0);
   }
   if (!real) return;
-  const float lower = __builtin_ldexpf(1.0f, -raise);
+  lower<T, ND>(dq, raise);
   if (a.splits > 1)
-    write_gradient<float, ND>(a.part + ((int64_t)blockIdx.y * a.n * a.hq * a.lq + stat) * D, dq, lower, D, lane);
+    write_gradient<float, ND>(a.part + ((int64_t)blockIdx.y * a.n * a.hq * a.lq + stat) * D, dq, 1.0f, D, lane);
   else
-    write_gradient<T, ND>(static_cast<T*>(a.dq) + b * a.dqb + h * a.dqh + (int64_t)i * a.dql, dq,
-                          ds_scale<T, CAP>(a) * lower, a.d, lane);
+    write_gradient<T, ND>(static_cast<T*>(a.dq) + b * a.dqb + h * a.dqh + (int64_t)i * a.dql, dq, ds_scale<T, CAP>(a),
+                          a.d, lane);
 }
 
 template <typename T, int D>
@@ -333,8 +366,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
     }
   };
   Scoring scoring = scoring_of(a, hk * a.group);
-  const int raise = ds_raise<T>(a, b, hk);
-  const float raised = __builtin_ldexpf(1.0f, raise - (int)kRaise);  // of ds, whose p is raised already
+  float raise = kDsRaise<T>;
   // One tile, while the next one is on its way into the other arrays.
   auto step = [&](bool more, char* qt, char* gt, float* stats, char* next_qt, char* next_gt, float* next_stats) {
     if (++tile == last) {
@@ -407,6 +439,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
       }
       const int at = i0 + 32 * u + 4 * half;
       const float c = scores<T, CAP>(scoring, s, ds, at, j - off);
+      const float raised = kHalf<T> ? __builtin_ldexpf(1.0f, (int)(raise - kRaise)) : 1.0f;  // p is raised already
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const f4 lse = *reinterpret_cast<const f4*>(stats + 32 * u + 8 * w + 4 * half);
@@ -438,6 +471,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
 #pragma unroll
           for (int r = 0; r < 16; ++r) hide(r, 8 * (r >> 2) + (r & 3) < j - off - at);
       }
+      if constexpr (kHalf<T>) keep_in_range<D == 128, ND>(ds, dk, raise);
       if constexpr (kAhead) {
         read_down(1);
         __builtin_amdgcn_sched_barrier(0);
@@ -479,55 +513,20 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
     if (s + 1 < mine.y) step(s + 2 < mine.y, qt1, gt1, stats1, qt0, gt0, stats0);
   }
   if (!real) return;
-  const float lower = __builtin_ldexpf(1.0f, -raise), lower_p = kHalf<T> ? __builtin_ldexpf(1.0f, -(int)kRaise) : 1.0f;
+  lower<T, ND>(dk, raise);
+  lower<T, ND>(dv, kRaise);
   if (a.splits > 1) {
     const int64_t rows = (int64_t)a.n * a.hk * a.lk;
     float* part = a.part + (2 * blockIdx.y * rows + ((int64_t)b * a.hk + hk) * a.lk + j) * D;
-    if (a.dk) write_gradient<float, ND>(part, dk, lower, D, lane);
-    if (a.dv) write_gradient<float, ND>(part + rows * D, dv, lower_p, D, lane);
+    if (a.dk) write_gradient<float, ND>(part, dk, 1.0f, D, lane);
+    if (a.dv) write_gradient<float, ND>(part + rows * D, dv, 1.0f, D, lane);
     return;
   }
   if (a.dk)
-    write_gradient<T, ND>(static_cast<T*>(a.dk) + b * a.dkb + hk * a.dkh + (int64_t)j * a.dkl, dk,
-                          ds_scale<T, CAP>(a) * lower, a.d, lane);
+    write_gradient<T, ND>(static_cast<T*>(a.dk) + b * a.dkb + hk * a.dkh + (int64_t)j * a.dkl, dk, ds_scale<T, CAP>(a),
+                          a.d, lane);
   if (a.dv)
-    write_gradient<T, ND>(static_cast<T*>(a.dv) + b * a.dvb + hk * a.dvh + (int64_t)j * a.dvl, dv, lower_p, a.d, lane);
-}
-
-// The largest finite |v| and |dout| of each key head, padding and rows that see nothing (lse is infinite) aside.
-// blockIdx.y: dout or v; blockIdx.x: part of a key head.  The maximum does not depend on the order.
-__global__ __launch_bounds__(kThreads) void attention_most_zero_kernel(unsigned* most, int count) {
-  const int i = blockIdx.x * kThreads + threadIdx.x;
-  if (i < count) most[i] = 0u;
-}
-
-__global__ __launch_bounds__(kThreads) void attention_most_kernel(Args a, int parts) {
-  const int item = blockIdx.x / parts, b = item / a.hk, hk = item % a.hk;
-  const bool values = blockIdx.y == 1;
-  const int rows = values ? a.lk : a.lq, pieces = a.d / 8;
-  const int* ids = values && a.kdoc.ids ? a.kdoc.ids + (int64_t)b * a.kdoc.stride : nullptr;
-  const int64_t count = (int64_t)rows * pieces * (values ? 1 : a.group);
-  unsigned top = 0u;
-  for (int64_t at = (int64_t)(blockIdx.x % parts) * kThreads + threadIdx.x; at < count; at += (int64_t)parts * kThreads) {
-    const int piece = (int)(at % pieces);
-    const int64_t line = at / pieces;
-    const int i = (int)(line % rows), h = hk * a.group + (int)(line / rows);
-    if (ids ? ids[i] < 0 : !values && a.lse[((int64_t)b * a.hq + h) * a.lq + i] == INFINITY) continue;
-    const _Float16* row = values ? static_cast<const _Float16*>(a.v) + b * a.vb + hk * a.vh + (int64_t)i * a.vl
-                                 : static_cast<const _Float16*>(a.dout) + b * a.gb + h * a.gh + (int64_t)i * a.gl;
-    const u4 v = *reinterpret_cast<const u4*>(row + 8 * piece);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const unsigned lo = v[w] & 0x7fffu, hi = (v[w] >> 16) & 0x7fffu;
-      top = max(top, lo < 0x7c00u ? lo : 0u);
-      top = max(top, hi < 0x7c00u ? hi : 0u);
-    }
-  }
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, m));
-  if (threadIdx.x % 64 == 0 && top)
-    atomicMax(a.most + 2 * (int64_t)item + (values ? 1 : 0),
-              __float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)top)));
+    write_gradient<T, ND>(static_cast<T*>(a.dv) + b * a.dvb + hk * a.dvh + (int64_t)j * a.dvl, dv, 1.0f, a.d, lane);
 }
 
 // Adds the parts of gradients in order: four values a thread.  blockIdx.y: which of up to two gradients.
@@ -575,31 +574,14 @@ int key_parts(const ctmr_masked_attention_desc* d) {
                     ceil_div(d->lq, kTile) * (d->q_heads / d->k_heads), d->elem, d->head_dim);
 }
 
-// Bytes of delta, and of fp16's maxima, in the workspace; the parts follow, dq's and then, in the same place, dk's and dv's.
+// Bytes of delta in the workspace; the parts follow, dq's and then, in the same place, dk's and dv's.
 int64_t delta_bytes(const ctmr_masked_attention_desc* d) {
   return ceil_div((int64_t)d->n * d->q_heads * d->lq * 4, 16) * 16;
-}
-
-int64_t most_bytes(const ctmr_masked_attention_desc* d) {
-  return d->elem == CTMR_ELEM_F16 ? ceil_div((int64_t)d->n * d->k_heads * 8, 16) * 16 : 0;
 }
 
 template <typename T, int D, bool CAP>
 int launch(Args a, int qparts, int kparts, hipStream_t st) {
   const unsigned parts = a.qdoc.ids ? 2u : 1u;
-  if constexpr (kHalf<T>) {
-    const int heads = a.n * a.hk;
-    hipLaunchKernelGGL(attention_most_zero_kernel, dim3((unsigned)ceil_div(2 * (int64_t)heads, kThreads)), dim3(kThreads), 0,
-                       st, a.most, 2 * heads);
-    int rc = check_launch("attention_most_zero");
-    if (rc) return rc;
-    // about 1024 workgroups, of 16 KB at least
-    const int64_t pieces = (int64_t)std::max<int64_t>(a.lk, (int64_t)a.lq * a.group) * (a.d / 8);
-    const int cut = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / heads, ceil_div(pieces, 4 * kThreads)));
-    hipLaunchKernelGGL(attention_most_kernel, dim3(heads * (unsigned)cut, 2), dim3(kThreads), 0, st, a, cut);
-    rc = check_launch("attention_most");
-    if (rc) return rc;
-  }
   a.splits = a.dq ? qparts : 1;
   const unsigned q_blocks = a.n * a.hq * (unsigned)ceil_div(a.lq, kOwn) * parts;
   hipLaunchKernelGGL((attention_dq_kernel<T, D, CAP>), dim3(q_blocks, a.splits), dim3(kThreads), 0, st, a);
@@ -641,7 +623,7 @@ int64_t ctmr_masked_attention_backward_workspace_bytes(const ctmr_masked_attenti
   const int64_t q = query_parts(d), k = key_parts(d);
   const int64_t qbytes = q > 1 ? q * d->n * d->q_heads * d->lq * padded(d->head_dim) * 4 : 0;
   const int64_t kbytes = k > 1 ? 2 * k * d->n * d->k_heads * d->lk * padded(d->head_dim) * 4 : 0;
-  return delta_bytes(d) + most_bytes(d) + std::max(qbytes, kbytes);
+  return delta_bytes(d) + std::max(qbytes, kbytes);
 }
 
 int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const void* q, const void* k, const void* v,
@@ -673,8 +655,7 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const vo
   Args a = make_args(d, q, k, v, slopes, prefixes, plan);
   a.out = const_cast<void*>(out), a.rest = const_cast<void*>(rest), a.lse = const_cast<float*>(lse), a.dout = dout;
   a.dq = dq, a.dk = dk, a.dv = dv, a.delta = (float*)workspace;
-  a.most = (unsigned*)((char*)workspace + delta_bytes(d));
-  a.part = (float*)((char*)workspace + delta_bytes(d) + most_bytes(d));
+  a.part = (float*)((char*)workspace + delta_bytes(d));
   a.ob = d->out_strides[0], a.oh = d->out_strides[1], a.ol = d->out_strides[2];
   a.gb = dout_strides[0], a.gh = dout_strides[1], a.gl = row_stride(dout_strides, d->lq, d->head_dim);
   if (dq) a.dqb = dq_strides[0], a.dqh = dq_strides[1], a.dql = dq_strides[2];
