@@ -491,6 +491,7 @@ int ctmr_documents(int32_t n, int32_t lq, int32_t lk, const int32_t* query_ids, 
  * values of a head lie side by side and rows do not overlap (those of batch items
  * and heads may).  Scores of row i and key j, p_i = i + lk - lq:
  *   s = scale q_i . k_j;  softcap > 0: s = softcap tanh(s / softcap)
+ *     (softcap up to 1e30, scale / softcap between 1e-30 and 1e30)
  *   slopes (q_heads) or NULL: s -= slopes[h] |p_i - j|
  * Key j is visible to row i if: with `prefixed`, j <= p_i or j < the prefix
  * (prefixes[item], or the descriptor's value where that is NULL); with a plan
@@ -498,7 +499,7 @@ int ctmr_documents(int32_t n, int32_t lq, int32_t lk, const int32_t* query_ids, 
  * no key gives zeros.  What masked places hold has no effect, NaN included.
  * rest or NULL: what the rounding of out left out, of type elem, with out's strides
  * (16 bits; not written for fp32).  lse (n, q_heads, lq) or NULL: log2 of each
- * row's sum (of 16-bit types with a cap: of the scores less the cap), +inf for an
+ * row's sum (of 16-bit types with a cap up to 256: of the scores less the cap), +inf for an
  * empty row.  The gradients read both.
  * The kernel splits long keys over workgroups where there are few rows: workspace
  * of ctmr_masked_attention_workspace_bytes, 16-byte aligned. */

@@ -44,8 +44,8 @@ struct RowMask {
 };
 
 // Raw products of NB 32-key blocks -> scores in units of 1 / c (c returned): the products, or with a cap cap_scores,
-// less the distance in these units.  Masked keys become -inf; ids: of the keys from k0 on, or null.
-template <typename T, int NB>
+// less the distance in these units.  CAP: the form of a cap, if there is one.  Masked keys become -inf; ids: of the keys from k0 on, or null.
+template <typename T, int NB, Cap CAP>
 __device__ __forceinline__ float score_blocks(const Scoring& a, f16v (&s)[NB], int k0, int pos, bool partial,
                                               const RowMask& m, const int* ids, int lane) {
   const int half = lane >> 5;
@@ -53,8 +53,8 @@ __device__ __forceinline__ float score_blocks(const Scoring& a, f16v (&s)[NB], i
   if (a.cap > 0.f) {
     const float in = a.scale / a.cap;
 #pragma unroll
-    for (int u = 0; u < NB; ++u) cap_scores<T>(s[u], in);
-    c = a.cap * (kLog2e * kCapUnits<T>);
+    for (int u = 0; u < NB; ++u) cap_scores<CAP>(s[u], in);
+    c = a.cap * (kLog2e * kCapUnits<CAP>);
   }
   if (a.sloped) {
     const float per = -a.slope * kLog2e / c, from = (float)(k0 + 4 * half - pos);
@@ -200,7 +200,7 @@ __device__ __forceinline__ void write_row(const Args& a, const f16v (&o)[ND], fl
 // The tiled form: a workgroup of four waves takes 128 query rows of a head, 32 a
 // wave, and streams K and V through LDS in 64-key tiles: the next tile is loaded
 // straight into a second pair of arrays while the current one is multiplied.
-template <typename T, int D>
+template <typename T, int D, Cap CAP>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void attention_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
 #pragma unroll
       for (int n = 0; n < ND; ++n) vf[w][n] = Lds::down(vt, 16 * w, n, at);
     const int* tile_ids = docs ? ids + k0 : nullptr;
-    const float c = score_blocks<T, 2>(scoring, s, k0, pos, meet.masked(tile), mask, tile_ids, lane);
+    const float c = score_blocks<T, 2, CAP>(scoring, s, k0, pos, meet.masked(tile), mask, tile_ids, lane);
     float alpha;
     Frag<T> p[2][2];
     if (softmax_blocks<T, 2>(s, p, c, m, l, alpha)) {
@@ -324,7 +324,7 @@ constexpr int few_lds() {  // bytes; the join takes four 32 x D blocks of fp32 a
   return tiles > join ? tiles : join;
 }
 
-template <typename T, int D>
+template <typename T, int D, Cap CAP>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 64 ? 2 : 1) void attention_few_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
@@ -385,7 +385,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 64 ? 2 : 1) void a
     f16v s[1] = {f16v(0.f)};
 #pragma unroll
     for (int n = 0; n < NK; ++n) s[0] = mma<T>(Lds::along(kt, 0, n, lane), qf[n], s[0]);
-    const float c = score_blocks<T, 1>(scoring, s, k0, pos, partial, mask, docs ? ids + k0 : nullptr, lane);
+    const float c = score_blocks<T, 1, CAP>(scoring, s, k0, pos, partial, mask, docs ? ids + k0 : nullptr, lane);
     float alpha;
     Frag<T> p[1][2];
     if (softmax_blocks<T, 1>(s, p, c, m, l, alpha)) {
@@ -642,14 +642,24 @@ int split_count(const ctmr_masked_attention_desc* d) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / least, kMostSplits}));
 }
 
-template <typename T, int D>
-int launch(const Args& a, bool few, hipStream_t st) {
+template <typename T, int D, Cap CAP>
+void launch_form(const Args& a, bool few, hipStream_t st) {
   if (few)
-    hipLaunchKernelGGL((attention_few_kernel<T, D>), dim3(a.n * a.hk, a.splits), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((attention_few_kernel<T, D, CAP>), dim3(a.n * a.hk, a.splits), dim3(kThreads), 0, st, a);
   else
-    hipLaunchKernelGGL((attention_kernel<T, D>),
+    hipLaunchKernelGGL((attention_kernel<T, D, CAP>),
                        dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kRows) * (a.qdoc.ids ? 2u : 1u), a.splits), dim3(kThreads),
                        0, st, a);
+}
+
+template <typename T, int D>
+int launch(const Args& a, bool few, hipStream_t st) {
+  bool shifted = false;
+  if constexpr (sizeof(T) == 2) {  // without a cap too
+    shifted = shifted_cap<T>(a.cap);
+    if (shifted) launch_form<T, D, kShiftedCap>(a, few, st);
+  }
+  if (!shifted) launch_form<T, D, kExactCap>(a, few, st);
   const int rc = check_launch("masked_attention");
   if (rc || a.splits == 1) return rc;
   const int64_t rows = (int64_t)a.n * a.hq * a.lq;
@@ -711,6 +721,8 @@ int check_desc(const ctmr_masked_attention_desc* d) {
     return fail(CTMR_E_INVALID, "scale must be positive, softcap not negative, both finite");
   if (d->softcap > 0.f && !(d->scale / d->softcap < 1e30f))
     return fail(CTMR_E_INVALID, "softcap too small for the scale");
+  if (d->softcap > 1e30f || (d->softcap > 0.f && d->scale / d->softcap < 1e-30f))  // fp32 ends not far above
+    return fail(CTMR_E_INVALID, "softcap too large for the scale");
   if (d->lq > (1 << 28) || d->lk > (1 << 28) ||
       (int64_t)d->n * d->q_heads * ceil_div(std::max(d->lq, d->lk), kTile) > (1ll << 23))  // 2^32 threads
     return fail(CTMR_E_UNSUPPORTED, "too many rows");

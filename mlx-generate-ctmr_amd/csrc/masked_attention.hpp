@@ -287,8 +287,8 @@ struct Args {
   const void *q, *k, *v;
   void* out;
   void* rest;             // what rounding took from out, as out lies, or null
-  float* lse;             // (n, hq, lq) log2 of a row's sum (of 16-bit operands with a cap: of the scores less cap),
-                          // +inf for an empty row
+  float* lse;             // (n, hq, lq) log2 of a row's sum (with a shifted cap: of the scores less cap), +inf for an
+                          // empty row
   float* part;            // split keys: (splits, n, hq, lq, D) sums, then (.., 2) maximum and total
   const void* dout;
   void *dq, *dk, *dv;
@@ -324,14 +324,24 @@ __device__ __forceinline__ int id_of(const Args& a, int b, int i) {
   return a.qdoc.ids[(int64_t)b * a.qdoc.stride + i];
 }
 
-// With t = tanh(x per): t itself in fp32, (t - 1) / 2 = -1 / (1 + e^(2 x per)) for 16-bit operands, one operation less;
-// the softmax does not see the shift, and lse has it too.  The hardware's exponential and reciprocal are exact to about
-// 1e-7, which moves scores by under 2^-17 at a cap of 50.
+// Forms of the cap, t = tanh(x per) of a raw product x, each in kernels of its own (a choice at run time takes a wave a
+// SIMD from the forward kernels' registers).  Exact: t itself, in fp32 and for caps past kShiftedMost.
+// Shifted, 16-bit operands: (t - 1) / 2 = -1 / (1 + e^(2 x per)), one operation less; the softmax does not see the shift,
+// and lse has it too.  The hardware's exponential and reciprocal are exact to about 1e-7, which near -1/2, where small
+// scores lie, is an error of the score of 1e-7 caps whatever the score: 2e-5 at most, where fp16 rounds weights by 2e-4.
+// Forward, 2 x 16 heads of 4096 rows of 64, bf16: no cap 167 us, shifted 223, exact 334; gradients 497, 671, 858.
+enum Cap { kNoCap, kShiftedCap, kExactCap };
+constexpr float kShiftedMost = 256.0f;
 template <typename T>
-constexpr float kCapUnits = sizeof(T) == 4 ? 1.0f : 2.0f;  // of t in what is returned
-template <typename T>
+inline bool shifted_cap(float cap) {
+  return sizeof(T) == 2 && cap <= kShiftedMost;
+}
+// Of t in what is returned.
+template <Cap CAP>
+constexpr float kCapUnits = CAP == kShiftedCap ? 2.0f : 1.0f;
+template <Cap CAP>
 __device__ __forceinline__ void cap_scores(f16v& s, float per) {
-  if constexpr (sizeof(T) == 4) {
+  if constexpr (CAP == kExactCap) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = tanhf(s[r] * per);
   } else {
@@ -348,11 +358,11 @@ __device__ __forceinline__ void cap_scores(f16v& s, float per) {
   }
 }
 // 1 - t^2 of it, in units of kCapSlope.
-template <typename T>
-constexpr float kCapSlope = sizeof(T) == 4 ? 1.0f : -4.0f;
-template <typename T>
+template <Cap CAP>
+constexpr float kCapSlope = CAP == kShiftedCap ? -4.0f : 1.0f;
+template <Cap CAP>
 __device__ __forceinline__ float cap_slope(float s) {
-  return sizeof(T) == 4 ? fmaf(-s, s, 1.0f) : fmaf(s, s, s);
+  return CAP == kExactCap ? fmaf(-s, s, 1.0f) : fmaf(s, s, s);
 }
 
 __device__ __forceinline__ float half_max(float v) {

@@ -45,9 +45,9 @@ constexpr int kOwn = kBlockRows;  // rows that a workgroup keeps in registers
 static_assert(kOwn == 32 * kWaves && kOwn == 4 * kGrain, "32 rows a wave");
 
 // What dq and dk are multiplied by at the end.
-template <typename T, bool CAP>
+template <Cap CAP>
 __host__ __device__ __forceinline__ float ds_scale(const Args& a) {
-  return a.scale * (CAP ? kCapSlope<T> : 1.0f);
+  return a.scale * (CAP == kNoCap ? 1.0f : kCapSlope<CAP>);
 }
 
 template <typename T>
@@ -87,14 +87,14 @@ __device__ __forceinline__ void keep_in_range(f16v& ds, f16v (&sums)[ND], float&
 // % 4; `x` is where the distance to it is zero.  With CAP g . v - delta, in `ds`, is multiplied by 1 - t^2
 // (in units of kCapSlope).  (As a branch on the cap the factor was 48 instructions of 145 a block for every call: the
 // compiler computes and selects.)
-template <typename T, bool CAP>
+template <typename T, Cap CAP>
 __device__ __forceinline__ float scores(const Scoring& a, f16v& s, f16v& ds, int at, int x) {
   float c = a.scale * kLog2e;
-  if constexpr (CAP) {
-    cap_scores<T>(s, a.scale / a.cap);
+  if constexpr (CAP != kNoCap) {
+    cap_scores<CAP>(s, a.scale / a.cap);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) ds[r] *= cap_slope<T>(s[r]);
-    c = a.cap * (kLog2e * kCapUnits<T>);
+    for (int r = 0; r < 16; ++r) ds[r] *= cap_slope<CAP>(s[r]);
+    c = a.cap * (kLog2e * kCapUnits<CAP>);
   }
   if (a.sloped) {
     const float per = -a.slope * kLog2e / c, from = (float)(at - x);
@@ -145,7 +145,7 @@ constexpr int dq_waves() {
 }
 
 // dq and delta: 128 query rows of a head, key tiles streaming.
-template <typename T, int D, bool CAP>
+template <typename T, int D, Cap CAP>
 __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
       __syncthreads();
     }
     if (meet.skips(tile)) return;
-    const int la = fresh<D == 128 && sizeof(T) == 2 && CAP>(lane);
+    const int la = fresh<D == 128 && sizeof(T) == 2 && CAP != kNoCap>(lane);
     const bool masked = meet.masked(tile) || (partial && (odd[0] | odd[1]) != 0u);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
   if (a.splits > 1)
     write_gradient<float, ND>(a.part + ((int64_t)blockIdx.y * a.n * a.hq * a.lq + stat) * D, dq, 1.0f, D, lane);
   else
-    write_gradient<T, ND>(static_cast<T*>(a.dq) + b * a.dqb + h * a.dqh + (int64_t)i * a.dql, dq, ds_scale<T, CAP>(a),
+    write_gradient<T, ND>(static_cast<T*>(a.dq) + b * a.dqb + h * a.dqh + (int64_t)i * a.dql, dq, ds_scale<CAP>(a),
                           a.d, lane);
 }
 
@@ -296,7 +296,7 @@ constexpr int dkv_waves() {
 }
 
 // dk and dv: 128 keys of a key head, the query tiles of its heads streaming.
-template <typename T, int D, bool CAP>
+template <typename T, int D, Cap CAP>
 __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_kernel(Args a) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
     return;
   }
   if (a.dk)
-    write_gradient<T, ND>(static_cast<T*>(a.dk) + b * a.dkb + hk * a.dkh + (int64_t)j * a.dkl, dk, ds_scale<T, CAP>(a),
+    write_gradient<T, ND>(static_cast<T*>(a.dk) + b * a.dkb + hk * a.dkh + (int64_t)j * a.dkl, dk, ds_scale<CAP>(a),
                           a.d, lane);
   if (a.dv)
     write_gradient<T, ND>(static_cast<T*>(a.dv) + b * a.dvb + hk * a.dvh + (int64_t)j * a.dvl, dv, 1.0f, a.d, lane);
@@ -579,7 +579,7 @@ int64_t delta_bytes(const ctmr_masked_attention_desc* d) {
   return ceil_div((int64_t)d->n * d->q_heads * d->lq * 4, 16) * 16;
 }
 
-template <typename T, int D, bool CAP>
+template <typename T, int D, Cap CAP>
 int launch(Args a, int qparts, int kparts, hipStream_t st) {
   const unsigned parts = a.qdoc.ids ? 2u : 1u;
   a.splits = a.dq ? qparts : 1;
@@ -588,7 +588,7 @@ int launch(Args a, int qparts, int kparts, hipStream_t st) {
   int rc = check_launch("attention_dq");
   if (rc) return rc;
   if (a.splits > 1) {
-    SumArgs s = {a.part, {a.dq, nullptr}, {a.dqb, 0}, {a.dqh, 0}, {a.dql, 0}, {ds_scale<T, CAP>(a), 0.f},
+    SumArgs s = {a.part, {a.dq, nullptr}, {a.dqb, 0}, {a.dqh, 0}, {a.dql, 0}, {ds_scale<CAP>(a), 0.f},
                  a.n * a.hq * a.lq, a.hq, a.lq, a.d, a.splits, 1};
     hipLaunchKernelGGL((attention_sum_kernel<T, D>), dim3((unsigned)ceil_div((int64_t)s.rows * (D / 4), kThreads)),
                        dim3(kThreads), 0, st, s);
@@ -601,7 +601,7 @@ int launch(Args a, int qparts, int kparts, hipStream_t st) {
   hipLaunchKernelGGL((attention_dkv_kernel<T, D, CAP>), dim3(k_blocks, a.splits), dim3(kThreads), 0, st, a);
   rc = check_launch("attention_dkv");
   if (rc || a.splits == 1) return rc;
-  SumArgs s = {a.part, {a.dk, a.dv}, {a.dkb, a.dvb}, {a.dkh, a.dvh}, {a.dkl, a.dvl}, {ds_scale<T, CAP>(a), 1.0f},
+  SumArgs s = {a.part, {a.dk, a.dv}, {a.dkb, a.dvb}, {a.dkh, a.dvh}, {a.dkl, a.dvl}, {ds_scale<CAP>(a), 1.0f},
                a.n * a.hk * a.lk, a.hk, a.lk, a.d, a.splits, 2};
   hipLaunchKernelGGL((attention_sum_kernel<T, D>), dim3((unsigned)ceil_div((int64_t)s.rows * (D / 4), kThreads), 2),
                      dim3(kThreads), 0, st, s);
@@ -664,8 +664,11 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* d, const vo
   const int qparts = query_parts(d), kparts = key_parts(d);
   hipStream_t st = (hipStream_t)stream;
   const bool cap = d->softcap > 0.f;
-#define CTMR_ATTENTION_CASE(T, D) \
-  return cap ? launch<T, D, true>(a, qparts, kparts, st) : launch<T, D, false>(a, qparts, kparts, st);
+#define CTMR_ATTENTION_CASE(T, D)                                             \
+  if (!cap) return launch<T, D, kNoCap>(a, qparts, kparts, st);               \
+  if constexpr (sizeof(T) == 2)                                               \
+    if (shifted_cap<T>(d->softcap)) return launch<T, D, kShiftedCap>(a, qparts, kparts, st); \
+  return launch<T, D, kExactCap>(a, qparts, kparts, st);
 #define CTMR_ATTENTION_TYPE(T)              \
   switch (padded(d->head_dim)) {            \
     case 32: CTMR_ATTENTION_CASE(T, 32)     \

@@ -310,7 +310,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
 
     Raises:
         ValueError: on other types, devices or shapes, a scale that is not positive and finite, a cap that is
-            negative or too small beside it, or slopes that need a gradient."""
+            negative or too small or large beside it, or slopes that need a gradient."""
     _activation(q, "q", 4)
     _like(k, q, "k", 4)
     _like(v, q, "v", 4)
@@ -327,6 +327,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
         raise ValueError(f"scale must be positive, softcap not negative, both finite; got {scale} and {softcap}")
     if softcap > 0.0 and not scale / softcap < 1e30:
         raise ValueError(f"softcap {softcap} is too small for a scale of {scale}")
+    if softcap > 1e30 or (softcap > 0.0 and scale / softcap < 1e-30):
+        raise ValueError(f"softcap {softcap} is too large for a scale of {scale}")
     if slopes is not None:
         if not isinstance(slopes, Tensor) or slopes.dtype != torch.float32 or tuple(slopes.shape) != (hq,) or (
                 slopes.device != q.device):
