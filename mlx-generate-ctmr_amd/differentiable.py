@@ -39,17 +39,29 @@ class _EagerGraph:
         self.leaves = [weakref.ref(t) for t in leaves]
 
 
+def _leaf(t: Tensor) -> Optional[Tensor]:
+    """The leaf that ``t`` is, or is made of by operators of one input: views, copies, casts."""
+    if t.is_leaf:
+        return t
+    node = t.grad_fn
+    while node is not None and node.name() != "torch::autograd::AccumulateGrad":
+        inputs = node.next_functions
+        node = inputs[0][0] if len(inputs) == 1 else None
+    return None if node is None else node.variable
+
+
 def _graph_token(*tensors: Optional[Tensor]) -> Optional[_EagerGraph]:
     """What an autograd node keeps while it lives: a mark on the leaves of a call made outside a capture.
 
     A leaf has one gradient accumulator for all graphs that hold it, bound to the stream of the first.  A
     backward pass captured into a HIP graph while an eager graph of the same leaf lives would make the
-    capture wait for a stream outside it, which ends the process; such a call is refused here.
+    capture wait for a stream outside it, which ends the process; such a call is refused here.  Leaves count
+    that these operators were given, or a view, copy or cast of.
 
     Raises:
         RuntimeError: in a capture, if a leaf belongs to a living graph recorded outside it."""
-    tracked = [t for t in tensors if t is not None and t.requires_grad]
-    leaves = [t for t in (t if t._base is None else t._base for t in tracked) if t.requires_grad and t.is_leaf]  # views'
+    leaves = [_leaf(t) for t in tensors if t is not None and t.requires_grad]
+    leaves = [t for t in leaves if t is not None]
     if not leaves:
         return None
     if not torch.cuda.is_current_stream_capturing():

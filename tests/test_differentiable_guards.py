@@ -17,3 +17,63 @@ def test_caps_at_the_end_of_the_range(ctmr, native_loaded, softcap, scale, good)
     d = L.MaskedAttentionDesc(1, 4, 4, 1, 1, 16, 0, 0, 0, scale, softcap, 0, *([(64, 64, 16)] * 4))
     code = native_loaded.ctmr_masked_attention_workspace_bytes(ctypes.byref(d))
     assert code == 0 if good else code == L.E_INVALID
+
+
+@pytest.fixture
+def capture(ctmr, monkeypatch):
+    """Sets whether a capture is under way."""
+    state = {"on": False}
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["on"])
+    return lambda on: state.update(on=on)
+
+
+def _made(f, kind):
+    """A leaf, and what an operator's own preparation makes of it before autograd sees it."""
+    big = torch.zeros(4, 6, 8, 16)
+    if kind == "a slice":
+        leaf = big[0:2].requires_grad_()
+        return leaf, leaf
+    if kind == "a transposed leaf":
+        leaf = big.transpose(1, 2).requires_grad_()
+        return leaf, leaf.contiguous()
+    if kind == "a strided leaf, norm":
+        leaf = big[..., ::2].requires_grad_()
+        return leaf, leaf.contiguous()
+    if kind == "heads, rotary":
+        leaf = big.transpose(2, 3).requires_grad_()
+        assert not leaf.is_contiguous()
+        return leaf, f._heads(leaf)
+    if kind == "heads, attention":
+        leaf = torch.zeros(4 * 6 * 8 * 16 + 1)[1:].view(4, 6, 8, 16).requires_grad_()
+        made = f._attention_heads(leaf)
+        assert made is not leaf
+        return leaf, made
+    leaf = big.requires_grad_()
+    return leaf, {"a view": leaf.flatten(0, 1), "views of views": leaf[1:].transpose(0, 1)[2].unbind(0)[1],
+                  "a cast": leaf.to(torch.bfloat16), "a cast view": leaf.to(torch.float16)[1].transpose(0, 1).contiguous()}[kind]
+
+
+@pytest.mark.parametrize("kind", ["a slice", "a transposed leaf", "a strided leaf, norm", "heads, rotary", "heads, attention",
+                                  "a view", "views of views", "a cast", "a cast view"])
+def test_leaves_behind_copies_casts_and_views_are_held(ctmr, capture, kind):
+    f = ctmr.differentiable
+    leaf, made = _made(f, kind)
+    token = f._graph_token(made)
+    assert token is not None
+    capture(True)
+    for t in (leaf, made, leaf.reshape(-1), leaf.to(torch.bfloat16)):
+        with pytest.raises(RuntimeError, match="outside this capture"):
+            f._graph_token(t)
+    assert f._graph_token(torch.zeros(2, requires_grad=True), leaf.detach()) is None
+    del token
+    assert f._graph_token(leaf) is None
+
+
+def test_a_held_leaf_is_found_whichever_way_it_was_recorded(ctmr, capture):
+    f = ctmr.differentiable
+    leaf = torch.zeros(3, 4).requires_grad_()
+    token = f._graph_token(leaf)
+    capture(True)
+    with pytest.raises(RuntimeError, match="outside this capture"):
+        f._graph_token(leaf.T.contiguous().half())
+    del token
