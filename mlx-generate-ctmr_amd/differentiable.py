@@ -1,4 +1,4 @@
-"""Operators of the networks' attention blocks with gradients, on fp32, bf16 and fp16 tensors.
+"""Operators of the networks' attention blocks with gradients (reverse mode), on fp32, bf16 and fp16 tensors.
 
 The reference is inference only; these are what fine-tuning its UNet and ControlNet (``unet.py``,
 ``attention.py``) needs beside the fp32 surface of ``fast_fp32``:
@@ -22,6 +22,7 @@ from typing import Optional, Union
 import torch
 import torch.nn.functional as F
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -102,6 +103,13 @@ def _activation(t, name: str, ndim: Optional[int] = None) -> Tensor:
     return t
 
 
+def _no_tangents(*tensors: Optional[Tensor]) -> None:
+    """Refuses dual tensors, whose tangents no kernel carries on."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise NotImplementedError("there are no forward-mode derivatives of this operator; use reverse mode")
+
+
 def _on_gpu(t: Tensor, name: str) -> None:
     if t.device.type != "cuda":
         raise ValueError(f"{name} must be on the GPU (there is no CPU path); got {t.device}")
@@ -146,7 +154,8 @@ def group_norm(x: Tensor, weight: Tensor, bias: Tensor, *, num_groups: int, eps:
 
     Raises:
         ValueError: on other types, devices or shapes, channels that the groups do not divide, or an ``eps``
-            that is negative or not finite."""
+            that is negative or not finite.
+        NotImplementedError: on forward-mode (dual) tensors."""
     _activation(x, "x")
     if x.dim() < 2:
         raise ValueError(f"x must be (N, ..., C); got shape {tuple(x.shape)}")
@@ -162,6 +171,7 @@ def group_norm(x: Tensor, weight: Tensor, bias: Tensor, *, num_groups: int, eps:
                              f"{tuple(t.shape)} {t.dtype} on {t.device}")
     if weight.dtype != bias.dtype:
         raise ValueError(f"weight and bias differ in type: {weight.dtype} and {bias.dtype}")
+    _no_tangents(x, weight, bias)
     _on_gpu(x, "x")
     x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias.requires_grad):
@@ -208,7 +218,8 @@ def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, *, sections: Seque
 
     Raises:
         ValueError: on other types, devices or shapes, sections that are odd, not positive, wider than the head
-            or not one for each axis, or a base that is not positive and finite."""
+            or not one for each axis, or a base that is not positive and finite.
+        NotImplementedError: on forward-mode (dual) tensors."""
     _activation(q, "q", 4)
     b, hq, l, d = (int(v) for v in q.shape)
     if hq < 1:
@@ -230,6 +241,7 @@ def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, *, sections: Seque
     if tuple(positions.shape) not in ((l, len(sections)), (1, l, len(sections)), (b, l, len(sections))):
         raise ValueError(f"positions must be ({l}, {len(sections)}) or ({b}, {l}, {len(sections)}); got "
                          f"{tuple(positions.shape)}")
+    _no_tangents(q, k, positions)
     _on_gpu(q, "q")
     positions = positions.detach().contiguous()
     q, k = _heads(q), None if k is None else _heads(k)
@@ -322,7 +334,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
 
     Raises:
         ValueError: on other types, devices or shapes, a scale that is not positive and finite, a cap that is
-            negative or too small or large beside it, or slopes that need a gradient."""
+            negative or too small or large beside it, or slopes that need a gradient.
+        NotImplementedError: on forward-mode (dual) tensors."""
     _activation(q, "q", 4)
     _like(k, q, "k", 4)
     _like(v, q, "v", 4)
@@ -359,6 +372,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
         raise ValueError(f"documents are for {documents.shape} rows on {documents.device}; got {(b, lq, lk)} on "
                          f"{q.device}")
     needs = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    _no_tangents(q, k, v, slopes)
     _on_gpu(q, "q")
     q, k, v = _attention_heads(q), _attention_heads(k), _attention_heads(v)
     plan = None if documents is None else documents.plan

@@ -77,3 +77,46 @@ def test_a_held_leaf_is_found_whichever_way_it_was_recorded(ctmr, capture):
     with pytest.raises(RuntimeError, match="outside this capture"):
         f._graph_token(leaf.T.contiguous().half())
     del token
+
+
+def _calls(f, dtype=torch.float32):
+    """Each operator as a function of one of its tensors, and that tensor."""
+    x, w = torch.zeros(2, 5, 8, dtype=dtype), torch.ones(8, dtype=dtype)
+    q, k = torch.zeros(2, 4, 6, 16, dtype=dtype), torch.zeros(2, 2, 6, 16, dtype=dtype)
+    at = torch.zeros(6, 1)
+    norm = lambda x, w, b: f.group_norm(x, w, b, num_groups=2, eps=1e-6)
+    turn = lambda q, k, at: f.rotary(q, k, at, sections=(16,))[0]
+    att = lambda q, k, v, s=None: f.attention(q, k, v, scale=1.0, slopes=s)
+    return {"norm x": (lambda t: norm(t, w, w), x), "norm weight": (lambda t: norm(x, t, w), w),
+            "norm bias": (lambda t: norm(x, w, t), w), "rotary q": (lambda t: turn(t, k, at), q),
+            "rotary k": (lambda t: turn(q, t, at), k), "rotary positions": (lambda t: turn(q, k, t), at),
+            "attention q": (lambda t: att(t, k, k), q), "attention k": (lambda t: att(q, t, k), k),
+            "attention v": (lambda t: att(q, k, t), k), "attention slopes": (lambda t: att(q, k, k, t), torch.zeros(4))}
+
+
+NAMES = ["norm x", "norm weight", "norm bias", "rotary q", "rotary k", "rotary positions", "attention q", "attention k",
+         "attention v", "attention slopes"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("tracked", [False, True])
+def test_forward_mode_is_refused(ctmr, name, tracked):
+    """A tangent would vanish without a word: the kernels have reverse-mode gradients only."""
+    call, t = _calls(ctmr.differentiable)[name]
+    t.requires_grad_(tracked and name != "attention slopes")
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(ValueError, match="on the GPU"):  # no tangent: as outside
+            call(t)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(call, (t.detach(),), (torch.ones_like(t),))
+
+
+def test_forward_mode_through_the_block_is_refused(ctmr):
+    c = 16
+    w = {f"attn.{n}.{p}": torch.zeros(*((c, c) if p == "weight" else (c,)))
+         for n in ("to_q", "to_k", "to_v", "out_proj") for p in ("weight", "bias")}
+    call = lambda t: ctmr.differentiable.self_attention_tokens(t, w, heads=2, scale=1.0, include_fc=True)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(call, (torch.zeros(1, 5, c),), (torch.ones(1, 5, c),))
