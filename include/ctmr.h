@@ -442,7 +442,8 @@ int ctmr_flash_attention_f16x2(const ctmr_attn_desc* desc, const float* q, const
 enum ctmr_elem { CTMR_ELEM_F32 = 0, CTMR_ELEM_BF16 = 1, CTMR_ELEM_F16 = 2 };
 
 /* Group norm (+ SiLU) of channels-last rows x (n, s voxels, c), statistics over
- * s x (c / groups) values, biased variance.  gamma and beta (c) are of type
+ * s x (c / groups) values, biased variance.  Sums are fp64, but for 32 voxels of a
+ * channel at a time in fp32 (again in fp64 where squares leave its range).  gamma and beta (c) are of type
  * param_elem.  saved (n, groups, 4) fp32, 16-byte aligned, is what the backward
  * call reads: the mean as two floats, 1 / sqrt(var + eps), and one unused.
  * y may equal x.  The workspace is 16-byte aligned (0 bytes for small groups). */

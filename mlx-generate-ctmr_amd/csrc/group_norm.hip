@@ -13,8 +13,9 @@
 // by HBM: x is read twice (the second time from the 256 MB memory-side cache
 // where it fits), in the backward pass dy too.  Sums are fp64, but for 32 rows at a
 // time in fp32, of x less the thread's first value: E[x^2] - mean^2 then keeps the
-// variance of a channel whose mean is a thousand times its spread.  The mean is kept
-// as two floats (hi + lo), so x - mean is exact to fp32 also there.
+// variance of a channel whose mean is a thousand times its spread.  Rows whose squares
+// leave fp32's range are added again in fp64.  The mean is kept as two floats (hi + lo),
+// so x - mean is exact to fp32 also there.
 // Measured: 80x128x128 voxels of 64 channels, bf16: forward 103 us, backward 194 (3.3
 // and 2.6 TB/s of the bytes that both passes would need at least, 4.7 a copy);
 // 45x90x117 of 128, fp16: 74 and 129; 2 x 8x8x4 of 512, bf16 (small form): 12 and 17,
@@ -30,6 +31,7 @@
 #include "elements.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ctmr {
 namespace {
@@ -117,6 +119,33 @@ __device__ __forceinline__ void reduce_rows(double (&v)[W], double* lds, int col
 // the channel, so that they lose nothing to a mean far above the spread.
 constexpr int kBatch = 32;
 
+// Whether fp32 lost a batch's squares: an overflow (spreads past 1.8e19, and NaN, which fp64 does not mend either), or
+// with an eps that is nothing beside them an underflow.  Never of fp16's range.
+template <typename T, int V>
+__device__ __forceinline__ bool outside_fp32(const Vec<float, V>& q, float eps) {
+  if constexpr (std::is_same_v<T, _Float16>) return false;
+  const float least = eps < 1e-18f ? 0x1p-90f : -1.0f;  // 32 squares, each off by 2^-150 at most
+  bool lost = false;
+#pragma unroll
+  for (int k = 0; k < V; ++k) lost |= !(q[k] < INFINITY) || q[k] < least;
+  return lost;
+}
+
+// Such a batch again, in fp64 throughout.
+template <typename T, int V>
+__device__ __forceinline__ void add_wide(double* acc, int slots, const T* x, int64_t step, int batch, Vec<float, V> x0) {
+#pragma unroll 1
+  for (int r = 0; r < batch; ++r) {
+    const Vec<float, V> v = load_as_float<T, V>(x + r * step);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const double d = (double)v[k] - (double)x0[k];
+      acc[k * slots] += d;
+      acc[(V + k) * slots] += d * d;
+    }
+  }
+}
+
 // The fp64 sums wait in LDS, where they are added up at the end.
 template <typename T, int V, bool BACKWARD>
 __global__ __launch_bounds__(kThreads, BACKWARD ? 4 : 5) void gn_sums_kernel(NormArgs a) {
@@ -152,6 +181,10 @@ __global__ __launch_bounds__(kThreads, BACKWARD ? 4 : 5) void gn_sums_kernel(Nor
           for (int k = 0; k < V; ++k) q[k] = fmaf(d[k], d[k], q[k]);
         }
         left -= batch;
+        if (__builtin_expect(outside_fp32<T, V>(q, a.eps), 0)) {
+          add_wide<T, V>(acc, slots, x - batch * step, step, batch, x0);
+          continue;
+        }
 #pragma unroll
         for (int k = 0; k < V; ++k) {
           acc[k * slots] += (double)p[k];

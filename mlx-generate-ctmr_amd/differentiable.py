@@ -149,8 +149,10 @@ def group_norm(x: Tensor, weight: Tensor, bias: Tensor, *, num_groups: int, eps:
     """Group norm, and SiLU with ``apply_silu``, of channels-last ``x`` ``(N, ..., C)``; differentiable.
 
     ``x`` is fp32, bf16 or fp16 (a copy is made where it is not contiguous); ``weight`` and ``bias`` ``(C,)``
-    are fp32 or ``x``'s type.  Statistics are fp64 sums over each batch item's voxels and ``C / num_groups``
-    channels with the biased variance; the output has ``x``'s type, the gradients their inputs' types.
+    are fp32 or ``x``'s type.  Statistics are over each batch item's voxels and ``C / num_groups`` channels, with the
+    biased variance.  Their sums, and the gradients', are fp64, but for 32 voxels of a channel at a time in fp32 (of
+    differences to one of the values; again in fp64 where squares leave fp32's range).  The output has ``x``'s type, the
+    gradients their inputs' types.
 
     Raises:
         ValueError: on other types, devices or shapes, channels that the groups do not divide, or an ``eps``
