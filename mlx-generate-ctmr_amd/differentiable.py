@@ -27,8 +27,9 @@ from torch.autograd.function import once_differentiable
 
 from . import ops
 
-# Autograd graphs recorded outside any capture that hold leaves, by what each saved (see _graph_token).
-_eager_graphs: "weakref.WeakSet[_EagerGraph]" = weakref.WeakSet()
+# Autograd graphs recorded outside any capture that hold leaves, by their identity (see _graph_token).  A plain dictionary:
+# its single operations, and the list of its values, are whole whatever other threads and the collector do meanwhile.
+_eager_graphs: dict[int, "weakref.ref[_EagerGraph]"] = {}
 
 
 class _EagerGraph:
@@ -38,6 +39,8 @@ class _EagerGraph:
 
     def __init__(self, leaves: list[Tensor]):
         self.leaves = [weakref.ref(t) for t in leaves]
+        key = id(self)
+        _eager_graphs[key] = weakref.ref(self, lambda _, graphs=_eager_graphs: graphs.pop(key, None))
 
 
 def _leaf(t: Tensor) -> Optional[Tensor]:
@@ -66,11 +69,10 @@ def _graph_token(*tensors: Optional[Tensor]) -> Optional[_EagerGraph]:
     if not leaves:
         return None
     if not torch.cuda.is_current_stream_capturing():
-        token = _EagerGraph(leaves)
-        _eager_graphs.add(token)
-        return token
-    for token in list(_eager_graphs):
-        for ref in token.leaves:
+        return _EagerGraph(leaves)
+    for graph in list(_eager_graphs.values()):
+        token = graph()
+        for ref in () if token is None else token.leaves:
             held = ref()
             if held is not None and any(held is t for t in leaves):
                 raise RuntimeError("an autograd graph recorded outside this capture still holds one of its leaves; "

@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import ctypes
+import sys
+import threading
 
 import pytest
 import torch
@@ -120,3 +122,37 @@ def test_forward_mode_through_the_block_is_refused(ctmr):
     call = lambda t: ctmr.differentiable.self_attention_tokens(t, w, heads=2, scale=1.0, include_fc=True)
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(call, (torch.zeros(1, 5, c),), (torch.ones(1, 5, c),))
+
+
+def test_a_capture_while_other_threads_record(ctmr, monkeypatch):
+    """The living graphs are walked while others come and go in threads of their own."""
+    f, main = ctmr.differentiable, threading.get_ident()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: threading.get_ident() == main)
+    stop, failures = threading.Event(), []
+
+    def record():
+        try:
+            leaf = torch.zeros(2, requires_grad=True)
+            kept = []
+            while not stop.is_set():
+                kept.append(f._graph_token(leaf))
+                if len(kept) > 200:
+                    kept.clear()
+        except Exception as error:
+            failures.append(error)
+
+    threads = [threading.Thread(target=record) for _ in range(4)]
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        for t in threads:
+            t.start()
+        leaf = torch.zeros(2, requires_grad=True)
+        for _ in range(1500):
+            assert f._graph_token(leaf) is None
+    finally:
+        sys.setswitchinterval(interval)
+        stop.set()
+        for t in threads:
+            t.join()
+    assert not failures
