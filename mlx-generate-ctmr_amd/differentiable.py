@@ -287,10 +287,17 @@ class Documents:
         return self.plan.device
 
 
+def _address(t: Tensor) -> int:
+    """Where ``t`` starts; what is traced has no address, and memory of its own starts on a multiple of 16 bytes."""
+    if type(t) in (Tensor, torch.nn.Parameter) and not torch.compiler.is_compiling():
+        return t.data_ptr()
+    return t.storage_offset() * t.element_size()
+
+
 def _attention_heads(t: Tensor) -> Tensor:
     """``t`` with a unit last stride and 16-byte aligned rows that do not overlap, in a stride that the kernels address."""
     size = t.element_size()
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0:
+    if t.stride(3) == 1 and _address(t) % 16 == 0:
         strides = ops._head_strides(t)
         if (all(s * size % 16 == 0 for s in strides) and strides[2] * size <= 1 << 23
                 and (t.shape[2] <= 1 or strides[2] >= t.shape[3])):

@@ -156,3 +156,29 @@ def test_a_capture_while_other_threads_record(ctmr, monkeypatch):
         for t in threads:
             t.join()
     assert not failures
+
+
+@pytest.mark.filterwarnings("error:Accessing the data pointer")
+@pytest.mark.parametrize("tracked", [False, True])
+def test_public_operators_trace(ctmr, monkeypatch, tracked):
+    """On fake tensors: shapes, types and strides without an address being read."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    f = ctmr.differentiable
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    with FakeTensorMode():
+        make = lambda *s, dtype=torch.bfloat16: torch.empty(*s, device="cuda", dtype=dtype)
+        q, k = (make(2, 6, h, 32).transpose(1, 2).requires_grad_(tracked) for h in (4, 2))
+        odd = make(2 * 2 * 6 * 32 + 1)[1:].view(2, 2, 6, 32)  # copied: its address is no multiple of 16 bytes
+        ids = make(2, 6, dtype=torch.int32)
+        for v in (k, odd, make(2, 2, 6, 64)[..., ::2]):
+            out = f.attention(q, k, v, scale=0.2, documents=f.Documents(ids))
+            assert out.shape == q.shape and out.dtype == q.dtype and out.transpose(1, 2).is_contiguous()
+        turned = f.rotary(q, k, make(6, 2, dtype=torch.int32), sections=(8, 8))
+        assert [t.shape for t in turned] == [q.shape, k.shape]
+        x, w = make(2, 5, 8).requires_grad_(tracked), make(8, dtype=torch.float32)
+        assert f.group_norm(x, w, w, num_groups=2, eps=1e-6).shape == x.shape
+        weights = {f"attn.{n}.{p}": make(*((64, 64) if p == "weight" else (64,)))
+                   for n in ("to_q", "to_k", "to_v", "out_proj") for p in ("weight", "bias")}
+        tokens = make(1, 5, 64).requires_grad_(tracked)
+        assert f.self_attention_tokens(tokens, weights, heads=2, scale=1.0, include_fc=True).shape == tokens.shape
