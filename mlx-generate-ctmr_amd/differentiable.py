@@ -258,13 +258,27 @@ def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, *, sections: Seque
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
+def _stream_of(t: Tensor) -> Optional[int]:
+    """The stream that ``t`` is being made on; None on the host and where calls are traced."""
+    return ops._raw_stream(t.device) if t.is_cuda and type(t) is Tensor else None
+
+
+def _used(t: Tensor, made: Optional[int]) -> Tensor:
+    """``t``, which was made on the stream ``made``: its memory stays until the current stream's work so far and the
+    call to come are done, also if its owner is gone before.  (A captured graph's user keeps the owner.)"""
+    if made is not None and ops._raw_stream(t.device) != made and not torch.cuda.is_current_stream_capturing():
+        t.record_stream(torch.cuda.current_stream(t.device))
+    return t
+
+
 class Documents:
     """Which query rows and keys belong together, laid out once for every ``attention`` of a batch.
 
     ``ids`` ``(B, Lq)`` int32 holds each query row's document, ``key_ids`` ``(B, Lk)`` each key's (the same rows
     if left out).  A row sees the keys of its own document; negative ids are padding, which sees and is seen by
     nothing.  Ids may come in any order, but only rows of a document that lie side by side let the kernels skip
-    the rest.  The ids are copied: changing the tensors afterwards changes nothing here.
+    the rest.  The ids are copied: changing the tensors afterwards changes nothing here.  Like a tensor, the documents are
+    made on the current stream, which other streams wait for, and outlive the graphs that captured them.
 
     Raises:
         ValueError: on ids that are not (B, L) int32 tensors of one device and batch on the GPU, or empty."""
@@ -281,6 +295,7 @@ class Documents:
         _on_gpu(ids, "ids")
         self.shape = (int(ids.shape[0]), int(ids.shape[1]), int(key_ids.shape[1]))
         self.plan = ops.documents(ids.contiguous(), key_ids.contiguous())
+        self._stream = _stream_of(self.plan)
 
     @property
     def device(self) -> torch.device:
@@ -386,7 +401,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
     _no_tangents(q, k, v, slopes)
     _on_gpu(q, "q")
     q, k, v = _attention_heads(q), _attention_heads(k), _attention_heads(v)
-    plan = None if documents is None else documents.plan
+    plan = None if documents is None else _used(documents.plan, documents._stream)
     if needs:
         return _Attention.apply(q, k, v, slopes, prefixes, plan, scale, softcap, prefix is not None, value)
     return ops.masked_attention(q, k, v, slopes, prefixes, plan, scale, softcap, prefix is not None, value, False)[0]
@@ -416,6 +431,7 @@ class PackedVolumes:
         grids = [torch.stack(torch.meshgrid(*(torch.arange(s, dtype=torch.int32) for s in shape), indexing="ij"),
                              dim=-1).reshape(-1, 3) for shape in self.shapes]
         self.positions = torch.cat(grids).to(device)
+        self._stream = _stream_of(self.positions)
         self.documents = None
         if len(self.shapes) > 1:
             ids = torch.repeat_interleave(torch.arange(len(self.shapes), dtype=torch.int32), torch.tensor(self.lengths))

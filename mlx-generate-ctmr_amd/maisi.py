@@ -147,7 +147,7 @@ def spatial_attention_volumes(volumes: Sequence[Tensor], weights: Mapping[str, T
     merged = df.self_attention_tokens(rows[0] if len(rows) == 1 else torch.cat(rows, dim=1), weights,
                                       heads=c // num_head_channels, scale=float(num_head_channels) ** -0.5,
                                       include_fc=include_fc, documents=packed.documents, sections=sections, base=base,
-                                      positions=None if sections is None else packed.positions)
+                                      positions=None if sections is None else df._used(packed.positions, packed._stream))
     return [v + part.reshape(v.shape) for v, part in zip(volumes, merged.split(packed.lengths, dim=1))]
 
 
