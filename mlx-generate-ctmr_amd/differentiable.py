@@ -105,6 +105,12 @@ def _activation(t, name: str, ndim: Optional[int] = None) -> Tensor:
     return t
 
 
+def _sizes(*sizes: int) -> None:
+    """Refuses sizes that the descriptors' 32 bits would cut short."""
+    if max(sizes) >= 1 << 31:
+        raise ValueError(f"sizes must be below 2^31; got {sizes}")
+
+
 def _no_tangents(*tensors: Optional[Tensor]) -> None:
     """Refuses dual tensors, whose tangents no kernel carries on."""
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
@@ -175,6 +181,7 @@ def group_norm(x: Tensor, weight: Tensor, bias: Tensor, *, num_groups: int, eps:
                              f"{tuple(t.shape)} {t.dtype} on {t.device}")
     if weight.dtype != bias.dtype:
         raise ValueError(f"weight and bias differ in type: {weight.dtype} and {bias.dtype}")
+    _sizes(int(x.shape[0]), c)
     _no_tangents(x, weight, bias)
     _on_gpu(x, "x")
     x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
@@ -245,6 +252,7 @@ def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, *, sections: Seque
     if tuple(positions.shape) not in ((l, len(sections)), (1, l, len(sections)), (b, l, len(sections))):
         raise ValueError(f"positions must be ({l}, {len(sections)}) or ({b}, {l}, {len(sections)}); got "
                          f"{tuple(positions.shape)}")
+    _sizes(b, hq, l)
     _no_tangents(q, k, positions)
     _on_gpu(q, "q")
     positions = positions.detach().contiguous()
@@ -292,6 +300,7 @@ class Documents:
                 raise ValueError(f"{name} is empty: {tuple(t.shape)}")
         if ids.device != key_ids.device or ids.shape[0] != key_ids.shape[0]:
             raise ValueError("ids and key_ids differ in device or batch")
+        _sizes(*ids.shape, *key_ids.shape)
         _on_gpu(ids, "ids")
         self.shape = (int(ids.shape[0]), int(ids.shape[1]), int(key_ids.shape[1]))
         self.plan = ops.documents(ids.contiguous(), key_ids.contiguous())
@@ -371,6 +380,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit each other")
     if hk < 1 or hq < 1 or hq % hk:
         raise ValueError(f"{hq} query heads are not a multiple of {hk} key heads")
+    _sizes(b, hq, lq, lk)
     if d < 8 or d % 8 or d > 128:
         raise ValueError(f"head width must be a multiple of 8 up to 128; got {d}")
     scale, softcap = float(scale), float(softcap)

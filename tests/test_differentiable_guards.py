@@ -182,3 +182,24 @@ def test_public_operators_trace(ctmr, monkeypatch, tracked):
                    for n in ("to_q", "to_k", "to_v", "out_proj") for p in ("weight", "bias")}
         tokens = make(1, 5, 64).requires_grad_(tracked)
         assert f.self_attention_tokens(tokens, weights, heads=2, scale=1.0, include_fc=True).shape == tokens.shape
+
+
+def test_sizes_past_32_bits_are_refused(ctmr):
+    """Sizes that would come out small in the descriptors' 32 bits: 2^32 + 64 rows are not 64."""
+    f, big = ctmr.differentiable, 2 ** 32 + 64
+    wide = lambda *s: torch.zeros(1).expand(*s)
+    row = torch.zeros(1, 1, 64, 8)
+    calls = [lambda: f.attention(wide(1, 1, big, 8), row, row, scale=1.0),
+             lambda: f.attention(row, wide(1, 1, big, 8), wide(1, 1, big, 8), scale=1.0),
+             lambda: f.attention(wide(big, 1, 1, 8), wide(big, 1, 1, 8), wide(big, 1, 1, 8), scale=1.0),
+             lambda: f.attention(wide(1, big, 1, 8), row[:, :, :1], row[:, :, :1], scale=1.0),
+             lambda: f.rotary(wide(1, 1, big, 8), None, wide(big, 1), sections=(8,)),
+             lambda: f.rotary(wide(big, 1, 1, 8), None, wide(1, 1), sections=(8,)),
+             lambda: f.rotary(wide(1, big, 1, 8), wide(1, big, 1, 8), wide(1, 1), sections=(8,)),
+             lambda: f.group_norm(wide(big, 1, 8), torch.zeros(8), torch.zeros(8), num_groups=2, eps=1e-6),
+             lambda: f.group_norm(wide(1, 1, big), wide(big), wide(big), num_groups=1, eps=1e-6),
+             lambda: f.Documents(torch.zeros(1, dtype=torch.int32).expand(1, big)),
+             lambda: f.Documents(torch.zeros(1, 64, dtype=torch.int32), torch.zeros(1, dtype=torch.int32).expand(1, big))]
+    for call in calls:
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()
