@@ -435,7 +435,7 @@ int ctmr_flash_attention_f16x2(const ctmr_attn_desc* desc, const float* q, const
  * Differentiable operators of the attention blocks, for activations of fp32,
  * bf16 or fp16.  No counterparts in the reference, which is inference only.
  * Sums, statistics and softmax are held in fp32 or fp64; each output is rounded
- * once.  No atomics: results are bit-identical run to run.  Like every entry
+ * once.  No sum is made by atomics: results are bit-identical run to run.  Like every entry
  * point they neither allocate nor synchronise, so calls may be captured into a
  * graph; two captures need workspaces of their own.
  */
@@ -443,9 +443,10 @@ enum ctmr_elem { CTMR_ELEM_F32 = 0, CTMR_ELEM_BF16 = 1, CTMR_ELEM_F16 = 2 };
 
 /* Group norm (+ SiLU) of channels-last rows x (n, s voxels, c), statistics over
  * s x (c / groups) values, biased variance.  Sums are fp64, but for 32 voxels of a
- * channel at a time in fp32 (again in fp64 where squares leave its range).  gamma and beta (c) are of type
- * param_elem.  saved (n, groups, 4) fp32, 16-byte aligned, is what the backward
- * call reads: the mean as two floats, 1 / sqrt(var + eps), and one unused.
+ * channel at a time in fp32 (again in fp64 where squares leave its range).  gamma
+ * and beta (c) are of type param_elem.  saved (n, groups, 4) fp32, 16-byte aligned,
+ * is what the backward call reads: the mean as two floats, 1 / sqrt(var + eps), and
+ * one unused.
  * y may equal x.  The workspace is 16-byte aligned (0 bytes for small groups). */
 int64_t ctmr_norm_workspace_bytes(int32_t n, int64_t s, int32_t c, int32_t groups, int32_t elem, int32_t backward);
 int ctmr_norm_forward(int32_t n, int64_t s, int32_t c, int32_t groups, float eps, int32_t elem, const void* x,
@@ -500,8 +501,8 @@ int ctmr_documents(int32_t n, int32_t lq, int32_t lk, const int32_t* query_ids, 
  * no key gives zeros.  What masked places hold has no effect, NaN included.
  * rest or NULL: what the rounding of out left out, of type elem, with out's strides
  * (16 bits; not written for fp32).  lse (n, q_heads, lq) or NULL: log2 of each
- * row's sum (of 16-bit types with a cap up to 256: of the scores less the cap), +inf for an
- * empty row.  The gradients read both.
+ * row's sum (of 16-bit types with a cap up to 256: of the scores less the cap), +inf
+ * for an empty row.  The gradients read both.
  * The kernel splits long keys over workgroups where there are few rows: workspace
  * of ctmr_masked_attention_workspace_bytes, 16-byte aligned. */
 typedef struct ctmr_masked_attention_desc {

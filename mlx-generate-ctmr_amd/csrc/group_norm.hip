@@ -18,8 +18,8 @@
 // so x - mean is exact to fp32 also there.
 // Measured: 80x128x128 voxels of 64 channels, bf16: forward 103 us, backward 194 (3.3
 // and 2.6 TB/s of the bytes that both passes would need at least, 4.7 a copy);
-// 45x90x117 of 128, fp16: 74 and 129; 2 x 8x8x4 of 512, bf16 (small form): 12 and 17,
-// the launches' time.
+// 45x90x117 of 128, fp16: 74 and 129 of values that the cache holds, 95 forward of
+// others; 2 x 8x8x4 of 512, bf16 (small form): 12 and 17, the launches' time.
 //
 // Two forms:
 //  * small (gn_small_*): a group's values stay in the registers of one

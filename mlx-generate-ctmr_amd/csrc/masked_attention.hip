@@ -43,8 +43,8 @@ struct RowMask {
   int limit, id;
 };
 
-// Raw products of NB 32-key blocks -> scores in units of 1 / c (c returned): the products, or with a cap cap_scores,
-// less the distance in these units.  CAP: the form of a cap, if there is one.  Masked keys become -inf; ids: of the keys from k0 on, or null.
+// Raw products of NB 32-key blocks -> scores in units of 1 / c (c returned): the products, or with a cap (in the form
+// CAP) cap_scores, less the distance in these units.  Masked keys become -inf; ids: of the keys from k0 on, or null.
 template <typename T, int NB, Cap CAP>
 __device__ __forceinline__ float score_blocks(const Scoring& a, f16v (&s)[NB], int k0, int pos, bool partial,
                                               const RowMask& m, const int* ids, int lane) {

@@ -13,10 +13,10 @@
 // Two kernels, each a stream of one side's tiles through LDS against 128 rows of
 // the other in registers: queries stay and keys stream for dq (and delta, which it
 // leaves for the other), keys stay and queries stream for dk and dv.  That is seven
-// products for the five of the formulas (scores and g . v twice), but no atomics:
-// each sum has one order, and the gradients are bit-identical run to run.  Where the
-// blocks of 128 rows do not fill the chip, each block's stream is cut into parts whose
-// fp32 sums a third kernel adds in order.  p and ds are rounded to the operands'
+// products for the five of the formulas (scores and g . v twice), but no additions in
+// memory: each sum has one order, and the gradients are bit-identical run to run.  Where
+// the blocks of 128 rows do not fill the chip, each block's stream is cut into parts
+// whose fp32 sums a third kernel adds in order.  p and ds are rounded to the operands'
 // type for their products, half a step of it on each term of an fp32 sum.
 //
 // Bound by the matrix products and, at their side, the exponentials: 2 x 16 heads of

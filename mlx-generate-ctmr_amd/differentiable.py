@@ -1,7 +1,7 @@
 """Operators of the networks' attention blocks with gradients (reverse mode), on fp32, bf16 and fp16 tensors.
 
-The reference is inference only; these are what fine-tuning its UNet and ControlNet (``unet.py``,
-``attention.py``) needs beside the fp32 surface of ``fast_fp32``:
+The reference is inference only; these are what fine-tuning its attention blocks (``attention.py``) needs beside the
+fp32 surface of ``fast_fp32``, whose convolutions have no gradients:
 
 * ``group_norm``  channels-last group norm + SiLU
 * ``rotary``      rotary positions over one to four axes (depth, height, width) for q and k
@@ -363,6 +363,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
     * ``documents`` hides the keys of other documents and padding (``Documents``).
 
     A row that sees no key gives zeros and gets no gradient.  What masked places hold has no effect, NaN included.
+    Scores are fp32: their size (the distance's too) is expected below some 2^20, where the weights still have digits.
     Statistics and sums are fp32; the softmax weights, and in the gradients those of the scores, are rounded to the
     inputs' type for their products (in fp16 raised by powers of two that keep them in its range).  The output has
     ``q``'s type and lies as ``(B, Lq, Hq, D)`` in memory, so merging the heads is a view.
