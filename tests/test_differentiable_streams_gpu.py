@@ -54,3 +54,34 @@ def test_packed_volumes(ctmr, dev):
     for part in (lambda packed: packed.positions, lambda packed: packed.documents.plan):
         got, reused = _while_another_stream_is_busy(make, use, part)
         assert not reused and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("kind", ["a slice", "a cast", "a strided leaf"])
+def test_a_refused_capture_leaves_the_process_sound(ctmr, dev, kind):
+    """The call is refused before it records anything; once the eager graph is gone the same capture works."""
+    f = ctmr.differentiable
+    g = torch.Generator(device=dev).manual_seed(2)
+    big = torch.randn(4, 60, 64, device=dev, generator=g)
+    leaf = {"a slice": big[1:3], "a cast": big, "a strided leaf": big[..., ::2]}[kind].requires_grad_()
+    w, b = torch.ones(leaf.shape[-1], device=dev), torch.zeros(leaf.shape[-1], device=dev)
+    dout = torch.randn(leaf.shape, device=dev, generator=g)
+
+    def step():
+        x = leaf.to(torch.bfloat16) if kind == "a cast" else leaf
+        y = f.group_norm(x, w, b, num_groups=4, eps=1e-6, apply_silu=True)
+        return y, torch.autograd.grad(y, leaf, dout.to(y.dtype))[0]
+
+    kept, want = step()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="outside this capture"):
+        with torch.cuda.graph(graph):
+            step()
+    del kept
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, grad = step()
+    for _ in range(3):
+        grad.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want)
