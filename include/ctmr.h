@@ -528,6 +528,40 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* desc, const
                                    const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
                                    const int64_t* dv_strides, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Lists of tensors (gradients, parameters): `count` tensors at tensors[i] (device
+ * memory, values side by side, on their type's own grid), of sizes[i] values and
+ * type elems[i]; the arrays are host memory, read before the call returns.  A tensor of
+ * no values may be NULL.  Sizes alone set the order of sums.
+ *
+ * The norm over all: norm_factor[0] = |scale| sqrt(sum g^2), squares added in fp64;
+ * norm_factor[1] = scale min(1, most / (norm + 1e-6)), NaN for a NaN (most INFINITY:
+ * scale).  The workspace is 16-byte aligned. */
+int64_t ctmr_gradients_workspace_bytes(int32_t count, const int64_t* sizes);
+int ctmr_gradient_norm(int32_t count, const void* const* gradients, const int64_t* sizes, const int32_t* elems,
+                       float scale, float most, float* norm_factor, void* workspace, size_t workspace_bytes, void* stream);
+/* Each value times factor[0] (device memory), rounded to its type.  Tensors may not overlap. */
+int ctmr_scale_tensors(int32_t count, void* const* tensors, const int64_t* sizes, const int32_t* elems,
+                       const float* factor, void* stream);
+/* One AdamW step t of parameters of the gradients' sizes and types, g = gradient times
+ * the factor that ctmr_gradient_norm gives for scale and most:
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   w -= lr decay w + lr m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps)
+ * m, v and, for parameters of 16 bits, w (the parameter is w rounded) are fp32, at
+ * starts[i] of exp_avg and exp_avg_sq and master_starts[i] of master (multiples of
+ * 4 values, 16-byte aligned memory); fp32 parameters are their own w.  steps (device) holds t - 1
+ * and gets t.  lr or NULL: device memory read in place of the descriptor's.  norm or
+ * NULL: gets the norm.  With `skip` a norm that is not finite leaves everything as it
+ * was.  The workspace is that of the sizes' norm.  Nothing may overlap. */
+typedef struct ctmr_adamw_desc {
+  double lr, beta1, beta2, eps, decay;
+  float scale, most;
+  int32_t skip, reserved;
+} ctmr_adamw_desc;
+int ctmr_adamw(const ctmr_adamw_desc* desc, int32_t count, void* const* parameters, const void* const* gradients,
+               const int64_t* sizes, const int32_t* elems, const int64_t* starts, const int64_t* master_starts,
+               float* exp_avg, float* exp_avg_sq, float* master, int64_t* steps, const float* lr, float* norm,
+               void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

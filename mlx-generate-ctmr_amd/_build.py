@@ -19,7 +19,7 @@ INCLUDE = REPO_DIR / "include"
 LIB_NAME = "libctmr_hip.so"
 LIB_PATH = PACKAGE_DIR / LIB_NAME
 SOURCES = ("conv.hip", "conv_lds.hip", "conv_march.hip", "norm.hip", "attention.hip", "noalloc.hip", "group_norm.hip",
-           "rotary.hip", "masked_attention.hip", "masked_attention_backward.hip")
+           "rotary.hip", "masked_attention.hip", "masked_attention_backward.hip", "gradients.hip")
 ARCH = "gfx950"
 
 # Packed FP32 VALU ops are disabled for every device pass; hipcc's host pass

@@ -73,6 +73,15 @@ class MaskedAttentionDesc(ctypes.Structure):
     )
 
 
+class AdamwDesc(ctypes.Structure):
+    """``ctmr_adamw_desc``."""
+
+    _fields_ = (
+        [(name, ctypes.c_double) for name in ("lr", "beta1", "beta2", "eps", "decay")]
+        + [("scale", ctypes.c_float), ("most", ctypes.c_float), ("skip", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+    )
+
+
 _c_int, _c_i32, _c_i64 = ctypes.c_int, ctypes.c_int32, ctypes.c_int64
 _vp, _sz, _f = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_float
 _desc_p = ctypes.POINTER(ConvDesc)
@@ -124,6 +133,10 @@ _PROTOTYPES = {
     "ctmr_masked_attention": (_c_int, [ctypes.POINTER(MaskedAttentionDesc)] + [_vp] * 10 + [_sz, _vp]),
     "ctmr_masked_attention_backward_workspace_bytes": (_c_i64, [ctypes.POINTER(MaskedAttentionDesc)]),
     "ctmr_masked_attention_backward": (_c_int, [ctypes.POINTER(MaskedAttentionDesc)] + [_vp] * 18 + [_sz, _vp]),
+    "ctmr_gradients_workspace_bytes": (_c_i64, [_c_i32, _vp]),
+    "ctmr_gradient_norm": (_c_int, [_c_i32, _vp, _vp, _vp, _f, _f, _vp, _vp, _sz, _vp]),
+    "ctmr_scale_tensors": (_c_int, [_c_i32, _vp, _vp, _vp, _vp, _vp]),
+    "ctmr_adamw": (_c_int, [ctypes.POINTER(AdamwDesc), _c_i32] + [_vp] * 13 + [_sz, _vp]),
 }
 
 _lock = threading.Lock()

@@ -10,6 +10,8 @@ fp32 surface of ``fast_fp32``, whose convolutions have no gradients:
 * ``PackedVolumes``  the documents and voxel positions of several volumes in one row
 * ``self_attention_tokens``  projections, rotary positions and attention of tokens
   (``maisi.spatial_attention_volumes`` is the networks' block over it)
+* ``gradient_norm``, ``clip_gradients``  the global norm of many gradients, and their clipping
+* ``AdamW``       steps of many parameters, clipping included
 """
 
 from __future__ import annotations
@@ -484,3 +486,230 @@ def self_attention_tokens(tokens: Tensor, weights: Mapping[str, Tensor], *, head
         merged = F.linear(merged, _like(weights[f"{prefix}.out_proj.weight"], tokens, f"{prefix}.out_proj.weight", 2),
                           _like(weights[f"{prefix}.out_proj.bias"], tokens, f"{prefix}.out_proj.bias", 1))
     return _hold(merged, token)
+
+
+# ---------------------------------------------------------------------------
+# lists of gradients and parameters
+# ---------------------------------------------------------------------------
+def _without_gaps(t: Tensor) -> bool:
+    """Whether ``t``'s values fill their memory, in any order of the axes."""
+    if t.is_contiguous():
+        return True
+    expected = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _listed(tensors, name: str) -> list[Tensor]:
+    """The tensors of a list, ``None`` left out, checked for type and device.  What autograd or tracing makes of them is not
+    looked at."""
+    if isinstance(tensors, Tensor):
+        raise ValueError(f"{name} must be a list of tensors")
+    out = [t for t in tensors if t is not None]
+    if not out:
+        raise ValueError(f"{name} holds no tensor")
+    device = out[0].device if isinstance(out[0], Tensor) else None
+    for t in out:
+        if not isinstance(t, Tensor) or t.layout != torch.strided:
+            raise ValueError(f"{name} must be dense tensors")
+        if t.dtype not in ops.ELEMENTS:
+            raise ValueError(f"{name} must be float32, bfloat16 or float16; got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{name} are on {device} and {t.device}")
+    _no_tangents(*out)
+    _on_gpu(out[0], name)
+    return out
+
+
+def _apart(tensors: Sequence[Tensor], name: str) -> None:
+    """Refuses tensors that are written and have gaps or share memory."""
+    if not all(_without_gaps(t) for t in tensors):
+        raise ValueError(f"{name} must fill their memory without gaps or overlaps")
+    if torch.compiler.is_compiling() or any(type(t) not in ops._PLAIN for t in tensors):
+        return  # what is traced has no address
+    spans = sorted([(t.data_ptr(), t.numel() * t.element_size()) for t in tensors if t.numel()])
+    if any(at + size > after for (at, size), (after, _) in zip(spans, spans[1:])):
+        raise ValueError(f"{name} share memory")
+
+
+def _most(max_norm) -> float:
+    max_norm = float(max_norm)
+    if not max_norm > 0.0:
+        raise ValueError(f"max_norm must be positive; got {max_norm}")
+    return max_norm
+
+
+@torch.no_grad()
+def gradient_norm(gradients: Sequence[Optional[Tensor]]) -> Tensor:
+    """The norm (square root of the sum of squares) over all values of a list of fp32, bf16 and fp16 gradients, 0-d fp32;
+    no gradient of its own.
+
+    ``None`` in the list is left out.  Squares are added in fp64, in an order that the sizes alone set.
+
+    Raises:
+        ValueError: on an empty list, other types, or tensors that are not on one GPU.
+        NotImplementedError: on forward-mode (dual) tensors."""
+    gradients = _listed(gradients, "gradients")
+    return ops.gradient_norm([t if _without_gaps(t) else t.contiguous() for t in gradients], 1.0, math.inf)[0]
+
+
+@torch.no_grad()
+def clip_gradients(gradients: Sequence[Optional[Tensor]], max_norm: float) -> Tensor:
+    """Multiplies gradients in place by ``min(1, max_norm / (norm + 1e-6))``; returns their ``gradient_norm`` before.
+
+    The factor stays on the device.  A norm that is not finite is not refused: an infinite one gives zeros (NaN where the
+    infinities were), a NaN gives NaN.  A factor of one writes nothing.
+
+    Raises:
+        ValueError: on what ``gradient_norm`` refuses, tensors that share memory or have gaps in it (expanded or sliced
+            ones), and a ``max_norm`` that is not positive.
+        NotImplementedError: on forward-mode (dual) tensors."""
+    max_norm, gradients = _most(max_norm), _listed(gradients, "gradients")
+    _apart(gradients, "gradients")
+    norm = ops.gradient_norm(gradients, 1.0, max_norm)
+    ops.scale_tensors(gradients, norm[1])
+    torch.autograd.graph.increment_version(gradients)
+    return norm[0]
+
+
+class AdamW:
+    """AdamW steps of a list of fp32, bf16 and fp16 parameters, in place and without a copy to the host.
+
+    ``w -= lr * weight_decay * w + lr * m_hat / (sqrt(v_hat) + eps)`` with the moments' usual bias corrections, all in
+    fp32.  Parameters of 16 bits have fp32 copies that the steps are made on, so that small steps are not lost to rounding;
+    what else changes such a parameter has to change its copy too (``load_masters``).
+
+    ``max_norm`` clips each step's gradients as ``clip_gradients`` does, without writing them; ``skip_non_finite`` leaves a
+    step out whose gradients have a norm that is not finite (for steps with a loss scale).
+
+    The state is public, on the parameters' device, and may be written between steps: ``steps`` (0-d int64), ``exp_avg``,
+    ``exp_avg_sq`` and ``master`` (1-d fp32; ``master`` of the 16-bit parameters only), where each parameter's values start
+    on a multiple of ``GRAIN``, in the list's order.  Steps may be captured into a graph; ``lr`` may then be a 0-d fp32 tensor.
+
+    Raises:
+        ValueError: on an empty list, other types, parameters that are not on one GPU, share memory or have gaps in it, and
+            settings out of their ranges."""
+
+    GRAIN = 64
+
+    @torch.no_grad()
+    def __init__(self, parameters: Sequence[Tensor], *, lr: Union[float, Tensor] = 1e-3,
+                 betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+                 max_norm: Optional[float] = None, skip_non_finite: bool = False):
+        parameters = parameters if isinstance(parameters, Tensor) else list(parameters)
+        if not isinstance(parameters, Tensor) and any(p is None for p in parameters):
+            raise ValueError("parameters must be dense tensors")
+        self.parameters = _listed(parameters, "parameters")
+        _apart(self.parameters, "parameters")
+        device = self.parameters[0].device
+        self.lr = self._rate(lr)
+        self.betas, self.eps, self.weight_decay = (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
+        if not all(0.0 <= b < 1.0 for b in self.betas):
+            raise ValueError(f"betas must be in [0, 1); got {self.betas}")
+        for name, value in (("eps", self.eps), ("weight_decay", self.weight_decay)):
+            if not (math.isfinite(value) and value >= 0.0):
+                raise ValueError(f"{name} must be finite and not negative; got {value}")
+        self.max_norm = math.inf if max_norm is None else _most(max_norm)
+        self.skip_non_finite = bool(skip_non_finite)
+        self._layouts = [(p.shape, p.stride(), p.dtype, p.device) for p in self.parameters]
+        self._starts, total = self._places(self.parameters)
+        half = [p for p in self.parameters if p.dtype != torch.float32]
+        starts, room = self._places(half)
+        starts = iter(starts)
+        self._master_starts = [0 if p.dtype == torch.float32 else next(starts) for p in self.parameters]
+        make = lambda n: torch.zeros(n, device=device, dtype=torch.float32)
+        self.exp_avg, self.exp_avg_sq, self.master = make(total), make(total), make(room)
+        self.steps = torch.zeros((), device=device, dtype=torch.int64)
+        self._stream = _stream_of(self.steps)
+        self.load_masters()
+
+    def _rate(self, lr: Union[float, Tensor]) -> Union[float, Tensor]:
+        if isinstance(lr, Tensor):
+            if lr.dtype != torch.float32 or lr.dim() != 0 or lr.device != self.parameters[0].device:
+                raise ValueError("lr must be a number or a 0-d float32 tensor on the parameters' device")
+            return lr
+        if not (math.isfinite(lr) and lr >= 0.0):
+            raise ValueError(f"lr must be finite and not negative; got {lr}")
+        return float(lr)
+
+    @classmethod
+    def _places(cls, parameters: Sequence[Tensor]) -> tuple[list[int], int]:
+        starts, at = [], 0
+        for p in parameters:
+            starts.append(at)
+            at += -(-p.numel() // cls.GRAIN) * cls.GRAIN
+        return starts, at
+
+    @staticmethod
+    def _values(p: Tensor) -> Tensor:
+        """The values in the order of their memory."""
+        return torch.as_strided(p, (p.numel(),), (1,))
+
+    @torch.no_grad()
+    def load_masters(self) -> None:
+        """Takes the fp32 copies from the parameters, after something else has changed these."""
+        for p, at in zip(self.parameters, self._master_starts):
+            if p.dtype != torch.float32:
+                self.master[at:at + p.numel()] = self._values(p)
+
+    def state_dict(self) -> dict[str, Tensor]:
+        """The state's tensors themselves, by name."""
+        return {name: getattr(self, name) for name in ("steps", "exp_avg", "exp_avg_sq", "master")}
+
+    @torch.no_grad()
+    def load_state_dict(self, state: Mapping[str, Tensor]) -> None:
+        """Copies a ``state_dict`` of the same parameters; the parameters of 16 bits become their copies, rounded.
+
+        Raises:
+            ValueError: on other names, or tensors of other shapes or types."""
+        own = self.state_dict()
+        if set(state) != set(own) or any(state[n].shape != t.shape or state[n].dtype != t.dtype for n, t in own.items()):
+            raise ValueError("the state is of other parameters")
+        for name, t in own.items():
+            t.copy_(state[name])
+        for p, at in zip(self.parameters, self._master_starts):
+            if p.dtype != torch.float32:
+                self._values(p).copy_(self.master[at:at + p.numel()])
+
+    @torch.no_grad()
+    def step(self, gradients: Sequence[Optional[Tensor]], *, lr: Union[float, Tensor, None] = None,
+             gradient_scale: float = 1.0) -> Tensor:
+        """One step from a gradient for each parameter (None: it and its moments stay); returns the norm, before clipping, of
+        the gradients times ``gradient_scale``, which is what the step takes (a loss scale's inverse).
+
+        Raises:
+            ValueError: on gradients of another count, or of other shapes, types or devices than their parameters', and an
+                ``lr`` or scale that is not finite.
+            NotImplementedError: on forward-mode (dual) tensors."""
+        gradients = list(gradients)
+        if len(gradients) != len(self.parameters):
+            raise ValueError(f"{len(gradients)} gradients for {len(self.parameters)} parameters")
+        lr, scale = self.lr if lr is None else self._rate(lr), float(gradient_scale)
+        if not math.isfinite(scale):
+            raise ValueError(f"gradient_scale must be finite; got {scale}")
+        _listed(gradients, "gradients")
+        used, taken = [], []
+        for i, (p, g) in enumerate(zip(self.parameters, gradients)):
+            if g is None:
+                continue
+            shape, strides, dtype, device = self._layouts[i]
+            if p.shape != shape or p.stride() != strides or p.dtype != dtype or p.device != device:
+                raise ValueError(f"parameter {i} has become another: {tuple(p.shape)} {p.stride()} {p.dtype} on {p.device}")
+            if g.shape != shape or g.dtype != dtype or g.device != device:
+                raise ValueError(f"gradient {i} is {tuple(g.shape)} {g.dtype} on {g.device}; its parameter {tuple(shape)} "
+                                 f"{dtype} on {device}")
+            if g.stride() != strides and not (g.is_contiguous() and p.is_contiguous()):
+                g = torch.empty_strided(shape, strides, dtype=dtype, device=device).copy_(g)
+            used.append(i)
+            taken.append(g)
+        parameters = self.parameters if len(used) == len(self.parameters) else [self.parameters[i] for i in used]
+        of = lambda values: values if len(used) == len(values) else [values[i] for i in used]
+        rate = (lr, 0.0) if isinstance(lr, Tensor) else (None, lr)
+        state = [_used(t, self._stream) for t in (self.exp_avg, self.exp_avg_sq, self.master, self.steps)]
+        norm = ops.adamw(parameters, taken, *state, rate[0], of(self._starts), of(self._master_starts), rate[1],
+                         *self.betas, self.eps, self.weight_decay, scale, self.max_norm, self.skip_non_finite)
+        torch.autograd.graph.increment_version([*parameters, *state])
+        return norm

@@ -32,8 +32,8 @@ class _CustomOp:
     """A registered ``ctmr::*`` operator (``.op``) whose eager calls on plain tensors skip the
     dispatcher."""
 
-    def __init__(self, name: str, fn: Callable):
-        self.op = torch.library.custom_op(name, mutates_args=())(fn)
+    def __init__(self, name: str, fn: Callable, mutates: Sequence[str] = ()):
+        self.op = torch.library.custom_op(name, mutates_args=tuple(mutates))(fn)
         self.fn = fn
         functools.update_wrapper(self, fn)
 
@@ -55,11 +55,16 @@ def _direct(values) -> bool:
     for v in values:
         if isinstance(v, Tensor) and (type(v) is not Tensor or (grad and v.requires_grad)):
             return False
+        if type(v) is list and not all(type(t) in _PLAIN and not (grad and t.requires_grad) for t in v):
+            return False
     return True
 
 
-def _custom_op(name: str) -> Callable[[Callable], _CustomOp]:
-    return lambda fn: _CustomOp(name, fn)
+_PLAIN = (Tensor, torch.nn.Parameter)  # of the tensors in lists
+
+
+def _custom_op(name: str, mutates: Sequence[str] = ()) -> Callable[[Callable], _CustomOp]:
+    return lambda fn: _CustomOp(name, fn, mutates)
 
 
 def _ptr(t: Optional[Tensor]) -> Optional[int]:
@@ -793,3 +798,91 @@ def _(q, k, v, slopes, prefixes, plan, out, rest, lse, dout, scale, softcap, pre
     none = (0,)
     return (_heads_like(q) if want_q else q.new_empty(none), _heads_like(k) if want_kv else k.new_empty(none),
             _heads_like(v) if want_kv else v.new_empty(none))
+
+
+# ---------------------------------------------------------------------------
+# lists of gradients and parameters
+# ---------------------------------------------------------------------------
+class _Sizes:
+    """Value counts and types of a list of tensors as the library takes them, and its workspace's bytes."""
+
+    __slots__ = ("count", "sizes", "elems", "nbytes")
+
+    def __init__(self, counts: Sequence[int], kinds: Sequence[torch.dtype]):
+        self.count = len(counts)
+        self.sizes = (ctypes.c_int64 * self.count)(*counts)
+        self.elems = (ctypes.c_int32 * self.count)(*[ELEMENTS[k] for k in kinds])
+        self.nbytes = _lib.check(_lib.lib().ctmr_gradients_workspace_bytes(self.count, self.sizes),
+                                 "ctmr_gradients_workspace_bytes")
+
+
+@functools.lru_cache(maxsize=64)
+def _sizes_of(counts: tuple[int, ...], kinds: tuple[torch.dtype, ...]) -> _Sizes:
+    return _Sizes(counts, kinds)
+
+
+def _list_sizes(tensors: Sequence[Tensor]) -> _Sizes:
+    return _sizes_of(tuple([t.numel() for t in tensors]), tuple([t.dtype for t in tensors]))
+
+
+def _addresses(tensors: Sequence[Tensor]):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+@_custom_op("ctmr::gradient_norm")
+def gradient_norm(gradients: Sequence[Tensor], scale: float, most: float) -> Tensor:
+    """``ctmr_gradient_norm`` of one or more tensors without gaps: (2,) fp32, the norm over all and the factor."""
+    _require_device(*gradients)
+    like, lib, sizes = gradients[0], _lib.lib(), _list_sizes(gradients)
+    out = torch.empty(2, device=like.device, dtype=torch.float32)
+    with _on(like):
+        ws = _workspace(sizes.nbytes, like.device)
+        _lib.check(lib.ctmr_gradient_norm(sizes.count, _addresses(gradients), sizes.sizes, sizes.elems, scale, most,
+                                          out.data_ptr(), ws.data_ptr(), sizes.nbytes, _raw_stream(like.device)),
+                   "ctmr_gradient_norm")
+    return out
+
+
+@gradient_norm.register_fake
+def _(gradients, scale, most):
+    return gradients[0].new_empty(2, dtype=torch.float32)
+
+
+@_custom_op("ctmr::scale_tensors", ("tensors",))
+def scale_tensors(tensors: Sequence[Tensor], factor: Tensor) -> None:
+    """``ctmr_scale_tensors``: tensors without gaps times the fp32 ``factor``, in place."""
+    _require_device(factor, *tensors)
+    sizes = _list_sizes(tensors)
+    with _on(factor):
+        _lib.check(_lib.lib().ctmr_scale_tensors(sizes.count, _addresses(tensors), sizes.sizes, sizes.elems,
+                                                 factor.data_ptr(), _raw_stream(factor.device)), "ctmr_scale_tensors")
+
+
+@scale_tensors.register_fake
+def _(tensors, factor):
+    return None
+
+
+@_custom_op("ctmr::adamw", ("parameters", "exp_avg", "exp_avg_sq", "master", "steps"))
+def adamw(parameters: Sequence[Tensor], gradients: Sequence[Tensor], exp_avg: Tensor, exp_avg_sq: Tensor, master: Tensor,
+          steps: Tensor, lr_tensor: Optional[Tensor], starts: Sequence[int], master_starts: Sequence[int], lr: float,
+          beta1: float, beta2: float, eps: float, decay: float, scale: float, most: float, skip: bool) -> Tensor:
+    """``ctmr_adamw``: a step of parameters without gaps in place; the gradients' norm, 0-d fp32."""
+    _require_device(exp_avg, *parameters)
+    sizes = _list_sizes(parameters)
+    norm = torch.empty((), device=exp_avg.device, dtype=torch.float32)
+    desc = _lib.AdamwDesc(lr, beta1, beta2, eps, decay, scale, most, skip)
+    places = lambda v: (ctypes.c_int64 * len(v))(*v)
+    with _on(exp_avg):
+        ws = _workspace(sizes.nbytes, exp_avg.device)
+        _lib.check(_lib.lib().ctmr_adamw(
+            ctypes.byref(desc), sizes.count, _addresses(parameters), _addresses(gradients), sizes.sizes, sizes.elems,
+            places(starts), places(master_starts), exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
+            master.data_ptr() if master.numel() else None, steps.data_ptr(), _ptr(lr_tensor), norm.data_ptr(), ws.data_ptr(),
+            sizes.nbytes, _raw_stream(exp_avg.device)), "ctmr_adamw")
+    return norm
+
+
+@adamw.register_fake
+def _(parameters, gradients, exp_avg, exp_avg_sq, master, steps, lr_tensor, *_):
+    return exp_avg.new_empty((), dtype=torch.float32)
