@@ -528,6 +528,45 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* desc, const
                                    const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
                                    const int64_t* dv_strides, void* workspace, size_t workspace_bytes, void* stream);
 
+/* A position bias for the two calls above: rows and keys lie at places of one to four
+ * axes, 0 .. extents[a] - 1 (the extents add up to 128 at most), and the scores, after
+ * their cap, get for each axis the table's value for the distance key - row on it:
+ *   s += sum_a table[rows[first_a + place_a(key) - place_a(row) + extents[a] - 1]][head]
+ * with first_a = sum over the axes before of 2 extents - 1; `rows` (host memory, read
+ * before the call returns) gives each distance's row of the table (its bucket).
+ * The plan (16-byte aligned) is made from query_places (query_items, lq, axes) and
+ * key_places (key_items, lk, axes), items 1 (all batch items alike) or the batch size;
+ * places outside are taken as the nearest inside.  With `same` the keys lie where the rows
+ * lie and key_places is not read.  table (table_rows, q_heads) of type table_elem; its
+ * values are expected below 2^20 in size like scores, or below -2^100 (-inf too), which hides a pair:
+ * a row left with no key gives zeros.  A value that is NaN or +inf makes NaN of all rows from
+ * whose place some place within the extents has that distance.
+ * The scale, or the cap with one, is at least 2^-20 here.
+ * `fine`: 16-bit softmax weights keep twice their type's bits in their products, which the
+ * table's gradient (dtable) needs of the forward call; no other result does.
+ * The forward workspace is ctmr_masked_attention's, the backward one has a size of its own
+ * (`documents`: with a plan of documents).  dtable, like table, may be NULL. */
+typedef struct ctmr_buckets_desc {
+  int32_t lq, lk, query_items, key_items, same, axes;
+  int32_t extents[4];
+  int32_t table_rows, table_elem;
+} ctmr_buckets_desc;
+int64_t ctmr_buckets_bytes(const ctmr_buckets_desc* buckets);
+int ctmr_buckets(const ctmr_buckets_desc* buckets, const int32_t* query_places, const int32_t* key_places,
+                 const int32_t* rows, void* plan, size_t plan_bytes, void* stream);
+int ctmr_biased_attention(const ctmr_masked_attention_desc* desc, const ctmr_buckets_desc* buckets, const void* q,
+                          const void* k, const void* v, const float* slopes, const int32_t* prefixes, const void* plan,
+                          const void* bucket_plan, const void* table, int32_t fine, void* out, void* rest,
+                          float* lse, void* workspace, size_t workspace_bytes, void* stream);
+int64_t ctmr_biased_attention_backward_workspace_bytes(const ctmr_masked_attention_desc* desc, int32_t documents);
+int ctmr_biased_attention_backward(const ctmr_masked_attention_desc* desc, const ctmr_buckets_desc* buckets, const void* q,
+                                   const void* k, const void* v, const float* slopes, const int32_t* prefixes,
+                                   const void* plan, const void* bucket_plan, const void* table, const void* out,
+                                   const void* rest, const float* lse, const void* dout, const int64_t* dout_strides,
+                                   void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                                   const int64_t* dv_strides, void* dtable, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
 /* Lists of tensors (gradients, parameters): `count` tensors at tensors[i] (device
  * memory, values side by side, on their type's own grid), of sizes[i] values and
  * type elems[i]; the arrays are host memory, read before the call returns.  A tensor of

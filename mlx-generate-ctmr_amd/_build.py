@@ -19,7 +19,9 @@ INCLUDE = REPO_DIR / "include"
 LIB_NAME = "libctmr_hip.so"
 LIB_PATH = PACKAGE_DIR / LIB_NAME
 SOURCES = ("conv.hip", "conv_lds.hip", "conv_march.hip", "norm.hip", "attention.hip", "noalloc.hip", "group_norm.hip",
-           "rotary.hip", "masked_attention.hip", "masked_attention_backward.hip", "gradients.hip")
+           "rotary.hip", "masked_attention.hip", "masked_attention_backward.hip", "gradients.hip",
+           "position_bias.hip", "biased_attention.hip", "biased_attention_backward.hip",
+           "biased_gradients_fp32.hip", "biased_gradients_bf16.hip", "biased_gradients_fp16.hip")
 ARCH = "gfx950"
 
 # Packed FP32 VALU ops are disabled for every device pass; hipcc's host pass

@@ -28,6 +28,7 @@ AVGPOOL2, NEAREST2X, TRILINEAR2X = 0, 1, 2
 ELEM_F32, ELEM_BF16, ELEM_F16 = 0, 1, 2
 POS_I32, POS_I64, POS_F32 = 0, 1, 2
 ROTARY_MAX_PAIRS = 256
+BUCKETS_MAX_PLACES = 128  # over all axes
 ABI_VERSION = 5
 NOALLOC_SCRATCH_BYTES = 256 << 20  # CTMR_NOALLOC_SCRATCH_BYTES
 
@@ -70,6 +71,15 @@ class MaskedAttentionDesc(ctypes.Structure):
                                              "prefix")]
         + [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("reserved", ctypes.c_int32)]
         + [(name, ctypes.c_int64 * 3) for name in ("q_strides", "k_strides", "v_strides", "out_strides")]
+    )
+
+
+class BucketsDesc(ctypes.Structure):
+    """``ctmr_buckets_desc``."""
+
+    _fields_ = (
+        [(name, ctypes.c_int32) for name in ("lq", "lk", "query_items", "key_items", "same", "axes")]
+        + [("extents", ctypes.c_int32 * 4), ("table_rows", ctypes.c_int32), ("table_elem", ctypes.c_int32)]
     )
 
 
@@ -133,6 +143,13 @@ _PROTOTYPES = {
     "ctmr_masked_attention": (_c_int, [ctypes.POINTER(MaskedAttentionDesc)] + [_vp] * 10 + [_sz, _vp]),
     "ctmr_masked_attention_backward_workspace_bytes": (_c_i64, [ctypes.POINTER(MaskedAttentionDesc)]),
     "ctmr_masked_attention_backward": (_c_int, [ctypes.POINTER(MaskedAttentionDesc)] + [_vp] * 18 + [_sz, _vp]),
+    "ctmr_buckets_bytes": (_c_i64, [ctypes.POINTER(BucketsDesc)]),
+    "ctmr_buckets": (_c_int, [ctypes.POINTER(BucketsDesc)] + [_vp] * 4 + [_sz, _vp]),
+    "ctmr_biased_attention": (_c_int, [ctypes.POINTER(MaskedAttentionDesc), ctypes.POINTER(BucketsDesc)] + [_vp] * 8
+                              + [_c_i32] + [_vp] * 4 + [_sz, _vp]),
+    "ctmr_biased_attention_backward_workspace_bytes": (_c_i64, [ctypes.POINTER(MaskedAttentionDesc), _c_i32]),
+    "ctmr_biased_attention_backward": (_c_int, [ctypes.POINTER(MaskedAttentionDesc), ctypes.POINTER(BucketsDesc)]
+                                       + [_vp] * 21 + [_sz, _vp]),
     "ctmr_gradients_workspace_bytes": (_c_i64, [_c_i32, _vp]),
     "ctmr_gradient_norm": (_c_int, [_c_i32, _vp, _vp, _vp, _f, _f, _vp, _vp, _sz, _vp]),
     "ctmr_scale_tensors": (_c_int, [_c_i32, _vp, _vp, _vp, _vp, _vp]),

@@ -1,0 +1,3 @@
+#include "biased_gradients.hpp"
+
+CTMR_BIASED_GRADIENTS(__bf16)

@@ -475,6 +475,15 @@ __device__ __forceinline__ Meeting meeting(int wave, int row0, int rows, F tiles
 
 int check_desc(const ctmr_masked_attention_desc* d);
 int check_strides(const ctmr_masked_attention_desc* d, const int64_t* strides, int rows);
+int check_call(const ctmr_masked_attention_desc* d, const void* q, const void* k, const void* v, const void* plan,
+               const void* out, const void* rest, const void* workspace, size_t workspace_bytes, int64_t need);
+// The arguments of the gradients' kernels, checked, in `a`.
+int check_gradients(const ctmr_masked_attention_desc* d, const void* q, const void* k, const void* v, const float* slopes,
+                    const int32_t* prefixes, const void* plan, const void* out, const void* rest, const float* lse,
+                    const void* dout, const int64_t* dout_strides, void* dq, const int64_t* dq_strides, void* dk,
+                    const int64_t* dk_strides, void* dv, const int64_t* dv_strides, void* workspace,
+                    size_t workspace_bytes, int64_t need, Args& a);
+int64_t delta_bytes(const ctmr_masked_attention_desc* d);  // of delta, the first in the gradients' workspace
 int64_t row_stride(const int64_t* strides, int rows, int head_dim);  // of one row: any that does not overlap
 int padded(int head_dim);
 Args make_args(const ctmr_masked_attention_desc* d, const void* q, const void* k, const void* v, const float* slopes,

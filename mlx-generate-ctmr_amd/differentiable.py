@@ -6,6 +6,7 @@ fp32 surface of ``fast_fp32``, whose convolutions have no gradients:
 * ``group_norm``  channels-last group norm + SiLU
 * ``rotary``      rotary positions over one to four axes (depth, height, width) for q and k
 * ``attention``   attention with grouped heads, a tanh cap, a distance bias, documents and a prefix
+* ``PositionBuckets``  where its rows and keys lie, for a learned bias by the buckets of their distances
 * ``Documents``   which tokens of a batch belong together (volumes of different sizes in one row, padding)
 * ``PackedVolumes``  the documents and voxel positions of several volumes in one row
 * ``self_attention_tokens``  projections, rotary positions and attention of tokens
@@ -16,7 +17,9 @@ fp32 surface of ``fast_fp32``, whose convolutions have no gradients:
 
 from __future__ import annotations
 
+import itertools
 import math
+import operator
 import weakref
 from collections.abc import Mapping, Sequence
 from typing import Optional, Union
@@ -331,6 +334,72 @@ def _attention_heads(t: Tensor) -> Tensor:
     return t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
 
 
+def distance_bucket(distance: int, num_buckets: int, max_distance: int) -> int:
+    """The bucket of a distance (a key's place less the row's): ``n = num_buckets // 2`` buckets for each sign, positive
+    ones from ``n``.  Distances below ``e = n // 2`` have buckets of their own, ``x`` beyond has ``e + floor((n - e)
+    log(x / e) / log(max_distance / e))``, at most the last.  In whole numbers, so a distance on a border is in the upper one."""
+    n, x = num_buckets // 2, abs(distance)
+    e = n // 2
+    bucket = min(x, e)
+    while x >= e and bucket < n - 1 and (x ** (n - e) * e ** (bucket + 1 - e) >= max_distance ** (bucket + 1 - e) * e ** (n - e)):
+        bucket += 1
+    return bucket + (n if distance > 0 else 0)
+
+
+class PositionBuckets:
+    """Where the rows and keys of a batch lie on one to four axes, and the buckets of their distances, laid out once for
+    every ``attention`` with a ``position_bias``.
+
+    ``positions`` ``(L, A)`` or ``(B, L, A)`` int32 holds the query rows' places (a voxel's depth, height, width),
+    ``key_positions`` the keys' (the same rows if left out).  Axis ``a`` has places ``0 .. extents[a] - 1``, others are taken
+    as the nearest of these; the extents add up to at most 128.  A distance on an axis is in one of ``num_buckets`` buckets
+    (``distance_bucket``), the same for all axes.  The positions are copied: changing the tensors afterwards changes nothing
+    here.  Like a tensor, the plan is made on the current stream, which other streams wait for, and outlives the graphs that
+    captured it.
+
+    Raises:
+        ValueError: on positions that are not int32 tensors of these shapes, of one device on the GPU, or empty; extents that
+            are not one for each axis, not positive or too large together; an odd or small ``num_buckets``, or a
+            ``max_distance`` within the buckets of single distances."""
+
+    def __init__(self, positions: Tensor, key_positions: Optional[Tensor] = None, *, extents: Sequence[int],
+                 num_buckets: int = 32, max_distance: int = 128):
+        self.extents = tuple(int(e) for e in extents)
+        if not 1 <= len(self.extents) <= 4 or min(self.extents) < 1 or sum(self.extents) > ops._lib.BUCKETS_MAX_PLACES:
+            raise ValueError(f"extents must be one to four positive sizes that add up to at most "
+                             f"{ops._lib.BUCKETS_MAX_PLACES}; got {self.extents}")
+        self.num_buckets, self.max_distance = int(num_buckets), int(max_distance)
+        if self.num_buckets < 4 or self.num_buckets % 2 or self.num_buckets > 512:
+            raise ValueError(f"num_buckets must be even, 4 to 512; got {num_buckets}")
+        if not self.num_buckets // 4 < self.max_distance < 1 << 31:
+            raise ValueError(f"max_distance must be above num_buckets // 4; got {max_distance}")
+        for t, name in ((positions, "positions"), (positions if key_positions is None else key_positions, "key_positions")):
+            if not isinstance(t, Tensor) or t.dtype != torch.int32 or t.dim() not in (2, 3) or (
+                    int(t.shape[-1]) != len(self.extents)):
+                raise ValueError(f"{name} must be an int32 (L, {len(self.extents)}) or (B, L, {len(self.extents)}) tensor")
+            if t.numel() == 0:
+                raise ValueError(f"{name} is empty: {tuple(t.shape)}")
+            _sizes(*t.shape)
+        if key_positions is not None and (key_positions.device != positions.device or len(
+                {int(t.shape[0]) for t in (positions, key_positions) if t.dim() == 3 and t.shape[0] > 1}) > 1):
+            raise ValueError("positions and key_positions differ in device or batch")
+        _on_gpu(positions, "positions")
+        lay = lambda t: (t[None] if t.dim() == 2 else t).contiguous()
+        places, keys = lay(positions), None if key_positions is None else lay(key_positions)
+        other = places if keys is None else keys
+        self.items = (int(places.shape[0]), int(other.shape[0]))
+        self.shape = (int(places.shape[1]), int(other.shape[1]))
+        rows = [a * self.num_buckets + distance_bucket(x, self.num_buckets, self.max_distance)
+                for a, e in enumerate(self.extents) for x in range(1 - e, e)]
+        self.plan = ops.buckets(places, keys, self.extents, rows, len(self.extents) * self.num_buckets)
+        self._places = (*self.items, int(keys is None), *self.extents)
+        self._stream = _stream_of(self.plan)
+
+    @property
+    def device(self) -> torch.device:
+        return self.plan.device
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, prefixes, plan, scale, softcap, prefixed, prefix):
@@ -350,15 +419,50 @@ class _Attention(torch.autograd.Function):
         return (dq if want_q else None, dk if want_k else None, dv if want_v else None, *(None,) * 7)
 
 
+class _BiasedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, slopes, prefixes, plan, bucket_plan, places, scale, softcap, prefixed, prefix):
+        out, rest, lse = ops.biased_attention(q, k, v, slopes, prefixes, plan, bucket_plan, table, places, scale, softcap,
+                                              prefixed, prefix, True, ctx.needs_input_grad[3])
+        ctx.save_for_backward(q, k, v, slopes, prefixes, plan, bucket_plan, table, out, rest, lse)
+        ctx.args = (places, scale, softcap, prefixed, prefix)
+        ctx.token, ctx.captured = _graph_token(q, k, v, table), torch.cuda.is_current_stream_capturing()
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        _check_capture(ctx.captured)
+        want_q, want_k, want_v, want_table = ctx.needs_input_grad[:4]
+        dq, dk, dv, dtable = ops.biased_attention_backward(*ctx.saved_tensors, _attention_heads(dout), *ctx.args, want_q,
+                                                           want_k or want_v, want_table)
+        return (dq if want_q else None, dk if want_k else None, dv if want_v else None, dtable if want_table else None,
+                *(None,) * 9)
+
+
+def _check_bias(table: Tensor, buckets: PositionBuckets, q: Tensor, lk: int) -> None:
+    b, hq, lq = (int(s) for s in q.shape[:3])
+    shape = (len(buckets.extents), buckets.num_buckets, hq)
+    if not isinstance(table, Tensor) or tuple(table.shape) != shape or table.device != q.device or (
+            table.dtype not in (torch.float32, q.dtype)):
+        raise ValueError(f"position_bias must be {shape} in float32 or {q.dtype} on {q.device}")
+    if buckets.shape != (lq, lk) or buckets.device != q.device or any(n not in (1, b) for n in buckets.items):
+        raise ValueError(f"buckets are for {buckets.items} items of {buckets.shape} rows on {buckets.device}; got {b} of "
+                         f"{(lq, lk)} on {q.device}")
+
+
 def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float = 0.0, slopes: Optional[Tensor] = None,
-              prefix: Union[int, Tensor, None] = None, documents: Optional[Documents] = None) -> Tensor:
-    """Masked attention of ``(B, H, L, D)`` heads; differentiable in ``q``, ``k`` and ``v``.
+              prefix: Union[int, Tensor, None] = None, documents: Optional[Documents] = None,
+              position_bias: Optional[Tensor] = None, buckets: Optional[PositionBuckets] = None) -> Tensor:
+    """Masked attention of ``(B, H, L, D)`` heads; differentiable in ``q``, ``k``, ``v`` and ``position_bias``.
 
     ``q`` has ``Hq`` heads and ``Lq`` rows, ``k`` and ``v`` ``Hk`` heads and ``Lk`` keys, ``Hq`` a multiple of
     ``Hk`` (query head ``h`` reads key head ``h // (Hq // Hk)``); ``D`` is a multiple of 8 up to 128.  With
     ``p_i = i + Lk - Lq`` the place of row ``i`` among the keys:
 
     * ``softcap`` > 0 caps the scores ``s = scale * q.k`` as ``softcap * tanh(s / softcap)``;
+    * ``position_bias`` ``(A, buckets, Hq)``, fp32 or ``q``'s type, with ``buckets`` (``PositionBuckets``) adds
+      ``position_bias[a, bucket, h]`` for the bucket of the distance from row to key on each axis ``a``;
     * ``slopes`` ``(Hq,)`` fp32 subtract ``slopes[h] * |p_i - j|`` (no gradient);
     * ``prefix``, an int or a ``(B,)`` int32 tensor, hides key ``j`` from row ``i`` unless ``j <= p_i`` or ``j <
       prefix`` (0: each row sees the keys up to its own place; None: every key);
@@ -367,12 +471,15 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
     A row that sees no key gives zeros and gets no gradient.  What masked places hold has no effect, NaN included.
     Scores are fp32: their size (the distance's too) is expected below some 2^20, where the weights still have digits.
     Statistics and sums are fp32; the softmax weights, and in the gradients those of the scores, are rounded to the
-    inputs' type for their products (in fp16 raised by powers of two that keep them in its range).  The output has
-    ``q``'s type and lies as ``(B, Lq, Hq, D)`` in memory, so merging the heads is a view.
+    inputs' type for their products (in fp16 raised by powers of two that keep them in its range).  The bias is added with
+    17 bits (all of its bits with fp32 heads), its gradient is summed in fp32 and fp64 from as many of the scores' gradients'; where it
+    is wanted the weights keep twice their bits, and outputs may differ in the last from those without it.
+    A bias below -2^100 (-inf too) hides its pairs; any other value that is not finite makes NaN of the rows within whose reach
+    it lies.  The output has ``q``'s type and lies as ``(B, Lq, Hq, D)`` in memory, so merging the heads is a view.
 
     Raises:
         ValueError: on other types, devices or shapes, a scale that is not positive and finite, a cap that is
-            negative or too small or large beside it, or slopes that need a gradient.
+            negative or too small or large beside it, slopes that need a gradient, or a bias without its buckets.
         NotImplementedError: on forward-mode (dual) tensors."""
     _activation(q, "q", 4)
     _like(k, q, "k", 4)
@@ -410,11 +517,23 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
     if documents is not None and (documents.shape != (b, lq, lk) or documents.device != q.device):
         raise ValueError(f"documents are for {documents.shape} rows on {documents.device}; got {(b, lq, lk)} on "
                          f"{q.device}")
-    needs = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-    _no_tangents(q, k, v, slopes)
+    if (position_bias is None) != (buckets is None):
+        raise ValueError("position_bias and buckets go together")
+    if position_bias is not None:
+        _check_bias(position_bias, buckets, q, lk)
+        if (softcap or scale) < 2.0 ** -20:
+            raise ValueError(f"scale {scale} or softcap {softcap} is too small for a position bias")
+    needs = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, position_bias))
+    _no_tangents(q, k, v, slopes, position_bias)
     _on_gpu(q, "q")
     q, k, v = _attention_heads(q), _attention_heads(k), _attention_heads(v)
     plan = None if documents is None else _used(documents.plan, documents._stream)
+    if position_bias is not None:
+        table, bucket_plan = position_bias.contiguous(), _used(buckets.plan, buckets._stream)
+        args = (buckets._places, scale, softcap, prefix is not None, value)
+        if needs:
+            return _BiasedAttention.apply(q, k, v, table, slopes, prefixes, plan, bucket_plan, *args)
+        return ops.biased_attention(q, k, v, slopes, prefixes, plan, bucket_plan, table, *args, False, False)[0]
     if needs:
         return _Attention.apply(q, k, v, slopes, prefixes, plan, scale, softcap, prefix is not None, value)
     return ops.masked_attention(q, k, v, slopes, prefixes, plan, scale, softcap, prefix is not None, value, False)[0]
@@ -450,16 +569,25 @@ class PackedVolumes:
             ids = torch.repeat_interleave(torch.arange(len(self.shapes), dtype=torch.int32), torch.tensor(self.lengths))
             self.documents = Documents(ids[None].to(self.positions.device))
 
+    def buckets(self, *, num_buckets: int = 32, max_distance: int = 128) -> PositionBuckets:
+        """The buckets of the voxels' distances, for ``attention``'s ``position_bias``; laid out anew by each call.
+
+        Raises:
+            ValueError: on what ``PositionBuckets`` refuses, such as volumes whose largest sizes add up to more than 128."""
+        return PositionBuckets(_used(self.positions, self._stream), extents=[max(axis) for axis in zip(*self.shapes)],
+                               num_buckets=num_buckets, max_distance=max_distance)
+
 
 def self_attention_tokens(tokens: Tensor, weights: Mapping[str, Tensor], *, heads: int, scale: float, include_fc: bool,
                           documents: Optional[Documents] = None, positions: Optional[Tensor] = None,
                           sections: Optional[Sequence[int]] = None, base: float = 10000.0, prefix: str = "attn",
-                          qkv_bias: bool = True) -> Tensor:
+                          qkv_bias: bool = True, buckets: Optional[PositionBuckets] = None) -> Tensor:
     """Q/K/V projections, rotary positions, self-attention and optional ``out_proj`` on ``(B, L, C)`` tokens;
     differentiable in the tokens and the weights.
 
     Takes the weights of ``fast_fp32.self_attention_tokens`` in the tokens' type.  ``documents`` keeps tokens apart;
     ``positions`` with ``sections`` (see ``rotary``) turns q and k, and is left out for attention without positions.
+    ``buckets`` adds the learned bias of ``weights[f"{prefix}.position_bias"]`` ``(A, buckets, heads)`` (see ``attention``).
 
     Raises:
         ValueError: on tokens that are not (B, L, C), heads that do not divide C, positions without sections or the
@@ -474,14 +602,16 @@ def self_attention_tokens(tokens: Tensor, weights: Mapping[str, Tensor], *, head
     names = [f"{prefix}.to_{m}" for m in ("q", "k", "v")]
     used = [weights[f"{m}.{part}"] for m in [*names, *([f"{prefix}.out_proj"] if include_fc else [])]
             for part in (("weight", "bias") if qkv_bias or m.endswith("out_proj") else ("weight",))]
-    token = _graph_token(tokens, *used) if torch.is_grad_enabled() and tokens.is_cuda else None
+    table = None if buckets is None else weights[f"{prefix}.position_bias"]
+    token = _graph_token(tokens, *used, table) if torch.is_grad_enabled() and tokens.is_cuda else None
     w = torch.cat([_like(weights[f"{m}.weight"], tokens, f"{m}.weight", 2) for m in names])
     b = torch.cat([_like(weights[f"{m}.bias"], tokens, f"{m}.bias", 1) for m in names]) if qkv_bias else None
     # (B, L, 3, H, D): q, k and v are strided views of the one product
     q, k, v = F.linear(tokens, w, b).reshape(n, length, 3, heads, c // heads).permute(2, 0, 3, 1, 4).unbind(0)
     if positions is not None:
         q, k = rotary(q, k, positions, sections=sections, base=base)
-    merged = attention(q, k, v, scale=scale, documents=documents).transpose(1, 2).reshape(n, length, c)
+    merged = attention(q, k, v, scale=scale, documents=documents, position_bias=table, buckets=buckets)
+    merged = merged.transpose(1, 2).reshape(n, length, c)
     if include_fc:
         merged = F.linear(merged, _like(weights[f"{prefix}.out_proj.weight"], tokens, f"{prefix}.out_proj.weight", 2),
                           _like(weights[f"{prefix}.out_proj.bias"], tokens, f"{prefix}.out_proj.bias", 1))
@@ -491,6 +621,9 @@ def self_attention_tokens(tokens: Tensor, weights: Mapping[str, Tensor], *, head
 # ---------------------------------------------------------------------------
 # lists of gradients and parameters
 # ---------------------------------------------------------------------------
+_kind, _layout, _device, _bytes = (operator.attrgetter(name) for name in ("dtype", "layout", "device", "nbytes"))
+
+
 def _without_gaps(t: Tensor) -> bool:
     """Whether ``t``'s values fill their memory, in any order of the axes."""
     if t.is_contiguous():
@@ -504,21 +637,21 @@ def _without_gaps(t: Tensor) -> bool:
 
 
 def _listed(tensors, name: str) -> list[Tensor]:
-    """The tensors of a list, ``None`` left out, checked for type and device.  What autograd or tracing makes of them is not
-    looked at."""
+    """The tensors of a list, ``None`` left out, checked for type and device."""
     if isinstance(tensors, Tensor):
         raise ValueError(f"{name} must be a list of tensors")
     out = [t for t in tensors if t is not None]
     if not out:
         raise ValueError(f"{name} holds no tensor")
-    device = out[0].device if isinstance(out[0], Tensor) else None
-    for t in out:
-        if not isinstance(t, Tensor) or t.layout != torch.strided:
-            raise ValueError(f"{name} must be dense tensors")
-        if t.dtype not in ops.ELEMENTS:
-            raise ValueError(f"{name} must be float32, bfloat16 or float16; got {t.dtype}")
-        if t.device != device:
-            raise ValueError(f"{name} are on {device} and {t.device}")
+    # the list as a whole (see ops._list_sizes); what is wrong is looked for only where something is
+    if not (all(map(isinstance, out, itertools.repeat(Tensor))) and set(map(_layout, out)) == {torch.strided}):
+        raise ValueError(f"{name} must be dense tensors")
+    for kind in set(map(_kind, out)):
+        if kind not in ops.ELEMENTS:
+            raise ValueError(f"{name} must be float32, bfloat16 or float16; got {kind}")
+    devices = set(map(_device, out))
+    if len(devices) != 1:
+        raise ValueError(f"{name} are on {' and '.join(sorted(map(str, devices)))}")
     _no_tangents(*out)
     _on_gpu(out[0], name)
     return out
@@ -526,12 +659,12 @@ def _listed(tensors, name: str) -> list[Tensor]:
 
 def _apart(tensors: Sequence[Tensor], name: str) -> None:
     """Refuses tensors that are written and have gaps or share memory."""
-    if not all(_without_gaps(t) for t in tensors):
+    if not (all(map(Tensor.is_contiguous, tensors)) or all(map(_without_gaps, tensors))):
         raise ValueError(f"{name} must fill their memory without gaps or overlaps")
-    if torch.compiler.is_compiling() or any(type(t) not in ops._PLAIN for t in tensors):
+    if torch.compiler.is_compiling() or not ops.PLAIN.issuperset(map(type, tensors)):
         return  # what is traced has no address
-    spans = sorted([(t.data_ptr(), t.numel() * t.element_size()) for t in tensors if t.numel()])
-    if any(at + size > after for (at, size), (after, _) in zip(spans, spans[1:])):
+    spans = sorted([span for span in zip(map(Tensor.data_ptr, tensors), map(_bytes, tensors)) if span[1]])
+    if any(at + size > after for (at, size), (after, _) in itertools.pairwise(spans)):
         raise ValueError(f"{name} share memory")
 
 
@@ -553,7 +686,9 @@ def gradient_norm(gradients: Sequence[Optional[Tensor]]) -> Tensor:
         ValueError: on an empty list, other types, or tensors that are not on one GPU.
         NotImplementedError: on forward-mode (dual) tensors."""
     gradients = _listed(gradients, "gradients")
-    return ops.gradient_norm([t if _without_gaps(t) else t.contiguous() for t in gradients], 1.0, math.inf)[0]
+    if not all(map(Tensor.is_contiguous, gradients)):
+        gradients = [t if _without_gaps(t) else t.contiguous() for t in gradients]
+    return ops.gradient_norm(gradients)[0]
 
 
 @torch.no_grad()
@@ -569,10 +704,13 @@ def clip_gradients(gradients: Sequence[Optional[Tensor]], max_norm: float) -> Te
         NotImplementedError: on forward-mode (dual) tensors."""
     max_norm, gradients = _most(max_norm), _listed(gradients, "gradients")
     _apart(gradients, "gradients")
-    norm = ops.gradient_norm(gradients, 1.0, max_norm)
-    ops.scale_tensors(gradients, norm[1])
+    norm = ops.clip_gradients(gradients, max_norm)
     torch.autograd.graph.increment_version(gradients)
     return norm[0]
+
+
+def _layout_of(t: Tensor) -> tuple:
+    return t.shape, t.stride(), t.dtype, t.device
 
 
 class AdamW:
@@ -614,7 +752,7 @@ class AdamW:
                 raise ValueError(f"{name} must be finite and not negative; got {value}")
         self.max_norm = math.inf if max_norm is None else _most(max_norm)
         self.skip_non_finite = bool(skip_non_finite)
-        self._layouts = [(p.shape, p.stride(), p.dtype, p.device) for p in self.parameters]
+        self._layouts = list(map(_layout_of, self.parameters))
         self._starts, total = self._places(self.parameters)
         half = [p for p in self.parameters if p.dtype != torch.float32]
         starts, room = self._places(half)
@@ -690,26 +828,26 @@ class AdamW:
         lr, scale = self.lr if lr is None else self._rate(lr), float(gradient_scale)
         if not math.isfinite(scale):
             raise ValueError(f"gradient_scale must be finite; got {scale}")
-        _listed(gradients, "gradients")
-        used, taken = [], []
-        for i, (p, g) in enumerate(zip(self.parameters, gradients)):
-            if g is None:
-                continue
-            shape, strides, dtype, device = self._layouts[i]
-            if p.shape != shape or p.stride() != strides or p.dtype != dtype or p.device != device:
-                raise ValueError(f"parameter {i} has become another: {tuple(p.shape)} {p.stride()} {p.dtype} on {p.device}")
-            if g.shape != shape or g.dtype != dtype or g.device != device:
-                raise ValueError(f"gradient {i} is {tuple(g.shape)} {g.dtype} on {g.device}; its parameter {tuple(shape)} "
-                                 f"{dtype} on {device}")
-            if g.stride() != strides and not (g.is_contiguous() and p.is_contiguous()):
-                g = torch.empty_strided(shape, strides, dtype=dtype, device=device).copy_(g)
-            used.append(i)
-            taken.append(g)
-        parameters = self.parameters if len(used) == len(self.parameters) else [self.parameters[i] for i in used]
-        of = lambda values: values if len(used) == len(values) else [values[i] for i in used]
+        taken = _listed(gradients, "gradients")
+        parameters, layouts, starts, masters = self.parameters, self._layouts, self._starts, self._master_starts
+        numbers = range(len(gradients))
+        if len(taken) != len(parameters):
+            used = [g is not None for g in gradients]
+            parameters, layouts, starts, masters, numbers = (
+                list(itertools.compress(v, used)) for v in (parameters, layouts, starts, masters, numbers))
+        if list(map(_layout_of, parameters)) != layouts:
+            i = next(i for i, p, want in zip(numbers, parameters, layouts) if _layout_of(p) != want)
+            raise ValueError(f"parameter {i} has become another than it was: {_layout_of(self.parameters[i])}")
+        if list(map(_layout_of, taken)) != layouts:
+            for at, (i, g, p) in enumerate(zip(numbers, taken, parameters)):
+                if g.shape != p.shape or g.dtype != p.dtype or g.device != p.device:
+                    raise ValueError(f"gradient {i} is {tuple(g.shape)} {g.dtype} on {g.device}; its parameter "
+                                     f"{tuple(p.shape)} {p.dtype} on {p.device}")
+                if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
+                    taken[at] = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
         rate = (lr, 0.0) if isinstance(lr, Tensor) else (None, lr)
         state = [_used(t, self._stream) for t in (self.exp_avg, self.exp_avg_sq, self.master, self.steps)]
-        norm = ops.adamw(parameters, taken, *state, rate[0], of(self._starts), of(self._master_starts), rate[1],
-                         *self.betas, self.eps, self.weight_decay, scale, self.max_norm, self.skip_non_finite)
+        norm = ops.adamw(parameters, taken, *state, rate[0], starts, masters, rate[1], *self.betas,
+                         self.eps, self.weight_decay, scale, self.max_norm, self.skip_non_finite)
         torch.autograd.graph.increment_version([*parameters, *state])
         return norm

@@ -117,13 +117,16 @@ def spatial_attention(x: Tensor, weights: Mapping[str, Tensor], *, num_groups: i
 
 def spatial_attention_volumes(volumes: Sequence[Tensor], weights: Mapping[str, Tensor], *, num_groups: int, eps: float,
                               num_head_channels: int, include_fc: bool, packed: Optional[df.PackedVolumes] = None,
-                              sections: Optional[Sequence[int]] = None, base: float = 10000.0) -> list[Tensor]:
+                              sections: Optional[Sequence[int]] = None, base: float = 10000.0,
+                              buckets: Optional[df.PositionBuckets] = None) -> list[Tensor]:
     """``spatial_attention`` of several DHWC volumes at once, each over its own voxels, differentiable in the volumes
     and the weights: what fine-tuning on volumes of different sizes runs.
 
     Each volume has group statistics of its own; the tokens of all lie in one row, whose documents the attention
     keeps apart, so no volume is padded to another's size.  ``packed`` is the batch's ``PackedVolumes`` where more
-    than one block uses it.  ``sections`` turns q and k by the voxels' (depth, height, width) (``differentiable.rotary``).
+    than one block uses it.  ``sections`` turns q and k by the voxels' (depth, height, width) (``differentiable.rotary``);
+    ``buckets``, the batch's ``packed.buckets(...)``, adds the bias ``weights["attn.position_bias"]`` learned for the distances
+    between voxels.
 
     Raises:
         ValueError: on no volumes, volumes that are not (D, H, W, C) of one C, type and device, channels that
@@ -147,6 +150,7 @@ def spatial_attention_volumes(volumes: Sequence[Tensor], weights: Mapping[str, T
     merged = df.self_attention_tokens(rows[0] if len(rows) == 1 else torch.cat(rows, dim=1), weights,
                                       heads=c // num_head_channels, scale=float(num_head_channels) ** -0.5,
                                       include_fc=include_fc, documents=packed.documents, sections=sections, base=base,
+                                      buckets=buckets,
                                       positions=None if sections is None else df._used(packed.positions, packed._stream))
     return [v + part.reshape(v.shape) for v, part in zip(volumes, merged.split(packed.lengths, dim=1))]
 

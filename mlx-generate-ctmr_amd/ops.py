@@ -20,6 +20,7 @@ import contextlib
 import ctypes
 import functools
 import math
+import operator
 from typing import Callable, Optional, Sequence
 
 import torch
@@ -55,12 +56,12 @@ def _direct(values) -> bool:
     for v in values:
         if isinstance(v, Tensor) and (type(v) is not Tensor or (grad and v.requires_grad)):
             return False
-        if type(v) is list and not all(type(t) in _PLAIN and not (grad and t.requires_grad) for t in v):
+        if type(v) is list and not (PLAIN.issuperset(map(type, v)) and not (grad and any(getattr(t, "requires_grad", False) for t in v))):
             return False
     return True
 
 
-_PLAIN = (Tensor, torch.nn.Parameter)  # of the tensors in lists
+PLAIN = {Tensor, torch.nn.Parameter, int}  # of what lists hold
 
 
 def _custom_op(name: str, mutates: Sequence[str] = ()) -> Callable[[Callable], _CustomOp]:
@@ -733,9 +734,13 @@ def _attention_desc(q_shape, k_shape, elem: int, q_strides, k_strides, v_strides
                        "ctmr_masked_attention_backward_workspace_bytes"))
 
 
-def _attention_desc_of(q: Tensor, k: Tensor, v: Tensor, scale: float, softcap: float, prefixed: bool, prefix: int):
-    return _attention_desc(tuple(q.shape), tuple(k.shape), ELEMENTS[q.dtype], _head_strides(q), _head_strides(k),
-                           _head_strides(v), scale, softcap, prefixed, prefix)
+def _attention_key(q: Tensor, k: Tensor, v: Tensor, scale: float, softcap: float, prefixed: bool, prefix: int) -> tuple:
+    return (tuple(q.shape), tuple(k.shape), ELEMENTS[q.dtype], _head_strides(q), _head_strides(k), _head_strides(v), scale,
+            softcap, prefixed, prefix)
+
+
+def _attention_desc_of(*call):
+    return _attention_desc(*_attention_key(*call))
 
 
 @_custom_op("ctmr::masked_attention")
@@ -800,6 +805,122 @@ def _(q, k, v, slopes, prefixes, plan, out, rest, lse, dout, scale, softcap, pre
             _heads_like(v) if want_kv else v.new_empty(none))
 
 
+@functools.lru_cache(maxsize=256)
+def buckets_desc(lq: int, lk: int, query_items: int, key_items: int, same: bool, extents: tuple[int, ...], table_rows: int,
+                 table_elem: int) -> _lib.BucketsDesc:
+    return _lib.BucketsDesc(lq, lk, query_items, key_items, same, len(extents), (*extents, *(0,) * (4 - len(extents))),
+                            table_rows, table_elem)
+
+
+def _places_desc(places: Tensor, key_places: Optional[Tensor], extents: Sequence[int], table_rows: int) -> _lib.BucketsDesc:
+    other = places if key_places is None else key_places
+    return buckets_desc(int(places.shape[1]), int(other.shape[1]), int(places.shape[0]), int(other.shape[0]),
+                        key_places is None, tuple(extents), table_rows, _lib.ELEM_F32)
+
+
+@_custom_op("ctmr::buckets")
+def buckets(places: Tensor, key_places: Optional[Tensor], extents: Sequence[int], rows: Sequence[int],
+            table_rows: int) -> Tensor:
+    """``ctmr_buckets``: the plan of contiguous (items, L, axes) int32 places, the keys' the same without ``key_places``, as
+    raw bytes."""
+    _require_device(places, key_places)
+    desc, lib = _places_desc(places, key_places, extents, table_rows), _lib.lib()
+    nbytes = _lib.check(lib.ctmr_buckets_bytes(ctypes.byref(desc)), "ctmr_buckets_bytes")
+    plan = torch.empty(nbytes, device=places.device, dtype=torch.uint8)
+    with _on(places):
+        _lib.check(lib.ctmr_buckets(ctypes.byref(desc), places.data_ptr(), _ptr(key_places), (ctypes.c_int32 * len(rows))(*rows),
+                                    plan.data_ptr(), nbytes, _raw_stream(plan.device)), "ctmr_buckets")
+    return plan
+
+
+@buckets.register_fake
+def _(places, key_places, extents, rows, table_rows):
+    desc = _places_desc(places, key_places, extents, table_rows)
+    return places.new_empty(_lib.lib().ctmr_buckets_bytes(ctypes.byref(desc)), dtype=torch.uint8)
+
+
+def _bias_desc(q: Tensor, k: Tensor, table: Tensor, places: Sequence[int]) -> _lib.BucketsDesc:
+    """``places``: (query items, key items, whether the sides are the same, the extents...)."""
+    return buckets_desc(int(q.shape[2]), int(k.shape[2]), places[0], places[1], bool(places[2]), tuple(places[3:]),
+                        table.numel() // int(q.shape[1]), ELEMENTS[table.dtype])
+
+
+@_custom_op("ctmr::biased_attention")
+def biased_attention(q: Tensor, k: Tensor, v: Tensor, slopes: Optional[Tensor], prefixes: Optional[Tensor],
+                     plan: Optional[Tensor], bucket_plan: Tensor, table: Tensor, places: Sequence[int], scale: float,
+                     softcap: float, prefixed: bool, prefix: int, want_grad: bool,
+                     want_table: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """``ctmr_biased_attention``: ``masked_attention`` with the bias of a contiguous (rows, Hq) ``table`` and a plan of
+    ``places`` (``_bias_desc``); ``want_table``: the table gets a gradient too."""
+    _require_device(q, k, v, slopes, prefixes, plan, bucket_plan, table)
+    out = _heads_like(q)
+    rest = _heads_like(q) if want_grad and q.element_size() == 2 else q.new_empty((0,))
+    lse = torch.empty(q.shape[:3] if want_grad else (0,), device=q.device, dtype=torch.float32)
+    if q.numel() == 0 or k.shape[2] == 0:
+        return out.zero_(), rest.zero_(), lse.fill_(math.inf)
+    desc, nbytes, _ = _attention_desc_of(q, k, v, scale, softcap, prefixed, prefix)
+    with _on(q):
+        ws = _workspace(nbytes, q.device)
+        _lib.check(_lib.lib().ctmr_biased_attention(
+            ctypes.byref(desc), ctypes.byref(_bias_desc(q, k, table, places)), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            _ptr(slopes), _ptr(prefixes), _ptr(plan), bucket_plan.data_ptr(), table.data_ptr(), want_table, out.data_ptr(),
+            rest.data_ptr() if rest.numel() else None, lse.data_ptr() if want_grad else None, _ptr(ws), nbytes,
+            _raw_stream(q.device)), "ctmr_biased_attention")
+    return out, rest, lse
+
+
+@biased_attention.register_fake
+def _(q, k, v, slopes, prefixes, plan, bucket_plan, table, places, scale, softcap, prefixed, prefix, want_grad, want_table):
+    return (_heads_like(q), _heads_like(q) if want_grad and q.element_size() == 2 else q.new_empty((0,)),
+            q.new_empty(q.shape[:3] if want_grad else (0,), dtype=torch.float32))
+
+
+@functools.lru_cache(maxsize=256)
+def _biased_backward_bytes(key, documents: bool) -> int:
+    """Of a call with ``_attention_desc``'s arguments."""
+    return _lib.check(_lib.lib().ctmr_biased_attention_backward_workspace_bytes(
+        ctypes.byref(_attention_desc(*key)[0]), documents), "ctmr_biased_attention_backward_workspace_bytes")
+
+
+@_custom_op("ctmr::biased_attention_backward")
+def biased_attention_backward(q: Tensor, k: Tensor, v: Tensor, slopes: Optional[Tensor], prefixes: Optional[Tensor],
+                              plan: Optional[Tensor], bucket_plan: Tensor, table: Tensor, out: Tensor, rest: Tensor,
+                              lse: Tensor, dout: Tensor, places: Sequence[int], scale: float, softcap: float, prefixed: bool,
+                              prefix: int, want_q: bool, want_kv: bool,
+                              want_table: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """``ctmr_biased_attention_backward``: gradients of ``q``, ``k`` and ``v``, which lie as (B, L, H, D), and of the table;
+    empty where not wanted."""
+    _require_device(q, k, v, slopes, prefixes, plan, bucket_plan, table, out, rest, lse, dout)
+    none = (0,)
+    dq = _heads_like(q) if want_q else q.new_empty(none)
+    dk, dv = (_heads_like(k), _heads_like(v)) if want_kv else (k.new_empty(none), v.new_empty(none))
+    dtable = torch.empty_like(table) if want_table else table.new_empty(none)
+    if q.numel() == 0 or k.shape[2] == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_(), dtable.zero_()
+    key = _attention_key(q, k, v, scale, softcap, prefixed, prefix)
+    desc, nbytes = _attention_desc(*key)[0], _biased_backward_bytes(key, plan is not None)
+    strides = lambda t, want=True: (ctypes.c_int64 * 3)(*_head_strides(t)) if want else None
+    with _on(q):
+        ws = _workspace(nbytes, q.device)
+        _lib.check(_lib.lib().ctmr_biased_attention_backward(
+            ctypes.byref(desc), ctypes.byref(_bias_desc(q, k, table, places)), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            _ptr(slopes), _ptr(prefixes), _ptr(plan), bucket_plan.data_ptr(), table.data_ptr(), out.data_ptr(),
+            rest.data_ptr() if rest.numel() else None, lse.data_ptr(), dout.data_ptr(), strides(dout),
+            dq.data_ptr() if want_q else None, strides(dq, want_q), dk.data_ptr() if want_kv else None, strides(dk, want_kv),
+            dv.data_ptr() if want_kv else None, strides(dv, want_kv), dtable.data_ptr() if want_table else None, _ptr(ws),
+            nbytes, _raw_stream(q.device)), "ctmr_biased_attention_backward")
+    return dq, dk, dv, dtable
+
+
+@biased_attention_backward.register_fake
+def _(q, k, v, slopes, prefixes, plan, bucket_plan, table, out, rest, lse, dout, places, scale, softcap, prefixed, prefix,
+      want_q, want_kv, want_table):
+    none = (0,)
+    return (_heads_like(q) if want_q else q.new_empty(none), _heads_like(k) if want_kv else k.new_empty(none),
+            _heads_like(v) if want_kv else v.new_empty(none),
+            torch.empty_like(table) if want_table else table.new_empty(none))
+
+
 # ---------------------------------------------------------------------------
 # lists of gradients and parameters
 # ---------------------------------------------------------------------------
@@ -816,51 +937,69 @@ class _Sizes:
                                  "ctmr_gradients_workspace_bytes")
 
 
-@functools.lru_cache(maxsize=64)
-def _sizes_of(counts: tuple[int, ...], kinds: tuple[torch.dtype, ...]) -> _Sizes:
-    return _Sizes(counts, kinds)
+_sizes_of = functools.lru_cache(maxsize=64)(_Sizes)
+# A list is walked by ``map`` and C getters, 40 ns a tensor and getter; a loop's body costs 1.5 us a tensor, which for
+# a few hundred tensors is longer than their kernels take.
+_dtype_of = operator.attrgetter("dtype")
 
 
 def _list_sizes(tensors: Sequence[Tensor]) -> _Sizes:
-    return _sizes_of(tuple([t.numel() for t in tensors]), tuple([t.dtype for t in tensors]))
+    return _sizes_of(tuple(map(Tensor.numel, tensors)), tuple(map(_dtype_of, tensors)))
 
 
 def _addresses(tensors: Sequence[Tensor]):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+    return (ctypes.c_void_p * len(tensors))(*map(Tensor.data_ptr, tensors))
+
+
+def _list_on_device(tensors: Sequence[Tensor]) -> Tensor:
+    """The first of tensors that are all on one GPU."""
+    devices = set(map(Tensor.get_device, tensors))
+    if len(devices) != 1 or -1 in devices:
+        raise RuntimeError("ctmr operators run only on the GPU (HIP), on tensors of one device")
+    return tensors[0]
 
 
 @_custom_op("ctmr::gradient_norm")
-def gradient_norm(gradients: Sequence[Tensor], scale: float, most: float) -> Tensor:
-    """``ctmr_gradient_norm`` of one or more tensors without gaps: (2,) fp32, the norm over all and the factor."""
-    _require_device(*gradients)
-    like, lib, sizes = gradients[0], _lib.lib(), _list_sizes(gradients)
+def gradient_norm(gradients: Sequence[Tensor]) -> Tensor:
+    """``ctmr_gradient_norm`` of one or more tensors without gaps: (2,) fp32, the norm over all and one."""
+    like, sizes = _list_on_device(gradients), _list_sizes(gradients)
     out = torch.empty(2, device=like.device, dtype=torch.float32)
     with _on(like):
         ws = _workspace(sizes.nbytes, like.device)
-        _lib.check(lib.ctmr_gradient_norm(sizes.count, _addresses(gradients), sizes.sizes, sizes.elems, scale, most,
-                                          out.data_ptr(), ws.data_ptr(), sizes.nbytes, _raw_stream(like.device)),
+        _lib.check(_lib.lib().ctmr_gradient_norm(sizes.count, _addresses(gradients), sizes.sizes, sizes.elems, 1.0, math.inf,
+                                                 out.data_ptr(), ws.data_ptr(), sizes.nbytes, _raw_stream(like.device)),
                    "ctmr_gradient_norm")
     return out
 
 
 @gradient_norm.register_fake
-def _(gradients, scale, most):
+def _(gradients):
     return gradients[0].new_empty(2, dtype=torch.float32)
 
 
-@_custom_op("ctmr::scale_tensors", ("tensors",))
-def scale_tensors(tensors: Sequence[Tensor], factor: Tensor) -> None:
-    """``ctmr_scale_tensors``: tensors without gaps times the fp32 ``factor``, in place."""
-    _require_device(factor, *tensors)
-    sizes = _list_sizes(tensors)
-    with _on(factor):
-        _lib.check(_lib.lib().ctmr_scale_tensors(sizes.count, _addresses(tensors), sizes.sizes, sizes.elems,
-                                                 factor.data_ptr(), _raw_stream(factor.device)), "ctmr_scale_tensors")
+@_custom_op("ctmr::clip_gradients", ("gradients",))
+def clip_gradients(gradients: Sequence[Tensor], most: float) -> Tensor:
+    """``ctmr_gradient_norm`` and ``ctmr_scale_tensors`` of one or more tensors without gaps, in place: (2,) fp32, the norm
+    over all before and the factor."""
+    like, sizes = _list_on_device(gradients), _list_sizes(gradients)
+    out, at = torch.empty(2, device=like.device, dtype=torch.float32), _addresses(gradients)
+    with _on(like):
+        ws, lib, stream = _workspace(sizes.nbytes, like.device), _lib.lib(), _raw_stream(like.device)
+        _lib.check(lib.ctmr_gradient_norm(sizes.count, at, sizes.sizes, sizes.elems, 1.0, most, out.data_ptr(),
+                                          ws.data_ptr(), sizes.nbytes, stream), "ctmr_gradient_norm")
+        _lib.check(lib.ctmr_scale_tensors(sizes.count, at, sizes.sizes, sizes.elems, out.data_ptr() + 4, stream),
+                   "ctmr_scale_tensors")
+    return out
 
 
-@scale_tensors.register_fake
-def _(tensors, factor):
-    return None
+@clip_gradients.register_fake
+def _(gradients, most):
+    return gradients[0].new_empty(2, dtype=torch.float32)
+
+
+@functools.lru_cache(maxsize=64)
+def _places(starts: tuple[int, ...]):
+    return (ctypes.c_int64 * len(starts))(*starts)
 
 
 @_custom_op("ctmr::adamw", ("parameters", "exp_avg", "exp_avg_sq", "master", "steps"))
@@ -868,18 +1007,17 @@ def adamw(parameters: Sequence[Tensor], gradients: Sequence[Tensor], exp_avg: Te
           steps: Tensor, lr_tensor: Optional[Tensor], starts: Sequence[int], master_starts: Sequence[int], lr: float,
           beta1: float, beta2: float, eps: float, decay: float, scale: float, most: float, skip: bool) -> Tensor:
     """``ctmr_adamw``: a step of parameters without gaps in place; the gradients' norm, 0-d fp32."""
-    _require_device(exp_avg, *parameters)
-    sizes = _list_sizes(parameters)
-    norm = torch.empty((), device=exp_avg.device, dtype=torch.float32)
+    like, sizes = _list_on_device(parameters), _list_sizes(parameters)
+    _list_on_device([exp_avg, gradients[0], like])
+    norm = torch.empty((), device=like.device, dtype=torch.float32)
     desc = _lib.AdamwDesc(lr, beta1, beta2, eps, decay, scale, most, skip)
-    places = lambda v: (ctypes.c_int64 * len(v))(*v)
-    with _on(exp_avg):
-        ws = _workspace(sizes.nbytes, exp_avg.device)
+    with _on(like):
+        ws = _workspace(sizes.nbytes, like.device)
         _lib.check(_lib.lib().ctmr_adamw(
             ctypes.byref(desc), sizes.count, _addresses(parameters), _addresses(gradients), sizes.sizes, sizes.elems,
-            places(starts), places(master_starts), exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
+            _places(tuple(starts)), _places(tuple(master_starts)), exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
             master.data_ptr() if master.numel() else None, steps.data_ptr(), _ptr(lr_tensor), norm.data_ptr(), ws.data_ptr(),
-            sizes.nbytes, _raw_stream(exp_avg.device)), "ctmr_adamw")
+            sizes.nbytes, _raw_stream(like.device)), "ctmr_adamw")
     return norm
 
 
