@@ -21,11 +21,15 @@ extern "C" int ctmr_biased_attention(const ctmr_masked_attention_desc* d, const 
   a.ob = d->out_strides[0], a.oh = d->out_strides[1], a.ol = d->out_strides[2];
   Bias bias = make_bias(d, buckets, bucket_plan, table);
   bias.fine = fine != 0;
-  const bool few = few_rows(d), narrow = bias_width(buckets) == 64;
+  const bool few = few_rows(d);
   hipStream_t st = (hipStream_t)stream;
-#define CTMR_BIASED_WIDTH(T, D)                                       \
-  if (narrow) return launch<T, D>(a, BiasOf<2>{bias}, few, st);       \
-  return launch<T, D>(a, BiasOf<4>{bias}, few, st);
+#define CTMR_BIASED_WIDTH(T, D)                                      \
+  switch (bias_steps(buckets)) {                                     \
+    case 3: return launch<T, D>(a, BiasOf<3>{bias}, few, st);        \
+    case 4: return launch<T, D>(a, BiasOf<4>{bias}, few, st);        \
+    case 6: return launch<T, D>(a, BiasOf<6>{bias}, few, st);        \
+    default: return launch<T, D>(a, BiasOf<8>{bias}, few, st);       \
+  }
 #define CTMR_BIASED_TYPE(T)              \
   switch (padded(d->head_dim)) {         \
     case 32: CTMR_BIASED_WIDTH(T, 32)    \

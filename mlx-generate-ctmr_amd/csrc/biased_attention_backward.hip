@@ -80,7 +80,7 @@ int ctmr_biased_attention_backward(const ctmr_masked_attention_desc* d, const ct
   const auto run = d->elem == CTMR_ELEM_F32    ? run_biased_gradients<float>
                    : d->elem == CTMR_ELEM_BF16 ? run_biased_gradients<__bf16>
                                                : run_biased_gradients<_Float16>;
-  rc = run(a, bias, bias_width(buckets) == 64, query_parts(d), key_parts(d), st);
+  rc = run(a, bias, bias_steps(buckets), query_parts(d), key_parts(d), st);
   if (rc || !dtable) return rc;
   hipLaunchKernelGGL(table_gradient_kernel, dim3(d->q_heads), dim3(1024), 0, st, bias.part, bias.rows, d->n, d->q_heads,
                      bias.slots, buckets->table_rows, buckets->table_elem, dtable);

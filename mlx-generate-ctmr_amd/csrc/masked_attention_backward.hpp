@@ -143,8 +143,8 @@ __device__ __forceinline__ int2 split_steps(int count, int split, int splits) {
 }
 
 // Adds to the gradient of r what a 32 x 32 block of scores' gradients gives, in parts as r's.
-template <typename T, int NE>
-__device__ __forceinline__ void add_row_gradient(f16v (&dr)[BiasOf<NE>::kBlocks], f16v ds, const char* hot, int row,
+template <typename T, int ST>
+__device__ __forceinline__ void add_row_gradient(f16v (&dr)[BiasOf<ST>::kBlocks], f16v ds, const char* hot, int row,
                                                  int lane) {
 #pragma unroll
   for (int p = 0; p < kParts<T>; ++p) {
@@ -152,8 +152,8 @@ __device__ __forceinline__ void add_row_gradient(f16v (&dr)[BiasOf<NE>::kBlocks]
     for (int w = 0; w < 2; ++w) {
       const Frag<__bf16> f = result_frag<__bf16>(ds, w);
 #pragma unroll
-      for (int n = 0; n < NE; ++n)
-        dr[n] = mma<__bf16>(Tile<__bf16, 32 * NE>::down(hot, row + 16 * w, n, lane), f, dr[n]);
+      for (int n = 0; n < BiasOf<ST>::kBlocks; ++n)
+        dr[n] = mma<__bf16>(Tile<__bf16, BiasOf<ST>::kWidth>::down(hot, row + 16 * w, n, lane), f, dr[n]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) ds[8 * w + e] -= (float)f[e];
     }
@@ -161,11 +161,11 @@ __device__ __forceinline__ void add_row_gradient(f16v (&dr)[BiasOf<NE>::kBlocks]
 }
 
 // A workgroup's gradients of r, added over its rows by distance: thread t's is distance t.  A wave's 32 rows at a time
-// go through LDS (32 x 32 NE floats, their pieces of four turned by the row).
-template <int NE>
-__device__ __forceinline__ void add_distances(const Bias& bias, const f16v (&dr)[BiasOf<NE>::kBlocks], unsigned places,
+// go through LDS (32 rows of the columns, their pieces of four turned by the row).
+template <int ST>
+__device__ __forceinline__ void add_distances(const Bias& bias, const f16v (&dr)[BiasOf<ST>::kBlocks], unsigned places,
                                               bool real, float* lds, float* out, int t) {
-  constexpr int kWidth = 32 * NE, kTurn = kWidth / 4 - 1;
+  constexpr int kWidth = BiasOf<ST>::kWidth, kTurn = kWidth / 4 - 1;
   __shared__ unsigned row_places[32];
   const int lane = t & 63, half = lane >> 5, wave = t >> 6, own = lane & 31;
   int axis = 0;  // of distance t; the last axis has the numbers that no distance has, too
@@ -177,7 +177,7 @@ __device__ __forceinline__ void add_distances(const Bias& bias, const f16v (&dr)
     if (wave == w) {
       if (half == 0) row_places[own] = places;
 #pragma unroll
-      for (int n = 0; n < NE; ++n)
+      for (int n = 0; n < BiasOf<ST>::kBlocks; ++n)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           f4 v = {0.f, 0.f, 0.f, 0.f};
@@ -199,18 +199,19 @@ __device__ __forceinline__ void add_distances(const Bias& bias, const f16v (&dr)
 // Waves a SIMD that the registers are kept for.  16-bit, 2 x 16 heads of 4096 rows, both kernels: heads of 32 with four
 // 327 us (a few registers spill), with three 351; heads of 64 with three for dk and dv too (20 spill) 577 us, with two
 // there 505.
-template <typename T, int D>
+template <typename T, int D, int ST>
 constexpr int dq_waves() {
+  if (ST > 0) return ST > 4 || D * sizeof(T) >= 256 ? 1 : 2;
   return D * sizeof(T) >= 512 ? 1 : D * sizeof(T) == 64 ? 4 : D * sizeof(T) == 128 ? 3 : 2;
 }
 
 // dq and delta: 128 query rows of a head, key tiles streaming.
-template <typename T, int D, Cap CAP, int NE>
-__global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_kernel(Args a, BiasOf<NE> bias) {
+template <typename T, int D, Cap CAP, int ST>
+__global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq_kernel(Args a, BiasOf<ST> bias) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
-  typedef Stream<__bf16, BiasOf<NE>::kWidth, kTile, kThreads> LoadHot;
-  constexpr bool kOneHot = one_hot<T, D, NE>();
+  typedef Stream<__bf16, BiasOf<ST>::kWidth, kTile, kThreads> LoadHot;
+  constexpr bool kOneHot = one_hot<T, D, ST>();
   __shared__ __attribute__((aligned(16))) char hot0[kTile * LoadHot::Lds::kRow];
   __shared__ __attribute__((aligned(16))) char hot1[kOneHot ? 16 : kTile * LoadHot::Lds::kRow];
   __shared__ __attribute__((aligned(16))) char kt0[kTile * Lds::kRow];
@@ -228,7 +229,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
   if (a.prefixed) block = blocks - 1 - block;
   const int b = item / a.hq, h = item % a.hq;
   float* table_part = nullptr;
-  if constexpr (NE > 0) {
+  if constexpr (ST > 0) {
     const int64_t slot = ((int64_t)blockIdx.y * (docs ? 2 : 1) + part.part) * blocks + block;
     if (bias.part) table_part = bias.part + (((int64_t)b * a.hq + h) * bias.slots + slot) * kDistances;
   }
@@ -280,13 +281,13 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
 #pragma unroll
   for (int n = 0; n < ND; ++n) dq[n] = f16v(0.f);
   unsigned places = 0u;
-  BiasRow<T, NE> bias_of_row;
-  f16v dr[BiasOf<NE>::kBlocks];  // of r
-  if constexpr (NE > 0) {
+  BiasRow<T, ST> bias_of_row;
+  f16v dr[BiasOf<ST>::kBlocks];  // of r
+  if constexpr (ST > 0) {
     if (real) places = bias.query_places[b * bias.query_item + i];
-    bias_row<T, NE, false>(bias, bias_of_row, places, h, a.hq, kLog2e / units_of<CAP>(scoring), lane);
+    bias_row<T, ST, false>(bias, bias_of_row, places, h, a.hq, kLog2e / units_of<CAP>(scoring), lane);
 #pragma unroll
-    for (int n = 0; n < NE; ++n) dr[n] = f16v(0.f);
+    for (int n = 0; n < BiasOf<ST>::kBlocks; ++n) dr[n] = f16v(0.f);
   }
 
   const Meeting meet = meeting<kWaves>(wave, i0, a.lq, [&](int row) { return key_tiles(a, b, row, prefix, &part); });
@@ -296,8 +297,8 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
   krows.begin(k, a.kl, first * kTile, a.lk, a.d);
   vrows.begin(v, a.vl, first * kTile, a.lk, a.d);
   Rows<__bf16, kTile> hot_rows;
-  if constexpr (NE > 0) {
-    constexpr int kWidth = BiasOf<NE>::kWidth;
+  if constexpr (ST > 0) {
+    constexpr int kWidth = BiasOf<ST>::kRow;
     hot_rows.begin(bias.key_hot + b * bias.key_item * kWidth, kWidth, first * kTile, a.lk, kWidth);
   }
   typedef Stream<T, D, kTile, kThreads> Load;
@@ -308,7 +309,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
   auto fetch = [&](char* kt, char* vt, char* hot) {
     Load::load(kt, krows, t);
     Load::load(vt, vrows, t);
-    if constexpr (NE > 0 && !kOneHot) fetch_hot(hot);
+    if constexpr (ST > 0 && !kOneHot) fetch_hot(hot);
     krows.next();
     vrows.next();
   };
@@ -317,7 +318,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
     const int k0 = tile * kTile;
     const bool partial = meet.partial(tile);
     arrive();
-    if constexpr (NE > 0 && kOneHot) {
+    if constexpr (ST > 0 && kOneHot) {
       fetch_hot(hot);
       arrive();
     }
@@ -342,9 +343,9 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
       const int at = k0 + 32 * u + 4 * half;
       f16v db = ds;  // of the bias: before the cap's slope
       const float c = scores<T, CAP>(scoring, s, ds, at, pos, [&](f16v& s) {
-        if constexpr (NE > 0) add_bias<T, NE>(s, bias_of_row, hot, 32 * u, la);
+        if constexpr (ST > 0) add_bias<T, ST>(s, bias_of_row, hot, 32 * u, la);
       });
-      if constexpr (NE > 0 && CAP != kNoCap) {
+      if constexpr (ST > 0 && CAP != kNoCap) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, kHalf<T> ? raise - lse : -lse));
@@ -375,14 +376,16 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
           for (int r = 0; r < 16; ++r) ds[r] = 8 * (r >> 2) + (r & 3) >= limit - at ? 0.f : ds[r];
       };
       if (masked) hide_keys(ds);
-      if constexpr (NE > 0) {
+      if constexpr (ST > 0) {
         if constexpr (CAP == kNoCap) {
           db = ds;
         } else if (masked) {
           hide_keys(db);
         }
-        if constexpr (kHalf<T>) db *= __builtin_ldexpf(1.0f, -(int)raise);
-        add_row_gradient<T, NE>(dr, db, hot, 32 * u, la);
+        if (table_part) {
+          if constexpr (kHalf<T>) db *= __builtin_ldexpf(1.0f, -(int)raise);
+          add_row_gradient<T, ST>(dr, db, hot, 32 * u, la);
+        }
       }
       if constexpr (kHalf<T>) keep_in_range<false, ND>(ds, dq, raise);
 #pragma unroll
@@ -399,8 +402,8 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
     step(tile, kt0, vt0, hot0, kt1, vt1, other);
     if (tile + 1 < last) step(tile + 1, kt1, vt1, other, kt0, vt0, hot0);
   }
-  if constexpr (NE > 0) {
-    if (table_part) add_distances<NE>(bias, dr, places, real, reinterpret_cast<float*>(hot0), table_part, t);
+  if constexpr (ST > 0) {
+    if (table_part) add_distances<ST>(bias, dr, places, real, reinterpret_cast<float*>(hot0), table_part, t);
     if (!a.dq) return;
   }
   if (!real) return;
@@ -412,18 +415,19 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D>())) void attention_dq_ker
                           a.d, lane);
 }
 
-template <typename T, int D>
+template <typename T, int D, int ST>
 constexpr int dkv_waves() {
+  if (ST > 0) return D * sizeof(T) >= 256 || (ST > 4 && D * sizeof(T) > 64) ? 1 : 2;
   return D * sizeof(T) >= 256 ? 1 : D * sizeof(T) == 64 ? 4 : 2;
 }
 
 // dk and dv: 128 keys of a key head, the query tiles of its heads streaming.
-template <typename T, int D, Cap CAP, int NE>
-__global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_kernel(Args a, BiasOf<NE> bias) {
+template <typename T, int D, Cap CAP, int ST>
+__global__ __launch_bounds__(kThreads, (dkv_waves<T, D, ST>())) void attention_dkv_kernel(Args a, BiasOf<ST> bias) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
-  typedef Stream<__bf16, BiasOf<NE>::kWidth, kTile, kThreads> LoadHot;
-  constexpr bool kOneHot = one_hot<T, D, NE>();
+  typedef Stream<__bf16, BiasOf<ST>::kWidth, kTile, kThreads> LoadHot;
+  constexpr bool kOneHot = one_hot<T, D, ST>();
   __shared__ __attribute__((aligned(16))) char hot0[kTile * LoadHot::Lds::kRow];
   __shared__ __attribute__((aligned(16))) char hot1[kOneHot ? 16 : kTile * LoadHot::Lds::kRow];
   __shared__ __attribute__((aligned(16))) char qt0[kTile * Lds::kRow];
@@ -475,14 +479,14 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
   int fetched = h, at_tile = tile + 1;  // head and tile of the next fetch
   bool begun = false;
   unsigned places = 0u;
-  BiasRow<T, NE> bias_of_row;
+  BiasRow<T, ST> bias_of_row;
   Rows<__bf16, kTile> hot_rows;
-  if constexpr (NE > 0) {
+  if constexpr (ST > 0) {
     if (real) places = bias.key_places[b * bias.key_item + j];
   }
   auto begin_hot = [&](int at) {
-    if constexpr (NE > 0) {
-      constexpr int kWidth = BiasOf<NE>::kWidth;
+    if constexpr (ST > 0) {
+      constexpr int kWidth = BiasOf<ST>::kRow;
       hot_rows.begin(bias.query_hot + b * bias.query_item * kWidth, kWidth, at * kTile, a.lq, kWidth);
     }
   };
@@ -493,13 +497,13 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
   auto fetch = [&](char* qt, char* gt, float* stats, char* hot) {
     if (at_tile == first || !begun) {
       begun = true;
-      if constexpr (NE > 0 && !kOneHot) begin_hot(at_tile);
+      if constexpr (ST > 0 && !kOneHot) begin_hot(at_tile);
       qrows.begin(static_cast<const T*>(a.q) + b * a.qb + fetched * a.qh, a.ql, at_tile * kTile, a.lq, a.d);
       grows.begin(static_cast<const T*>(a.dout) + b * a.gb + fetched * a.gh, a.gl, at_tile * kTile, a.lq, a.d);
     }
     Load::load(qt, qrows, t);
     Load::load(gt, grows, t);
-    if constexpr (NE > 0 && !kOneHot) fetch_hot(hot);
+    if constexpr (ST > 0 && !kOneHot) fetch_hot(hot);
     qrows.next();
     grows.next();
     const int64_t row = ((int64_t)b * a.hq + fetched) * a.lq;
@@ -522,7 +526,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
     const bool partial = meet.partial(tile);
     if (a.slopes) scoring.slope = a.slopes[h];
     arrive();
-    if constexpr (NE > 0 && kOneHot) {
+    if constexpr (ST > 0 && kOneHot) {
       begin_hot(tile);
       fetch_hot(hot);
       arrive();
@@ -589,7 +593,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
       }
       const int at = i0 + 32 * u + 4 * half;
       const float c = scores<T, CAP>(scoring, s, ds, at, j - off, [&](f16v& s) {
-        if constexpr (NE > 0) add_bias<T, NE>(s, bias_of_row, hot, 32 * u, la);
+        if constexpr (ST > 0) add_bias<T, ST>(s, bias_of_row, hot, 32 * u, la);
       });
       const float raised = kHalf<T> ? __builtin_ldexpf(1.0f, (int)(raise - kRaise)) : 1.0f;  // p is raised already
 #pragma unroll
@@ -663,11 +667,11 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_k
   if (mine.x < mine.y) fetch(qt0, gt0, stats0, hot0);
   int head = -1;  // whose r' the registers hold
   auto turn = [&]() {
-    if constexpr (NE > 0) {
+    if constexpr (ST > 0) {
       const int next = h + (tile + 1 == last ? 1 : 0);  // of the next step
       if (next == head) return;
       head = next;
-      bias_row<T, NE, true>(bias, bias_of_row, places, head, a.hq, kLog2e / units_of<CAP>(scoring), lane);
+      bias_row<T, ST, true>(bias, bias_of_row, places, head, a.hq, kLog2e / units_of<CAP>(scoring), lane);
     }
   };
   for (int s = mine.x; s < mine.y; s += 2) {
@@ -740,14 +744,14 @@ int key_parts(const ctmr_masked_attention_desc* d) {
                     ceil_div(d->lq, kTile) * (d->q_heads / d->k_heads), d->elem, d->head_dim);
 }
 
-template <typename T, int D, Cap CAP, int NE>
-int launch(Args a, const BiasOf<NE>& bias, int qparts, int kparts, hipStream_t st) {
+template <typename T, int D, Cap CAP, int ST>
+int launch(Args a, const BiasOf<ST>& bias, int qparts, int kparts, hipStream_t st) {
   const unsigned parts = a.qdoc.ids ? 2u : 1u;
   bool table = false;
-  if constexpr (NE > 0) table = bias.part != nullptr;
+  if constexpr (ST > 0) table = bias.part != nullptr;
   a.splits = a.dq || table ? qparts : 1;
   const unsigned q_blocks = a.n * a.hq * (unsigned)ceil_div(a.lq, kOwn) * parts;
-  hipLaunchKernelGGL((attention_dq_kernel<T, D, CAP, NE>), dim3(q_blocks, a.splits), dim3(kThreads), 0, st, a, bias);
+  hipLaunchKernelGGL((attention_dq_kernel<T, D, CAP, ST>), dim3(q_blocks, a.splits), dim3(kThreads), 0, st, a, bias);
   int rc = check_launch("attention_dq");
   if (rc) return rc;
   if (a.splits > 1 && a.dq) {
@@ -761,7 +765,7 @@ int launch(Args a, const BiasOf<NE>& bias, int qparts, int kparts, hipStream_t s
   if (!a.dk && !a.dv) return rc;
   a.splits = kparts;
   const unsigned k_blocks = a.n * a.hk * (unsigned)ceil_div(a.lk, kOwn) * parts;
-  hipLaunchKernelGGL((attention_dkv_kernel<T, D, CAP, NE>), dim3(k_blocks, a.splits), dim3(kThreads), 0, st, a, bias);
+  hipLaunchKernelGGL((attention_dkv_kernel<T, D, CAP, ST>), dim3(k_blocks, a.splits), dim3(kThreads), 0, st, a, bias);
   rc = check_launch("attention_dkv");
   if (rc || a.splits == 1) return rc;
   SumArgs s = {a.part, {a.dk, a.dv}, {a.dkb, a.dvb}, {a.dkh, a.dvh}, {a.dkl, a.dvl}, {ds_scale<CAP>(a), 1.0f},

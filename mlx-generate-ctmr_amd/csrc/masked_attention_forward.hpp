@@ -221,13 +221,18 @@ __device__ __forceinline__ void write_row(const Args& a, const f16v (&o)[ND], fl
 // The tiled form: a workgroup of four waves takes 128 query rows of a head, 32 a
 // wave, and streams K and V through LDS in 64-key tiles: the next tile is loaded
 // straight into a second pair of arrays while the current one is multiplied.
-template <typename T, int D, Cap CAP, int NE>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void attention_kernel(Args a,
-                                                                                                 BiasOf<NE> bias) {
+template <typename T, int D, int ST>
+constexpr int tiled_waves() {
+  if (ST > 0) return D == 128 || (ST > 4 && D * sizeof(T) > 64) || D * sizeof(T) > 128 ? 1 : 2;
+  return sizeof(T) == 4 && D == 128 ? 1 : 2;
+}
+
+template <typename T, int D, Cap CAP, int ST>
+__global__ __launch_bounds__(kThreads, (tiled_waves<T, D, ST>())) void attention_kernel(Args a, BiasOf<ST> bias) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
-  typedef Stream<__bf16, BiasOf<NE>::kWidth, kTile, kThreads> LoadHot;
-  constexpr bool kOneHot = one_hot<T, D, NE>();
+  typedef Stream<__bf16, BiasOf<ST>::kWidth, kTile, kThreads> LoadHot;
+  constexpr bool kOneHot = one_hot<T, D, ST>();
   __shared__ __attribute__((aligned(16))) char kt0[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) char vt0[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) char kt1[kTile * Lds::kRow];
@@ -274,12 +279,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
   Rows<T, kTile> krows, vrows;
   krows.begin(k, a.kl, first * kTile, a.lk, a.d);
   vrows.begin(v, a.vl, first * kTile, a.lk, a.d);
-  BiasRow<T, NE> bias_of_row;
+  BiasRow<T, ST> bias_of_row;
   Rows<__bf16, kTile> hot_rows;
-  if constexpr (NE > 0) {
+  if constexpr (ST > 0) {
     const unsigned places = mine ? bias.query_places[b * bias.query_item + i] : 0u;
-    bias_row<T, NE, false>(bias, bias_of_row, places, h, a.hq, kLog2e / units_of<CAP>(scoring), lane);
-    constexpr int kWidth = BiasOf<NE>::kWidth;
+    bias_row<T, ST, false>(bias, bias_of_row, places, h, a.hq, kLog2e / units_of<CAP>(scoring), lane);
+    constexpr int kWidth = BiasOf<ST>::kRow;
     hot_rows.begin(bias.key_hot + b * bias.key_item * kWidth, kWidth, first * kTile, a.lk, kWidth);
   }
   typedef Stream<T, D, kTile, kThreads> Load;
@@ -290,7 +295,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
   auto fetch = [&](char* kt, char* vt, char* hot) {
     Load::load(kt, krows, t);
     Load::load(vt, vrows, t);
-    if constexpr (NE > 0 && !kOneHot) fetch_hot(hot);
+    if constexpr (ST > 0 && !kOneHot) fetch_hot(hot);
     krows.next();
     vrows.next();
   };
@@ -299,7 +304,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
     const int k0 = tile * kTile;
     const bool partial = meet.partial(tile);  // some row of the workgroup has a masked key in it
     arrive();
-    if constexpr (NE > 0 && kOneHot) {
+    if constexpr (ST > 0 && kOneHot) {
       fetch_hot(hot);
       arrive();
     }
@@ -326,9 +331,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
       for (int n = 0; n < ND; ++n) vf[w][n] = Lds::down(vt, 16 * w, n, at);
     const int* tile_ids = docs ? ids + k0 : nullptr;
     const float c = score_blocks<T, 2, CAP>(scoring, s, k0, pos, meet.masked(tile), mask, tile_ids, lane, [&](auto& s) {
-      if constexpr (NE > 0)
+      if constexpr (ST > 0)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) add_bias<T, NE>(s[u], bias_of_row, hot, 32 * u, at);
+        for (int u = 0; u < 2; ++u) add_bias<T, ST>(s[u], bias_of_row, hot, 32 * u, at);
     });
     float alpha;
     Frag<T> p[2][2];
@@ -348,7 +353,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
             if constexpr (fine) o[n] = mma<T>(f, fine_weights<T>(s[u], p[u][w], w), o[n]);
           }
     };
-    if constexpr (NE > 0 && sizeof(T) == 2) {
+    if constexpr (ST > 0 && sizeof(T) == 2) {
       if (bias.fine) products(std::true_type());
       else products(std::false_type());
     } else {
@@ -383,12 +388,12 @@ constexpr int few_lds() {  // bytes; the join takes four 32 x D blocks of fp32 a
   return tiles > join ? tiles : join;
 }
 
-template <typename T, int D, Cap CAP, int NE>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 64 ? 2 : 1) void attention_few_kernel(Args a,
-                                                                                                    BiasOf<NE> bias) {
+template <typename T, int D, Cap CAP, int ST>
+__global__ __launch_bounds__(kThreads, ST == 0 && sizeof(T) == 4 && D == 64 ? 2 : 1) void attention_few_kernel(
+    Args a, BiasOf<ST> bias) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
-  typedef Stream<__bf16, BiasOf<NE>::kWidth, kFewTile, 64> LoadHot;
+  typedef Stream<__bf16, BiasOf<ST>::kWidth, kFewTile, 64> LoadHot;
   __shared__ __attribute__((aligned(16))) char hots[kWaves][kFewTile * LoadHot::Lds::kRow];
   __shared__ __attribute__((aligned(16))) char lds[few_lds<T, D>()];
   __shared__ unsigned odd[kWaves];
@@ -424,9 +429,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 64 ? 2 : 1) void a
   for (int n = 0; n < ND; ++n) o[n] = f16v(0.f);
   float m = kNone, l = 0.f;
 
-  BiasRow<T, NE> bias_of_row;
-  if constexpr (NE > 0)
-    bias_row<T, NE, false>(bias, bias_of_row, bias.query_places[b * bias.query_item + i], h, a.hq,
+  BiasRow<T, ST> bias_of_row;
+  if constexpr (ST > 0)
+    bias_row<T, ST, false>(bias, bias_of_row, bias.query_places[b * bias.query_item + i], h, a.hq,
                            kLog2e / units_of<CAP>(scoring), lane);
   Stream<T, D, kFewTile, 64> ks, vs;
   LoadHot hot;
@@ -437,8 +442,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 64 ? 2 : 1) void a
     vrows.begin(v, a.vl, at, a.lk, a.d);
     ks.fetch(krows, lane);
     vs.fetch(vrows, lane);
-    if constexpr (NE > 0) {
-      constexpr int kWidth = BiasOf<NE>::kWidth;
+    if constexpr (ST > 0) {
+      constexpr int kWidth = BiasOf<ST>::kRow;
       Rows<__bf16, kFewTile> rows;
       rows.begin(bias.key_hot + b * bias.key_item * kWidth, kWidth, at, a.lk, kWidth);
       hot.fetch(rows, lane);
@@ -452,7 +457,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 64 ? 2 : 1) void a
     ks.template store<false>(kt, nullptr, lane);
     if (partial) vs.template store<true>(vt, &odd[wave], lane);
     else vs.template store<false>(vt, nullptr, lane);
-    if constexpr (NE > 0) hot.template store<false>(hots[wave], nullptr, lane);
+    if constexpr (ST > 0) hot.template store<false>(hots[wave], nullptr, lane);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const int next = k0 + kWaves * kFewTile;
     if (next < end) fetch(next);
@@ -461,7 +466,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 64 ? 2 : 1) void a
     for (int n = 0; n < NK; ++n) s[0] = mma<T>(Lds::along(kt, 0, n, lane), qf[n], s[0]);
     const float c = score_blocks<T, 1, CAP>(scoring, s, k0, pos, partial, mask, docs ? ids + k0 : nullptr, lane,
                                             [&](auto& s) {
-                                              if constexpr (NE > 0) add_bias<T, NE>(s[0], bias_of_row, hots[wave], 0, lane);
+                                              if constexpr (ST > 0) add_bias<T, ST>(s[0], bias_of_row, hots[wave], 0, lane);
                                             });
     float alpha;
     Frag<T> p[1][2];
@@ -475,7 +480,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 64 ? 2 : 1) void a
       for (int n = 0; n < ND; ++n) {
         const Frag<T> f = Lds::down(vt, 16 * w, n, lane);
         o[n] = mma<T>(f, p[0][w], o[n]);
-        if constexpr (NE > 0 && sizeof(T) == 2)
+        if constexpr (ST > 0 && sizeof(T) == 2)
           if (bias.fine) o[n] = mma<T>(f, fine_weights<T>(s[0], p[0][w], w), o[n]);
       }
     if (partial) {
@@ -624,23 +629,23 @@ int split_count(const ctmr_masked_attention_desc* d) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / least, kMostSplits}));
 }
 
-template <typename T, int D, Cap CAP, int NE>
-void launch_form(const Args& a, const BiasOf<NE>& bias, bool few, hipStream_t st) {
+template <typename T, int D, Cap CAP, int ST>
+void launch_form(const Args& a, const BiasOf<ST>& bias, bool few, hipStream_t st) {
   // With fp32 heads of 128 and the widest bias the few-row form's tiles do not fit LDS.
-  constexpr bool kFits = few_lds<T, D>() + kWaves * kFewTile * 64 * NE + 2048 <= 160 * 1024;
+  constexpr bool kFits = few_lds<T, D>() + kWaves * kFewTile * 2 * BiasOf<ST>::kWidth + 2048 <= 160 * 1024;
   if constexpr (kFits) {
     if (few) {
-      hipLaunchKernelGGL((attention_few_kernel<T, D, CAP, NE>), dim3(a.n * a.hk, a.splits), dim3(kThreads), 0, st, a, bias);
+      hipLaunchKernelGGL((attention_few_kernel<T, D, CAP, ST>), dim3(a.n * a.hk, a.splits), dim3(kThreads), 0, st, a, bias);
       return;
     }
   }
-  hipLaunchKernelGGL((attention_kernel<T, D, CAP, NE>),
+  hipLaunchKernelGGL((attention_kernel<T, D, CAP, ST>),
                      dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kRows) * (a.qdoc.ids ? 2u : 1u), a.splits), dim3(kThreads), 0,
                      st, a, bias);
 }
 
-template <typename T, int D, int NE>
-int launch(const Args& a, const BiasOf<NE>& bias, bool few, hipStream_t st) {
+template <typename T, int D, int ST>
+int launch(const Args& a, const BiasOf<ST>& bias, bool few, hipStream_t st) {
   bool shifted = false;
   if constexpr (sizeof(T) == 2) {  // without a cap too
     shifted = shifted_cap<T>(a.cap);

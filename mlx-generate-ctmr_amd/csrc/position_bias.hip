@@ -6,10 +6,10 @@
 namespace ctmr {
 namespace attn {
 
-int bias_width(const ctmr_buckets_desc* b) {
+int bias_steps(const ctmr_buckets_desc* b) {
   int columns = 0;
   for (int a = 0; a < b->axes; ++a) columns += b->extents[a];
-  return columns <= 64 ? 64 : 128;
+  return columns <= 48 ? 3 : columns <= 64 ? 4 : columns <= 96 ? 6 : 8;
 }
 
 namespace {
@@ -38,7 +38,7 @@ struct Parts {
 // Where a plan's parts start.  One-hot rows of equal sides are the same.
 Parts parts_of(const ctmr_buckets_desc* b) {
   Parts p = {};
-  const int64_t width = bias_width(b) * 2, q = (int64_t)b->query_items * b->lq, k = (int64_t)b->key_items * b->lk;
+  const int64_t width = bias_steps(b) * 32, q = (int64_t)b->query_items * b->lq, k = (int64_t)b->key_items * b->lk;
   auto take = [&](int64_t size) {
     const int64_t at = p.bytes;
     p.bytes += round_up(size, 256);
@@ -189,7 +189,7 @@ int ctmr_buckets(const ctmr_buckets_desc* b, const int32_t* query_places, const 
   a.hot[0] = reinterpret_cast<__bf16*>(base + p.query_hot), a.hot[1] = reinterpret_cast<__bf16*>(base + p.key_hot);
   a.rows[0] = (int64_t)b->query_items * b->lq, a.rows[1] = b->same ? 0 : (int64_t)b->key_items * b->lk;
   a.table = reinterpret_cast<int*>(base + p.rows);
-  a.axes = b->axes, a.width = bias_width(b);
+  a.axes = b->axes, a.width = 16 * bias_steps(b);
   std::copy(b->extents, b->extents + 4, a.extents);
   static_assert(kNumbers * 4 % 256 == 0 && kColumns * 4 % 256 == 0, "the tables lie one behind the other");
   hipLaunchKernelGGL(places_kernel, dim3((unsigned)ceil_div(std::max(a.rows[0], a.rows[1]), 256), b->same ? 1 : 2), dim3(256),

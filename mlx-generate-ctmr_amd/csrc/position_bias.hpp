@@ -33,7 +33,7 @@ struct Bias {
   const int* query_columns;  // (kColumns) axis << 16 | the number of column c's distance from place 0
   const int* key_columns;    // likewise to place 0
   const unsigned *query_places, *key_places;  // (items, rows) a byte for each axis
-  const __bf16 *query_hot, *key_hot;          // (items, rows, 32 NE) o
+  const __bf16 *query_hot, *key_hot;          // (items, rows, 16 ST) o
   int64_t query_item, key_item;               // rows from item to item (0: all have the same)
   const void* table;         // (table_rows, hq)
   int elem, table_rows, axes;
@@ -43,23 +43,25 @@ struct Bias {
   int slots;
 };
 
-// 32-column blocks of r and o; 0: no bias.
-template <int NE>
+// ST: contraction steps of 16 columns, 3, 4, 6 or 8; 0: no bias.
+template <int ST>
 struct BiasOf : Bias {
-  static constexpr int kBlocks = NE, kSteps = 2 * NE, kWidth = 32 * NE;
+  static constexpr int kSteps = ST, kBlocks = (ST + 1) / 2;  // 32-column blocks
+  static constexpr int kRow = 16 * ST;                       // columns of a row of o in memory
+  static constexpr int kWidth = ST <= 4 ? 64 : 128;          // and of a tile in LDS, zeros past them
 };
 template <>
 struct BiasOf<0> {
-  static constexpr int kBlocks = 1, kSteps = 1, kWidth = 32;  // of arrays that nothing uses
+  static constexpr int kSteps = 1, kBlocks = 1, kRow = 32, kWidth = 32;  // of arrays that nothing uses
 };
 
 template <typename T>
 constexpr int kParts = sizeof(T) == 4 ? 3 : 2;
 
 // A lane's r of one row, in parts.
-template <typename T, int NE>
+template <typename T, int ST>
 struct BiasRow {
-  Frag<__bf16> part[BiasOf<NE>::kSteps][kParts<T>];
+  Frag<__bf16> part[BiasOf<ST>::kSteps][kParts<T>];
 };
 
 // The table's value for a distance's number, in units of 1 / `unit`.  What is below -2^100 hides a pair: the score that it
@@ -72,12 +74,12 @@ __device__ __forceinline__ float bias_value(const Bias& b, int number, int h, in
 }
 
 // r of a row at `places` for head h.  KEYS: of a key (r').
-template <typename T, int NE, bool KEYS>
-__device__ __forceinline__ void bias_row(const Bias& b, BiasRow<T, NE>& out, unsigned places, int h, int hq, float unit,
+template <typename T, int ST, bool KEYS>
+__device__ __forceinline__ void bias_row(const Bias& b, BiasRow<T, ST>& out, unsigned places, int h, int hq, float unit,
                                          int lane) {
   const int* columns = KEYS ? b.key_columns : b.query_columns;
 #pragma unroll
-  for (int n = 0; n < 2 * NE; ++n)
+  for (int n = 0; n < ST; ++n)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int c = columns[16 * n + 8 * (lane >> 5) + e];
@@ -93,35 +95,35 @@ __device__ __forceinline__ void bias_row(const Bias& b, BiasRow<T, NE>& out, uns
 }
 
 // Adds the bias of 32 rows of one-hot values in LDS to raw scores.
-template <typename T, int NE>
-__device__ __forceinline__ void add_bias(f16v& s, const BiasRow<T, NE>& r, const char* hot, int row, int lane) {
+template <typename T, int ST>
+__device__ __forceinline__ void add_bias(f16v& s, const BiasRow<T, ST>& r, const char* hot, int row, int lane) {
 #pragma unroll
-  for (int n = 0; n < 2 * NE; ++n) {
-    const Frag<__bf16> o = Tile<__bf16, 32 * NE>::along(hot, row, n, lane);
+  for (int n = 0; n < ST; ++n) {
+    const Frag<__bf16> o = Tile<__bf16, BiasOf<ST>::kWidth>::along(hot, row, n, lane);
 #pragma unroll
     for (int p = 0; p < kParts<T>; ++p) s = mma<__bf16>(o, r.part[n][p], s);
   }
 }
 
 // Whether the one-hot rows of a bias have one array instead of two: where LDS holds no more.
-template <typename T, int D, int NE>
+template <typename T, int D, int ST>
 constexpr bool one_hot() {
-  return 4 * kTile * Tile<T, D>::kRow + 2 * kTile * 64 * NE + 2048 > 160 * 1024;
+  return 4 * kTile * Tile<T, D>::kRow + 4 * kTile * BiasOf<ST>::kWidth + 2048 > 160 * 1024;
 }
 
 int check_buckets(const ctmr_masked_attention_desc* d, const ctmr_buckets_desc* b);
 Bias make_bias(const ctmr_masked_attention_desc* d, const ctmr_buckets_desc* b, const void* plan, const void* table);
-int bias_width(const ctmr_buckets_desc* b);  // columns, rounded up to what the kernels have
+int bias_steps(const ctmr_buckets_desc* b);  // contraction steps that the kernels have
 
-// The gradients' kernels for heads of T; narrow: 64 columns.
+// The gradients' kernels for heads of T.
 template <typename T>
-int run_biased_gradients(const Args& a, const Bias& bias, bool narrow, int qparts, int kparts, hipStream_t st);
+int run_biased_gradients(const Args& a, const Bias& bias, int steps, int qparts, int kparts, hipStream_t st);
 template <>
-int run_biased_gradients<float>(const Args&, const Bias&, bool, int, int, hipStream_t);
+int run_biased_gradients<float>(const Args&, const Bias&, int, int, int, hipStream_t);
 template <>
-int run_biased_gradients<__bf16>(const Args&, const Bias&, bool, int, int, hipStream_t);
+int run_biased_gradients<__bf16>(const Args&, const Bias&, int, int, int, hipStream_t);
 template <>
-int run_biased_gradients<_Float16>(const Args&, const Bias&, bool, int, int, hipStream_t);
+int run_biased_gradients<_Float16>(const Args&, const Bias&, int, int, int, hipStream_t);
 
 }  // namespace attn
 }  // namespace ctmr
