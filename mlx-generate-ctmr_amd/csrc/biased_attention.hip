@@ -19,26 +19,18 @@ extern "C" int ctmr_biased_attention(const ctmr_masked_attention_desc* d, const 
   Args a = make_args(d, q, k, v, slopes, prefixes, plan);
   a.out = out, a.rest = rest, a.lse = lse, a.part = (float*)workspace, a.splits = split_count(d);
   a.ob = d->out_strides[0], a.oh = d->out_strides[1], a.ol = d->out_strides[2];
-  Bias bias = make_bias(d, buckets, bucket_plan, table);
+  BiasOf<kForwardBias> bias{make_bias(d, buckets, bucket_plan, table)};
   bias.fine = fine != 0;
   const bool few = few_rows(d);
   hipStream_t st = (hipStream_t)stream;
-#define CTMR_BIASED_WIDTH(T, D)                                      \
-  switch (bias_steps(buckets)) {                                     \
-    case 3: return launch<T, D>(a, BiasOf<3>{bias}, few, st);        \
-    case 4: return launch<T, D>(a, BiasOf<4>{bias}, few, st);        \
-    case 6: return launch<T, D>(a, BiasOf<6>{bias}, few, st);        \
-    default: return launch<T, D>(a, BiasOf<8>{bias}, few, st);       \
-  }
-#define CTMR_BIASED_TYPE(T)              \
-  switch (padded(d->head_dim)) {         \
-    case 32: CTMR_BIASED_WIDTH(T, 32)    \
-    case 64: CTMR_BIASED_WIDTH(T, 64)    \
-    default: CTMR_BIASED_WIDTH(T, 128)   \
+#define CTMR_BIASED_TYPE(T)                           \
+  switch (padded(d->head_dim)) {                      \
+    case 32: return launch<T, 32>(a, bias, few, st);  \
+    case 64: return launch<T, 64>(a, bias, few, st);  \
+    default: return launch<T, 128>(a, bias, few, st); \
   }
   if (d->elem == CTMR_ELEM_F32) CTMR_BIASED_TYPE(float)
   if (d->elem == CTMR_ELEM_BF16) CTMR_BIASED_TYPE(__bf16)
   CTMR_BIASED_TYPE(_Float16)
 #undef CTMR_BIASED_TYPE
-#undef CTMR_BIASED_WIDTH
 }

@@ -174,8 +174,9 @@ __device__ __forceinline__ void arrive() {
   __syncthreads();
 }
 
-// A wave's 64 floats from place `first` of `count` straight into LDS, zeros past the end.  Complete after arrive().
-__device__ __forceinline__ void load_floats(float* to, const float* from, int first, int count, int lane) {
+// A wave's 64 words from place `first` of `count` straight into LDS, zeros past the end.  Complete after arrive().
+template <typename W>
+__device__ __forceinline__ void load_words(W* to, const W* from, int first, int count, int lane) {
   typedef __attribute__((address_space(3))) void lds_void;
   const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
       (void*)(from + first), (short)0, max(min(count - first, 64), 0) * 4, 0x00020000);

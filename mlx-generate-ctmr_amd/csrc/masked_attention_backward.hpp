@@ -205,6 +205,8 @@ constexpr int dq_waves() {
   return D * sizeof(T) >= 512 ? 1 : D * sizeof(T) == 64 ? 4 : D * sizeof(T) == 128 ? 3 : 2;
 }
 
+extern __shared__ __attribute__((aligned(16))) char bias_values[];  // of a position bias (lay_out_bias)
+
 // dq and delta: 128 query rows of a head, key tiles streaming.
 template <typename T, int D, Cap CAP, int ST>
 __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq_kernel(Args a, BiasOf<ST> bias) {
@@ -214,6 +216,8 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
   constexpr bool kOneHot = one_hot<T, D, ST>();
   __shared__ __attribute__((aligned(16))) char hot0[kTile * LoadHot::Lds::kRow];
   __shared__ __attribute__((aligned(16))) char hot1[kOneHot ? 16 : kTile * LoadHot::Lds::kRow];
+  __shared__ __attribute__((aligned(16))) unsigned words0[kTile];
+  __shared__ __attribute__((aligned(16))) unsigned words1[kTile];
   __shared__ __attribute__((aligned(16))) char kt0[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) char vt0[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) char kt1[kTile * Lds::kRow];
@@ -281,11 +285,13 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
 #pragma unroll
   for (int n = 0; n < ND; ++n) dq[n] = f16v(0.f);
   unsigned places = 0u;
-  BiasRow<T, ST> bias_of_row;
+  unsigned word = 0u;
   f16v dr[BiasOf<ST>::kBlocks];  // of r
   if constexpr (ST > 0) {
     if (real) places = bias.query_places[b * bias.query_item + i];
-    bias_row<T, ST, false>(bias, bias_of_row, places, h, a.hq, kLog2e / units_of<CAP>(scoring), lane);
+    word = row_word<kSingle<T, D>>(bias, b, i, a.lq);
+    lay_out_bias<kSingle<T, D>, kThreads>(bias, bias_values, h, a.hq, kLog2e / units_of<CAP>(scoring),
+                                          t);  // arrive() comes before its use
 #pragma unroll
     for (int n = 0; n < BiasOf<ST>::kBlocks; ++n) dr[n] = f16v(0.f);
   }
@@ -299,30 +305,35 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
   Rows<__bf16, kTile> hot_rows;
   if constexpr (ST > 0) {
     constexpr int kWidth = BiasOf<ST>::kRow;
-    hot_rows.begin(bias.key_hot + b * bias.key_item * kWidth, kWidth, first * kTile, a.lk, kWidth);
+    hot_rows.begin(bias.key_hot + b * bias.hot_item * kWidth, kWidth, first * kTile, a.lk, kWidth);
   }
   typedef Stream<T, D, kTile, kThreads> Load;
   auto fetch_hot = [&](char* hot) {
     LoadHot::load(hot, hot_rows, t);
     hot_rows.next();
   };
-  auto fetch = [&](char* kt, char* vt, char* hot) {
+  auto fetch = [&](int tile, char* kt, char* vt, char* hot, unsigned* words) {
     Load::load(kt, krows, t);
     Load::load(vt, vrows, t);
-    if constexpr (ST > 0 && !kOneHot) fetch_hot(hot);
+    if constexpr (ST > 0) {
+      if (!kOneHot && table_part) fetch_hot(hot);
+      if (wave == 0) load_words(words, (kSingle<T, D> ? bias.key_places : bias.key_codes) + b * bias.key_item, tile * kTile, a.lk, lane);
+    }
     krows.next();
     vrows.next();
   };
   // One tile, while the next one is on its way into the other pair of arrays.
-  auto step = [&](int tile, char* kt, char* vt, char* hot, char* next_kt, char* next_vt, char* next_hot) {
+  auto step = [&](int tile, char* kt, char* vt, char* hot, unsigned* words, char* next_kt, char* next_vt, char* next_hot,
+                  unsigned* next_words) {
     const int k0 = tile * kTile;
     const bool partial = meet.partial(tile);
     arrive();
-    if constexpr (ST > 0 && kOneHot) {
-      fetch_hot(hot);
-      arrive();
-    }
-    if (tile + 1 < last) fetch(next_kt, next_vt, next_hot);
+    if constexpr (ST > 0 && kOneHot)
+      if (table_part) {
+        fetch_hot(hot);
+        arrive();
+      }
+    if (tile + 1 < last) fetch(tile + 1, next_kt, next_vt, next_hot, next_words);
     if (partial) {
       if (t < 2) odd[t] = 0u;
       __syncthreads();
@@ -343,7 +354,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
       const int at = k0 + 32 * u + 4 * half;
       f16v db = ds;  // of the bias: before the cap's slope
       const float c = scores<T, CAP>(scoring, s, ds, at, pos, [&](f16v& s) {
-        if constexpr (ST > 0) add_bias<T, ST>(s, bias_of_row, hot, 32 * u, la);
+        if constexpr (ST > 0) add_bias<kSingle<T, D>, true>(s, bias_values, word, words + 32 * u, la);
       });
       if constexpr (ST > 0 && CAP != kNoCap) {
 #pragma unroll
@@ -397,10 +408,10 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
     }
   };
   char* const other = kOneHot ? hot0 : hot1;
-  if (first < last) fetch(kt0, vt0, hot0);
+  if (first < last) fetch(first, kt0, vt0, hot0, words0);
   for (int tile = first; tile < last; tile += 2) {
-    step(tile, kt0, vt0, hot0, kt1, vt1, other);
-    if (tile + 1 < last) step(tile + 1, kt1, vt1, other, kt0, vt0, hot0);
+    step(tile, kt0, vt0, hot0, words0, kt1, vt1, other, words1);
+    if (tile + 1 < last) step(tile + 1, kt1, vt1, other, words1, kt0, vt0, hot0, words0);
   }
   if constexpr (ST > 0) {
     if (table_part) add_distances<ST>(bias, dr, places, real, reinterpret_cast<float*>(hot0), table_part, t);
@@ -426,10 +437,8 @@ template <typename T, int D, Cap CAP, int ST>
 __global__ __launch_bounds__(kThreads, (dkv_waves<T, D, ST>())) void attention_dkv_kernel(Args a, BiasOf<ST> bias) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
-  typedef Stream<__bf16, BiasOf<ST>::kWidth, kTile, kThreads> LoadHot;
-  constexpr bool kOneHot = one_hot<T, D, ST>();
-  __shared__ __attribute__((aligned(16))) char hot0[kTile * LoadHot::Lds::kRow];
-  __shared__ __attribute__((aligned(16))) char hot1[kOneHot ? 16 : kTile * LoadHot::Lds::kRow];
+  __shared__ __attribute__((aligned(16))) unsigned words0[kTile];
+  __shared__ __attribute__((aligned(16))) unsigned words1[kTile];
   __shared__ __attribute__((aligned(16))) char qt0[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) char gt0[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) char qt1[kTile * Lds::kRow];
@@ -478,36 +487,26 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D, ST>())) void attention_d
   int h = hk * a.group + (tiles > 0 ? mine.x / tiles : 0), tile = first + (tiles > 0 ? mine.x % tiles : 0) - 1;
   int fetched = h, at_tile = tile + 1;  // head and tile of the next fetch
   bool begun = false;
-  unsigned places = 0u;
-  BiasRow<T, ST> bias_of_row;
-  Rows<__bf16, kTile> hot_rows;
+  unsigned word = 0u;
   if constexpr (ST > 0) {
-    if (real) places = bias.key_places[b * bias.key_item + j];
+    word = key_word<kSingle<T, D>>(bias, b, j, a.lk) - (kSingle<T, D> ? bias.reach : 0u);
   }
-  auto begin_hot = [&](int at) {
-    if constexpr (ST > 0) {
-      constexpr int kWidth = BiasOf<ST>::kRow;
-      hot_rows.begin(bias.query_hot + b * bias.query_item * kWidth, kWidth, at * kTile, a.lq, kWidth);
-    }
-  };
-  auto fetch_hot = [&](char* hot) {
-    LoadHot::load(hot, hot_rows, t);
-    hot_rows.next();
-  };
-  auto fetch = [&](char* qt, char* gt, float* stats, char* hot) {
+  const int query_room = (a.lq + kTile - 1) / kTile * kTile;  // words past the last row are a row's, too
+  auto fetch = [&](char* qt, char* gt, float* stats, unsigned* words) {
     if (at_tile == first || !begun) {
       begun = true;
-      if constexpr (ST > 0 && !kOneHot) begin_hot(at_tile);
       qrows.begin(static_cast<const T*>(a.q) + b * a.qb + fetched * a.qh, a.ql, at_tile * kTile, a.lq, a.d);
       grows.begin(static_cast<const T*>(a.dout) + b * a.gb + fetched * a.gh, a.gl, at_tile * kTile, a.lq, a.d);
     }
     Load::load(qt, qrows, t);
     Load::load(gt, grows, t);
-    if constexpr (ST > 0 && !kOneHot) fetch_hot(hot);
+    if constexpr (ST > 0)
+      if (wave == 2) load_words(words, (kSingle<T, D> ? bias.query_places : bias.query_codes) + b * bias.query_item, at_tile * kTile,
+                   query_room, lane);
     qrows.next();
     grows.next();
     const int64_t row = ((int64_t)b * a.hq + fetched) * a.lq;
-    if (wave < 2) load_floats(stats + wave * kTile, (wave == 0 ? a.lse : a.delta) + row, at_tile * kTile, a.lq, lane);
+    if (wave < 2) load_words(stats + wave * kTile, (wave == 0 ? a.lse : a.delta) + row, at_tile * kTile, a.lq, lane);
     if (++at_tile == last) {
       at_tile = first;
       ++fetched;
@@ -516,8 +515,8 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D, ST>())) void attention_d
   Scoring scoring = scoring_of(a, hk * a.group);
   float raise = kDsRaise<T>;
   // One tile, while the next one is on its way into the other arrays.
-  auto step = [&](bool more, char* qt, char* gt, float* stats, char* hot, char* next_qt, char* next_gt, float* next_stats,
-                  char* next_hot) {
+  auto step = [&](bool more, char* qt, char* gt, float* stats, unsigned* words, char* next_qt, char* next_gt,
+                  float* next_stats, unsigned* next_words) {
     if (++tile == last) {
       tile = first;
       ++h;
@@ -526,12 +525,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D, ST>())) void attention_d
     const bool partial = meet.partial(tile);
     if (a.slopes) scoring.slope = a.slopes[h];
     arrive();
-    if constexpr (ST > 0 && kOneHot) {
-      begin_hot(tile);
-      fetch_hot(hot);
-      arrive();
-    }
-    if (more) fetch(next_qt, next_gt, next_stats, next_hot);
+    if (more) fetch(next_qt, next_gt, next_stats, next_words);
     if (partial) {
       if (t < 4) odd[t >> 1][t & 1] = 0u;
       __syncthreads();
@@ -593,7 +587,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D, ST>())) void attention_d
       }
       const int at = i0 + 32 * u + 4 * half;
       const float c = scores<T, CAP>(scoring, s, ds, at, j - off, [&](f16v& s) {
-        if constexpr (ST > 0) add_bias<T, ST>(s, bias_of_row, hot, 32 * u, la);
+        if constexpr (ST > 0) add_bias<kSingle<T, D>, false>(s, bias_values, word, words + 32 * u, la);
       });
       const float raised = kHalf<T> ? __builtin_ldexpf(1.0f, (int)(raise - kRaise)) : 1.0f;  // p is raised already
 #pragma unroll
@@ -663,23 +657,23 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D, ST>())) void attention_d
       }
     }
   };
-  char* const other = kOneHot ? hot0 : hot1;
-  if (mine.x < mine.y) fetch(qt0, gt0, stats0, hot0);
-  int head = -1;  // whose r' the registers hold
+  if (mine.x < mine.y) fetch(qt0, gt0, stats0, words0);
+  int head = -1;  // whose bias LDS holds
   auto turn = [&]() {
     if constexpr (ST > 0) {
       const int next = h + (tile + 1 == last ? 1 : 0);  // of the next step
       if (next == head) return;
       head = next;
-      bias_row<T, ST, true>(bias, bias_of_row, places, head, a.hq, kLog2e / units_of<CAP>(scoring), lane);
+      __syncthreads();  // the last head's is read; arrive() comes before the next one's use
+      lay_out_bias<kSingle<T, D>, kThreads>(bias, bias_values, head, a.hq, kLog2e / units_of<CAP>(scoring), t);
     }
   };
   for (int s = mine.x; s < mine.y; s += 2) {
     turn();
-    step(s + 1 < mine.y, qt0, gt0, stats0, hot0, qt1, gt1, stats1, other);
+    step(s + 1 < mine.y, qt0, gt0, stats0, words0, qt1, gt1, stats1, words1);
     if (s + 1 < mine.y) {
       turn();
-      step(s + 2 < mine.y, qt1, gt1, stats1, other, qt0, gt0, stats0, hot0);
+      step(s + 2 < mine.y, qt1, gt1, stats1, words1, qt0, gt0, stats0, words0);
     }
   }
   if (!real) return;
@@ -746,12 +740,13 @@ int key_parts(const ctmr_masked_attention_desc* d) {
 
 template <typename T, int D, Cap CAP, int ST>
 int launch(Args a, const BiasOf<ST>& bias, int qparts, int kparts, hipStream_t st) {
-  const unsigned parts = a.qdoc.ids ? 2u : 1u;
+  const unsigned parts = a.qdoc.ids ? 2u : 1u, bytes = bias_bytes<T, D>(bias);
   bool table = false;
   if constexpr (ST > 0) table = bias.part != nullptr;
   a.splits = a.dq || table ? qparts : 1;
   const unsigned q_blocks = a.n * a.hq * (unsigned)ceil_div(a.lq, kOwn) * parts;
-  hipLaunchKernelGGL((attention_dq_kernel<T, D, CAP, ST>), dim3(q_blocks, a.splits), dim3(kThreads), 0, st, a, bias);
+  hipLaunchKernelGGL((attention_dq_kernel<T, D, CAP, ST>), dim3(q_blocks, a.splits), dim3(kThreads), bytes, st, a,
+                     bias);
   int rc = check_launch("attention_dq");
   if (rc) return rc;
   if (a.splits > 1 && a.dq) {
@@ -765,7 +760,12 @@ int launch(Args a, const BiasOf<ST>& bias, int qparts, int kparts, hipStream_t s
   if (!a.dk && !a.dv) return rc;
   a.splits = kparts;
   const unsigned k_blocks = a.n * a.hk * (unsigned)ceil_div(a.lk, kOwn) * parts;
-  hipLaunchKernelGGL((attention_dkv_kernel<T, D, CAP, ST>), dim3(k_blocks, a.splits), dim3(kThreads), 0, st, a, bias);
+  constexpr int kAny = ST > 0 ? kForwardBias : 0;
+  if constexpr (ST > 0)
+    hipLaunchKernelGGL((attention_dkv_kernel<T, D, CAP, kAny>), dim3(k_blocks, a.splits), dim3(kThreads), bytes, st, a,
+                       BiasOf<kAny>{bias});
+  else
+    hipLaunchKernelGGL((attention_dkv_kernel<T, D, CAP, 0>), dim3(k_blocks, a.splits), dim3(kThreads), 0, st, a, bias);
   rc = check_launch("attention_dkv");
   if (rc || a.splits == 1) return rc;
   SumArgs s = {a.part, {a.dk, a.dv}, {a.dkb, a.dvb}, {a.dkh, a.dvh}, {a.dkl, a.dvl}, {ds_scale<CAP>(a), 1.0f},

@@ -218,27 +218,21 @@ __device__ __forceinline__ void write_row(const Args& a, const f16v (&o)[ND], fl
     a.lse[((int64_t)b * a.hq + h) * a.lq + i] = l == 0.f ? INFINITY : m + log2f(l) - kLift<T>;
 }
 
+extern __shared__ __attribute__((aligned(16))) char bias_values[];  // of a position bias (lay_out_bias)
+
 // The tiled form: a workgroup of four waves takes 128 query rows of a head, 32 a
 // wave, and streams K and V through LDS in 64-key tiles: the next tile is loaded
 // straight into a second pair of arrays while the current one is multiplied.
-template <typename T, int D, int ST>
-constexpr int tiled_waves() {
-  if (ST > 0) return D == 128 || (ST > 4 && D * sizeof(T) > 64) || D * sizeof(T) > 128 ? 1 : 2;
-  return sizeof(T) == 4 && D == 128 ? 1 : 2;
-}
-
 template <typename T, int D, Cap CAP, int ST>
-__global__ __launch_bounds__(kThreads, (tiled_waves<T, D, ST>())) void attention_kernel(Args a, BiasOf<ST> bias) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void attention_kernel(Args a, BiasOf<ST> bias) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
-  typedef Stream<__bf16, BiasOf<ST>::kWidth, kTile, kThreads> LoadHot;
-  constexpr bool kOneHot = one_hot<T, D, ST>();
   __shared__ __attribute__((aligned(16))) char kt0[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) char vt0[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) char kt1[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) char vt1[kTile * Lds::kRow];
-  __shared__ __attribute__((aligned(16))) char hot0[kTile * LoadHot::Lds::kRow];
-  __shared__ __attribute__((aligned(16))) char hot1[kOneHot ? 16 : kTile * LoadHot::Lds::kRow];
+  __shared__ __attribute__((aligned(16))) unsigned words0[kTile];
+  __shared__ __attribute__((aligned(16))) unsigned words1[kTile];
   __shared__ unsigned odd[2];
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -279,36 +273,27 @@ __global__ __launch_bounds__(kThreads, (tiled_waves<T, D, ST>())) void attention
   Rows<T, kTile> krows, vrows;
   krows.begin(k, a.kl, first * kTile, a.lk, a.d);
   vrows.begin(v, a.vl, first * kTile, a.lk, a.d);
-  BiasRow<T, ST> bias_of_row;
-  Rows<__bf16, kTile> hot_rows;
+  unsigned word = 0u;
   if constexpr (ST > 0) {
-    const unsigned places = mine ? bias.query_places[b * bias.query_item + i] : 0u;
-    bias_row<T, ST, false>(bias, bias_of_row, places, h, a.hq, kLog2e / units_of<CAP>(scoring), lane);
-    constexpr int kWidth = BiasOf<ST>::kRow;
-    hot_rows.begin(bias.key_hot + b * bias.key_item * kWidth, kWidth, first * kTile, a.lk, kWidth);
+    word = row_word<kSingle<T, D>>(bias, b, i, a.lq);
+    lay_out_bias<kSingle<T, D>, kThreads>(bias, bias_values, h, a.hq, kLog2e / units_of<CAP>(scoring),
+                                          t);  // arrive() comes before its use
   }
   typedef Stream<T, D, kTile, kThreads> Load;
-  auto fetch_hot = [&](char* hot) {
-    LoadHot::load(hot, hot_rows, t);
-    hot_rows.next();
-  };
-  auto fetch = [&](char* kt, char* vt, char* hot) {
+  auto fetch = [&](int tile, char* kt, char* vt, unsigned* words) {
     Load::load(kt, krows, t);
     Load::load(vt, vrows, t);
-    if constexpr (ST > 0 && !kOneHot) fetch_hot(hot);
+    if constexpr (ST > 0)
+      if (wave == 0) load_words(words, (kSingle<T, D> ? bias.key_places : bias.key_codes) + b * bias.key_item, tile * kTile, a.lk, lane);
     krows.next();
     vrows.next();
   };
   // One tile, while the next one is on its way into the other pair of arrays.
-  auto step = [&](int tile, char* kt, char* vt, char* hot, char* next_kt, char* next_vt, char* next_hot) {
+  auto step = [&](int tile, char* kt, char* vt, unsigned* words, char* next_kt, char* next_vt, unsigned* next_words) {
     const int k0 = tile * kTile;
     const bool partial = meet.partial(tile);  // some row of the workgroup has a masked key in it
     arrive();
-    if constexpr (ST > 0 && kOneHot) {
-      fetch_hot(hot);
-      arrive();
-    }
-    if (tile + 1 < last) fetch(next_kt, next_vt, next_hot);
+    if (tile + 1 < last) fetch(tile + 1, next_kt, next_vt, next_words);
     if (partial) {
       if (t < 2) odd[t] = 0u;
       __syncthreads();
@@ -333,7 +318,7 @@ __global__ __launch_bounds__(kThreads, (tiled_waves<T, D, ST>())) void attention
     const float c = score_blocks<T, 2, CAP>(scoring, s, k0, pos, meet.masked(tile), mask, tile_ids, lane, [&](auto& s) {
       if constexpr (ST > 0)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) add_bias<T, ST>(s[u], bias_of_row, hot, 32 * u, at);
+        for (int u = 0; u < 2; ++u) add_bias<kSingle<T, D>, true>(s[u], bias_values, word, words + 32 * u, at);
     });
     float alpha;
     Frag<T> p[2][2];
@@ -364,11 +349,10 @@ __global__ __launch_bounds__(kThreads, (tiled_waves<T, D, ST>())) void attention
       if (lo | hi) add_odd_values<T, ND>(a, o, v, k0, lo, hi, mask, tile_ids, lane);
     }
   };
-  char* const other = kOneHot ? hot0 : hot1;
-  if (first < last) fetch(kt0, vt0, hot0);
+  if (first < last) fetch(first, kt0, vt0, words0);
   for (int tile = first; tile < last; tile += 2) {
-    step(tile, kt0, vt0, hot0, kt1, vt1, other);
-    if (tile + 1 < last) step(tile + 1, kt1, vt1, other, kt0, vt0, hot0);
+    step(tile, kt0, vt0, words0, kt1, vt1, words1);
+    if (tile + 1 < last) step(tile + 1, kt1, vt1, words1, kt0, vt0, words0);
   }
   l = half_sum(l);
   if (mine) write_row<T, ND>(a, o, m, l, b, h, i, blockIdx.y, lane);
@@ -393,8 +377,7 @@ __global__ __launch_bounds__(kThreads, ST == 0 && sizeof(T) == 4 && D == 64 ? 2 
     Args a, BiasOf<ST> bias) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
-  typedef Stream<__bf16, BiasOf<ST>::kWidth, kFewTile, 64> LoadHot;
-  __shared__ __attribute__((aligned(16))) char hots[kWaves][kFewTile * LoadHot::Lds::kRow];
+  __shared__ __attribute__((aligned(16))) unsigned words[kWaves][kFewTile];
   __shared__ __attribute__((aligned(16))) char lds[few_lds<T, D>()];
   __shared__ unsigned odd[kWaves];
   __shared__ float2 state[kWaves][32];
@@ -429,12 +412,20 @@ __global__ __launch_bounds__(kThreads, ST == 0 && sizeof(T) == 4 && D == 64 ? 2 
   for (int n = 0; n < ND; ++n) o[n] = f16v(0.f);
   float m = kNone, l = 0.f;
 
-  BiasRow<T, ST> bias_of_row;
-  if constexpr (ST > 0)
-    bias_row<T, ST, false>(bias, bias_of_row, bias.query_places[b * bias.query_item + i], h, a.hq,
-                           kLog2e / units_of<CAP>(scoring), lane);
+  // The heads of a group have values of their own, one behind the other.
+  unsigned word = 0u, key = 0u;
+  const char* values = bias_values;
+  if constexpr (ST > 0) {
+    word = row_word<kSingle<T, D>>(bias, b, i, a.lq);
+    const int bytes = kSingle<T, D> ? 4096 : 4 * bias.values;
+    values += (row / a.lq) * bytes;
+    for (int g = 0; g < a.group; ++g) {
+      lay_out_bias<kSingle<T, D>, kThreads>(bias, bias_values + g * bytes, hk * a.group + g, a.hq,
+                                            kLog2e / units_of<CAP>(scoring), t);
+      __syncthreads();
+    }
+  }
   Stream<T, D, kFewTile, 64> ks, vs;
-  LoadHot hot;
   Rows<T, kFewTile> krows, vrows;
   int k0 = first * kTile + wave * kFewTile;
   auto fetch = [&](int at) {
@@ -442,12 +433,8 @@ __global__ __launch_bounds__(kThreads, ST == 0 && sizeof(T) == 4 && D == 64 ? 2 
     vrows.begin(v, a.vl, at, a.lk, a.d);
     ks.fetch(krows, lane);
     vs.fetch(vrows, lane);
-    if constexpr (ST > 0) {
-      constexpr int kWidth = BiasOf<ST>::kRow;
-      Rows<__bf16, kFewTile> rows;
-      rows.begin(bias.key_hot + b * bias.key_item * kWidth, kWidth, at, a.lk, kWidth);
-      hot.fetch(rows, lane);
-    }
+    if constexpr (ST > 0)
+      if (lane < kFewTile) key = key_word<kSingle<T, D>>(bias, b, at + lane, a.lk);
   };
   if (k0 < end) fetch(k0);
   for (; k0 < end; k0 += kWaves * kFewTile) {
@@ -457,7 +444,8 @@ __global__ __launch_bounds__(kThreads, ST == 0 && sizeof(T) == 4 && D == 64 ? 2 
     ks.template store<false>(kt, nullptr, lane);
     if (partial) vs.template store<true>(vt, &odd[wave], lane);
     else vs.template store<false>(vt, nullptr, lane);
-    if constexpr (ST > 0) hot.template store<false>(hots[wave], nullptr, lane);
+    if constexpr (ST > 0)
+      if (lane < kFewTile) words[wave][lane] = key;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const int next = k0 + kWaves * kFewTile;
     if (next < end) fetch(next);
@@ -466,7 +454,7 @@ __global__ __launch_bounds__(kThreads, ST == 0 && sizeof(T) == 4 && D == 64 ? 2 
     for (int n = 0; n < NK; ++n) s[0] = mma<T>(Lds::along(kt, 0, n, lane), qf[n], s[0]);
     const float c = score_blocks<T, 1, CAP>(scoring, s, k0, pos, partial, mask, docs ? ids + k0 : nullptr, lane,
                                             [&](auto& s) {
-                                              if constexpr (ST > 0) add_bias<T, ST>(s[0], bias_of_row, hots[wave], 0, lane);
+                                              if constexpr (ST > 0) add_bias<kSingle<T, D>, true>(s[0], values, word, words[wave], lane);
                                             });
     float alpha;
     Frag<T> p[1][2];
@@ -631,17 +619,19 @@ int split_count(const ctmr_masked_attention_desc* d) {
 
 template <typename T, int D, Cap CAP, int ST>
 void launch_form(const Args& a, const BiasOf<ST>& bias, bool few, hipStream_t st) {
-  // With fp32 heads of 128 and the widest bias the few-row form's tiles do not fit LDS.
-  constexpr bool kFits = few_lds<T, D>() + kWaves * kFewTile * 2 * BiasOf<ST>::kWidth + 2048 <= 160 * 1024;
-  if constexpr (kFits) {
-    if (few) {
-      hipLaunchKernelGGL((attention_few_kernel<T, D, CAP, ST>), dim3(a.n * a.hk, a.splits), dim3(kThreads), 0, st, a, bias);
-      return;
-    }
+  const unsigned bytes = bias_bytes<T, D>(bias);
+  if constexpr (ST > 0) {
+    // In the few-row form each head of a group has its values in LDS; where they do not fit the tiled form takes the call.
+    constexpr unsigned kRoom = 160 * 1024 - 4096 - few_lds<T, D>();
+    few = few && bytes * a.group <= kRoom;
   }
-  hipLaunchKernelGGL((attention_kernel<T, D, CAP, ST>),
-                     dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kRows) * (a.qdoc.ids ? 2u : 1u), a.splits), dim3(kThreads), 0,
-                     st, a, bias);
+  if (few)
+    hipLaunchKernelGGL((attention_few_kernel<T, D, CAP, ST>), dim3(a.n * a.hk, a.splits), dim3(kThreads), bytes * a.group, st,
+                       a, bias);
+  else
+    hipLaunchKernelGGL((attention_kernel<T, D, CAP, ST>),
+                       dim3(a.n * a.hq * (unsigned)ceil_div(a.lq, kRows) * (a.qdoc.ids ? 2u : 1u), a.splits), dim3(kThreads),
+                       bytes, st, a, bias);
 }
 
 template <typename T, int D, int ST>

@@ -31,88 +31,115 @@ int check_plan(const ctmr_buckets_desc* b) {
   return CTMR_OK;
 }
 
+// The axes in two pairs, the pairing with the fewest values.
+struct Pairs {
+  int axis[kAxes], extent[kAxes];  // extent 1: no axis
+  int values[2];
+};
+Pairs pairs_of(const ctmr_buckets_desc* b) {
+  static const int kPairings[3][kAxes] = {{0, 1, 2, 3}, {0, 2, 1, 3}, {0, 3, 1, 2}};
+  Pairs best = {};
+  for (const auto& pairing : kPairings) {
+    Pairs p;
+    for (int i = 0; i < kAxes; ++i) {
+      p.axis[i] = pairing[i] < b->axes ? pairing[i] : -1;
+      p.extent[i] = p.axis[i] < 0 ? 1 : b->extents[p.axis[i]];
+    }
+    for (int i = 0; i < 2; ++i) p.values[i] = (2 * p.extent[2 * i] - 1) * (2 * p.extent[2 * i + 1] - 1);
+    if (!best.values[0] || p.values[0] + p.values[1] < best.values[0] + best.values[1]) best = p;
+  }
+  return best;
+}
+
 struct Parts {
-  int64_t rows, query_columns, key_columns, query_places, key_places, query_hot, key_hot, bytes;
+  int64_t rows, query_codes, key_codes, query_places, key_places, hot, bytes;
 };
 
-// Where a plan's parts start.  One-hot rows of equal sides are the same.
+int64_t room_of(int rows) { return round_up(rows, kTile); }
+
+// Where a plan's parts start.
 Parts parts_of(const ctmr_buckets_desc* b) {
   Parts p = {};
-  const int64_t width = bias_steps(b) * 32, q = (int64_t)b->query_items * b->lq, k = (int64_t)b->key_items * b->lk;
+  const int64_t q = b->query_items * room_of(b->lq), k = b->key_items * room_of(b->lk);
   auto take = [&](int64_t size) {
     const int64_t at = p.bytes;
     p.bytes += round_up(size, 256);
     return at;
   };
-  p.rows = take(kNumbers * 4);
-  p.query_columns = take(kColumns * 4);
-  p.key_columns = take(kColumns * 4);
+  p.rows = take(kDistances * 4);
+  p.query_codes = take(q * 4);
+  p.key_codes = take(k * 4);
   p.query_places = take(q * 4);
-  p.query_hot = take(q * width);
-  p.key_places = b->same ? p.query_places : take(k * 4);
-  p.key_hot = b->same ? p.query_hot : take(k * width);
+  p.key_places = take(k * 4);
+  p.hot = take((int64_t)b->key_items * b->lk * bias_steps(b) * 32);
   return p;
 }
 
 struct PlanArgs {
-  const int* positions[2];  // (items, rows, axes)
-  unsigned* places[2];
-  __bf16* hot[2];
-  int64_t rows[2];
+  const int* positions[2];  // of rows and keys: (items, rows, axes)
+  unsigned *codes[2], *places[2];
+  int64_t count[2];  // words of all items
+  int rows[2], room[2];
+  __bf16* hot;
   int* table;
-  int axes, extents[4], width;
+  int axes, extents[kAxes], width;
+  Pairs pairs;
   unsigned short of[kDistances];  // the table's row of each distance's number
+  int numbers;
 };
 
-// blockIdx.y: the side; a thread makes a row's place and its one-hot row in pieces of eight columns.  The first
-// workgroup also lays out the tables.
+// blockIdx.y: rows or keys; a thread makes the words of one of them, and a key's one-hot row.  The first workgroup also lays
+// out the table's rows.
 __global__ __launch_bounds__(256) void places_kernel(PlanArgs a) {
   const int side = blockIdx.y;
-  if (side == 0 && blockIdx.x == 0) {
-    for (int n = threadIdx.x; n < kNumbers; n += 256) a.table[n] = -1;
-    __syncthreads();
-    int number = 0, column = 0;
-    for (int x = 0; x < a.axes; ++x) {
-      const int extent = a.extents[x];
-      for (int n = threadIdx.x; n < 2 * extent - 1; n += 256) a.table[number + n] = a.of[number + n];
-      // from a query row at place 0 to column c's: its coordinate; from there to a key at place 0: less it
-      for (int c = threadIdx.x; c < extent; c += 256) {
-        a.table[kNumbers + column + c] = x << 16 | (number + extent - 1 + c);
-        a.table[kNumbers + kColumns + column + c] = x << 16 | (number + extent - 1 - c);
-      }
-      number += 2 * extent - 1;
-      column += extent;
-    }
-    // numbers that no distance has, whichever place is added or taken
-    for (int c = column + threadIdx.x; c < kColumns; c += 256) {
-      a.table[kNumbers + c] = kNumbers - 1;
-      a.table[kNumbers + kColumns + c] = kNumbers - kColumns;
-    }
-  }
-  const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (row >= a.rows[side]) return;
+  if (side == 0 && blockIdx.x == 0)
+    for (int n = threadIdx.x; n < kDistances; n += 256) a.table[n] = n < a.numbers ? a.of[n] : -1;
+  const int64_t word = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (word >= a.count[side]) return;
+  const int64_t item = word / a.room[side];
+  const int i = (int)(word - item * a.room[side]);
+  const bool real = i < a.rows[side];
   unsigned places = 0u;
-  int columns[4], start = 0;
+  int place[kAxes], columns[kAxes], start = 0;
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
+  for (int x = 0; x < kAxes; ++x) {
+    place[x] = 0;
     columns[x] = -1;
     if (x >= a.axes) continue;
-    const int place = max(0, min(a.positions[side][row * a.axes + x], a.extents[x] - 1));
-    places |= (unsigned)place << (8 * x);
-    columns[x] = start + place;
+    if (real) place[x] = max(0, min(a.positions[side][(item * a.rows[side] + i) * a.axes + x], a.extents[x] - 1));
+    places |= (unsigned)place[x] << (8 * x);
+    columns[x] = start + place[x];
     start += a.extents[x];
   }
-  a.places[side][row] = places;
+  // Bytes of a pair's value: a row's from its far end, so that no difference is negative; the second pair's are behind.
+  unsigned code = 0u;
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    unsigned at = 0u;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int n = 2 * p + e, axis = a.pairs.axis[n], extent = a.pairs.extent[n];
+      int x = 0;
+#pragma unroll
+      for (int y = 0; y < kAxes; ++y) x = axis == y ? place[y] : x;
+      at = at * (2 * extent - 1) + x + (side == 0 ? extent - 1 : 0);
+    }
+    if (p == 1 && side == 0) at += a.pairs.values[0];
+    code |= at * 4 << (16 * p);
+  }
+  a.codes[side][word] = code;
+  a.places[side][word] = places;
+  if (side == 0 || !real) return;
   for (int c = 0; c < a.width; c += 8) {
     Vec<unsigned short, 8> v;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       bool hot = false;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) hot |= columns[x] == c + e;
+      for (int x = 0; x < kAxes; ++x) hot |= columns[x] == c + e;
       v[e] = hot ? 0x3f80 : 0;  // 1 in bf16
     }
-    *reinterpret_cast<Vec<unsigned short, 8>*>(a.hot[side] + row * a.width + c) = v;
+    *reinterpret_cast<Vec<unsigned short, 8>*>(a.hot + (item * a.rows[1] + i) * a.width + c) = v;
   }
 }
 
@@ -135,20 +162,26 @@ Bias make_bias(const ctmr_masked_attention_desc* d, const ctmr_buckets_desc* b, 
   const char* base = static_cast<const char*>(plan);
   Bias r = {};
   r.rows = reinterpret_cast<const int*>(base + p.rows);
-  r.query_columns = reinterpret_cast<const int*>(base + p.query_columns);
-  r.key_columns = reinterpret_cast<const int*>(base + p.key_columns);
-  r.query_places = reinterpret_cast<const unsigned*>(base + p.query_places);
-  r.key_places = reinterpret_cast<const unsigned*>(base + p.key_places);
-  r.query_hot = reinterpret_cast<const __bf16*>(base + p.query_hot);
-  r.key_hot = reinterpret_cast<const __bf16*>(base + p.key_hot);
-  r.query_item = b->query_items > 1 ? b->lq : 0;
-  r.key_item = b->key_items > 1 ? b->lk : 0;
+  auto words = [&](int64_t at) { return reinterpret_cast<const unsigned*>(base + at); };
+  r.query_codes = words(p.query_codes), r.key_codes = words(p.key_codes);
+  r.query_places = words(p.query_places), r.key_places = words(p.key_places);
+  r.key_hot = reinterpret_cast<const __bf16*>(base + p.hot);
+  r.query_item = b->query_items > 1 ? room_of(b->lq) : 0;
+  r.key_item = b->key_items > 1 ? room_of(b->lk) : 0;
+  r.hot_item = b->key_items > 1 ? b->lk : 0;
   r.table = table, r.elem = b->table_elem, r.table_rows = b->table_rows, r.axes = b->axes;
   int column = 0, number = 0;
   for (int a = 0; a < b->axes; ++a) {
     r.extents[a] = b->extents[a], r.first_column[a] = column, r.first_number[a] = number;
+    r.reach |= (unsigned)(b->extents[a] - 1) << (8 * a);
     column += b->extents[a], number += 2 * b->extents[a] - 1;
   }
+  const Pairs pairs = pairs_of(b);
+  for (int i = 0; i < kAxes; ++i) {
+    r.pair_extents[i] = pairs.extent[i];
+    r.pair_number[i] = pairs.axis[i] < 0 ? -1 : r.first_number[pairs.axis[i]];
+  }
+  r.values = pairs.values[0] + pairs.values[1];
   return r;
 }
 
@@ -175,25 +208,26 @@ int ctmr_buckets(const ctmr_buckets_desc* b, const int32_t* query_places, const 
   if ((int64_t)plan_bytes < need || ((uintptr_t)plan & 15) != 0)
     return fail(CTMR_E_WORKSPACE, "plan of places too small or not on a 16-byte boundary");
   PlanArgs a = {};
-  int numbers = 0;
-  for (int x = 0; x < b->axes; ++x) numbers += 2 * b->extents[x] - 1;
-  for (int n = 0; n < numbers; ++n) {
+  for (int x = 0; x < b->axes; ++x) a.numbers += 2 * b->extents[x] - 1;
+  for (int n = 0; n < a.numbers; ++n) {
     if (rows[n] < 0 || rows[n] >= b->table_rows) return fail(CTMR_E_INVALID, "a row that the table does not have");
     a.of[n] = (unsigned short)rows[n];
   }
   const Parts p = parts_of(b);
   char* base = static_cast<char*>(plan);
-  a.positions[0] = query_places, a.positions[1] = key_places;
-  a.places[0] = reinterpret_cast<unsigned*>(base + p.query_places);
-  a.places[1] = reinterpret_cast<unsigned*>(base + p.key_places);
-  a.hot[0] = reinterpret_cast<__bf16*>(base + p.query_hot), a.hot[1] = reinterpret_cast<__bf16*>(base + p.key_hot);
-  a.rows[0] = (int64_t)b->query_items * b->lq, a.rows[1] = b->same ? 0 : (int64_t)b->key_items * b->lk;
+  auto words = [&](int64_t at) { return reinterpret_cast<unsigned*>(base + at); };
+  a.positions[0] = query_places, a.positions[1] = b->same ? query_places : key_places;
+  a.codes[0] = words(p.query_codes), a.codes[1] = words(p.key_codes);
+  a.places[0] = words(p.query_places), a.places[1] = words(p.key_places);
+  a.rows[0] = b->lq, a.rows[1] = b->lk;
+  a.room[0] = (int)room_of(b->lq), a.room[1] = (int)room_of(b->lk);
+  a.count[0] = (int64_t)b->query_items * a.room[0], a.count[1] = (int64_t)b->key_items * a.room[1];
+  a.hot = reinterpret_cast<__bf16*>(base + p.hot);
   a.table = reinterpret_cast<int*>(base + p.rows);
-  a.axes = b->axes, a.width = 16 * bias_steps(b);
-  std::copy(b->extents, b->extents + 4, a.extents);
-  static_assert(kNumbers * 4 % 256 == 0 && kColumns * 4 % 256 == 0, "the tables lie one behind the other");
-  hipLaunchKernelGGL(places_kernel, dim3((unsigned)ceil_div(std::max(a.rows[0], a.rows[1]), 256), b->same ? 1 : 2), dim3(256),
-                     0, (hipStream_t)stream, a);
+  a.axes = b->axes, a.width = 16 * bias_steps(b), a.pairs = pairs_of(b);
+  std::copy(b->extents, b->extents + kAxes, a.extents);
+  hipLaunchKernelGGL(places_kernel, dim3((unsigned)ceil_div(std::max(a.count[0], a.count[1]), 256), 2), dim3(256), 0,
+                     (hipStream_t)stream, a);
   return check_launch("places");
 }
 

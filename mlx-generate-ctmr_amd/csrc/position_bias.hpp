@@ -1,21 +1,27 @@
 // A learned bias of attention scores by the distance of a row and a key on each of
-// up to four axes, in matrix products.
+// up to four axes.
 //
 //   bias_ij = sum_a table[row_a(x_a(j) - x_a(i))][h]
 // where x_a is a token's place on axis a, 0 .. extent_a - 1, and row_a the table's row
-// for a distance (its bucket).  For a query row i that is a function of the key's place
-// on each axis, so with a column c = (a, x) for each place of each axis
-//   bias_ij = sum_c r_i[c] o_j[c],  r_i[a, x] = table[row_a(x - x_a(i))][h],  o_j[a, x] = (x_a(j) == x)
-// and likewise with the sides exchanged, r'_j[a, x] = table[row_a(x_a(j) - x)][h].  The
-// table's gradient is that of r_i, which is one product more over the scores' gradients,
-//   dr_i[c] = sum_j ds_ij o_j[c],
-// added up over the distances of each row of the table.
+// for a distance (its bucket).  A workgroup lays the head's values out in LDS, the axes
+// in two pairs: one value for each two distances of a pair, (2 e - 1) (2 e' - 1) of
+// them, summed, in the scores' units.  Tokens have codes, places times strides, whose
+// difference is the LDS address of both pairs' values: a score costs a subtraction, a
+// mask, a shift and two reads and additions, whatever the places and their order.
 //
-// The one-hot rows o are exact in bf16 and the same for all heads: they stream through
-// LDS beside the keys (or the query rows).  r has kParts bf16 parts, whose products with
-// o are exact, so the bias is r to 2^-17 (16-bit heads; their weights are rounded by
-// 2^-9 or 2^-12) or to all of fp32's bits (fp32 heads); ds likewise.  A wave keeps r as
-// the B operand.
+// The table's gradient is the sum of the scores' gradients ds of a head over all pairs of
+// a distance.  For a row i, ds_ij counts by the key's place on each axis, so with a
+// column c = (a, x) for each place of each axis and one-hot rows o_j[a, x] = (x_a(j) == x)
+//   dr_i[c] = sum_j ds_ij o_j[c]
+// is a matrix product, which the matrix units sum without an addition in memory; the
+// rows' dr are then added by distance.  o is exact in bf16 and the same for all heads: it
+// streams through LDS beside the keys.  ds goes in kParts bf16 parts, 2^-17 of it with
+// 16-bit heads and all of fp32's bits with fp32 heads.
+//
+// (The bias itself as a product too, of o_j and each row's r_i[c] = table[row_a(x - x_a(i))]
+// in parts, has no reads of single values, but r takes 24 to 64 registers and the product
+// as long as that of keys of as many values: 2 x 16 heads of 4096 rows on 16x16x16, bf16,
+// forward, heads of 64 KA us, of 128 KB; so KC and KD.)
 #pragma once
 
 #include "masked_attention.hpp"
@@ -23,92 +29,121 @@
 namespace ctmr {
 namespace attn {
 
-constexpr int kColumns = 128;   // at most, over all axes
-constexpr int kNumbers = 512;   // of distances: two for a column, and room past them for columns that no place has
-constexpr int kDistances = 256;  // numbers that a distance may have
+constexpr int kColumns = 128;    // at most, over all axes
+constexpr int kDistances = 256;  // numbers of distances: two for a place, and one to spare
+constexpr int kAxes = 4;
+constexpr int kMostValues = 8192;  // of both pairs: with 128 places on four axes 7938 at most
 
 // A plan of places (ctmr_buckets), and the table.
 struct Bias {
-  const int* rows;           // (kNumbers) the table's row of a distance's number, -1 for none
-  const int* query_columns;  // (kColumns) axis << 16 | the number of column c's distance from place 0
-  const int* key_columns;    // likewise to place 0
-  const unsigned *query_places, *key_places;  // (items, rows) a byte for each axis
-  const __bf16 *query_hot, *key_hot;          // (items, rows, 16 ST) o
-  int64_t query_item, key_item;               // rows from item to item (0: all have the same)
-  const void* table;         // (table_rows, hq)
+  const int* rows;                             // (kDistances) the table's row of a distance's number, -1 for none
+  const unsigned *query_codes, *key_codes;     // (items, rows up to a multiple of kTile), of the axes in pairs
+  const unsigned *query_places, *key_places;   // likewise: a byte for each axis
+  const __bf16* key_hot;                       // (items, lk, 16 ST) o
+  int64_t query_item, key_item, hot_item;      // from item to item in rows; 0: all have the same
+  const void* table;                           // (table_rows, hq)
   int elem, table_rows, axes;
-  int extents[4], first_column[4], first_number[4];  // of each axis
+  int extents[kAxes], first_column[kAxes], first_number[kAxes];  // of each axis
+  int pair_extents[kAxes], pair_number[kAxes];  // the axes in pairs, 0 and 1, 2 and 3; extent 1 and number -1: no axis
+  int values;      // of both pairs
+  unsigned reach;  // extent - 1 of each axis in its byte
   bool fine;    // forward, 16-bit heads: weights in two parts (see fine_weights)
   float* part;  // the gradient: (n, hq, slots, kDistances) sums over a block's rows, or null
   int slots;
 };
 
-// ST: contraction steps of 16 columns, 3, 4, 6 or 8; 0: no bias.
+// ST: contraction steps of 16 columns, 3, 4, 6 or 8, in the gradients' products; 0: no bias.
 template <int ST>
 struct BiasOf : Bias {
-  static constexpr int kSteps = ST, kBlocks = (ST + 1) / 2;  // 32-column blocks
-  static constexpr int kRow = 16 * ST;                       // columns of a row of o in memory
-  static constexpr int kWidth = ST <= 4 ? 64 : 128;          // and of a tile in LDS, zeros past them
+  static constexpr int kBlocks = (ST + 1) / 2;       // of 32 columns
+  static constexpr int kRow = 16 * ST;               // columns of a row of o in memory
+  static constexpr int kWidth = ST <= 4 ? 64 : 128;  // and of a tile in LDS, zeros past them
 };
 template <>
 struct BiasOf<0> {
-  static constexpr int kSteps = 1, kBlocks = 1, kRow = 32, kWidth = 32;  // of arrays that nothing uses
+  static constexpr int kBlocks = 1, kRow = 32, kWidth = 32;  // of arrays that nothing uses
 };
+constexpr int kForwardBias = 4;  // the forward call and dk and dv have no columns; any number does
 
 template <typename T>
 constexpr int kParts = sizeof(T) == 4 ? 3 : 2;
 
-// A lane's r of one row, in parts.
-template <typename T, int ST>
-struct BiasRow {
-  Frag<__bf16> part[BiasOf<ST>::kSteps][kParts<T>];
-};
+// With fp32 heads of 128 LDS has no room for pairs: the axes are looked up one by one, in tables of 256 values, by the
+// bytes of the difference of places.
+template <typename T, int D>
+constexpr bool kSingle = sizeof(T) == 4 && D == 128;
 
-// The table's value for a distance's number, in units of 1 / `unit`.  What is below -2^100 hides a pair: the score that it
-// makes is below kNone in log2 units (the host keeps c from 2^-20), and zero times it is zero.
-__device__ __forceinline__ float bias_value(const Bias& b, int number, int h, int hq, float unit) {
-  const int row = b.rows[number];
-  if (row < 0) return 0.f;
-  const float v = load_param(b.table, b.elem, (int64_t)row * hq + h);
-  return v < -0x1p100f ? -0x1p127f : v * unit;
+// What a row's word and a key's differ by says where their values are.  Every lane has one: past the end that of the last.
+template <bool SINGLE>
+__device__ __forceinline__ unsigned row_word(const Bias& b, int item, int i, int lq) {
+  const int64_t at = item * b.query_item + min(i, lq - 1);
+  return SINGLE ? b.query_places[at] + b.reach : b.query_codes[at];
+}
+template <bool SINGLE>
+__device__ __forceinline__ unsigned key_word(const Bias& b, int item, int j, int lk) {
+  const int64_t at = item * b.key_item + min(j, lk - 1);
+  return SINGLE ? b.key_places[at] : b.key_codes[at];
 }
 
-// r of a row at `places` for head h.  KEYS: of a key (r').
-template <typename T, int ST, bool KEYS>
-__device__ __forceinline__ void bias_row(const Bias& b, BiasRow<T, ST>& out, unsigned places, int h, int hq, float unit,
-                                         int lane) {
-  const int* columns = KEYS ? b.key_columns : b.query_columns;
+// Lays out head h's values in `values`, in units of 1 / `unit`, by all threads of the workgroup between its barriers.  A
+// value below -2^100 hides a pair: the score that it makes is below kNone in log2 units (the host keeps the units so), also
+// where several are summed.
+template <bool SINGLE, int THREADS>
+__device__ __forceinline__ void lay_out_bias(const Bias& b, char* values, int h, int hq, float unit, int t) {
+  __shared__ float of[kDistances];
+  for (int n = t; n < kDistances; n += THREADS) {
+    const int row = b.rows[n];
+    const float v = row < 0 ? 0.f : load_param(b.table, b.elem, (int64_t)row * hq + h);
+    of[n] = v < -0x1p100f ? -0x1p127f : v * unit;
+  }
+  __syncthreads();
+  float* out = reinterpret_cast<float*>(values);
+  // Words count from the key to the row, numbers from the row to the key.
+  if constexpr (SINGLE) {
 #pragma unroll
-  for (int n = 0; n < ST; ++n)
+    for (int a = 0; a < kAxes; ++a)
+      for (int i = t; i < 256; i += THREADS)
+        out[256 * a + i] = a < b.axes && i < 2 * b.extents[a] - 1 ? of[b.first_number[a] + 2 * b.extents[a] - 2 - i] : 0.f;
+  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = columns[16 * n + 8 * (lane >> 5) + e];
-      const int place = (places >> (8 * (c >> 16))) & 255, number = (c & 0xffff) + (KEYS ? place : -place);
-      float v = bias_value(b, number, h, hq, unit);
-#pragma unroll
-      for (int p = 0; p < kParts<T>; ++p) {
-        const __bf16 part = (__bf16)v;
-        out.part[n][p][e] = part;
-        v -= (float)part;
+    for (int p = 0; p < kAxes; p += 2) {
+      const int n0 = 2 * b.pair_extents[p] - 1, n1 = 2 * b.pair_extents[p + 1] - 1;
+      const int at0 = b.pair_number[p], at1 = b.pair_number[p + 1];
+      for (int i = t; i < n0 * n1; i += THREADS) {
+        const int x0 = i / n1, x1 = i - x0 * n1;
+        out[i] = (at0 < 0 ? 0.f : of[at0 + n0 - 1 - x0]) + (at1 < 0 ? 0.f : of[at1 + n1 - 1 - x1]);
       }
+      out += n0 * n1;
     }
-}
-
-// Adds the bias of 32 rows of one-hot values in LDS to raw scores.
-template <typename T, int ST>
-__device__ __forceinline__ void add_bias(f16v& s, const BiasRow<T, ST>& r, const char* hot, int row, int lane) {
-#pragma unroll
-  for (int n = 0; n < ST; ++n) {
-    const Frag<__bf16> o = Tile<__bf16, BiasOf<ST>::kWidth>::along(hot, row, n, lane);
-#pragma unroll
-    for (int p = 0; p < kParts<T>; ++p) s = mma<__bf16>(o, r.part[n][p], s);
   }
 }
 
-// Whether the one-hot rows of a bias have one array instead of two: where LDS holds no more.
+// The bias of a row and a key from the difference of their words.
+template <bool SINGLE>
+__device__ __forceinline__ float bias_of(const char* values, unsigned at) {
+  const auto value = [&](unsigned byte) { return *reinterpret_cast<const float*>(values + byte); };
+  if constexpr (SINGLE)
+    return (value((at & 255u) * 4) + value(1024 + (at >> 8 & 255u) * 4)) +
+           (value(2048 + (at >> 16 & 255u) * 4) + value(3072 + (at >> 24) * 4));
+  else
+    return value(at & 0xffffu) + value(at >> 16);
+}
+
+// Adds the bias to a lane's 16 scores, whose rows have `words` (32 of them, in LDS).  KEYS: the rows are keys.
+template <bool SINGLE, bool KEYS>
+__device__ __forceinline__ void add_bias(f16v& s, const char* values, unsigned own, const unsigned* words, int lane) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const u4 w = *reinterpret_cast<const u4*>(words + 8 * g + 4 * (lane >> 5));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[4 * g + r] += bias_of<SINGLE>(values, KEYS ? own - w[r] : w[r] - own);
+  }
+}
+
+// Whether the gradients' one-hot rows have one array instead of two: where LDS holds no more.
 template <typename T, int D, int ST>
 constexpr bool one_hot() {
-  return 4 * kTile * Tile<T, D>::kRow + 4 * kTile * BiasOf<ST>::kWidth + 2048 > 160 * 1024;
+  return 4 * kTile * Tile<T, D>::kRow + 4 * kTile * BiasOf<ST>::kWidth + kMostValues * 4 + 2048 > 160 * 1024;
 }
 
 int check_buckets(const ctmr_masked_attention_desc* d, const ctmr_buckets_desc* b);
@@ -124,6 +159,12 @@ template <>
 int run_biased_gradients<__bf16>(const Args&, const Bias&, int, int, int, hipStream_t);
 template <>
 int run_biased_gradients<_Float16>(const Args&, const Bias&, int, int, int, hipStream_t);
+
+// Bytes of the values in LDS, the kernels' dynamic part.
+template <typename T, int D>
+inline unsigned bias_bytes(const Bias& b) { return kSingle<T, D> ? 4096u : 4u * b.values; }
+template <typename T, int D>
+inline unsigned bias_bytes(const BiasOf<0>&) { return 0u; }
 
 }  // namespace attn
 }  // namespace ctmr

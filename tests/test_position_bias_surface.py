@@ -111,9 +111,10 @@ def _desc(L, lq=6, lk=6, qi=1, ki=1, same=1, axes=2, extents=(3, 4, 0, 0), rows=
 def test_host_checks(ctmr, native_loaded):
     L, lib, p = ctmr._lib, native_loaded, 4096
     space = lambda **kw: lib.ctmr_buckets_bytes(ctypes.byref(_desc(L, **kw)))
-    # tables 2048 + 2 x 512, six places 24 -> 256, six rows of 64 columns 768
-    assert space() == 3072 + 256 + 768 and space(same=0) == 3072 + 2 * (256 + 768)
-    assert space(extents=(60, 5, 0, 0)) == 3072 + 256 + 1536
+    # 256 rows of the table, four times 64 words, six one-hot rows of 48 columns (576 bytes) or 96, in pieces of 256 bytes
+    assert space() == 1024 + 4 * 256 + 768 and space(same=0) == space()
+    assert space(extents=(60, 5, 0, 0)) == 1024 + 4 * 256 + 1280 and space(lq=65, same=0) == space() + 2 * 256
+    assert space(same=0, ki=3) == 1024 + 2 * 256 + 2 * 768 + 1792
     assert lib.ctmr_buckets_bytes(None) == L.E_INVALID
     for kw in ({"lq": 0, "lk": 0}, {"qi": 0, "ki": 0}, {"axes": 0}, {"axes": 5}, {"extents": (3, 0, 0, 0)}, {"rows": 0},
                {"rows": 65537}, {"lk": 5}, {"qi": 2}, {"extents": (129, 1, 0, 0)}):
