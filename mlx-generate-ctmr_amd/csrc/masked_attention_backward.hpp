@@ -346,6 +346,8 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f16v s = f16v(0.f), ds = f16v(-delta);
+      if constexpr (ST > 0 && CAP == kNoCap)  // the products are added to the bias
+        apply_bias<kSingle<T, D>, true, false>(s, bias_values, word, words + 32 * u, la);
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
         s = mma<T>(Lds::along(kt, 32 * u, n, la), qf[n], s);
@@ -354,7 +356,8 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
       const int at = k0 + 32 * u + 4 * half;
       f16v db = ds;  // of the bias: before the cap's slope
       const float c = scores<T, CAP>(scoring, s, ds, at, pos, [&](f16v& s) {
-        if constexpr (ST > 0) add_bias<kSingle<T, D>, true>(s, bias_values, word, words + 32 * u, la);
+        if constexpr (ST > 0 && CAP != kNoCap)
+          apply_bias<kSingle<T, D>, true, true>(s, bias_values, word, words + 32 * u, la);
       });
       if constexpr (ST > 0 && CAP != kNoCap) {
 #pragma unroll
@@ -539,6 +542,8 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D, ST>())) void attention_d
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f16v s = f16v(0.f), ds;
+      if constexpr (ST > 0 && CAP == kNoCap)  // the products are added to the bias
+        apply_bias<kSingle<T, D>, false, false>(s, bias_values, word, words + 32 * u, la);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const f4 delta = *reinterpret_cast<const f4*>(stats + kTile + 32 * u + 8 * w + 4 * half);
@@ -587,7 +592,8 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D, ST>())) void attention_d
       }
       const int at = i0 + 32 * u + 4 * half;
       const float c = scores<T, CAP>(scoring, s, ds, at, j - off, [&](f16v& s) {
-        if constexpr (ST > 0) add_bias<kSingle<T, D>, false>(s, bias_values, word, words + 32 * u, la);
+        if constexpr (ST > 0 && CAP != kNoCap)
+          apply_bias<kSingle<T, D>, false, true>(s, bias_values, word, words + 32 * u, la);
       });
       const float raised = kHalf<T> ? __builtin_ldexpf(1.0f, (int)(raise - kRaise)) : 1.0f;  // p is raised already
 #pragma unroll

@@ -303,6 +303,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
     if (meet.skips(tile)) return;
     const int at = fresh<D == 128 && sizeof(T) == 4>(lane);
     f16v s[2] = {f16v(0.f), f16v(0.f)};
+    if constexpr (ST > 0)  // without a cap the products are added to the bias
+      if (scoring.cap == 0.f) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) apply_bias<kSingle<T, D>, true, false>(s[u], bias_values, word, words + 32 * u, at);
+      }
 #pragma unroll
     for (int n = 0; n < NK; ++n)
 #pragma unroll
@@ -317,8 +322,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
     const int* tile_ids = docs ? ids + k0 : nullptr;
     const float c = score_blocks<T, 2, CAP>(scoring, s, k0, pos, meet.masked(tile), mask, tile_ids, lane, [&](auto& s) {
       if constexpr (ST > 0)
+        if (scoring.cap > 0.f) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) add_bias<kSingle<T, D>, true>(s[u], bias_values, word, words + 32 * u, at);
+          for (int u = 0; u < 2; ++u) apply_bias<kSingle<T, D>, true, true>(s[u], bias_values, word, words + 32 * u, at);
+        }
     });
     float alpha;
     Frag<T> p[2][2];
@@ -454,7 +461,8 @@ __global__ __launch_bounds__(kThreads, ST == 0 && sizeof(T) == 4 && D == 64 ? 2 
     for (int n = 0; n < NK; ++n) s[0] = mma<T>(Lds::along(kt, 0, n, lane), qf[n], s[0]);
     const float c = score_blocks<T, 1, CAP>(scoring, s, k0, pos, partial, mask, docs ? ids + k0 : nullptr, lane,
                                             [&](auto& s) {
-                                              if constexpr (ST > 0) add_bias<kSingle<T, D>, true>(s[0], values, word, words[wave], lane);
+                                              if constexpr (ST > 0) apply_bias<kSingle<T, D>, true, true>(s[0], values, word,
+                                                                                             words[wave], lane);
                                             });
     float alpha;
     Frag<T> p[1][2];

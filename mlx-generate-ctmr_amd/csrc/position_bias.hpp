@@ -129,14 +129,18 @@ __device__ __forceinline__ float bias_of(const char* values, unsigned at) {
     return value(at & 0xffffu) + value(at >> 16);
 }
 
-// Adds the bias to a lane's 16 scores, whose rows have `words` (32 of them, in LDS).  KEYS: the rows are keys.
-template <bool SINGLE, bool KEYS>
-__device__ __forceinline__ void add_bias(f16v& s, const char* values, unsigned own, const unsigned* words, int lane) {
+// The bias of a lane's 16 scores, whose rows have `words` (32 of them, in LDS), or that added to the scores.  KEYS: the rows
+// are keys.
+template <bool SINGLE, bool KEYS, bool ADD>
+__device__ __forceinline__ void apply_bias(f16v& s, const char* values, unsigned own, const unsigned* words, int lane) {
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const u4 w = *reinterpret_cast<const u4*>(words + 8 * g + 4 * (lane >> 5));
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s[4 * g + r] += bias_of<SINGLE>(values, KEYS ? own - w[r] : w[r] - own);
+    for (int r = 0; r < 4; ++r) {
+      const float v = bias_of<SINGLE>(values, KEYS ? own - w[r] : w[r] - own);
+      s[4 * g + r] = ADD ? s[4 * g + r] + v : v;
+    }
   }
 }
 
