@@ -19,18 +19,23 @@ extern "C" int ctmr_biased_attention(const ctmr_masked_attention_desc* d, const 
   Args a = make_args(d, q, k, v, slopes, prefixes, plan);
   a.out = out, a.rest = rest, a.lse = lse, a.part = (float*)workspace, a.splits = split_count(d);
   a.ob = d->out_strides[0], a.oh = d->out_strides[1], a.ol = d->out_strides[2];
-  BiasOf<kForwardBias> bias{make_bias(d, buckets, bucket_plan, table)};
-  bias.fine = fine != 0;
+  const Bias bias = make_bias(d, buckets, bucket_plan, table);
   const bool few = few_rows(d);
   hipStream_t st = (hipStream_t)stream;
-#define CTMR_BIASED_TYPE(T)                           \
-  switch (padded(d->head_dim)) {                      \
-    case 32: return launch<T, 32>(a, bias, few, st);  \
-    case 64: return launch<T, 64>(a, bias, few, st);  \
-    default: return launch<T, 128>(a, bias, few, st); \
-  }
-  if (d->elem == CTMR_ELEM_F32) CTMR_BIASED_TYPE(float)
-  if (d->elem == CTMR_ELEM_BF16) CTMR_BIASED_TYPE(__bf16)
-  CTMR_BIASED_TYPE(_Float16)
-#undef CTMR_BIASED_TYPE
+  auto run = [&](auto type, auto width) {
+    typedef decltype(type) T;
+    constexpr int D = decltype(width)::value;
+    if constexpr (sizeof(T) == 2)
+      if (fine) return launch<T, D>(a, BiasOf<kFineBias>{bias}, few, st);
+    return launch<T, D>(a, BiasOf<kBias>{bias}, few, st);
+  };
+  auto of_type = [&](auto type) {
+    switch (padded(d->head_dim)) {
+      case 32: return run(type, std::integral_constant<int, 32>());
+      case 64: return run(type, std::integral_constant<int, 64>());
+      default: return run(type, std::integral_constant<int, 128>());
+    }
+  };
+  if (d->elem == CTMR_ELEM_F32) return of_type(0.0f);
+  return d->elem == CTMR_ELEM_BF16 ? of_type((__bf16)0.0f) : of_type((_Float16)0.0f);
 }

@@ -347,7 +347,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
     for (int u = 0; u < 2; ++u) {
       f16v s = f16v(0.f), ds = f16v(-delta);
       if constexpr (ST > 0 && CAP == kNoCap)  // the products are added to the bias
-        apply_bias<kSingle<T, D>, true, false>(s, bias_values, word, words + 32 * u, la);
+        apply_bias<kSingle<T, D>, true, false, kBiasRows<D>>(s, bias_values, word, words + 32 * u, la);
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
         s = mma<T>(Lds::along(kt, 32 * u, n, la), qf[n], s);
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
       f16v db = ds;  // of the bias: before the cap's slope
       const float c = scores<T, CAP>(scoring, s, ds, at, pos, [&](f16v& s) {
         if constexpr (ST > 0 && CAP != kNoCap)
-          apply_bias<kSingle<T, D>, true, true>(s, bias_values, word, words + 32 * u, la);
+          apply_bias<kSingle<T, D>, true, true, kBiasRows<D>>(s, bias_values, word, words + 32 * u, la);
       });
       if constexpr (ST > 0 && CAP != kNoCap) {
 #pragma unroll
@@ -543,7 +543,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D, ST>())) void attention_d
     for (int u = 0; u < 2; ++u) {
       f16v s = f16v(0.f), ds;
       if constexpr (ST > 0 && CAP == kNoCap)  // the products are added to the bias
-        apply_bias<kSingle<T, D>, false, false>(s, bias_values, word, words + 32 * u, la);
+        apply_bias<kSingle<T, D>, false, false, kBiasRows<D>>(s, bias_values, word, words + 32 * u, la);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const f4 delta = *reinterpret_cast<const f4*>(stats + kTile + 32 * u + 8 * w + 4 * half);
@@ -593,7 +593,7 @@ __global__ __launch_bounds__(kThreads, (dkv_waves<T, D, ST>())) void attention_d
       const int at = i0 + 32 * u + 4 * half;
       const float c = scores<T, CAP>(scoring, s, ds, at, j - off, [&](f16v& s) {
         if constexpr (ST > 0 && CAP != kNoCap)
-          apply_bias<kSingle<T, D>, false, true>(s, bias_values, word, words + 32 * u, la);
+          apply_bias<kSingle<T, D>, false, true, kBiasRows<D>>(s, bias_values, word, words + 32 * u, la);
       });
       const float raised = kHalf<T> ? __builtin_ldexpf(1.0f, (int)(raise - kRaise)) : 1.0f;  // p is raised already
 #pragma unroll
@@ -766,7 +766,7 @@ int launch(Args a, const BiasOf<ST>& bias, int qparts, int kparts, hipStream_t s
   if (!a.dk && !a.dv) return rc;
   a.splits = kparts;
   const unsigned k_blocks = a.n * a.hk * (unsigned)ceil_div(a.lk, kOwn) * parts;
-  constexpr int kAny = ST > 0 ? kForwardBias : 0;
+  constexpr int kAny = ST > 0 ? kBias : 0;
   if constexpr (ST > 0)
     hipLaunchKernelGGL((attention_dkv_kernel<T, D, CAP, kAny>), dim3(k_blocks, a.splits), dim3(kThreads), bytes, st, a,
                        BiasOf<kAny>{bias});

@@ -306,7 +306,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
     if constexpr (ST > 0)  // without a cap the products are added to the bias
       if (scoring.cap == 0.f) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) apply_bias<kSingle<T, D>, true, false>(s[u], bias_values, word, words + 32 * u, at);
+        for (int u = 0; u < 2; ++u) apply_bias<kSingle<T, D>, true, false, kBiasRows<D>>(s[u], bias_values, word, words + 32 * u, at);
       }
 #pragma unroll
     for (int n = 0; n < NK; ++n)
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
       if constexpr (ST > 0)
         if (scoring.cap > 0.f) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) apply_bias<kSingle<T, D>, true, true>(s[u], bias_values, word, words + 32 * u, at);
+          for (int u = 0; u < 2; ++u) apply_bias<kSingle<T, D>, true, true, kBiasRows<D>>(s[u], bias_values, word, words + 32 * u, at);
         }
     });
     float alpha;
@@ -333,24 +333,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void 
 #pragma unroll
       for (int n = 0; n < ND; ++n) o[n] *= alpha;
     }
-    auto products = [&](auto fine) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
+      for (int w = 0; w < 2; ++w)
 #pragma unroll
-          for (int n = 0; n < ND; ++n) {
-            const Frag<T> f = u == 0 && w < kEarly ? vf[w][n] : Lds::down(vt, 32 * u + 16 * w, n, at);
-            o[n] = mma<T>(f, p[u][w], o[n]);
-            if constexpr (fine) o[n] = mma<T>(f, fine_weights<T>(s[u], p[u][w], w), o[n]);
-          }
-    };
-    if constexpr (ST > 0 && sizeof(T) == 2) {
-      if (bias.fine) products(std::true_type());
-      else products(std::false_type());
-    } else {
-      products(std::false_type());
-    }
+        for (int n = 0; n < ND; ++n) {
+          const Frag<T> f = u == 0 && w < kEarly ? vf[w][n] : Lds::down(vt, 32 * u + 16 * w, n, at);
+          o[n] = mma<T>(f, p[u][w], o[n]);
+          if constexpr (ST == kFineBias) o[n] = mma<T>(f, fine_weights<T>(s[u], p[u][w], w), o[n]);
+        }
     if (partial) {
       const unsigned lo = odd[0], hi = odd[1];
       if (lo | hi) add_odd_values<T, ND>(a, o, v, k0, lo, hi, mask, tile_ids, lane);
@@ -461,7 +453,7 @@ __global__ __launch_bounds__(kThreads, ST == 0 && sizeof(T) == 4 && D == 64 ? 2 
     for (int n = 0; n < NK; ++n) s[0] = mma<T>(Lds::along(kt, 0, n, lane), qf[n], s[0]);
     const float c = score_blocks<T, 1, CAP>(scoring, s, k0, pos, partial, mask, docs ? ids + k0 : nullptr, lane,
                                             [&](auto& s) {
-                                              if constexpr (ST > 0) apply_bias<kSingle<T, D>, true, true>(s[0], values, word,
+                                              if constexpr (ST > 0) apply_bias<kSingle<T, D>, true, true, kBiasRows<D>>(s[0], values, word,
                                                                                              words[wave], lane);
                                             });
     float alpha;
@@ -476,8 +468,7 @@ __global__ __launch_bounds__(kThreads, ST == 0 && sizeof(T) == 4 && D == 64 ? 2 
       for (int n = 0; n < ND; ++n) {
         const Frag<T> f = Lds::down(vt, 16 * w, n, lane);
         o[n] = mma<T>(f, p[0][w], o[n]);
-        if constexpr (ST > 0 && sizeof(T) == 2)
-          if (bias.fine) o[n] = mma<T>(f, fine_weights<T>(s[0], p[0][w], w), o[n]);
+        if constexpr (ST == kFineBias) o[n] = mma<T>(f, fine_weights<T>(s[0], p[0][w], w), o[n]);
       }
     if (partial) {
       const unsigned set = odd[wave];

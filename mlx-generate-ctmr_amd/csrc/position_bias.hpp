@@ -47,7 +47,6 @@ struct Bias {
   int pair_extents[kAxes], pair_number[kAxes];  // the axes in pairs, 0 and 1, 2 and 3; extent 1 and number -1: no axis
   int values;      // of both pairs
   unsigned reach;  // extent - 1 of each axis in its byte
-  bool fine;    // forward, 16-bit heads: weights in two parts (see fine_weights)
   float* part;  // the gradient: (n, hq, slots, kDistances) sums over a block's rows, or null
   int slots;
 };
@@ -63,7 +62,8 @@ template <>
 struct BiasOf<0> {
   static constexpr int kBlocks = 1, kRow = 32, kWidth = 32;  // of arrays that nothing uses
 };
-constexpr int kForwardBias = 4;  // the forward call and dk and dv have no columns; any number does
+// In the forward call and in dk and dv, which have no columns: a bias, and one with fine weights (fine_weights).
+constexpr int kBias = 1, kFineBias = 2;
 
 template <typename T>
 constexpr int kParts = sizeof(T) == 4 ? 3 : 2;
@@ -118,29 +118,44 @@ __device__ __forceinline__ void lay_out_bias(const Bias& b, char* values, int h,
   }
 }
 
-// The bias of a row and a key from the difference of their words.
-template <bool SINGLE>
-__device__ __forceinline__ float bias_of(const char* values, unsigned at) {
-  const auto value = [&](unsigned byte) { return *reinterpret_cast<const float*>(values + byte); };
-  if constexpr (SINGLE)
-    return (value((at & 255u) * 4) + value(1024 + (at >> 8 & 255u) * 4)) +
-           (value(2048 + (at >> 16 & 255u) * 4) + value(3072 + (at >> 24) * 4));
-  else
-    return value(at & 0xffffu) + value(at >> 16);
-}
+template <int D>
+constexpr int kBiasRows = D == 128 ? 4 : 16;
 
 // The bias of a lane's 16 scores, whose rows have `words` (32 of them, in LDS), or that added to the scores.  KEYS: the rows
-// are keys.
-template <bool SINGLE, bool KEYS, bool ADD>
+// are keys.  Pairs: the lane's own two addresses less the halves of a word, two subtractions; ROWS rows' reads are on their
+// way at once.
+template <bool SINGLE, bool KEYS, bool ADD, int ROWS>
 __device__ __forceinline__ void apply_bias(f16v& s, const char* values, unsigned own, const unsigned* words, int lane) {
+  typedef __attribute__((address_space(3))) const char lds_char;
+  typedef __attribute__((address_space(3))) const float lds_float;
+  const unsigned base = (unsigned)(uintptr_t)(lds_char*)values;
+  const auto value = [](unsigned at) { return *(lds_float*)(uintptr_t)at; };
+  const unsigned own0 = KEYS ? base + (own & 0xffffu) : base - (own & 0xffffu);
+  const unsigned own1 = KEYS ? base + (own >> 16) : base - (own >> 16);
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const u4 w = *reinterpret_cast<const u4*>(words + 8 * g + 4 * (lane >> 5));
+  for (int g = 0; g < 16; g += ROWS) {
+    unsigned w[ROWS];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float v = bias_of<SINGLE>(values, KEYS ? own - w[r] : w[r] - own);
-      s[4 * g + r] = ADD ? s[4 * g + r] + v : v;
+    for (int r = 0; r < ROWS; r += 4) {
+      const u4 v = *reinterpret_cast<const u4*>(words + 2 * (g + r) + 4 * (lane >> 5));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[r + e] = v[e];
     }
+    float first[ROWS], second[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if constexpr (SINGLE) {
+        const unsigned at = KEYS ? own - w[r] : w[r] - own;
+        first[r] = value(base + (at & 255u) * 4) + value(base + 1024 + (at >> 8 & 255u) * 4);
+        second[r] = value(base + 2048 + (at >> 16 & 255u) * 4) + value(base + 3072 + (at >> 24) * 4);
+      } else {
+        first[r] = value(KEYS ? own0 - (w[r] & 0xffffu) : own0 + (w[r] & 0xffffu));
+        second[r] = value(KEYS ? own1 - (w[r] >> 16) : own1 + (w[r] >> 16));
+      }
+    }
+    if constexpr (!SINGLE && ROWS == 16) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) s[g + r] = (ADD ? s[g + r] + first[r] : first[r]) + second[r];
   }
 }
 
