@@ -25,11 +25,15 @@ __global__ __launch_bounds__(1024) void table_gradient_kernel(const float* part,
   __syncthreads();
   if (quarter == 0) sums[0][number] = (sums[0][number] + sums[1][number]) + (sums[2][number] + sums[3][number]);
   __syncthreads();
-  for (int row = threadIdx.x; row < table_rows; row += 1024) {
+  // Eight threads a row, a distance each in turn.
+  const int lane = threadIdx.x & 7;
+  for (int row = threadIdx.x >> 3; row < table_rows; row += 128) {
     double total = 0.0;
-    for (int n = 0; n < kDistances; ++n)
-      if (row_of[n] == row) total += sums[0][n];
-    store_param(out, elem, (int64_t)row * hq + h, (float)total);
+#pragma unroll 4
+    for (int n = lane; n < kDistances; n += 8) total += row_of[n] == row ? sums[0][n] : 0.0;
+#pragma unroll
+    for (int m = 4; m > 0; m >>= 1) total += __shfl_xor(total, m);
+    if (lane == 0) store_param(out, elem, (int64_t)row * hq + h, (float)total);
   }
 }
 

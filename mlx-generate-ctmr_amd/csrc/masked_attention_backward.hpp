@@ -144,7 +144,7 @@ __device__ __forceinline__ int2 split_steps(int count, int split, int splits) {
 
 // Adds to the gradient of r what a 32 x 32 block of scores' gradients gives, in parts as r's.
 template <typename T, int ST>
-__device__ __forceinline__ void add_row_gradient(f16v (&dr)[BiasOf<ST>::kBlocks], f16v ds, const char* hot, int row,
+__device__ __forceinline__ void add_row_gradient(f16v (&dr)[HotTile<ST>::kBlocks], f16v ds, const char* hot, int row,
                                                  int lane) {
 #pragma unroll
   for (int p = 0; p < kParts<T>; ++p) {
@@ -152,8 +152,8 @@ __device__ __forceinline__ void add_row_gradient(f16v (&dr)[BiasOf<ST>::kBlocks]
     for (int w = 0; w < 2; ++w) {
       const Frag<__bf16> f = result_frag<__bf16>(ds, w);
 #pragma unroll
-      for (int n = 0; n < BiasOf<ST>::kBlocks; ++n)
-        dr[n] = mma<__bf16>(Tile<__bf16, BiasOf<ST>::kWidth>::down(hot, row + 16 * w, n, lane), f, dr[n]);
+      for (int n = 0; n < HotTile<ST>::kBlocks; ++n)
+        dr[n] = mma<__bf16>(HotTile<ST>::down(hot, row + 16 * w, n, lane), f, dr[n]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) ds[8 * w + e] -= (float)f[e];
     }
@@ -163,9 +163,10 @@ __device__ __forceinline__ void add_row_gradient(f16v (&dr)[BiasOf<ST>::kBlocks]
 // A workgroup's gradients of r, added over its rows by distance: thread t's is distance t.  A wave's 32 rows at a time
 // go through LDS (32 rows of the columns, their pieces of four turned by the row).
 template <int ST>
-__device__ __forceinline__ void add_distances(const Bias& bias, const f16v (&dr)[BiasOf<ST>::kBlocks], unsigned places,
+__device__ __forceinline__ void add_distances(const Bias& bias, const f16v (&dr)[HotTile<ST>::kBlocks], unsigned places,
                                               bool real, float* lds, float* out, int t) {
-  constexpr int kWidth = BiasOf<ST>::kWidth, kTurn = kWidth / 4 - 1;
+  constexpr int kWidth = 32 * HotTile<ST>::kBlocks;
+  const auto turned = [](int piece, int row) { return piece ^ (row & (ST == 6 && piece >= 16 ? 7 : 15)); };
   __shared__ unsigned row_places[32];
   const int lane = t & 63, half = lane >> 5, wave = t >> 6, own = lane & 31;
   int axis = 0;  // of distance t; the last axis has the numbers that no distance has, too
@@ -177,12 +178,12 @@ __device__ __forceinline__ void add_distances(const Bias& bias, const f16v (&dr)
     if (wave == w) {
       if (half == 0) row_places[own] = places;
 #pragma unroll
-      for (int n = 0; n < BiasOf<ST>::kBlocks; ++n)
+      for (int n = 0; n < HotTile<ST>::kBlocks; ++n)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           f4 v = {0.f, 0.f, 0.f, 0.f};
           if (real) v = f4{dr[n][4 * q], dr[n][4 * q + 1], dr[n][4 * q + 2], dr[n][4 * q + 3]};
-          *reinterpret_cast<f4*>(lds + own * kWidth + 4 * ((8 * n + 2 * q + half) ^ (own & kTurn))) = v;
+          *reinterpret_cast<f4*>(lds + own * kWidth + 4 * turned(8 * n + 2 * q + half, own)) = v;
         }
     }
     __syncthreads();
@@ -190,7 +191,7 @@ __device__ __forceinline__ void add_distances(const Bias& bias, const f16v (&dr)
       const int x = (int)((row_places[i] >> (8 * axis)) & 255) + distance;
       if (x < 0 || x >= extent) continue;
       const int column = bias.first_column[axis] + x;
-      sum += lds[i * kWidth + 4 * ((column >> 2) ^ (i & kTurn)) + (column & 3)];
+      sum += lds[i * kWidth + 4 * turned(column >> 2, i) + (column & 3)];
     }
   }
   out[t] = sum;
@@ -201,7 +202,7 @@ __device__ __forceinline__ void add_distances(const Bias& bias, const f16v (&dr)
 // there 505.
 template <typename T, int D, int ST>
 constexpr int dq_waves() {
-  if (ST > 0) return ST > 4 || D * sizeof(T) >= 256 ? 1 : 2;
+  if (ST > 0) return D * sizeof(T) >= 256 ? 1 : 2;
   return D * sizeof(T) >= 512 ? 1 : D * sizeof(T) == 64 ? 4 : D * sizeof(T) == 128 ? 3 : 2;
 }
 
@@ -212,10 +213,9 @@ template <typename T, int D, Cap CAP, int ST>
 __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq_kernel(Args a, BiasOf<ST> bias) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
-  typedef Stream<__bf16, BiasOf<ST>::kWidth, kTile, kThreads> LoadHot;
   constexpr bool kOneHot = one_hot<T, D, ST>();
-  __shared__ __attribute__((aligned(16))) char hot0[kTile * LoadHot::Lds::kRow];
-  __shared__ __attribute__((aligned(16))) char hot1[kOneHot ? 16 : kTile * LoadHot::Lds::kRow];
+  __shared__ __attribute__((aligned(16))) char hot0[HotTile<ST>::kBytes];
+  __shared__ __attribute__((aligned(16))) char hot1[kOneHot ? 16 : HotTile<ST>::kBytes];
   __shared__ __attribute__((aligned(16))) unsigned words0[kTile];
   __shared__ __attribute__((aligned(16))) unsigned words1[kTile];
   __shared__ __attribute__((aligned(16))) char kt0[kTile * Lds::kRow];
@@ -286,14 +286,14 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
   for (int n = 0; n < ND; ++n) dq[n] = f16v(0.f);
   unsigned places = 0u;
   unsigned word = 0u;
-  f16v dr[BiasOf<ST>::kBlocks];  // of r
+  f16v dr[HotTile<ST>::kBlocks];  // of r
   if constexpr (ST > 0) {
     if (real) places = bias.query_places[b * bias.query_item + i];
     word = row_word<kSingle<T, D>>(bias, b, i, a.lq);
     lay_out_bias<kSingle<T, D>, kThreads>(bias, bias_values, h, a.hq, kLog2e / units_of<CAP>(scoring),
                                           t);  // arrive() comes before its use
 #pragma unroll
-    for (int n = 0; n < BiasOf<ST>::kBlocks; ++n) dr[n] = f16v(0.f);
+    for (int n = 0; n < HotTile<ST>::kBlocks; ++n) dr[n] = f16v(0.f);
   }
 
   const Meeting meet = meeting<kWaves>(wave, i0, a.lq, [&](int row) { return key_tiles(a, b, row, prefix, &part); });
@@ -302,21 +302,16 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
   Rows<T, kTile> krows, vrows;
   krows.begin(k, a.kl, first * kTile, a.lk, a.d);
   vrows.begin(v, a.vl, first * kTile, a.lk, a.d);
-  Rows<__bf16, kTile> hot_rows;
-  if constexpr (ST > 0) {
-    constexpr int kWidth = BiasOf<ST>::kRow;
-    hot_rows.begin(bias.key_hot + b * bias.hot_item * kWidth, kWidth, first * kTile, a.lk, kWidth);
-  }
   typedef Stream<T, D, kTile, kThreads> Load;
-  auto fetch_hot = [&](char* hot) {
-    LoadHot::load(hot, hot_rows, t);
-    hot_rows.next();
+  auto fetch_hot = [&](int tile, char* hot) {
+    if constexpr (ST > 0)
+      HotTile<ST>::template load<kThreads>(hot, bias.key_hot + b * bias.hot_item * HotTile<ST>::kRow, tile * kTile, a.lk, t);
   };
   auto fetch = [&](int tile, char* kt, char* vt, char* hot, unsigned* words) {
     Load::load(kt, krows, t);
     Load::load(vt, vrows, t);
     if constexpr (ST > 0) {
-      if (!kOneHot && table_part) fetch_hot(hot);
+      if (!kOneHot && table_part) fetch_hot(tile, hot);
       if (wave == 0) load_words(words, (kSingle<T, D> ? bias.key_places : bias.key_codes) + b * bias.key_item, tile * kTile, a.lk, lane);
     }
     krows.next();
@@ -330,7 +325,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
     arrive();
     if constexpr (ST > 0 && kOneHot)
       if (table_part) {
-        fetch_hot(hot);
+        fetch_hot(tile, hot);
         arrive();
       }
     if (tile + 1 < last) fetch(tile + 1, next_kt, next_vt, next_hot, next_words);
@@ -390,17 +385,9 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
           for (int r = 0; r < 16; ++r) ds[r] = 8 * (r >> 2) + (r & 3) >= limit - at ? 0.f : ds[r];
       };
       if (masked) hide_keys(ds);
-      if constexpr (ST > 0) {
-        if constexpr (CAP == kNoCap) {
-          db = ds;
-        } else if (masked) {
-          hide_keys(db);
-        }
-        if (table_part) {
-          if constexpr (kHalf<T>) db *= __builtin_ldexpf(1.0f, -(int)raise);
-          add_row_gradient<T, ST>(dr, db, hot, 32 * u, la);
-        }
-      }
+      const float raised = raise;  // of db
+      if constexpr (ST > 0 && CAP != kNoCap)
+        if (masked) hide_keys(db);
       if constexpr (kHalf<T>) keep_in_range<false, ND>(ds, dq, raise);
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
@@ -408,6 +395,12 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
 #pragma unroll
         for (int n = 0; n < ND; ++n) dq[n] = mma<T>(Lds::down(kt, 32 * u + 16 * w, n, la), f, dq[n]);
       }
+      if constexpr (ST > 0)
+        if (table_part) {
+          if constexpr (CAP == kNoCap) db = ds;
+          if constexpr (kHalf<T>) db *= __builtin_ldexpf(1.0f, -(int)(CAP == kNoCap ? raise : raised));
+          add_row_gradient<T, ST>(dr, db, hot, 32 * u, la);
+        }
     }
   };
   char* const other = kOneHot ? hot0 : hot1;
@@ -431,7 +424,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
 
 template <typename T, int D, int ST>
 constexpr int dkv_waves() {
-  if (ST > 0) return D * sizeof(T) >= 256 || (ST > 4 && D * sizeof(T) > 64) ? 1 : 2;
+  if (ST > 0) return D * sizeof(T) >= 256 ? 1 : D * sizeof(T) == 64 ? 4 : 2;
   return D * sizeof(T) >= 256 ? 1 : D * sizeof(T) == 64 ? 4 : 2;
 }
 

@@ -223,8 +223,14 @@ extern __shared__ __attribute__((aligned(16))) char bias_values[];  // of a posi
 // The tiled form: a workgroup of four waves takes 128 query rows of a head, 32 a
 // wave, and streams K and V through LDS in 64-key tiles: the next tile is loaded
 // straight into a second pair of arrays while the current one is multiplied.
+// Waves a SIMD that the registers are kept for.
+template <typename T, int D, int ST>
+constexpr int tiled_waves() {
+  return sizeof(T) == 4 && D == 128 ? 1 : ST == kBias && D * sizeof(T) == 64 ? 4 : 2;
+}
+
 template <typename T, int D, Cap CAP, int ST>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 ? 1 : 2) void attention_kernel(Args a, BiasOf<ST> bias) {
+__global__ __launch_bounds__(kThreads, (tiled_waves<T, D, ST>())) void attention_kernel(Args a, BiasOf<ST> bias) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
   __shared__ __attribute__((aligned(16))) char kt0[kTile * Lds::kRow];

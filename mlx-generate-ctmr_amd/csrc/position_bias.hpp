@@ -51,16 +51,36 @@ struct Bias {
   int slots;
 };
 
-// ST: contraction steps of 16 columns, 3, 4, 6 or 8, in the gradients' products; 0: no bias.
+// ST: contraction steps of 16 columns, 3, 4, 6 or 8, in the table's gradient; 0: no bias.
 template <int ST>
-struct BiasOf : Bias {
-  static constexpr int kBlocks = (ST + 1) / 2;       // of 32 columns
-  static constexpr int kRow = 16 * ST;               // columns of a row of o in memory
-  static constexpr int kWidth = ST <= 4 ? 64 : 128;  // and of a tile in LDS, zeros past them
-};
+struct BiasOf : Bias {};
 template <>
-struct BiasOf<0> {
-  static constexpr int kBlocks = 1, kRow = 32, kWidth = 32;  // of arrays that nothing uses
+struct BiasOf<0> {};
+
+// A tile of one-hot rows in LDS: 64 columns, and 32 or 64 more behind them; zeros past 16 ST.
+template <int ST>
+struct HotTile {
+  static constexpr int kBlocks = ST == 6 ? 3 : ST == 8 ? 4 : 2;  // of 32 columns
+  static constexpr int kRow = 16 * ST;                           // columns of a row in memory
+  static constexpr int kFirst = kTile * 128, kBytes = kTile * 64 * kBlocks;
+  typedef Tile<__bf16, 64> First;
+  typedef Tile<__bf16, ST == 6 ? 32 : 64> Second;
+
+  // A operand whose rows are the columns 32 block .. + 31 (Tile::down).
+  static __device__ __forceinline__ Frag<__bf16> down(const char* tile, int row, int block, int lane) {
+    return block < 2 ? First::down(tile, row, block, lane) : Second::down(tile + kFirst, row, block - 2, lane);
+  }
+  // Rows from `first` of `count` straight into LDS.
+  template <int THREADS>
+  static __device__ __forceinline__ void load(char* tile, const __bf16* rows, int first, int count, int t) {
+    Rows<__bf16, kTile> r;
+    r.begin(rows, kRow, first, count, kRow < 64 ? kRow : 64);
+    Stream<__bf16, 64, kTile, THREADS>::load(tile, r, t);
+    if constexpr (ST > 4) {
+      r.begin(rows + 64, kRow, first, count, kRow - 64);
+      Stream<__bf16, ST == 6 ? 32 : 64, kTile, THREADS>::load(tile + kFirst, r, t);
+    }
+  }
 };
 // In the forward call and in dk and dv, which have no columns: a bias, and one with fine weights (fine_weights).
 constexpr int kBias = 1, kFineBias = 2;
@@ -162,7 +182,7 @@ __device__ __forceinline__ void apply_bias(f16v& s, const char* values, unsigned
 // Whether the gradients' one-hot rows have one array instead of two: where LDS holds no more.
 template <typename T, int D, int ST>
 constexpr bool one_hot() {
-  return 4 * kTile * Tile<T, D>::kRow + 4 * kTile * BiasOf<ST>::kWidth + kMostValues * 4 + 2048 > 160 * 1024;
+  return 4 * kTile * Tile<T, D>::kRow + 2 * HotTile<ST>::kBytes + kMostValues * 4 + 2048 > 160 * 1024;
 }
 
 int check_buckets(const ctmr_masked_attention_desc* d, const ctmr_buckets_desc* b);
