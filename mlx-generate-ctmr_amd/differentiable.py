@@ -621,7 +621,7 @@ def self_attention_tokens(tokens: Tensor, weights: Mapping[str, Tensor], *, head
 # ---------------------------------------------------------------------------
 # lists of gradients and parameters
 # ---------------------------------------------------------------------------
-_kind, _layout, _device, _bytes = (operator.attrgetter(name) for name in ("dtype", "layout", "device", "nbytes"))
+_shape, _kind, _device, _bytes = (operator.attrgetter(name) for name in ("shape", "dtype", "device", "nbytes"))
 
 
 def _without_gaps(t: Tensor) -> bool:
@@ -636,35 +636,46 @@ def _without_gaps(t: Tensor) -> bool:
     return True
 
 
-def _listed(tensors, name: str) -> list[Tensor]:
-    """The tensors of a list, ``None`` left out, checked for type and device."""
+def _listed(tensors, name: str) -> tuple[list[Tensor], bool]:
+    """The tensors of a list, ``None`` left out, checked for type and device, and whether all are contiguous."""
     if isinstance(tensors, Tensor):
         raise ValueError(f"{name} must be a list of tensors")
     out = [t for t in tensors if t is not None]
     if not out:
         raise ValueError(f"{name} holds no tensor")
-    # the list as a whole (see ops._list_sizes); what is wrong is looked for only where something is
-    if not (all(map(isinstance, out, itertools.repeat(Tensor))) and set(map(_layout, out)) == {torch.strided}):
+    # the list as a whole, a getter at a time (see ops._list_sizes)
+    if not all(issubclass(kind, Tensor) for kind in set(map(type, out))):
         raise ValueError(f"{name} must be dense tensors")
     for kind in set(map(_kind, out)):
         if kind not in ops.ELEMENTS:
             raise ValueError(f"{name} must be float32, bfloat16 or float16; got {kind}")
-    devices = set(map(_device, out))
-    if len(devices) != 1:
-        raise ValueError(f"{name} are on {' and '.join(sorted(map(str, devices)))}")
+    numbers = set(map(Tensor.get_device, out))
+    if len(numbers) != 1 or -1 in numbers:
+        devices = set(map(_device, out))
+        if len(devices) != 1:
+            raise ValueError(f"{name} are on {' and '.join(sorted(map(str, devices)))}")
+    try:
+        contiguous = all(map(Tensor.is_contiguous, out))
+    except RuntimeError:  # a layout that has no strides
+        contiguous = False
+    if not contiguous and any(t.layout != torch.strided for t in out):
+        raise ValueError(f"{name} must be dense tensors")
     _no_tangents(*out)
     _on_gpu(out[0], name)
-    return out
+    return out, contiguous
 
 
-def _apart(tensors: Sequence[Tensor], name: str) -> None:
+def _apart(tensors: Sequence[Tensor], name: str, contiguous: bool) -> None:
     """Refuses tensors that are written and have gaps or share memory."""
-    if not (all(map(Tensor.is_contiguous, tensors)) or all(map(_without_gaps, tensors))):
+    if not (contiguous or all(map(_without_gaps, tensors))):
         raise ValueError(f"{name} must fill their memory without gaps or overlaps")
     if torch.compiler.is_compiling() or not ops.PLAIN.issuperset(map(type, tensors)):
         return  # what is traced has no address
-    spans = sorted([span for span in zip(map(Tensor.data_ptr, tensors), map(_bytes, tensors)) if span[1]])
-    if any(at + size > after for (at, size), (after, _) in itertools.pairwise(spans)):
+    starts = list(map(Tensor.data_ptr, tensors))
+    ends = sorted(map(operator.add, starts, map(_bytes, tensors)))
+    starts.sort()
+    # apart if each end, in order, is before the next start; tensors of no values start and end at address zero
+    if any(map(operator.gt, ends, starts[1:])):
         raise ValueError(f"{name} share memory")
 
 
@@ -685,8 +696,8 @@ def gradient_norm(gradients: Sequence[Optional[Tensor]]) -> Tensor:
     Raises:
         ValueError: on an empty list, other types, or tensors that are not on one GPU.
         NotImplementedError: on forward-mode (dual) tensors."""
-    gradients = _listed(gradients, "gradients")
-    if not all(map(Tensor.is_contiguous, gradients)):
+    gradients, contiguous = _listed(gradients, "gradients")
+    if not contiguous:
         gradients = [t if _without_gaps(t) else t.contiguous() for t in gradients]
     return ops.gradient_norm(gradients)[0]
 
@@ -702,15 +713,16 @@ def clip_gradients(gradients: Sequence[Optional[Tensor]], max_norm: float) -> Te
         ValueError: on what ``gradient_norm`` refuses, tensors that share memory or have gaps in it (expanded or sliced
             ones), and a ``max_norm`` that is not positive.
         NotImplementedError: on forward-mode (dual) tensors."""
-    max_norm, gradients = _most(max_norm), _listed(gradients, "gradients")
-    _apart(gradients, "gradients")
+    max_norm, (gradients, contiguous) = _most(max_norm), _listed(gradients, "gradients")
+    _apart(gradients, "gradients", contiguous)
     norm = ops.clip_gradients(gradients, max_norm)
     torch.autograd.graph.increment_version(gradients)
     return norm[0]
 
 
-def _layout_of(t: Tensor) -> tuple:
-    return t.shape, t.stride(), t.dtype, t.device
+def _layouts_of(tensors: Sequence[Tensor]) -> tuple[list, ...]:
+    """Shapes, strides, types and devices."""
+    return tuple(list(map(get, tensors)) for get in (_shape, Tensor.stride, _kind, Tensor.get_device))
 
 
 class AdamW:
@@ -740,8 +752,8 @@ class AdamW:
         parameters = parameters if isinstance(parameters, Tensor) else list(parameters)
         if not isinstance(parameters, Tensor) and any(p is None for p in parameters):
             raise ValueError("parameters must be dense tensors")
-        self.parameters = _listed(parameters, "parameters")
-        _apart(self.parameters, "parameters")
+        self.parameters, contiguous = _listed(parameters, "parameters")
+        _apart(self.parameters, "parameters", contiguous)
         device = self.parameters[0].device
         self.lr = self._rate(lr)
         self.betas, self.eps, self.weight_decay = (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
@@ -752,7 +764,7 @@ class AdamW:
                 raise ValueError(f"{name} must be finite and not negative; got {value}")
         self.max_norm = math.inf if max_norm is None else _most(max_norm)
         self.skip_non_finite = bool(skip_non_finite)
-        self._layouts = list(map(_layout_of, self.parameters))
+        self._layouts = _layouts_of(self.parameters)
         self._starts, total = self._places(self.parameters)
         half = [p for p in self.parameters if p.dtype != torch.float32]
         starts, room = self._places(half)
@@ -828,17 +840,18 @@ class AdamW:
         lr, scale = self.lr if lr is None else self._rate(lr), float(gradient_scale)
         if not math.isfinite(scale):
             raise ValueError(f"gradient_scale must be finite; got {scale}")
-        taken = _listed(gradients, "gradients")
+        taken, _ = _listed(gradients, "gradients")
         parameters, layouts, starts, masters = self.parameters, self._layouts, self._starts, self._master_starts
         numbers = range(len(gradients))
         if len(taken) != len(parameters):
             used = [g is not None for g in gradients]
-            parameters, layouts, starts, masters, numbers = (
-                list(itertools.compress(v, used)) for v in (parameters, layouts, starts, masters, numbers))
-        if list(map(_layout_of, parameters)) != layouts:
-            i = next(i for i, p, want in zip(numbers, parameters, layouts) if _layout_of(p) != want)
-            raise ValueError(f"parameter {i} has become another than it was: {_layout_of(self.parameters[i])}")
-        if list(map(_layout_of, taken)) != layouts:
+            of = lambda values: list(itertools.compress(values, used))
+            parameters, starts, masters, numbers = map(of, (parameters, starts, masters, numbers))
+            layouts = tuple(map(of, layouts))
+        if _layouts_of(parameters) != layouts:
+            i = next(i for i, *pair in zip(numbers, zip(*_layouts_of(parameters)), zip(*layouts)) if pair[0] != pair[1])
+            raise ValueError(f"parameter {i} has become another than it was: {tuple(self.parameters[i].shape)}")
+        if _layouts_of(taken) != layouts:
             for at, (i, g, p) in enumerate(zip(numbers, taken, parameters)):
                 if g.shape != p.shape or g.dtype != p.dtype or g.device != p.device:
                     raise ValueError(f"gradient {i} is {tuple(g.shape)} {g.dtype} on {g.device}; its parameter "

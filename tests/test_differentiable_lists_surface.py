@@ -18,7 +18,8 @@ def _calls(f):
     ("tensors", "message"),
     [([], "no tensor"), ([None], "no tensor|dense"), (torch.zeros(3), "list of tensors"), ([1.0], "dense"),
      ([torch.zeros(3, dtype=torch.float64)], "float32, bfloat16"), ([torch.zeros(3, dtype=torch.int32)], "float32"),
-     ([torch.zeros(3).to_sparse()], "dense"), ([torch.zeros(3)], "on the GPU"),
+     ([torch.zeros(3).to_sparse()], "dense"),
+     ([torch.eye(3).to_sparse_csr()], "dense"), ([torch.zeros(3)], "on the GPU"),
      ([torch.zeros(3), torch.zeros(3, device="meta")], "cpu and meta")])
 def test_lists_are_refused(ctmr, name, tensors, message):
     with pytest.raises(ValueError, match=message):
@@ -52,7 +53,8 @@ def test_shared_memory_and_gaps_are_refused(on_cpu):
         for call in (lambda t: on_cpu.clip_gradients(t, 1.0), on_cpu.AdamW):
             with pytest.raises(ValueError, match="share memory|without gaps"):
                 call(tensors)
-    on_cpu._apart([flat[:32], flat[32:], torch.zeros(4, 3, 2).permute(2, 0, 1), torch.zeros(0)], "gradients")
+    on_cpu._apart([flat[:32], flat[32:], torch.zeros(4, 3, 2).permute(2, 0, 1), torch.zeros(0), flat[5:5]], "gradients",
+                  False)
 
 
 @pytest.mark.parametrize("value", [0.0, -1.0, math.nan])
