@@ -581,6 +581,9 @@ int ctmr_gradient_norm(int32_t count, const void* const* gradients, const int64_
 /* Each value times factor[0] (device memory), rounded to its type.  Tensors may not overlap. */
 int ctmr_scale_tensors(int32_t count, void* const* tensors, const int64_t* sizes, const int32_t* elems,
                        const float* factor, void* stream);
+/* Both at once: values times factor, norm_factor as ctmr_gradient_norm leaves it (scale 1). */
+int ctmr_clip_gradients(int32_t count, void* const* gradients, const int64_t* sizes, const int32_t* elems, float most,
+                        float* norm_factor, void* workspace, size_t workspace_bytes, void* stream);
 /* One AdamW step t of parameters of the gradients' sizes and types, g = gradient times
  * the factor that ctmr_gradient_norm gives for scale and most:
  *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2

@@ -153,6 +153,7 @@ _PROTOTYPES = {
     "ctmr_gradients_workspace_bytes": (_c_i64, [_c_i32, _vp]),
     "ctmr_gradient_norm": (_c_int, [_c_i32, _vp, _vp, _vp, _f, _f, _vp, _vp, _sz, _vp]),
     "ctmr_scale_tensors": (_c_int, [_c_i32, _vp, _vp, _vp, _vp, _vp]),
+    "ctmr_clip_gradients": (_c_int, [_c_i32, _vp, _vp, _vp, _f, _vp, _vp, _sz, _vp]),
     "ctmr_adamw": (_c_int, [ctypes.POINTER(AdamwDesc), _c_i32] + [_vp] * 13 + [_sz, _vp]),
 }
 

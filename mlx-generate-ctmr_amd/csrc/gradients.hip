@@ -76,17 +76,24 @@ __device__ __forceinline__ double block_sum(double v) {
 
 template <typename T>
 __device__ __forceinline__ double square_sum(const T* p, int64_t count) {
-  constexpr int kWide = 16 / sizeof(T);
-  const int64_t wide = count / kWide;
+  constexpr int kWide = 16 / sizeof(T), kAhead = 4;  // loads on their way at once
+  const int64_t wide = count / kWide, rounds = wide / (kAhead * kThreads) * kAhead * kThreads;
   double sum = 0.0;
-  for (int64_t i = threadIdx.x; i < wide; i += kThreads) {
-    const Wide<T> v = reinterpret_cast<const Wide<T>*>(p)[i];
+  auto add = [&](const Wide<T>& v) {
 #pragma unroll
     for (int e = 0; e < kWide; ++e) {
       const double x = (double)(float)v[e];
       sum = fma(x, x, sum);
     }
+  };
+  for (int64_t i = threadIdx.x; i < rounds; i += kAhead * kThreads) {
+    Wide<T> v[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) v[a] = reinterpret_cast<const Wide<T>*>(p)[i + a * kThreads];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) add(v[a]);
   }
+  for (int64_t i = rounds + threadIdx.x; i < wide; i += kThreads) add(reinterpret_cast<const Wide<T>*>(p)[i]);
   for (int64_t i = wide * kWide + threadIdx.x; i < count; i += kThreads) {
     const double x = (double)(float)p[i];
     sum = fma(x, x, sum);
@@ -162,10 +169,27 @@ __device__ __forceinline__ void scale_values(T* p, int64_t count, float factor) 
   for (int64_t i = wide * kWide + threadIdx.x; i < count; i += kThreads) p[i] = (T)((float)p[i] * factor);
 }
 
-__global__ __launch_bounds__(kThreads) void scale_kernel(List list, const float* factor) {
+// With sums (`count` of them, a thread each at most) a workgroup makes the factor itself, and the first one leaves norm
+// and factor in `out`: a launch less where the launches are what a call takes.
+struct Sums {
+  const double* sums;
+  int count;
+  float most;
+  float* out;
+};
+
+__global__ __launch_bounds__(kThreads) void scale_kernel(List list, const float* factor, Sums sums) {
   const Entry& e = list.entry[entry_of(list, blockIdx.x)];
   const int64_t at = (blockIdx.x - e.first) * list.chunk, count = min(list.chunk, e.count - at);
-  const float f = factor[0];
+  float f;
+  if (sums.sums) {
+    const double sum = block_sum<kThreads / 64>((int)threadIdx.x < sums.count ? sums.sums[threadIdx.x] : 0.0);
+    const float norm = (float)sqrt(sum);
+    f = clip_factor(norm, 1.0f, sums.most);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && sums.out) sums.out[0] = norm, sums.out[1] = f;
+  } else {
+    f = factor[0];
+  }
   if (f == 1.0f) return;  // nothing would change
   if (e.elem == CTMR_ELEM_F32) scale_values(static_cast<float*>(e.data) + at, count, f);
   else if (e.elem == CTMR_ELEM_BF16) scale_values(static_cast<__bf16*>(e.data) + at, count, f);
@@ -322,7 +346,7 @@ int check_workspace(const void* ws, size_t bytes, int64_t need) {
 }
 
 constexpr int64_t kControlBytes = 64;
-static_assert(sizeof(Control) <= kControlBytes && sizeof(List) <= 4080 && sizeof(StepList) <= 4096, "argument sizes");
+static_assert(sizeof(Control) <= kControlBytes && sizeof(List) + sizeof(Sums) + 16 <= 4096 && sizeof(StepList) <= 4096, "argument sizes");
 
 }  // namespace
 }  // namespace ctmr
@@ -363,8 +387,37 @@ int ctmr_scale_tensors(int32_t count, void* const* tensors, const int64_t* sizes
   if (rc) return rc;
   if (!factor) return fail(CTMR_E_INVALID, "null pointer");
   return for_lists(count, tensors, sizes, elems, kChunk, [&](const List& list, int chunks) {
-    hipLaunchKernelGGL(scale_kernel, dim3(chunks), dim3(kThreads), 0, (hipStream_t)stream, list, factor);
+    hipLaunchKernelGGL(scale_kernel, dim3(chunks), dim3(kThreads), 0, (hipStream_t)stream, list, factor, Sums{});
     return check_launch("scale_tensors");
+  });
+}
+
+int ctmr_clip_gradients(int32_t count, void* const* gradients, const int64_t* sizes, const int32_t* elems, float most,
+                        float* norm_factor, void* workspace, size_t workspace_bytes, void* stream) {
+  const int64_t need = ctmr_gradients_workspace_bytes(count, sizes);
+  if (need < 0) return (int)need;
+  // Up to as many sums as a workgroup has threads: 10 tensors of 64 channels, bf16, 26 us for 30; with more of them each
+  // workgroup would add too many.
+  const int64_t chunks = chunks_of(count, sizes, sum_chunk(total_of(count, sizes)));
+  if (chunks == 0 || chunks > kThreads) {
+    const int rc = ctmr_gradient_norm(count, gradients, sizes, elems, 1.0f, most, norm_factor, workspace, workspace_bytes,
+                                      stream);
+    return rc ? rc : ctmr_scale_tensors(count, gradients, sizes, elems, norm_factor + 1, stream);
+  }
+  int rc = check_list(count, gradients, sizes, elems);
+  if (rc) return rc;
+  if (!norm_factor) return fail(CTMR_E_INVALID, "null pointer");
+  if (!(most > 0.f)) return fail(CTMR_E_INVALID, "most must be positive");
+  rc = check_workspace(workspace, workspace_bytes, need);
+  if (rc) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  Sums sums = {reinterpret_cast<double*>((char*)workspace + kControlBytes), 0, most, norm_factor};
+  rc = square_sums(count, gradients, sizes, elems, const_cast<double*>(sums.sums), &sums.count, st);
+  if (rc) return rc;
+  return for_lists(count, gradients, sizes, elems, kChunk, [&](const List& list, int blocks) {
+    hipLaunchKernelGGL(scale_kernel, dim3(blocks), dim3(kThreads), 0, st, list, nullptr, sums);
+    sums.out = nullptr;
+    return check_launch("clip_gradients");
   });
 }
 

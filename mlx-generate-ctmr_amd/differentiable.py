@@ -765,6 +765,8 @@ class AdamW:
         self.max_norm = math.inf if max_norm is None else _most(max_norm)
         self.skip_non_finite = bool(skip_non_finite)
         self._layouts = _layouts_of(self.parameters)
+        self._counts = tuple(p.numel() for p in self.parameters)
+        self._elems = tuple(ops.ELEMENTS[p.dtype] for p in self.parameters)
         self._starts, total = self._places(self.parameters)
         half = [p for p in self.parameters if p.dtype != torch.float32]
         starts, room = self._places(half)
@@ -824,6 +826,24 @@ class AdamW:
             if p.dtype != torch.float32:
                 self._values(p).copy_(self.master[at:at + p.numel()])
 
+    @staticmethod
+    def _check_parameters(parameters: Sequence[Tensor], layouts: tuple[list, ...], numbers: Sequence[int]) -> None:
+        now = _layouts_of(parameters)
+        if now != layouts:
+            i = next(i for i, *pair in zip(numbers, zip(*now), zip(*layouts)) if pair[0] != pair[1])
+            raise ValueError(f"parameter {i} has become another than it was, by its shape, strides, type or device")
+
+    @staticmethod
+    def _brought(gradients: list[Tensor], parameters: Sequence[Tensor], numbers: Sequence[int]) -> list[Tensor]:
+        """The gradients in their parameters' layouts."""
+        for at, (i, g, p) in enumerate(zip(numbers, gradients, parameters)):
+            if g.shape != p.shape or g.dtype != p.dtype or g.device != p.device:
+                raise ValueError(f"gradient {i} is {tuple(g.shape)} {g.dtype} on {g.device}; its parameter "
+                                 f"{tuple(p.shape)} {p.dtype} on {p.device}")
+            if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
+                gradients[at] = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
+        return gradients
+
     @torch.no_grad()
     def step(self, gradients: Sequence[Optional[Tensor]], *, lr: Union[float, Tensor, None] = None,
              gradient_scale: float = 1.0) -> Tensor:
@@ -840,27 +860,25 @@ class AdamW:
         lr, scale = self.lr if lr is None else self._rate(lr), float(gradient_scale)
         if not math.isfinite(scale):
             raise ValueError(f"gradient_scale must be finite; got {scale}")
-        taken, _ = _listed(gradients, "gradients")
-        parameters, layouts, starts, masters = self.parameters, self._layouts, self._starts, self._master_starts
-        numbers = range(len(gradients))
-        if len(taken) != len(parameters):
+        plan = (self.parameters, self._counts, self._elems, self._starts, self._master_starts, range(len(gradients)))
+        layouts = self._layouts
+        if any(g is None for g in gradients):
             used = [g is not None for g in gradients]
             of = lambda values: list(itertools.compress(values, used))
-            parameters, starts, masters, numbers = map(of, (parameters, starts, masters, numbers))
-            layouts = tuple(map(of, layouts))
-        if _layouts_of(parameters) != layouts:
-            i = next(i for i, *pair in zip(numbers, zip(*_layouts_of(parameters)), zip(*layouts)) if pair[0] != pair[1])
-            raise ValueError(f"parameter {i} has become another than it was: {tuple(self.parameters[i].shape)}")
-        if _layouts_of(taken) != layouts:
-            for at, (i, g, p) in enumerate(zip(numbers, taken, parameters)):
-                if g.shape != p.shape or g.dtype != p.dtype or g.device != p.device:
-                    raise ValueError(f"gradient {i} is {tuple(g.shape)} {g.dtype} on {g.device}; its parameter "
-                                     f"{tuple(p.shape)} {p.dtype} on {p.device}")
-                if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
-                    taken[at] = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
+            plan, layouts, gradients = tuple(map(of, plan)), tuple(map(of, layouts)), of(gradients)
+        parameters, *places, numbers = plan
+        self._check_parameters(parameters, layouts, numbers)
+        try:  # gradients laid out as their parameters need no other check than this
+            alike = bool(gradients) and _layouts_of(gradients) == layouts
+        except (AttributeError, TypeError, RuntimeError):
+            alike = False
+        if alike:
+            _no_tangents(*gradients)
+        else:
+            gradients = self._brought(_listed(gradients, "gradients")[0], parameters, numbers)
         rate = (lr, 0.0) if isinstance(lr, Tensor) else (None, lr)
         state = [_used(t, self._stream) for t in (self.exp_avg, self.exp_avg_sq, self.master, self.steps)]
-        norm = ops.adamw(parameters, taken, *state, rate[0], starts, masters, rate[1], *self.betas,
-                         self.eps, self.weight_decay, scale, self.max_norm, self.skip_non_finite)
+        norm = ops.adamw(parameters, gradients, *state, rate[0], *places, rate[1], *self.betas, self.eps, self.weight_decay,
+                         scale, self.max_norm, self.skip_non_finite)
         torch.autograd.graph.increment_version([*parameters, *state])
         return norm

@@ -929,10 +929,10 @@ class _Sizes:
 
     __slots__ = ("count", "sizes", "elems", "nbytes")
 
-    def __init__(self, counts: Sequence[int], kinds: Sequence[torch.dtype]):
+    def __init__(self, counts: Sequence[int], kinds: Sequence):  # torch's types, or the library's
         self.count = len(counts)
         self.sizes = (ctypes.c_int64 * self.count)(*counts)
-        self.elems = (ctypes.c_int32 * self.count)(*[ELEMENTS[k] for k in kinds])
+        self.elems = (ctypes.c_int32 * self.count)(*[ELEMENTS.get(k, k) for k in kinds])
         self.nbytes = _lib.check(_lib.lib().ctmr_gradients_workspace_bytes(self.count, self.sizes),
                                  "ctmr_gradients_workspace_bytes")
 
@@ -979,16 +979,15 @@ def _(gradients):
 
 @_custom_op("ctmr::clip_gradients", ("gradients",))
 def clip_gradients(gradients: Sequence[Tensor], most: float) -> Tensor:
-    """``ctmr_gradient_norm`` and ``ctmr_scale_tensors`` of one or more tensors without gaps, in place: (2,) fp32, the norm
-    over all before and the factor."""
+    """``ctmr_clip_gradients`` of one or more tensors without gaps, in place: (2,) fp32, the norm over all before and the
+    factor."""
     like, sizes = _list_on_device(gradients), _list_sizes(gradients)
-    out, at = torch.empty(2, device=like.device, dtype=torch.float32), _addresses(gradients)
+    out = torch.empty(2, device=like.device, dtype=torch.float32)
     with _on(like):
-        ws, lib, stream = _workspace(sizes.nbytes, like.device), _lib.lib(), _raw_stream(like.device)
-        _lib.check(lib.ctmr_gradient_norm(sizes.count, at, sizes.sizes, sizes.elems, 1.0, most, out.data_ptr(),
-                                          ws.data_ptr(), sizes.nbytes, stream), "ctmr_gradient_norm")
-        _lib.check(lib.ctmr_scale_tensors(sizes.count, at, sizes.sizes, sizes.elems, out.data_ptr() + 4, stream),
-                   "ctmr_scale_tensors")
+        ws = _workspace(sizes.nbytes, like.device)
+        _lib.check(_lib.lib().ctmr_clip_gradients(sizes.count, _addresses(gradients), sizes.sizes, sizes.elems, most,
+                                                  out.data_ptr(), ws.data_ptr(), sizes.nbytes, _raw_stream(like.device)),
+                   "ctmr_clip_gradients")
     return out
 
 
@@ -1004,11 +1003,12 @@ def _places(starts: tuple[int, ...]):
 
 @_custom_op("ctmr::adamw", ("parameters", "exp_avg", "exp_avg_sq", "master", "steps"))
 def adamw(parameters: Sequence[Tensor], gradients: Sequence[Tensor], exp_avg: Tensor, exp_avg_sq: Tensor, master: Tensor,
-          steps: Tensor, lr_tensor: Optional[Tensor], starts: Sequence[int], master_starts: Sequence[int], lr: float,
+          steps: Tensor, lr_tensor: Optional[Tensor], counts: Sequence[int], elems: Sequence[int], starts: Sequence[int],
+          master_starts: Sequence[int], lr: float,
           beta1: float, beta2: float, eps: float, decay: float, scale: float, most: float, skip: bool) -> Tensor:
-    """``ctmr_adamw``: a step of parameters without gaps in place; the gradients' norm, 0-d fp32."""
-    like, sizes = _list_on_device(parameters), _list_sizes(parameters)
-    _list_on_device([exp_avg, gradients[0], like])
+    """``ctmr_adamw``: a step of parameters without gaps, of ``counts`` values and ``elems`` types, in place; the gradients'
+    norm, 0-d fp32."""
+    like, sizes = _list_on_device([exp_avg, *parameters, *gradients]), _sizes_of(tuple(counts), tuple(elems))
     norm = torch.empty((), device=like.device, dtype=torch.float32)
     desc = _lib.AdamwDesc(lr, beta1, beta2, eps, decay, scale, most, skip)
     with _on(like):
@@ -1022,5 +1022,5 @@ def adamw(parameters: Sequence[Tensor], gradients: Sequence[Tensor], exp_avg: Te
 
 
 @adamw.register_fake
-def _(parameters, gradients, exp_avg, exp_avg_sq, master, steps, lr_tensor, *_):
+def _(parameters, gradients, exp_avg, exp_avg_sq, master, steps, lr_tensor, *rest):
     return exp_avg.new_empty((), dtype=torch.float32)

@@ -88,7 +88,7 @@ def test_steps_are_refused(on_cpu):
     assert not on_cpu.launched
     o.step(good)
     o.step([None, good[1]])
-    assert [len(a[0]) for a in on_cpu.launched] == [2, 1] and on_cpu.launched[1][7] == [64]
+    assert [len(a[0]) for a in on_cpu.launched] == [2, 1] and on_cpu.launched[1][9] == [64]
     p.data = torch.zeros(6, 4).t()
     with pytest.raises(ValueError, match="parameter 0 has become"):
         o.step(good)
@@ -136,6 +136,12 @@ def test_host_checks(ctmr, native_loaded):
     assert space() == 64 and space(0, 0) == 64 and space(4096) == 80 and space(4097, 1) == 64 + 32
     assert space(1 << 30) == 64 + 2048 * 8 and space(-1) == L.E_INVALID and space(1 << 41) == L.E_UNSUPPORTED
     one = lambda kind, v: (kind * 1)(v)
+    clip = lambda ptr=p, out=p, ws=p, nbytes=1 << 20, size=5, most=1.0: lib.ctmr_clip_gradients(
+        1, one(ctypes.c_void_p, ptr), one(ctypes.c_int64, size), one(ctypes.c_int32, 0), most, out, ws, nbytes, None)
+    for size in (5, 1 << 30):  # both forms
+        assert clip(ptr=p + 2, size=size) == clip(out=None, size=size) == clip(most=0.0, size=size) == L.E_INVALID
+        assert clip(nbytes=64, size=size) == clip(ws=None, size=size) == L.E_WORKSPACE
+    assert clip(size=-1) == L.E_INVALID and clip(size=1 << 41) == L.E_UNSUPPORTED
     scale = lambda ptr=p, factor=p, size=5: lib.ctmr_scale_tensors(1, one(ctypes.c_void_p, ptr), one(ctypes.c_int64, size),
                                                                   one(ctypes.c_int32, 0), factor, None)
     assert scale(factor=None) == L.E_INVALID and scale(ptr=p + 2) == L.E_INVALID and scale(size=-1) == L.E_INVALID
