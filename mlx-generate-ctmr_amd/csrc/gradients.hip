@@ -118,9 +118,10 @@ struct Control {
   float lr_decay, rate, root, go;  // lr decay, lr / (1 - b1^t), 1 / sqrt(1 - b2^t), whether there is a step
 };
 
+// Without a limit the norm, which may be infinite or NaN, has no part in it.
 __device__ __forceinline__ float clip_factor(float norm, float scale, float most) {
   const float f = most / (norm + 1e-6f);
-  return scale * (f > 1.0f ? 1.0f : f);  // a NaN stays
+  return most == INFINITY ? scale : scale * (f > 1.0f ? 1.0f : f);  // a NaN stays
 }
 
 __global__ __launch_bounds__(1024) void finish_norm_kernel(const double* sums, int count, float scale, float most,

@@ -223,10 +223,12 @@ extern __shared__ __attribute__((aligned(16))) char bias_values[];  // of a posi
 // The tiled form: a workgroup of four waves takes 128 query rows of a head, 32 a
 // wave, and streams K and V through LDS in 64-key tiles: the next tile is loaded
 // straight into a second pair of arrays while the current one is multiplied.
-// Waves a SIMD that the registers are kept for.
+// Waves a SIMD that the registers are kept for.  With a bias, 2 x 16 heads of 4096 rows on 16x16x16, bf16: heads of 32 with
+// four 187 us (13 registers spill), with three 217; heads of 64 with three 257 (14 spill), with two 264.
 template <typename T, int D, int ST>
 constexpr int tiled_waves() {
-  return sizeof(T) == 4 && D == 128 ? 1 : ST == kBias && D * sizeof(T) == 64 ? 4 : 2;
+  if (ST == kBias && sizeof(T) == 2 && D < 128) return D == 32 ? 4 : 3;
+  return sizeof(T) == 4 && D == 128 ? 1 : 2;
 }
 
 template <typename T, int D, Cap CAP, int ST>

@@ -173,7 +173,6 @@ __device__ __forceinline__ void apply_bias(f16v& s, const char* values, unsigned
         second[r] = value(KEYS ? own1 - (w[r] >> 16) : own1 + (w[r] >> 16));
       }
     }
-    if constexpr (!SINGLE && ROWS == 16) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) s[g + r] = (ADD ? s[g + r] + first[r] : first[r]) + second[r];
   }

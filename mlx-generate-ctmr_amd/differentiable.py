@@ -707,7 +707,7 @@ def clip_gradients(gradients: Sequence[Optional[Tensor]], max_norm: float) -> Te
     """Multiplies gradients in place by ``min(1, max_norm / (norm + 1e-6))``; returns their ``gradient_norm`` before.
 
     The factor stays on the device.  A norm that is not finite is not refused: an infinite one gives zeros (NaN where the
-    infinities were), a NaN gives NaN.  A factor of one writes nothing.
+    infinities were), a NaN gives NaN.  A factor of one writes nothing, and an infinite ``max_norm`` is one.
 
     Raises:
         ValueError: on what ``gradient_norm`` refuses, tensors that share memory or have gaps in it (expanded or sliced

@@ -123,6 +123,20 @@ def test_what_is_not_finite(ctmr, dev):
     assert bool(f.clip_gradients([t, torch.ones(5, device=dev)], 1.0).isnan()) and bool(t.isnan().all())
 
 
+def test_without_a_limit_what_is_not_finite_stays_where_it_is(ctmr, dev):
+    f = ctmr.differentiable
+    t = torch.ones(3000, device=dev)
+    t[7], t[8] = math.inf, math.nan
+    kept = t.clone()
+    assert bool(f.clip_gradients([t], math.inf).isnan()) and torch.equal(t.nan_to_num(9.0), kept.nan_to_num(9.0))
+    p = torch.zeros(3000, device=dev)
+    o = f.AdamW([p], lr=0.5, weight_decay=0.0)
+    o.step([t], gradient_scale=2.0)
+    # every finite gradient moves its value by the rate, to the roundings of a step and eps 1e-8
+    assert bool(((p[9:] + 0.5).abs() < 1e-6).all()) and bool(((p[:7] + 0.5).abs() < 1e-6).all())
+    assert bool(p[7:9].isnan().all())
+
+
 def test_same_bits_again(ctmr, dev):
     grads = _list(dev, [(300001,), (777,)], torch.float32)
     first = ctmr.differentiable.gradient_norm(grads)

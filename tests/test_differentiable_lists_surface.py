@@ -19,7 +19,7 @@ def _calls(f):
     [([], "no tensor"), ([None], "no tensor|dense"), (torch.zeros(3), "list of tensors"), ([1.0], "dense"),
      ([torch.zeros(3, dtype=torch.float64)], "float32, bfloat16"), ([torch.zeros(3, dtype=torch.int32)], "float32"),
      ([torch.zeros(3).to_sparse()], "dense"),
-     ([torch.eye(3).to_sparse_csr()], "dense"), ([torch.zeros(3)], "on the GPU"),
+ ([torch.zeros(3)], "on the GPU"),
      ([torch.zeros(3), torch.zeros(3, device="meta")], "cpu and meta")])
 def test_lists_are_refused(ctmr, name, tensors, message):
     with pytest.raises(ValueError, match=message):
@@ -171,3 +171,12 @@ def test_lists_trace(ctmr):
         make = lambda *s, dtype=torch.float32: torch.empty(*s, device="cuda", dtype=dtype)
         grads = [make(3, 4), make(5, dtype=torch.bfloat16), None]
         assert f.gradient_norm(grads).shape == () and f.clip_gradients(grads, 1.0).dtype == torch.float32
+        o = f.AdamW(grads[:2], max_norm=1.0)
+        assert o.step([make(3, 4), make(5, dtype=torch.bfloat16)]).shape == () and o.master.shape == (64,)
+
+
+@pytest.mark.filterwarnings("ignore:Sparse CSR")
+def test_layouts_without_strides_are_refused(ctmr):
+    for call in _calls(ctmr.differentiable).values():
+        with pytest.raises(ValueError, match="dense"):
+            call([torch.eye(3).to_sparse_csr()])
