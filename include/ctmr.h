@@ -538,9 +538,9 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* desc, const
  * key_places (key_items, lk, axes), items 1 (all batch items alike) or the batch size;
  * places outside are taken as the nearest inside.  With `same` the keys lie where the rows
  * lie and key_places is not read.  table (table_rows, q_heads) of type table_elem; its
- * values are expected below 2^20 in size like scores, or below -2^100 (-inf too), which hides a pair:
- * a row left with no key gives zeros.  A value that is NaN or +inf makes NaN of all rows from
- * whose place some place within the extents has that distance.
+ * values are expected below 2^20 in size like scores, or below -2^100 (-inf too), which hides
+ * a pair: a row left with no key gives zeros.  NaN or inf makes NaN of the rows that see a
+ * key at that distance.
  * The scale, or the cap with one, is at least 2^-20 here.
  * `fine`: 16-bit softmax weights keep twice their type's bits in their products, which the
  * table's gradient (dtable) needs of the forward call; no other result does.

@@ -1,5 +1,5 @@
 // Masked attention with a position bias: the entry point of its forward call.  The
-// kernels are those of masked_attention_forward.hpp with the bias's products.
+// kernels are those of masked_attention_forward.hpp with the bias looked up.
 #include "masked_attention_forward.hpp"
 
 using namespace ctmr;

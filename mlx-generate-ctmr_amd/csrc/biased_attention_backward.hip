@@ -1,6 +1,7 @@
 // Gradients of the masked attention with a position bias, the table's among them.  The
-// kernels are those of masked_attention_backward.hpp with the bias's products, each type's
-// compiled in a source of its own (biased_gradients_*.hip); the table's gradient comes from the workgroups' sums by distance.
+// kernels are those of masked_attention_backward.hpp with the bias looked up, each type's
+// compiled in a source of its own (biased_gradients_*.hip); the table's gradient comes from
+// the workgroups' sums by distance.
 #include "masked_attention_backward.hpp"
 
 namespace ctmr {

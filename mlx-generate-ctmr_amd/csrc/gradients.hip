@@ -15,7 +15,10 @@
 // set by the sizes alone.
 //
 // Bound by memory: the norm reads each gradient once, the scaling reads and writes
-// it, a step moves 28 bytes a parameter.
+// it, a step moves 28 bytes an fp32 parameter.  24 matrices of 1024 x 4096 and as many
+// turned, fp32 (805 MB): the norm 2 x 79 us (5.1 TB/s), the steps of a third of them each
+// 184 (4.9 TB/s, a copy's rate); clipped at half the size 2 x 48 + 5 + 2 x 15.  Small
+// lists are bound by the host: 320 tensors, fp16, 105 us for 18 of kernels.
 #include "elements.hpp"
 
 #include <algorithm>
@@ -397,8 +400,8 @@ int ctmr_clip_gradients(int32_t count, void* const* gradients, const int64_t* si
                         float* norm_factor, void* workspace, size_t workspace_bytes, void* stream) {
   const int64_t need = ctmr_gradients_workspace_bytes(count, sizes);
   if (need < 0) return (int)need;
-  // Up to as many sums as a workgroup has threads: 10 tensors of 64 channels, bf16, 26 us for 30; with more of them each
-  // workgroup would add too many.
+  // Up to as many sums as a workgroup has threads, each workgroup adds them by itself: two launches instead of three, 26 us
+  // for 30 with 10 tensors of 64 channels, bf16; with more of them each would add too many.
   const int64_t chunks = chunks_of(count, sizes, sum_chunk(total_of(count, sizes)));
   if (chunks == 0 || chunks > kThreads) {
     const int rc = ctmr_gradient_norm(count, gradients, sizes, elems, 1.0f, most, norm_factor, workspace, workspace_bytes,

@@ -130,7 +130,8 @@ __device__ __forceinline__ bool softmax_blocks(f16v (&s)[NB], Frag<T> (&p)[NB][2
 // What rounding 16-bit weights left of them, as operands.  Where a table gets a gradient the weights' products take both
 // parts: each ds_ij = p_ij (g_i . v_j - delta_i) has an error of p_ij times that of delta_i = g_i . out_i, the same for a
 // whole row, which the sums over rows and keys of a bucket do not average out.  With weights rounded once the table's
-// gradient is off by 2e-4 (4096 rows and keys, bf16), so by 3e-6.
+// gradient is off by 4.6e-4 (2 x 16 heads of 64, 4096 rows on 16x16x16, bf16; fp16 5.8e-5), so by 3.6e-6 (3.7e-6), for
+// 320 us where one rounding takes 255.
 template <typename T>
 __device__ __forceinline__ Frag<T> fine_weights(const f16v& s, const Frag<T>& p, int step) {
   f16v rest = s;
@@ -224,7 +225,7 @@ extern __shared__ __attribute__((aligned(16))) char bias_values[];  // of a posi
 // wave, and streams K and V through LDS in 64-key tiles: the next tile is loaded
 // straight into a second pair of arrays while the current one is multiplied.
 // Waves a SIMD that the registers are kept for.  With a bias, 2 x 16 heads of 4096 rows on 16x16x16, bf16: heads of 32 with
-// four 187 us (13 registers spill), with three 217; heads of 64 with three 257 (14 spill), with two 264.
+// four 187 us (13 registers spill), with three 217; heads of 64 with three 255 (14 spill), with two 264.
 template <typename T, int D, int ST>
 constexpr int tiled_waves() {
   if (ST == kBias && sizeof(T) == 2 && D < 128) return D == 32 ? 4 : 3;

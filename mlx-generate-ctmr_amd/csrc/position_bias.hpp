@@ -6,8 +6,12 @@
 // for a distance (its bucket).  A workgroup lays the head's values out in LDS, the axes
 // in two pairs: one value for each two distances of a pair, (2 e - 1) (2 e' - 1) of
 // them, summed, in the scores' units.  Tokens have codes, places times strides, whose
-// difference is the LDS address of both pairs' values: a score costs a subtraction, a
-// mask, a shift and two reads and additions, whatever the places and their order.
+// difference is the LDS address of both pairs' values: a score costs two subtractions, two
+// reads and an addition, whatever the places and their order (without a cap the products
+// are added to it by the matrix units).  That is what bounds the forward pass: 2 x 16 heads
+// of 64, 4096 rows on 16x16x16, bf16, 255 us where no bias takes 162: 4 LDS instructions
+// where 1 was, LDS busy for 37 % of the time, vector units for 52, matrix units for 21
+// (38); no bank conflicts.  Heads of 32 187 us (116), of 128 361 (272).
 //
 // The table's gradient is the sum of the scores' gradients ds of a head over all pairs of
 // a distance.  For a row i, ds_ij counts by the key's place on each axis, so with a
@@ -20,8 +24,11 @@
 //
 // (The bias itself as a product too, of o_j and each row's r_i[c] = table[row_a(x - x_a(i))]
 // in parts, has no reads of single values, but r takes 24 to 64 registers and the product
-// as long as that of keys of as many values: 2 x 16 heads of 4096 rows on 16x16x16, bf16,
-// forward, heads of 64 KA us, of 128 KB; so KC and KD.)
+// as long as that of keys of as many values.  Forward, bf16, 4096 rows on 16x16x16, heads
+// of 64 243 us and of 128 557, where reads take 255 and 361; 16 heads of 64, 8192 rows on
+// 32x32x8, 874 and 489; a row over 13824 keys 66 and 52.  Tiles whose lanes share the reads
+// of four keys in a line take 261 us for heads of 64, but 260 for 245 where keys are in no
+// order and 294 for 192 with heads of 32: one form for all.)
 #pragma once
 
 #include "masked_attention.hpp"
@@ -138,12 +145,12 @@ __device__ __forceinline__ void lay_out_bias(const Bias& b, char* values, int h,
   }
 }
 
+// Rows whose reads apply_bias has on their way at once, 32 registers for 16: heads of 128 have none to spare.
 template <int D>
 constexpr int kBiasRows = D == 128 ? 4 : 16;
 
 // The bias of a lane's 16 scores, whose rows have `words` (32 of them, in LDS), or that added to the scores.  KEYS: the rows
-// are keys.  Pairs: the lane's own two addresses less the halves of a word, two subtractions; ROWS rows' reads are on their
-// way at once.
+// are keys.  Pairs: the lane's own two addresses less the halves of a word; else single axes, by the difference's bytes.
 template <bool SINGLE, bool KEYS, bool ADD, int ROWS>
 __device__ __forceinline__ void apply_bias(f16v& s, const char* values, unsigned own, const unsigned* words, int lane) {
   typedef __attribute__((address_space(3))) const char lds_char;

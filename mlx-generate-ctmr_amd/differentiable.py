@@ -471,11 +471,10 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
     A row that sees no key gives zeros and gets no gradient.  What masked places hold has no effect, NaN included.
     Scores are fp32: their size (the distance's too) is expected below some 2^20, where the weights still have digits.
     Statistics and sums are fp32; the softmax weights, and in the gradients those of the scores, are rounded to the
-    inputs' type for their products (in fp16 raised by powers of two that keep them in its range).  The bias is added with
-    17 bits (all of its bits with fp32 heads), its gradient is summed in fp32 and fp64 from as many of the scores' gradients'; where it
-    is wanted the weights keep twice their bits, and outputs may differ in the last from those without it.
-    A bias below -2^100 (-inf too) hides its pairs; any other value that is not finite makes NaN of the rows within whose reach
-    it lies.  The output has ``q``'s type and lies as ``(B, Lq, Hq, D)`` in memory, so merging the heads is a view.
+    inputs' type for their products (in fp16 raised by powers of two that keep them in its range).  The bias is added in
+    fp32; its gradient is summed in fp32 and fp64 from 17 bits of each score's gradient (all with fp32 heads), and where it is
+    wanted the weights keep twice their bits, so outputs may differ in the last from those without it.  A bias below -2^100
+    (-inf too) hides its pairs; NaN or inf makes NaN of the rows that see a key at that distance.  The output has ``q``'s type and lies as ``(B, Lq, Hq, D)`` in memory, so merging the heads is a view.
 
     Raises:
         ValueError: on other types, devices or shapes, a scale that is not positive and finite, a cap that is
