@@ -4,7 +4,8 @@ Modules:
   fast_fp32  the reference's fast-FP32 arithmetic surface (NDHWC-native plus
              ``*_ncdhw`` adapters with the reference's names)
   differentiable  group norm, rotary positions and masked attention with
-             gradients, in fp32, bf16 and fp16
+             gradients, position biases, gradient norms and AdamW steps, in
+             fp32, bf16 and fp16
   maisi      UNet / ControlNet / VAE decoder / sliding-window decode / rflow
              sampler composed over fast_fp32 (the callers of the hot path)
   weights    safetensors checkpoints (channels-last conv weights on disk)
