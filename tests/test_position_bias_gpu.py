@@ -149,11 +149,45 @@ def test_masks_caps_and_slopes(ctmr, dev, dtype, softcap, prefix, slopes, length
              slopes=0.1 * torch.rand(hq, device=dev) if slopes else None)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d", [32, 120, 128])
+@pytest.mark.parametrize(("softcap", "prefix", "lengths"), [(7.0, 40, [100, 29, 64]), (400.0, 0, [130, 71]), (0.0, 150, [90, 110])],
+                         ids=str)
+def test_masks_and_caps_of_narrow_and_wide_heads(ctmr, dev, dtype, d, softcap, prefix, lengths):
+    n, hq, l, extents = 2, 4, 205, (43, 43, 41)
+    prefix = torch.tensor([prefix, 3], dtype=torch.int32, device=dev)
+    _compare(ctmr, *_inputs(dev, n, hq, 2, l, l, d, dtype), _table(dev, extents, 32, hq, dtype), _places(dev, n, l, extents),
+             extents=extents, max_distance=40, softcap=softcap, prefix=prefix, ids=_rows(dev, n, lengths, l))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
 def test_long_rows_split_over_workgroups(ctmr, dev, dtype):
     for shape, extents in (((1, 4, 2, 150, 5000, 64), (30, 20, 20)), ((1, 2, 1, 2500, 40, 32), (60, 60))):
         _compare(ctmr, *_inputs(dev, *shape, dtype), _table(dev, extents, 32, shape[1], torch.float32),
                  _places(dev, 0, shape[3], extents), _places(dev, 0, shape[4], extents, seed=4), extents=extents)
+
+
+@pytest.mark.parametrize("kw", [{}, {"softcap": 2.0}, {"prefix": 20}, {"ids": True}], ids=str)
+def test_differences(ctmr, dev, kw):
+    f, extents, kw = ctmr.differentiable, (8, 10), dict(kw)
+    q, k, v, dout = _inputs(dev, 1, 4, 2, 80, 80, 32, torch.float32)
+    table = _table(dev, extents, 8, 4, torch.float32)
+    if kw.pop("ids", None):
+        kw["documents"] = f.Documents(_rows(dev, 1, [30, 41], 80))
+    kw |= {"buckets": f.PositionBuckets(_grid(dev, extents), extents=extents, num_buckets=8, max_distance=7), "scale": 0.3}
+    grads = _run(f, q, k, v, table, dout, **kw)[1:]
+    h = 1e-2
+    for i, g in enumerate(grads):
+        u = torch.randn(g.shape, device=dev, generator=torch.Generator(device=dev).manual_seed(40 + i))
+
+        def at(by):
+            x = [t + by * h * u if j == i else t for j, t in enumerate((q, k, v, table))]
+            return float((f.attention(*x[:3], position_bias=x[3], **kw).double() * dout.double()).sum())
+
+        # cut-off: h^2 / 6 = 1.7e-5 of a third derivative, that of scores that move by 2 or 3 at most below 100 slopes'
+        # sizes; noise 10240^(1/2) 2^-24 / h = 6e-4
+        slope = (at(1.0) - at(-1.0)) / (2 * h)
+        assert abs(slope - float((g.double() * u.double()).sum())) <= 2e-3 * float(g.norm() * u.norm())
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
