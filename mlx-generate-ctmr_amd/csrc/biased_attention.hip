@@ -17,7 +17,7 @@ extern "C" int ctmr_biased_attention(const ctmr_masked_attention_desc* d, const 
   if (!bucket_plan || !table || ((uintptr_t)bucket_plan & 15) != 0)
     return fail(CTMR_E_INVALID, "a bias needs its table and a plan of places on a 16-byte boundary");
   Args a = make_args(d, q, k, v, slopes, prefixes, plan);
-  a.out = out, a.rest = rest, a.lse = lse, a.part = (float*)workspace, a.splits = split_count(d);
+  a.out = out, a.rest = rest, a.wide_rest = 1, a.lse = lse, a.part = (float*)workspace, a.splits = split_count(d);
   a.ob = d->out_strides[0], a.oh = d->out_strides[1], a.ol = d->out_strides[2];
   const Bias bias = make_bias(d, buckets, bucket_plan, table);
   const bool few = few_rows(d);

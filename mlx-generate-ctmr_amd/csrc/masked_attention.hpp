@@ -287,7 +287,7 @@ struct Side {        // documents of the query or key rows
 struct Args {
   const void *q, *k, *v;
   void* out;
-  void* rest;             // what rounding took from out, as out lies, or null
+  void* rest;             // what rounding took from out, as out lies, or null; with wide_rest in fp32
   float* lse;             // (n, hq, lq) log2 of a row's sum (with a shifted cap: of the scores less cap), +inf for an
                           // empty row
   float* part;            // split keys: (splits, n, hq, lq, D) sums, then (.., 2) maximum and total
@@ -300,7 +300,7 @@ struct Args {
   int64_t qb, qh, ql, kb, kh, kl, vb, vh, vl, ob, oh, ol, gb, gh, gl;  // strides; g: dout
   int64_t dqb, dqh, dql, dkb, dkh, dkl, dvb, dvh, dvl;
   int n, lq, lk, hq, hk, group, d;
-  int prefixed, prefix, splits;
+  int prefixed, prefix, splits, wide_rest;
   float scale, cap;
 };
 

@@ -144,12 +144,12 @@ __device__ __forceinline__ int2 split_steps(int count, int split, int splits) {
   return {first, min(count, first + per)};
 }
 
-// Adds to the gradient of r what a 32 x 32 block of scores' gradients gives, in parts as r's.
-template <typename T, int ST>
+// Adds to the gradient of r what a 32 x 32 block of scores' gradients gives, in kParts parts.
+template <int ST>
 __device__ __forceinline__ void add_row_gradient(f16v (&dr)[HotTile<ST>::kBlocks], f16v ds, const char* hot, int row,
                                                  int lane) {
 #pragma unroll
-  for (int p = 0; p < kParts<T>; ++p) {
+  for (int p = 0; p < kParts; ++p) {
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const Frag<__bf16> f = result_frag<__bf16>(ds, w);
@@ -271,9 +271,13 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
 #pragma unroll
     for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[s][e], (float)of[e], delta);
     if constexpr (sizeof(T) == 2) {
-      if (a.rest) {
-        const T* rest = static_cast<const T*>(a.rest) + b * a.ob + h * a.oh + (int64_t)i * a.ol;
-        const Frag<T> rf = frag_global(rest, s, a.d, lane, real);
+      const int64_t at = b * a.ob + h * a.oh + (int64_t)i * a.ol;
+      if (ST > 0 && a.rest) {  // fp32
+        const Frag<float> rf = frag_global(static_cast<const float*>(a.rest) + at, s, a.d, lane, real);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[s][e], rf[e], delta);
+      } else if (a.rest) {
+        const Frag<T> rf = frag_global(static_cast<const T*>(a.rest) + at, s, a.d, lane, real);
 #pragma unroll
         for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[s][e], (float)rf[e], delta);
       }
@@ -402,7 +406,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
         if (table_part) {
           if constexpr (CAP == kNoCap) db = ds;
           if constexpr (kHalf<T>) db *= __builtin_ldexpf(1.0f, -(int)(CAP == kNoCap ? raise : raised));
-          add_row_gradient<T, ST>(dr, db, hot, 32 * u, la);
+          add_row_gradient<ST>(dr, db, hot, 32 * u, la);
         }
     }
   };

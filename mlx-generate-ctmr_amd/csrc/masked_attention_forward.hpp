@@ -127,17 +127,20 @@ __device__ __forceinline__ bool softmax_blocks(f16v (&s)[NB], Frag<T> (&p)[NB][2
   return __any(move);
 }
 
+// Parts of fine weights besides the first: bf16 24 bits in three, fp16 22 in two.
+template <typename T>
+constexpr int kMoreParts = std::is_same_v<T, __bf16> ? 2 : 1;
+
 // What rounding 16-bit weights left of them, as operands.  Where a table gets a gradient the weights' products take both
 // parts: each ds_ij = p_ij (g_i . v_j - delta_i) has an error of p_ij times that of delta_i = g_i . out_i, the same for a
 // whole row, which the sums over rows and keys of a bucket do not average out.  With weights rounded once the table's
 // gradient is off by 4.6e-4 (2 x 16 heads of 64, 4096 rows on 16x16x16, bf16; fp16 5.8e-5), so by 3.6e-6 (3.7e-6), for
 // 320 us where one rounding takes 255.
 template <typename T>
-__device__ __forceinline__ Frag<T> fine_weights(const f16v& s, const Frag<T>& p, int step) {
-  f16v rest = s;
+__device__ __forceinline__ Frag<T> fine_weights(f16v& s, const Frag<T>& p, int step) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) rest[8 * step + e] -= (float)p[e];
-  return result_frag<T>(rest, step);
+  for (int e = 0; e < 8; ++e) s[8 * step + e] -= (float)p[e];
+  return result_frag<T>(s, step);
 }
 
 // The values of V that store<true> left out, added to the rows that see their keys.
@@ -178,7 +181,9 @@ __device__ __forceinline__ void store_output(const Args& a, int64_t at, const Ve
   if constexpr (sizeof(T) == 2) {
     if (a.rest) {
       const Vec<T, 4> r = __builtin_convertvector(v, Vec<T, 4>);
-      store_rounded<T, 4>(static_cast<T*>(a.rest) + at, v - __builtin_convertvector(r, Vec<float, 4>));
+      const Vec<float, 4> rest = v - __builtin_convertvector(r, Vec<float, 4>);
+      if (a.wide_rest) *reinterpret_cast<Vec<float, 4>*>(static_cast<float*>(a.rest) + at) = rest;
+      else store_rounded<T, 4>(static_cast<T*>(a.rest) + at, rest);
     }
   }
 }
@@ -234,7 +239,7 @@ constexpr int tiled_waves() {
 
 template <typename T, int D, Cap CAP, int ST>
 __global__ __launch_bounds__(kThreads, (tiled_waves<T, D, ST>())) void attention_kernel(Args a, BiasOf<ST> bias) {
-  constexpr int NK = D / 16, ND = D / 32;
+  constexpr int NK = D / 16, ND = D / 32, kMore = ST == kFineBias ? kMoreParts<T> : 0;
   typedef Tile<T, D> Lds;
   __shared__ __attribute__((aligned(16))) char kt0[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) char vt0[kTile * Lds::kRow];
@@ -345,13 +350,18 @@ __global__ __launch_bounds__(kThreads, (tiled_waves<T, D, ST>())) void attention
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int w = 0; w < 2; ++w)
+      for (int w = 0; w < 2; ++w) {
+        Frag<T> more[kMore > 0 ? kMore : 1];
+#pragma unroll
+        for (int e = 0; e < kMore; ++e) more[e] = fine_weights<T>(s[u], e == 0 ? p[u][w] : more[e - 1], w);
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
           const Frag<T> f = u == 0 && w < kEarly ? vf[w][n] : Lds::down(vt, 32 * u + 16 * w, n, at);
           o[n] = mma<T>(f, p[u][w], o[n]);
-          if constexpr (ST == kFineBias) o[n] = mma<T>(f, fine_weights<T>(s[u], p[u][w], w), o[n]);
+#pragma unroll
+          for (int e = 0; e < kMore; ++e) o[n] = mma<T>(f, more[e], o[n]);
         }
+      }
     if (partial) {
       const unsigned lo = odd[0], hi = odd[1];
       if (lo | hi) add_odd_values<T, ND>(a, o, v, k0, lo, hi, mask, tile_ids, lane);
@@ -383,7 +393,7 @@ constexpr int few_lds() {  // bytes; the join takes four 32 x D blocks of fp32 a
 template <typename T, int D, Cap CAP, int ST>
 __global__ __launch_bounds__(kThreads, ST == 0 && sizeof(T) == 4 && D == 64 ? 2 : 1) void attention_few_kernel(
     Args a, BiasOf<ST> bias) {
-  constexpr int NK = D / 16, ND = D / 32;
+  constexpr int NK = D / 16, ND = D / 32, kMore = ST == kFineBias ? kMoreParts<T> : 0;
   typedef Tile<T, D> Lds;
   __shared__ __attribute__((aligned(16))) unsigned words[kWaves][kFewTile];
   __shared__ __attribute__((aligned(16))) char lds[few_lds<T, D>()];
@@ -472,13 +482,18 @@ __global__ __launch_bounds__(kThreads, ST == 0 && sizeof(T) == 4 && D == 64 ? 2 
       for (int n = 0; n < ND; ++n) o[n] *= alpha;
     }
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
+    for (int w = 0; w < 2; ++w) {
+      Frag<T> more[kMore > 0 ? kMore : 1];
+#pragma unroll
+      for (int e = 0; e < kMore; ++e) more[e] = fine_weights<T>(s[0], e == 0 ? p[0][w] : more[e - 1], w);
 #pragma unroll
       for (int n = 0; n < ND; ++n) {
         const Frag<T> f = Lds::down(vt, 16 * w, n, lane);
         o[n] = mma<T>(f, p[0][w], o[n]);
-        if constexpr (ST == kFineBias) o[n] = mma<T>(f, fine_weights<T>(s[0], p[0][w], w), o[n]);
+#pragma unroll
+        for (int e = 0; e < kMore; ++e) o[n] = mma<T>(f, more[e], o[n]);
       }
+    }
     if (partial) {
       const unsigned set = odd[wave];
       if (set) add_odd_values<T, ND>(a, o, v, k0, set, 0u, mask, docs ? ids + k0 : nullptr, lane);

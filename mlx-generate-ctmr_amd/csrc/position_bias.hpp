@@ -92,8 +92,7 @@ struct HotTile {
 // In the forward call and in dk and dv, which have no columns: a bias, and one with fine weights (fine_weights).
 constexpr int kBias = 1, kFineBias = 2;
 
-template <typename T>
-constexpr int kParts = sizeof(T) == 4 ? 3 : 2;
+constexpr int kParts = 3;  // of ds
 
 // With fp32 heads of 128 LDS has no room for pairs: the axes are looked up one by one, in tables of 256 values, by the
 // bytes of the difference of places.

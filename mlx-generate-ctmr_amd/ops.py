@@ -845,6 +845,12 @@ def _bias_desc(q: Tensor, k: Tensor, table: Tensor, places: Sequence[int]) -> _l
                         table.numel() // int(q.shape[1]), ELEMENTS[table.dtype])
 
 
+def _rest_like(q: Tensor, wanted: bool) -> Tensor:
+    """For what rounding takes from a biased call's output, in fp32; empty where nothing is."""
+    b, h, l, d = q.shape if wanted and q.element_size() == 2 else (0, 0, 0, 0)
+    return torch.empty_strided((b, h, l, d), (l * h * d, d, h * d, 1), device=q.device, dtype=torch.float32)
+
+
 @_custom_op("ctmr::biased_attention")
 def biased_attention(q: Tensor, k: Tensor, v: Tensor, slopes: Optional[Tensor], prefixes: Optional[Tensor],
                      plan: Optional[Tensor], bucket_plan: Tensor, table: Tensor, places: Sequence[int], scale: float,
@@ -854,7 +860,7 @@ def biased_attention(q: Tensor, k: Tensor, v: Tensor, slopes: Optional[Tensor], 
     ``places`` (``_bias_desc``); ``want_table``: the table gets a gradient too."""
     _require_device(q, k, v, slopes, prefixes, plan, bucket_plan, table)
     out = _heads_like(q)
-    rest = _heads_like(q) if want_grad and q.element_size() == 2 else q.new_empty((0,))
+    rest = _rest_like(q, want_grad)
     lse = torch.empty(q.shape[:3] if want_grad else (0,), device=q.device, dtype=torch.float32)
     if q.numel() == 0 or k.shape[2] == 0:
         return out.zero_(), rest.zero_(), lse.fill_(math.inf)
@@ -871,7 +877,7 @@ def biased_attention(q: Tensor, k: Tensor, v: Tensor, slopes: Optional[Tensor], 
 
 @biased_attention.register_fake
 def _(q, k, v, slopes, prefixes, plan, bucket_plan, table, places, scale, softcap, prefixed, prefix, want_grad, want_table):
-    return (_heads_like(q), _heads_like(q) if want_grad and q.element_size() == 2 else q.new_empty((0,)),
+    return (_heads_like(q), _rest_like(q, want_grad),
             q.new_empty(q.shape[:3] if want_grad else (0,), dtype=torch.float32))
 
 
