@@ -261,6 +261,10 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
   const T* k = static_cast<const T*>(a.k) + b * a.kb + (h / a.group) * a.kh;
   const T* v = static_cast<const T*>(a.v) + b * a.vb + (h / a.group) * a.vh;
 
+  // The matrix units drop bits of sums of 16-bit products downwards, for every ds of a row, a bias that the table's sums over
+  // rows and keys add up.  Odd rows have g and all that is made of it with the other sign, so that it cancels.
+  constexpr bool kFlips = ST > 0 && sizeof(T) == 2;
+  const float flip = kFlips && (lane & 1) ? -1.f : 1.f;
   Frag<T> qf[NK], gf[NK];
   float delta = 0.f;
 #pragma unroll
@@ -286,6 +290,11 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
   delta = half_sum(delta);
   if (real && half == 0 && blockIdx.y == 0) a.delta[stat] = -delta;
   if (!a.dq && !table_part) return;
+  if constexpr (kFlips) {
+    delta *= flip;
+#pragma unroll
+    for (int s = 0; s < NK; ++s) gf[s] = __builtin_bit_cast(Frag<T>, __builtin_bit_cast(u4, gf[s]) ^ (lane & 1 ? 0x80008000u : 0u));
+  }
   const float lse = real ? a.lse[stat] : INFINITY;
   float raise = kDsRaise<T>;
   f16v dq[ND];
@@ -415,6 +424,12 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
   for (int tile = first; tile < last; tile += 2) {
     step(tile, kt0, vt0, hot0, words0, kt1, vt1, other, words1);
     if (tile + 1 < last) step(tile + 1, kt1, vt1, other, words1, kt0, vt0, hot0, words0);
+  }
+  if constexpr (kFlips) {
+#pragma unroll
+    for (int n = 0; n < ND; ++n) dq[n] *= flip;
+#pragma unroll
+    for (int n = 0; n < HotTile<ST>::kBlocks; ++n) dr[n] *= flip;
   }
   if constexpr (ST > 0) {
     if (table_part) add_distances<ST>(bias, dr, places, real, reinterpret_cast<float*>(hot0), table_part, t);
