@@ -542,8 +542,9 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* desc, const
  * a pair: a row left with no key gives zeros.  NaN or inf makes NaN of the rows that see a
  * key at that distance.
  * The scale, or the cap with one, is at least 2^-20 here.
- * `fine`: 16-bit softmax weights keep twice their type's bits in their products, which the
- * table's gradient (dtable) needs of the forward call; no other result does.
+ * `fine`: 16-bit softmax weights keep twice their type's bits in their products (bf16 with an
+ * fp32 table three times), which the table's gradient (dtable) needs of the forward call; no
+ * other result does.  rest is fp32 here, its strides out's in values.
  * The forward workspace is ctmr_masked_attention's, the backward one has a size of its own
  * (`documents`: with a plan of documents).  dtable, like table, may be NULL. */
 typedef struct ctmr_buckets_desc {

@@ -26,7 +26,11 @@ extern "C" int ctmr_biased_attention(const ctmr_masked_attention_desc* d, const 
     typedef decltype(type) T;
     constexpr int D = decltype(width)::value;
     if constexpr (sizeof(T) == 2)
-      if (fine) return launch<T, D>(a, BiasOf<kFineBias>{bias}, few, st);
+      if (fine) {
+        if constexpr (std::is_same_v<T, __bf16>)
+          if (bias.elem == CTMR_ELEM_F32) return launch<T, D>(a, BiasOf<kFinestBias>{bias}, few, st);
+        return launch<T, D>(a, BiasOf<kFineBias>{bias}, few, st);
+      }
     return launch<T, D>(a, BiasOf<kBias>{bias}, few, st);
   };
   auto of_type = [&](auto type) {

@@ -25,7 +25,7 @@
 // two below: two operations a score in dk and dv, half a one in dq); fp32, 2 x 8 heads of
 // 2048 rows of 32: 252 (119 of the seven, where a library product of 8192^3 reaches 153).
 // With a position bias on 16x16x16 and its table's gradient (position_bias.hpp): bf16, heads
-// of 32 608 us, of 64 757, of 128 1770; fp32 as above on 16x16x8 317.
+// of 32 660 us, of 64 826, of 128 1870; fp32 as above on 16x16x8 318.
 //
 // fp16's range is far smaller than what ds spans, so every row of dq and every key of
 // dk (a lane's column) has a power of two of its own that ds is multiplied by: the sums
@@ -144,12 +144,13 @@ __device__ __forceinline__ int2 split_steps(int count, int split, int splits) {
   return {first, min(count, first + per)};
 }
 
-// Adds to the gradient of r what a 32 x 32 block of scores' gradients gives, in kParts parts.
+// Adds to the gradient of r what a 32 x 32 block of scores' gradients gives, in two parts or three.
 template <int ST>
-__device__ __forceinline__ void add_row_gradient(f16v (&dr)[HotTile<ST>::kBlocks], f16v ds, const char* hot, int row,
-                                                 int lane) {
+__device__ __forceinline__ void add_row_gradient(f16v (&dr)[HotTile<ST>::kBlocks], f16v ds, bool third, const char* hot,
+                                                 int row, int lane) {
 #pragma unroll
-  for (int p = 0; p < kParts; ++p) {
+  for (int p = 0; p < 3; ++p) {
+    if (p == 2 && !third) break;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const Frag<__bf16> f = result_frag<__bf16>(ds, w);
@@ -202,7 +203,7 @@ __device__ __forceinline__ void add_distances(const Bias& bias, const f16v (&dr)
 // Waves a SIMD that the registers are kept for.  16-bit, 2 x 16 heads of 4096 rows, both kernels: heads of 32 with four
 // 327 us (a few registers spill), with three 351; heads of 64 with three for dk and dv too (20 spill) 577 us, with two
 // there 505.  With a bias dq has up to 64 more sums a lane: heads of 32 with 96 columns, 8192 rows on 32x32x8, both kernels
-// with two 1182 us, with three 1514.
+// with two 1182 us, with three 1514 (ds in two parts).
 template <typename T, int D, int ST>
 constexpr int dq_waves() {
   if (ST > 0) return D * sizeof(T) >= 256 ? 1 : 2;
@@ -261,8 +262,9 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
   const T* k = static_cast<const T*>(a.k) + b * a.kb + (h / a.group) * a.kh;
   const T* v = static_cast<const T*>(a.v) + b * a.vb + (h / a.group) * a.vh;
 
-  // The matrix units drop bits of sums of 16-bit products downwards, for every ds of a row, a bias that the table's sums over
-  // rows and keys add up.  Odd rows have g and all that is made of it with the other sign, so that it cancels.
+  // The matrix units round sums of 16-bit products to one side, so each ds has a bias that the table's sums over rows and
+  // keys add up (2.5e-6 of its gradient at 4096 rows, growing with their number).  Odd rows have g and all that is made of
+  // it with the other sign, and it cancels (5e-7, at any length).
   constexpr bool kFlips = ST > 0 && sizeof(T) == 2;
   const float flip = kFlips && (lane & 1) ? -1.f : 1.f;
   Frag<T> qf[NK], gf[NK];
@@ -415,7 +417,7 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
         if (table_part) {
           if constexpr (CAP == kNoCap) db = ds;
           if constexpr (kHalf<T>) db *= __builtin_ldexpf(1.0f, -(int)(CAP == kNoCap ? raise : raised));
-          add_row_gradient<ST>(dr, db, hot, 32 * u, la);
+          add_row_gradient<ST>(dr, db, sizeof(T) == 4 || wide_table(bias), hot, 32 * u, la);
         }
     }
   };

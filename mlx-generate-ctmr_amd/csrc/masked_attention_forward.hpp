@@ -127,15 +127,11 @@ __device__ __forceinline__ bool softmax_blocks(f16v (&s)[NB], Frag<T> (&p)[NB][2
   return __any(move);
 }
 
-// Parts of fine weights besides the first: bf16 24 bits in three, fp16 22 in two.
-template <typename T>
-constexpr int kMoreParts = std::is_same_v<T, __bf16> ? 2 : 1;
-
-// What rounding 16-bit weights left of them, as operands.  Where a table gets a gradient the weights' products take both
-// parts: each ds_ij = p_ij (g_i . v_j - delta_i) has an error of p_ij times that of delta_i = g_i . out_i, the same for a
+// What rounding 16-bit weights left of them, as operands.  Where a table gets a gradient the weights' products take two or
+// three parts: each ds_ij = p_ij (g_i . v_j - delta_i) has an error of p_ij times that of delta_i = g_i . out_i, the same for a
 // whole row, which the sums over rows and keys of a bucket do not average out.  With weights rounded once the table's
-// gradient is off by 4.6e-4 (2 x 16 heads of 64, 4096 rows on 16x16x16, bf16; fp16 5.8e-5), so by 3.6e-6 (3.7e-6), for
-// 320 us where one rounding takes 255.
+// gradient is off by 4.6e-4 (2 x 16 heads of 64, 4096 rows on 16x16x16, bf16; fp16 5.8e-5), with two parts by 1.2e-6
+// (5e-7), with three, which bf16 has for fp32 tables, by 5e-7; the forward call takes 255, 320 and 384 us.
 template <typename T>
 __device__ __forceinline__ Frag<T> fine_weights(f16v& s, const Frag<T>& p, int step) {
 #pragma unroll
@@ -239,7 +235,7 @@ constexpr int tiled_waves() {
 
 template <typename T, int D, Cap CAP, int ST>
 __global__ __launch_bounds__(kThreads, (tiled_waves<T, D, ST>())) void attention_kernel(Args a, BiasOf<ST> bias) {
-  constexpr int NK = D / 16, ND = D / 32, kMore = ST == kFineBias ? kMoreParts<T> : 0;
+  constexpr int NK = D / 16, ND = D / 32, kMore = ST == 0 ? 0 : ST - kBias;
   typedef Tile<T, D> Lds;
   __shared__ __attribute__((aligned(16))) char kt0[kTile * Lds::kRow];
   __shared__ __attribute__((aligned(16))) char vt0[kTile * Lds::kRow];
@@ -393,7 +389,7 @@ constexpr int few_lds() {  // bytes; the join takes four 32 x D blocks of fp32 a
 template <typename T, int D, Cap CAP, int ST>
 __global__ __launch_bounds__(kThreads, ST == 0 && sizeof(T) == 4 && D == 64 ? 2 : 1) void attention_few_kernel(
     Args a, BiasOf<ST> bias) {
-  constexpr int NK = D / 16, ND = D / 32, kMore = ST == kFineBias ? kMoreParts<T> : 0;
+  constexpr int NK = D / 16, ND = D / 32, kMore = ST == 0 ? 0 : ST - kBias;
   typedef Tile<T, D> Lds;
   __shared__ __attribute__((aligned(16))) unsigned words[kWaves][kFewTile];
   __shared__ __attribute__((aligned(16))) char lds[few_lds<T, D>()];

@@ -19,8 +19,9 @@
 //   dr_i[c] = sum_j ds_ij o_j[c]
 // is a matrix product, which the matrix units sum without an addition in memory; the
 // rows' dr are then added by distance.  o is exact in bf16 and the same for all heads: it
-// streams through LDS beside the keys.  ds goes in kParts bf16 parts, 2^-17 of it with
-// 16-bit heads and all of fp32's bits with fp32 heads.
+// streams through LDS beside the keys.  ds goes in three bf16 parts, all of fp32's bits, or
+// two, 2^-17 of it, where the table has 16 bits (both kernels of the backward pass, heads of
+// 64, 4096 rows: 826 us, 775).
 //
 // (The bias itself as a product too, of o_j and each row's r_i[c] = table[row_a(x - x_a(i))]
 // in parts, has no reads of single values, but r takes 24 to 64 registers and the product
@@ -89,10 +90,12 @@ struct HotTile {
     }
   }
 };
-// In the forward call and in dk and dv, which have no columns: a bias, and one with fine weights (fine_weights).
-constexpr int kBias = 1, kFineBias = 2;
+// In the forward call and in dk and dv, which have no columns: a bias, and one with weights in two and three parts
+// (fine_weights).
+constexpr int kBias = 1, kFineBias = 2, kFinestBias = 3;
 
-constexpr int kParts = 3;  // of ds
+// Whether the table's gradient has more digits than two bf16 parts of each ds.
+__device__ __forceinline__ bool wide_table(const Bias& b) { return b.elem == CTMR_ELEM_F32; }
 
 // With fp32 heads of 128 LDS has no room for pairs: the axes are looked up one by one, in tables of 256 values, by the
 // bytes of the difference of places.
