@@ -131,7 +131,7 @@ __device__ __forceinline__ bool softmax_blocks(f16v (&s)[NB], Frag<T> (&p)[NB][2
 // three parts: each ds_ij = p_ij (g_i . v_j - delta_i) has an error of p_ij times that of delta_i = g_i . out_i, the same for a
 // whole row, which the sums over rows and keys of a bucket do not average out.  With weights rounded once the table's
 // gradient is off by 4.6e-4 (2 x 16 heads of 64, 4096 rows on 16x16x16, bf16; fp16 5.8e-5), with two parts by 1.2e-6
-// (5e-7), with three, which bf16 has for fp32 tables, by 5e-7; the forward call takes 255, 320 and 384 us.
+// (7e-7), with three, which bf16 has for fp32 tables, by 5e-7; the forward call takes 255, 320 and 384 us.
 template <typename T>
 __device__ __forceinline__ Frag<T> fine_weights(f16v& s, const Frag<T>& p, int step) {
 #pragma unroll
