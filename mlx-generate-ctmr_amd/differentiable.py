@@ -736,7 +736,10 @@ class AdamW:
 
     The state is public, on the parameters' device, and may be written between steps: ``steps`` (0-d int64), ``exp_avg``,
     ``exp_avg_sq`` and ``master`` (1-d fp32; ``master`` of the 16-bit parameters only), where each parameter's values start
-    on a multiple of ``GRAIN``, in the list's order.  Steps may be captured into a graph; ``lr`` may then be a 0-d fp32 tensor.
+    on a multiple of ``GRAIN``, in the list's order.  Steps may be captured into a graph; ``lr`` may then be a 0-d fp32 tensor.  Replays
+    raise no ``_version``: from the capture on, ``fast_fp32`` and ``maisi`` derive what they keep of the parameters (packed and
+    fused weights) anew at each use, until ``fast_fp32.settle_weights`` after the last replay; a ``maisi.UNetGraph`` recorded
+    before the capture keeps the old ones.
 
     Raises:
         ValueError: on an empty list, other types, parameters that are not on one GPU, share memory or have gaps in it, and

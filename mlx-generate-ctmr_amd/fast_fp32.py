@@ -161,6 +161,9 @@ def _vec(t: Optional[Tensor], n: int, name: str, device: torch.device) -> Option
 # references to the same source objects are alive and each source's
 # ``_version`` is what it was when the entry was built (torch tensors, unlike
 # MLX arrays, can change in place: ``copy_`` or an in-place reload bumps it).
+# Tensors that a step recorded into a graph writes change with every replay and
+# no version does: what is derived of them is derived anew each time, until
+# ``settle_weights``.
 # ---------------------------------------------------------------------------
 _packed: dict[tuple, tuple[tuple[weakref.ref, ...], tuple[int, ...], Tensor]] = {}
 _packed_lock = threading.RLock()  # re-entrant: a weakref eviction may run inside a locked section
@@ -200,8 +203,12 @@ def retain_cached(sink: list) -> Iterator[list]:
 
 def cached_derived(cache: dict, lock: threading.Lock, key: tuple, sources: tuple[Tensor, ...], build):
     """The cache entry for ``key`` built from ``sources`` by ``build()``, rebuilt when a source was
-    collected, replaced or modified in place since.  ``build`` returns a tensor or a tuple whose
-    tensors are the derived data (recorded for ``retain_cached``)."""
+    collected, replaced or modified in place since, and not kept while a recorded graph writes one.
+    ``build`` returns a tensor or a tuple whose tensors are the derived data (recorded for ``retain_cached``)."""
+    if ops._rewritten and any(map(ops._is_rewritten, sources)):
+        value = build()
+        _note_use(*(value if isinstance(value, tuple) else (value,)))
+        return value
     with lock:
         hit = cache.get(key)
         if hit is not None and _sources_match(hit[0], hit[1], sources):
@@ -298,6 +305,17 @@ def drop_packed_weights(weights: Iterable[Tensor]) -> None:
         with lock:
             for key in [k for k, entry in cache.items() if any(id(r()) in ids for r in entry[0] if r() is not None)]:
                 del cache[key]
+
+
+def settle_weights(weights: Iterable[Tensor]) -> None:
+    """Says that no recorded graph changes ``weights`` from here on, after the last replay of a captured
+    ``differentiable.AdamW`` step: what is derived of them is kept from call to call again, as
+    ``drop_packed_weights`` leaves it.  Until then every use derives it anew, also in a pass that a
+    ``maisi.UNetGraph`` records.  Capturing another step ends it."""
+    weights = list(weights)
+    for w in weights:
+        ops._rewritten.pop(id(w.untyped_storage()), None)
+    drop_packed_weights(weights)
 
 
 def register_cache(cache: dict, lock) -> None:

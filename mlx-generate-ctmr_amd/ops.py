@@ -21,6 +21,7 @@ import ctypes
 import functools
 import math
 import operator
+import weakref
 from typing import Callable, Optional, Sequence
 
 import torch
@@ -965,6 +966,27 @@ def _list_on_device(tensors: Sequence[Tensor]) -> Tensor:
     return tensors[0]
 
 
+# Storages that a call recorded into a HIP graph writes, by identity.  A replay writes them without a step of their version
+# counters, so that nothing derived of them may be kept by these (``fast_fp32.cached_derived``).
+_rewritten: dict[int, "weakref.ref[torch.UntypedStorage]"] = {}
+
+
+def _note_writes(tensors: Sequence[Tensor]) -> None:
+    """Marks what a call writes, if it is recorded into a graph."""
+    if not torch.cuda.is_current_stream_capturing():
+        return
+    for t in tensors:
+        storage = t.untyped_storage()
+        key = id(storage)
+        if key not in _rewritten:
+            _rewritten[key] = weakref.ref(storage, lambda _, key=key, marks=_rewritten: marks.pop(key, None))
+
+
+def _is_rewritten(t: Tensor) -> bool:
+    """Whether a recorded call writes the memory of ``t``, whichever view of it."""
+    return id(t.untyped_storage()) in _rewritten
+
+
 @_custom_op("ctmr::gradient_norm")
 def gradient_norm(gradients: Sequence[Tensor]) -> Tensor:
     """``ctmr_gradient_norm`` of one or more tensors without gaps: (2,) fp32, the norm over all and one."""
@@ -994,6 +1016,7 @@ def clip_gradients(gradients: Sequence[Tensor], most: float) -> Tensor:
         _lib.check(_lib.lib().ctmr_clip_gradients(sizes.count, _addresses(gradients), sizes.sizes, sizes.elems, most,
                                                   out.data_ptr(), ws.data_ptr(), sizes.nbytes, _raw_stream(like.device)),
                    "ctmr_clip_gradients")
+        _note_writes(gradients)
     return out
 
 
@@ -1024,6 +1047,7 @@ def adamw(parameters: Sequence[Tensor], gradients: Sequence[Tensor], exp_avg: Te
             _places(tuple(starts)), _places(tuple(master_starts)), exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
             master.data_ptr() if master.numel() else None, steps.data_ptr(), _ptr(lr_tensor), norm.data_ptr(), ws.data_ptr(),
             sizes.nbytes, _raw_stream(like.device)), "ctmr_adamw")
+        _note_writes(parameters)
     return norm
 
 
