@@ -734,7 +734,8 @@ class AdamW:
     ``max_norm`` clips each step's gradients as ``clip_gradients`` does, without writing them; ``skip_non_finite`` leaves a
     step out whose gradients have a norm that is not finite (for steps with a loss scale).
 
-    The state is public, on the parameters' device, and may be written between steps: ``steps`` (0-d int64), ``exp_avg``,
+    The settings may be changed between steps, ``lr`` by a number or a 0-d fp32 tensor on the parameters' device.
+    The state is public, on the parameters' device, and may be written or bound anew between steps: ``steps`` (0-d int64), ``exp_avg``,
     ``exp_avg_sq`` and ``master`` (1-d fp32; ``master`` of the 16-bit parameters only), where each parameter's values start
     on a multiple of ``GRAIN``, in the list's order.  Steps may be captured into a graph; ``lr`` may then be a 0-d fp32 tensor.  Replays
     raise no ``_version``: from the capture on, ``fast_fp32`` and ``maisi`` derive what they keep of the parameters (packed and
@@ -758,14 +759,8 @@ class AdamW:
         _apart(self.parameters, "parameters", contiguous)
         device = self.parameters[0].device
         self.lr = self._rate(lr)
-        self.betas, self.eps, self.weight_decay = (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
-        if not all(0.0 <= b < 1.0 for b in self.betas):
-            raise ValueError(f"betas must be in [0, 1); got {self.betas}")
-        for name, value in (("eps", self.eps), ("weight_decay", self.weight_decay)):
-            if not (math.isfinite(value) and value >= 0.0):
-                raise ValueError(f"{name} must be finite and not negative; got {value}")
-        self.max_norm = math.inf if max_norm is None else _most(max_norm)
-        self.skip_non_finite = bool(skip_non_finite)
+        self._given = self._taken = self._checked(betas, eps, weight_decay, max_norm, skip_non_finite)
+        self.betas, self.eps, self.weight_decay, self.max_norm, self.skip_non_finite = self._taken
         self._layouts = _layouts_of(self.parameters)
         self._counts = tuple(p.numel() for p in self.parameters)
         self._elems = tuple(ops.ELEMENTS[p.dtype] for p in self.parameters)
@@ -777,8 +772,41 @@ class AdamW:
         make = lambda n: torch.zeros(n, device=device, dtype=torch.float32)
         self.exp_avg, self.exp_avg_sq, self.master = make(total), make(total), make(room)
         self.steps = torch.zeros((), device=device, dtype=torch.int64)
+        self._state_layouts = _layouts_of(self._state())
         self._stream = _stream_of(self.steps)
         self.load_masters()
+
+    @staticmethod
+    def _checked(betas, eps, weight_decay, max_norm, skip_non_finite) -> tuple:
+        """The settings as the steps take them, checked."""
+        betas, eps, weight_decay = (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
+        if not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"betas must be in [0, 1); got {betas}")
+        for name, value in (("eps", eps), ("weight_decay", weight_decay)):
+            if not (math.isfinite(value) and value >= 0.0):
+                raise ValueError(f"{name} must be finite and not negative; got {value}")
+        return betas, eps, weight_decay, math.inf if max_norm is None else _most(max_norm), bool(skip_non_finite)
+
+    def _settings(self) -> tuple:
+        """``_checked`` of the settings as they are now."""
+        given = self.betas, self.eps, self.weight_decay, self.max_norm, self.skip_non_finite
+        if given != self._given:
+            self._taken, self._given = self._checked(*given), given
+        return self._taken
+
+    def _state(self) -> list[Tensor]:
+        return [self.exp_avg, self.exp_avg_sq, self.master, self.steps]
+
+    def _checked_state(self) -> list[Tensor]:
+        """The state's tensors, which may have been bound anew: the kernels take their addresses."""
+        state = self._state()
+        try:
+            alike = _layouts_of(state) == self._state_layouts
+        except (AttributeError, TypeError, RuntimeError):  # no tensors, or of a layout without strides
+            alike = False
+        if not alike:
+            raise ValueError("exp_avg, exp_avg_sq, master and steps must keep their shapes, types and device, without gaps")
+        return state
 
     def _rate(self, lr: Union[float, Tensor]) -> Union[float, Tensor]:
         if isinstance(lr, Tensor):
@@ -853,13 +881,17 @@ class AdamW:
         the gradients times ``gradient_scale``, which is what the step takes (a loss scale's inverse).
 
         Raises:
-            ValueError: on gradients of another count, or of other shapes, types or devices than their parameters', and an
-                ``lr`` or scale that is not finite.
+            ValueError: on gradients of another count, or of other shapes, types or devices than their parameters', an ``lr``
+                or scale that is not finite, and settings, parameters or a state that have been changed to what the constructor
+                would not have or make.
             NotImplementedError: on forward-mode (dual) tensors."""
         gradients = list(gradients)
         if len(gradients) != len(self.parameters):
             raise ValueError(f"{len(gradients)} gradients for {len(self.parameters)} parameters")
-        lr, scale = self.lr if lr is None else self._rate(lr), float(gradient_scale)
+        if len(self.parameters) != len(self._counts):
+            raise ValueError(f"{len(self.parameters)} parameters where there were {len(self._counts)}")
+        lr, scale = self._rate(self.lr if lr is None else lr), float(gradient_scale)
+        settings, state = self._settings(), self._checked_state()
         if not math.isfinite(scale):
             raise ValueError(f"gradient_scale must be finite; got {scale}")
         plan = (self.parameters, self._counts, self._elems, self._starts, self._master_starts, range(len(gradients)))
@@ -879,8 +911,9 @@ class AdamW:
         else:
             gradients = self._brought(_listed(gradients, "gradients")[0], parameters, numbers)
         rate = (lr, 0.0) if isinstance(lr, Tensor) else (None, lr)
-        state = [_used(t, self._stream) for t in (self.exp_avg, self.exp_avg_sq, self.master, self.steps)]
-        norm = ops.adamw(parameters, gradients, *state, rate[0], *places, rate[1], *self.betas, self.eps, self.weight_decay,
-                         scale, self.max_norm, self.skip_non_finite)
+        if self._stream is not None and ops._raw_stream(state[0].device) != self._stream:
+            state = [_used(t, self._stream) for t in state]
+        betas, eps, decay, most, skip = settings
+        norm = ops.adamw(parameters, gradients, *state, rate[0], *places, rate[1], *betas, eps, decay, scale, most, skip)
         torch.autograd.graph.increment_version([*parameters, *state])
         return norm

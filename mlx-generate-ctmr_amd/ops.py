@@ -1037,7 +1037,8 @@ def adamw(parameters: Sequence[Tensor], gradients: Sequence[Tensor], exp_avg: Te
           beta1: float, beta2: float, eps: float, decay: float, scale: float, most: float, skip: bool) -> Tensor:
     """``ctmr_adamw``: a step of parameters without gaps, of ``counts`` values and ``elems`` types, in place; the gradients'
     norm, 0-d fp32."""
-    like, sizes = _list_on_device([exp_avg, *parameters, *gradients]), _sizes_of(tuple(counts), tuple(elems))
+    state = [exp_avg, exp_avg_sq, master, steps] if lr_tensor is None else [exp_avg, exp_avg_sq, master, steps, lr_tensor]
+    like, sizes = _list_on_device([*state, *parameters, *gradients]), _sizes_of(tuple(counts), tuple(elems))
     norm = torch.empty((), device=like.device, dtype=torch.float32)
     desc = _lib.AdamwDesc(lr, beta1, beta2, eps, decay, scale, most, skip)
     with _on(like):
