@@ -604,6 +604,16 @@ int ctmr_adamw(const ctmr_adamw_desc* desc, int32_t count, void* const* paramete
                const int64_t* sizes, const int32_t* elems, const int64_t* starts, const int64_t* master_starts,
                float* exp_avg, float* exp_avg_sq, float* master, int64_t* steps, const float* lr, float* norm,
                void* workspace, size_t workspace_bytes, void* stream);
+/* The same where each of `parameters` parameters has steps of its own: parameter n's t is the
+ * list's less missed[n] (device memory, 1 at least), for parameters that steps left out.
+ * Entry i of the lists is parameter numbers[i] (host memory, rising; NULL: i); the missed
+ * of the others grows by one with a step that is taken. */
+int64_t ctmr_adamw_workspace_bytes(int32_t count, const int64_t* sizes, int32_t parameters);
+int ctmr_adamw_counted(const ctmr_adamw_desc* desc, int32_t count, void* const* data, const void* const* gradients,
+                       const int64_t* sizes, const int32_t* elems, const int64_t* starts, const int64_t* master_starts,
+                       float* exp_avg, float* exp_avg_sq, float* master, int64_t* steps, int32_t parameters,
+                       const int32_t* numbers, int64_t* missed, const float* lr, float* norm, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -155,6 +155,8 @@ _PROTOTYPES = {
     "ctmr_scale_tensors": (_c_int, [_c_i32, _vp, _vp, _vp, _vp, _vp]),
     "ctmr_clip_gradients": (_c_int, [_c_i32, _vp, _vp, _vp, _f, _vp, _vp, _sz, _vp]),
     "ctmr_adamw": (_c_int, [ctypes.POINTER(AdamwDesc), _c_i32] + [_vp] * 13 + [_sz, _vp]),
+    "ctmr_adamw_workspace_bytes": (_c_i64, [_c_i32, _vp, _c_i32]),
+    "ctmr_adamw_counted": (_c_int, [ctypes.POINTER(AdamwDesc), _c_i32] + [_vp] * 10 + [_c_i32] + [_vp] * 5 + [_sz, _vp]),
 }
 
 _lock = threading.Lock()

@@ -6,7 +6,8 @@
 //   m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
 //   w -= lr decay w + lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
 // with w the parameter, or its fp32 copy where the parameter has 16 bits and gets
-// the copy rounded.  Squares are added in fp64, which none of the types' values
+// the copy rounded, and t its own steps: all of the list's but those it had no
+// gradient in.  Squares are added in fp64, which none of the types' values
 // leave; moments, copies and all arithmetic of the step are fp32.
 //
 // The tensors of a list are passed in the kernels' arguments, so a launch takes up
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(kThreads) void square_sums_kernel(List list, double
 // What a step reads: the norm and the factor first, as ctmr_gradient_norm leaves them.
 struct Control {
   float norm, factor;
-  float lr_decay, rate, root, go;  // lr decay, lr / (1 - b1^t), 1 / sqrt(1 - b2^t), whether there is a step
+  float lr_decay, go;  // lr decay, whether there is a step
 };
 
 // Without a limit the norm, which may be infinite or NaN, has no part in it.
@@ -141,26 +142,47 @@ __global__ __launch_bounds__(1024) void finish_norm_kernel(const double* sums, i
   }
 }
 
-// The control of a step from the norm (count 0: none is taken) and the steps so far.
+// What the bias corrections make of a parameter's steps.
+struct Correction {
+  float rate, root;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+};
+
+// The control of a step from the norm (count 0: none is taken) and the steps so far, and the corrections of each of
+// `parameters`, a thread each; `missed`: the steps that they had no part in, or null.
 __global__ __launch_bounds__(1024) void begin_step_kernel(const double* sums, int count, ctmr_adamw_desc d, const float* lr,
-                                                          int64_t* steps, Control* control, float* norm) {
+                                                          int64_t* steps, int parameters, const int64_t* missed,
+                                                          Control* control, Correction* corrections, float* norm) {
+  const int64_t before = steps[0];  // the first thread writes it after the barrier
   double sum = 0.0;
   for (int i = threadIdx.x; i < count; i += 1024) sum += sums[i];
   sum = block_sum<16>(sum);
-  if (threadIdx.x != 0) return;
   Control c;
   c.norm = (float)(sqrt(sum) * fabs((double)d.scale));
   c.factor = count > 0 ? clip_factor(c.norm, d.scale, d.most) : d.scale;
   const bool go = !d.skip || fabsf(c.norm) < INFINITY;
-  const int64_t t = steps[0] + (go ? 1 : 0);
-  if (go) steps[0] = t;
+  const int64_t now = before + (go ? 1 : 0);
   const double rate = lr ? (double)lr[0] : d.lr;
+  for (int i = threadIdx.x; i < parameters; i += 1024) {
+    const double t = (double)max(now - (missed ? missed[i] : (int64_t)0), (int64_t)1);
+    corrections[i] = {(float)(rate / (1.0 - pow(d.beta1, t))), (float)(1.0 / sqrt(1.0 - pow(d.beta2, t)))};
+  }
+  if (threadIdx.x != 0) return;
+  if (go) steps[0] = now;
   c.lr_decay = (float)(rate * d.decay);
-  c.rate = (float)(rate / (1.0 - pow(d.beta1, (double)t)));
-  c.root = (float)(1.0 / sqrt(1.0 - pow(d.beta2, (double)t)));
   c.go = go ? 1.f : 0.f;
   *control = c;
   if (norm) norm[0] = c.norm;
+}
+
+// Counts a step as missed for parameters that had no gradient, if it is taken.
+constexpr int kMostNumbers = 960;
+struct Numbers {
+  int number[kMostNumbers];
+  int count;
+};
+__global__ __launch_bounds__(kThreads) void count_missed_kernel(Numbers list, const Control* control, int64_t* missed) {
+  const int i = blockIdx.x * kThreads + threadIdx.x;
+  if (i < list.count && control->go != 0.f) ++missed[list.number[i]];
 }
 
 template <typename T>
@@ -208,13 +230,15 @@ struct StepEntry {
   const void* gradient;
   int64_t count;
   int64_t start, master;  // of its moments and its fp32 copy
-  int first, elem;
+  int first;
+  unsigned elem : 2, number : 30;  // its correction's
 };
 constexpr int kMostSteps = 80;
 struct StepList {
   StepEntry entry[kMostSteps];
   float *m, *v, *master;
   const Control* control;
+  const Correction* corrections;
   float beta1, beta2, eps;
   float rest1, rest2;  // 1 - beta
   int64_t chunk;
@@ -269,7 +293,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(StepList list) {
   const int64_t at = (blockIdx.x - e.first) * list.chunk, count = min(list.chunk, e.count - at);
   const Control c = *list.control;
   if (c.go == 0.f) return;
-  const StepRule rule = {c.factor, c.lr_decay, c.rate, c.root, list.beta1, list.beta2, list.rest1, list.rest2, list.eps};
+  const Correction by = list.corrections[e.number];
+  const StepRule rule = {c.factor, c.lr_decay, by.rate, by.root, list.beta1, list.beta2, list.rest1, list.rest2, list.eps};
   float *m = list.m + e.start + at, *v = list.v + e.start + at;
   float* master = list.master ? list.master + e.master + at : nullptr;
   auto step = [&](auto* p, const auto* g) { step_values(rule, p + at, g + at, m, v, master, count); };
@@ -353,7 +378,88 @@ int check_workspace(const void* ws, size_t bytes, int64_t need) {
 }
 
 constexpr int64_t kControlBytes = 64;
-static_assert(sizeof(Control) <= kControlBytes && sizeof(List) + sizeof(Sums) + 16 <= 4096 && sizeof(StepList) <= 4096, "argument sizes");
+constexpr int64_t kCorrectionAt = 32;  // of all parameters' where they have the same steps
+static_assert(sizeof(Control) <= kCorrectionAt && kCorrectionAt + sizeof(Correction) <= kControlBytes && sizeof(List) + sizeof(Sums) + 16 <= 4096 && sizeof(StepList) <= 4096 &&
+                  sizeof(Numbers) + 16 <= 4096,
+              "argument sizes");
+constexpr int kMostParameters = 1 << 24;
+
+// The steps of `parameters` parameters, `count` of which have a gradient: entry i of the lists is number numbers[i], in
+// order (null: i).  missed or null: all have the same steps.
+int adamw(const ctmr_adamw_desc* d, int count, void* const* data, const void* const* gradients, const int64_t* sizes,
+          const int32_t* elems, const int64_t* starts, const int64_t* master_starts, float* exp_avg, float* exp_avg_sq,
+          float* master, int64_t* steps, int parameters, const int32_t* numbers, int64_t* missed, const float* lr, float* norm,
+          void* workspace, size_t workspace_bytes, int64_t need, hipStream_t st) {
+  int rc = check_list(count, data, sizes, elems);
+  if (!rc) rc = check_list(count, gradients, sizes, elems);
+  if (rc) return rc;
+  if (!(d->beta1 >= 0.0 && d->beta1 < 1.0 && d->beta2 >= 0.0 && d->beta2 < 1.0) || !(d->eps >= 0.0) ||
+      !(d->decay >= 0.0) || !(d->most > 0.f) || std::isnan(d->scale) || !(d->lr >= 0.0))
+    return fail(CTMR_E_INVALID, "bad step: betas in [0, 1), eps, decay and lr not negative, most positive");
+  if (!steps || (count > 0 && (!starts || !exp_avg || !exp_avg_sq))) return fail(CTMR_E_INVALID, "null pointer");
+  bool half = false;
+  for (int i = 0; i < count; ++i) {
+    half |= elems[i] != CTMR_ELEM_F32;
+    if (starts[i] < 0 || starts[i] % 4 != 0) return fail(CTMR_E_INVALID, "starts must be multiples of 4");
+    if (numbers && (numbers[i] >= parameters || numbers[i] < (i > 0 ? numbers[i - 1] + 1 : 0)))
+      return fail(CTMR_E_INVALID, "numbers must rise and be below the parameters'");
+  }
+  if (half && (!master || !master_starts)) return fail(CTMR_E_INVALID, "16-bit parameters need an fp32 copy");
+  for (int i = 0; half && i < count; ++i)
+    if (elems[i] != CTMR_ELEM_F32 && (master_starts[i] < 0 || master_starts[i] % 4 != 0))
+      return fail(CTMR_E_INVALID, "starts must be multiples of 4");
+  if ((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq | (uintptr_t)master) & 15) != 0)
+    return fail(CTMR_E_INVALID, "moments and copies must start on 16-byte boundaries");
+  rc = check_workspace(workspace, workspace_bytes, need);
+  if (rc) return rc;
+  Control* control = static_cast<Control*>(workspace);
+  double* sums = reinterpret_cast<double*>((char*)workspace + kControlBytes);
+  Correction* corrections = reinterpret_cast<Correction*>(
+      (char*)workspace + (missed ? ctmr_gradients_workspace_bytes(count, sizes) : kCorrectionAt));
+  int sums_taken = 0;
+  if (d->most < INFINITY || d->skip || norm) {
+    rc = square_sums(count, gradients, sizes, elems, sums, &sums_taken, st);
+    if (rc) return rc;
+  }
+  hipLaunchKernelGGL(begin_step_kernel, dim3(1), dim3(1024), 0, st, sums, sums_taken, *d, lr, steps, missed ? parameters : 1,
+                     missed, control, corrections, norm);
+  rc = check_launch("begin_step");
+  if (rc) return rc;
+  StepList list;
+  list.m = exp_avg, list.v = exp_avg_sq, list.master = master, list.control = control, list.corrections = corrections;
+  list.beta1 = (float)d->beta1, list.beta2 = (float)d->beta2, list.eps = (float)d->eps;
+  list.rest1 = (float)(1.0 - d->beta1), list.rest2 = (float)(1.0 - d->beta2), list.chunk = kChunk;
+  int i = 0;
+  while (i < count) {
+    int chunks = 0;
+    for (list.entries = 0; i < count && list.entries < kMostSteps; ++i) {
+      if (sizes[i] == 0) continue;
+      StepEntry& e = list.entry[list.entries++];
+      e.parameter = data[i], e.gradient = gradients[i], e.count = sizes[i], e.start = starts[i];
+      e.master = elems[i] != CTMR_ELEM_F32 ? master_starts[i] : 0;
+      e.first = chunks, e.elem = (unsigned)elems[i], e.number = (unsigned)(!missed ? 0 : numbers ? numbers[i] : i);
+      chunks += (int)ceil_div(sizes[i], kChunk);
+    }
+    if (list.entries == 0) break;
+    hipLaunchKernelGGL(adamw_kernel, dim3(chunks), dim3(kThreads), 0, st, list);
+    rc = check_launch("adamw");
+    if (rc) return rc;
+  }
+  if (!missed || count == parameters) return CTMR_OK;
+  Numbers absent;
+  for (int number = 0, at = 0; number < parameters;) {
+    for (absent.count = 0; number < parameters && absent.count < kMostNumbers; ++number) {
+      if (at < count && (numbers ? numbers[at] : at) == number) ++at;
+      else absent.number[absent.count++] = number;
+    }
+    if (absent.count == 0) break;
+    hipLaunchKernelGGL(count_missed_kernel, dim3((unsigned)ceil_div(absent.count, kThreads)), dim3(kThreads), 0, st, absent,
+                       control, missed);
+    rc = check_launch("count_missed");
+    if (rc) return rc;
+  }
+  return CTMR_OK;
+}
 
 }  // namespace
 }  // namespace ctmr
@@ -428,61 +534,36 @@ int ctmr_clip_gradients(int32_t count, void* const* gradients, const int64_t* si
   });
 }
 
+int64_t ctmr_adamw_workspace_bytes(int32_t count, const int64_t* sizes, int32_t parameters) {
+  const int64_t bytes = ctmr_gradients_workspace_bytes(count, sizes);
+  if (bytes < 0) return bytes;
+  if (parameters < count) return fail(CTMR_E_INVALID, "more gradients than parameters");
+  if (parameters > kMostParameters) return fail(CTMR_E_UNSUPPORTED, "too many parameters");
+  return bytes + round_up(parameters * (int64_t)sizeof(Correction), 16);
+}
+
 int ctmr_adamw(const ctmr_adamw_desc* d, int32_t count, void* const* parameters, const void* const* gradients,
                const int64_t* sizes, const int32_t* elems, const int64_t* starts, const int64_t* master_starts,
                float* exp_avg, float* exp_avg_sq, float* master, int64_t* steps, const float* lr, float* norm,
                void* workspace, size_t workspace_bytes, void* stream) {
   if (!d) return fail(CTMR_E_INVALID, "null descriptor");
-  int rc = check_list(count, parameters, sizes, elems);
-  if (!rc) rc = check_list(count, gradients, sizes, elems);
-  if (rc) return rc;
-  if (!(d->beta1 >= 0.0 && d->beta1 < 1.0 && d->beta2 >= 0.0 && d->beta2 < 1.0) || !(d->eps >= 0.0) ||
-      !(d->decay >= 0.0) || !(d->most > 0.f) || std::isnan(d->scale) || !(d->lr >= 0.0))
-    return fail(CTMR_E_INVALID, "bad step: betas in [0, 1), eps, decay and lr not negative, most positive");
-  if (!steps || (count > 0 && (!starts || !exp_avg || !exp_avg_sq))) return fail(CTMR_E_INVALID, "null pointer");
-  bool half = false;
-  for (int i = 0; i < count; ++i) {
-    half |= elems[i] != CTMR_ELEM_F32;
-    if (starts[i] < 0 || starts[i] % 4 != 0) return fail(CTMR_E_INVALID, "starts must be multiples of 4");
-  }
-  if (half && (!master || !master_starts)) return fail(CTMR_E_INVALID, "16-bit parameters need an fp32 copy");
-  for (int i = 0; half && i < count; ++i)
-    if (elems[i] != CTMR_ELEM_F32 && (master_starts[i] < 0 || master_starts[i] % 4 != 0))
-      return fail(CTMR_E_INVALID, "starts must be multiples of 4");
-  if ((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq | (uintptr_t)master) & 15) != 0)
-    return fail(CTMR_E_INVALID, "moments and copies must start on 16-byte boundaries");
-  rc = check_workspace(workspace, workspace_bytes, ctmr_gradients_workspace_bytes(count, sizes));
-  if (rc) return rc;
-  hipStream_t st = (hipStream_t)stream;
-  Control* control = static_cast<Control*>(workspace);
-  double* sums = reinterpret_cast<double*>((char*)workspace + kControlBytes);
-  int sums_taken = 0;
-  if (d->most < INFINITY || d->skip || norm) {
-    rc = square_sums(count, gradients, sizes, elems, sums, &sums_taken, st);
-    if (rc) return rc;
-  }
-  hipLaunchKernelGGL(begin_step_kernel, dim3(1), dim3(1024), 0, st, sums, sums_taken, *d, lr, steps, control, norm);
-  rc = check_launch("begin_step");
-  if (rc) return rc;
-  StepList list;
-  list.m = exp_avg, list.v = exp_avg_sq, list.master = master, list.control = control;
-  list.beta1 = (float)d->beta1, list.beta2 = (float)d->beta2, list.eps = (float)d->eps;
-  list.rest1 = (float)(1.0 - d->beta1), list.rest2 = (float)(1.0 - d->beta2), list.chunk = kChunk;
-  int i = 0;
-  while (i < count) {
-    int chunks = 0;
-    for (list.entries = 0; i < count && list.entries < kMostSteps; ++i) {
-      if (sizes[i] == 0) continue;
-      list.entry[list.entries++] = {parameters[i], gradients[i], sizes[i], starts[i],
-                                    elems[i] != CTMR_ELEM_F32 ? master_starts[i] : 0, chunks, elems[i]};
-      chunks += (int)ceil_div(sizes[i], kChunk);
-    }
-    if (list.entries == 0) break;
-    hipLaunchKernelGGL(adamw_kernel, dim3(chunks), dim3(kThreads), 0, st, list);
-    rc = check_launch("adamw");
-    if (rc) return rc;
-  }
-  return CTMR_OK;
+  const int64_t need = ctmr_gradients_workspace_bytes(count, sizes);
+  if (need < 0) return (int)need;
+  return adamw(d, count, parameters, gradients, sizes, elems, starts, master_starts, exp_avg, exp_avg_sq, master, steps, count,
+               nullptr, nullptr, lr, norm, workspace, workspace_bytes, need, (hipStream_t)stream);
+}
+
+int ctmr_adamw_counted(const ctmr_adamw_desc* d, int32_t count, void* const* data, const void* const* gradients,
+                       const int64_t* sizes, const int32_t* elems, const int64_t* starts, const int64_t* master_starts,
+                       float* exp_avg, float* exp_avg_sq, float* master, int64_t* steps, int32_t parameters,
+                       const int32_t* numbers, int64_t* missed, const float* lr, float* norm, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  if (!d) return fail(CTMR_E_INVALID, "null descriptor");
+  const int64_t need = ctmr_adamw_workspace_bytes(count, sizes, parameters);
+  if (need < 0) return (int)need;
+  if (!missed && parameters > 0) return fail(CTMR_E_INVALID, "null pointer");
+  return adamw(d, count, data, gradients, sizes, elems, starts, master_starts, exp_avg, exp_avg_sq, master, steps, parameters,
+               numbers, missed, lr, norm, workspace, workspace_bytes, need, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -727,20 +727,24 @@ def _layouts_of(tensors: Sequence[Tensor]) -> tuple[list, ...]:
 class AdamW:
     """AdamW steps of a list of fp32, bf16 and fp16 parameters, in place and without a copy to the host.
 
-    ``w -= lr * weight_decay * w + lr * m_hat / (sqrt(v_hat) + eps)`` with the moments' usual bias corrections, all in
-    fp32.  Parameters of 16 bits have fp32 copies that the steps are made on, so that small steps are not lost to rounding;
-    what else changes such a parameter has to change its copy too (``load_masters``).
+    ``w -= lr * weight_decay * w + lr * m_hat / (sqrt(v_hat) + eps)`` with the moments' usual bias corrections, each
+    parameter's by the steps that it had a gradient in, all in fp32.  Parameters of 16 bits have fp32 copies that the steps
+    are made on, so that small steps are not lost to rounding; what else changes such a parameter has to change its copy
+    too (``load_masters``).
 
     ``max_norm`` clips each step's gradients as ``clip_gradients`` does, without writing them; ``skip_non_finite`` leaves a
     step out whose gradients have a norm that is not finite (for steps with a loss scale).
 
-    The settings may be changed between steps, ``lr`` by a number or a 0-d fp32 tensor on the parameters' device.
-    The state is public, on the parameters' device, and may be written or bound anew between steps: ``steps`` (0-d int64), ``exp_avg``,
-    ``exp_avg_sq`` and ``master`` (1-d fp32; ``master`` of the 16-bit parameters only), where each parameter's values start
-    on a multiple of ``GRAIN``, in the list's order.  Steps may be captured into a graph; ``lr`` may then be a 0-d fp32 tensor.  Replays
-    raise no ``_version``: from the capture on, ``fast_fp32`` and ``maisi`` derive what they keep of the parameters (packed and
-    fused weights) anew at each use, until ``fast_fp32.settle_weights`` after the last replay; a ``maisi.UNetGraph`` recorded
-    before the capture keeps the old ones.
+    The settings may be changed between steps, ``lr`` by a number or a 0-d fp32 tensor on the parameters' device.  The
+    state is public, on the parameters' device, and may be written or bound anew between steps: ``steps`` (0-d int64),
+    ``missed`` (1-d int64: those of them that each parameter had no gradient in), ``exp_avg``, ``exp_avg_sq`` and ``master``
+    (1-d fp32; ``master`` of the 16-bit parameters only), where each parameter's values start on a multiple of ``GRAIN``, in
+    the list's order.
+
+    Steps may be captured into a graph; ``lr`` may then be a 0-d fp32 tensor.  Replays raise no ``_version``: from the
+    capture on, ``fast_fp32`` and ``maisi`` derive what they keep of the parameters (packed and fused weights) anew at each
+    use, until ``fast_fp32.settle_weights`` after the last replay; a ``maisi.UNetGraph`` recorded before the capture keeps
+    the old ones.
 
     Raises:
         ValueError: on an empty list, other types, parameters that are not on one GPU, share memory or have gaps in it, and
@@ -772,6 +776,7 @@ class AdamW:
         make = lambda n: torch.zeros(n, device=device, dtype=torch.float32)
         self.exp_avg, self.exp_avg_sq, self.master = make(total), make(total), make(room)
         self.steps = torch.zeros((), device=device, dtype=torch.int64)
+        self.missed = torch.zeros(len(self.parameters), device=device, dtype=torch.int64)
         self._state_layouts = _layouts_of(self._state())
         self._stream = _stream_of(self.steps)
         self.load_masters()
@@ -795,7 +800,7 @@ class AdamW:
         return self._taken
 
     def _state(self) -> list[Tensor]:
-        return [self.exp_avg, self.exp_avg_sq, self.master, self.steps]
+        return [self.exp_avg, self.exp_avg_sq, self.master, self.steps, self.missed]
 
     def _checked_state(self) -> list[Tensor]:
         """The state's tensors, which may have been bound anew: the kernels take their addresses."""
@@ -805,7 +810,7 @@ class AdamW:
         except (AttributeError, TypeError, RuntimeError):  # no tensors, or of a layout without strides
             alike = False
         if not alike:
-            raise ValueError("exp_avg, exp_avg_sq, master and steps must keep their shapes, types and device, without gaps")
+            raise ValueError("exp_avg, exp_avg_sq, master, steps and missed must keep their shapes, types and device, without gaps")
         return state
 
     def _rate(self, lr: Union[float, Tensor]) -> Union[float, Tensor]:
@@ -839,15 +844,18 @@ class AdamW:
 
     def state_dict(self) -> dict[str, Tensor]:
         """The state's tensors themselves, by name."""
-        return {name: getattr(self, name) for name in ("steps", "exp_avg", "exp_avg_sq", "master")}
+        return {name: getattr(self, name) for name in ("steps", "exp_avg", "exp_avg_sq", "master", "missed")}
 
     @torch.no_grad()
     def load_state_dict(self, state: Mapping[str, Tensor]) -> None:
-        """Copies a ``state_dict`` of the same parameters; the parameters of 16 bits become their copies, rounded.
+        """Copies a ``state_dict`` of the same parameters (without ``missed`` none missed a step); the parameters of 16 bits
+        become their copies, rounded.
 
         Raises:
             ValueError: on other names, or tensors of other shapes or types."""
         own = self.state_dict()
+        if "missed" not in state:
+            state = {**state, "missed": torch.zeros_like(self.missed)}
         if set(state) != set(own) or any(state[n].shape != t.shape or state[n].dtype != t.dtype for n, t in own.items()):
             raise ValueError("the state is of other parameters")
         for name, t in own.items():
@@ -877,12 +885,13 @@ class AdamW:
     @torch.no_grad()
     def step(self, gradients: Sequence[Optional[Tensor]], *, lr: Union[float, Tensor, None] = None,
              gradient_scale: float = 1.0) -> Tensor:
-        """One step from a gradient for each parameter (None: it and its moments stay); returns the norm, before clipping, of
-        the gradients times ``gradient_scale``, which is what the step takes (a loss scale's inverse).
+        """One step from a gradient for each parameter (None, but not for all: it and its moments stay, and the step does not
+        count among its own); returns the norm, before clipping, of the gradients times ``gradient_scale``, which is what the
+        step takes (a loss scale's inverse).
 
         Raises:
             ValueError: on gradients of another count, or of other shapes, types or devices than their parameters', an ``lr``
-                or scale that is not finite, and settings, parameters or a state that have been changed to what the constructor
+                or scale that is not finite, gradients that are all None, and settings, parameters or a state that have been changed to what the constructor
                 would not have or make.
             NotImplementedError: on forward-mode (dual) tensors."""
         gradients = list(gradients)
@@ -895,11 +904,13 @@ class AdamW:
         if not math.isfinite(scale):
             raise ValueError(f"gradient_scale must be finite; got {scale}")
         plan = (self.parameters, self._counts, self._elems, self._starts, self._master_starts, range(len(gradients)))
+        given = ()  # numbers of the parameters that have a gradient; all of them
         layouts = self._layouts
         if any(g is None for g in gradients):
             used = [g is not None for g in gradients]
             of = lambda values: list(itertools.compress(values, used))
             plan, layouts, gradients = tuple(map(of, plan)), tuple(map(of, layouts)), of(gradients)
+            given = plan[-1]
         parameters, *places, numbers = plan
         self._check_parameters(parameters, layouts, numbers)
         try:  # gradients laid out as their parameters need no other check than this
@@ -914,6 +925,7 @@ class AdamW:
         if self._stream is not None and ops._raw_stream(state[0].device) != self._stream:
             state = [_used(t, self._stream) for t in state]
         betas, eps, decay, most, skip = settings
-        norm = ops.adamw(parameters, gradients, *state, rate[0], *places, rate[1], *betas, eps, decay, scale, most, skip)
+        norm = ops.adamw(parameters, gradients, *state[:4], rate[0], *places, rate[1], *betas, eps, decay, scale, most, skip,
+                         state[4], given)
         torch.autograd.graph.increment_version([*parameters, *state])
         return norm

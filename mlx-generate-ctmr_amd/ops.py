@@ -934,7 +934,7 @@ def _(q, k, v, slopes, prefixes, plan, bucket_plan, table, out, rest, lse, dout,
 class _Sizes:
     """Value counts and types of a list of tensors as the library takes them, and its workspace's bytes."""
 
-    __slots__ = ("count", "sizes", "elems", "nbytes")
+    __slots__ = ("count", "sizes", "elems", "nbytes", "step_bytes")
 
     def __init__(self, counts: Sequence[int], kinds: Sequence):  # torch's types, or the library's
         self.count = len(counts)
@@ -942,6 +942,15 @@ class _Sizes:
         self.elems = (ctypes.c_int32 * self.count)(*[ELEMENTS.get(k, k) for k in kinds])
         self.nbytes = _lib.check(_lib.lib().ctmr_gradients_workspace_bytes(self.count, self.sizes),
                                  "ctmr_gradients_workspace_bytes")
+        self.step_bytes: dict[int, int] = {}
+
+    def bytes_of_step(self, parameters: int) -> int:
+        """A step's workspace, of these and the parameters without a gradient."""
+        nbytes = self.step_bytes.get(parameters)
+        if nbytes is None:
+            nbytes = self.step_bytes[parameters] = _lib.check(
+                _lib.lib().ctmr_adamw_workspace_bytes(self.count, self.sizes, parameters), "ctmr_adamw_workspace_bytes")
+        return nbytes
 
 
 _sizes_of = functools.lru_cache(maxsize=64)(_Sizes)
@@ -1030,24 +1039,33 @@ def _places(starts: tuple[int, ...]):
     return (ctypes.c_int64 * len(starts))(*starts)
 
 
-@_custom_op("ctmr::adamw", ("parameters", "exp_avg", "exp_avg_sq", "master", "steps"))
+@functools.lru_cache(maxsize=64)
+def _numbers(numbers: tuple[int, ...]):
+    return (ctypes.c_int32 * len(numbers))(*numbers)
+
+
+@_custom_op("ctmr::adamw", ("parameters", "exp_avg", "exp_avg_sq", "master", "steps", "missed"))
 def adamw(parameters: Sequence[Tensor], gradients: Sequence[Tensor], exp_avg: Tensor, exp_avg_sq: Tensor, master: Tensor,
           steps: Tensor, lr_tensor: Optional[Tensor], counts: Sequence[int], elems: Sequence[int], starts: Sequence[int],
           master_starts: Sequence[int], lr: float,
-          beta1: float, beta2: float, eps: float, decay: float, scale: float, most: float, skip: bool) -> Tensor:
-    """``ctmr_adamw``: a step of parameters without gaps, of ``counts`` values and ``elems`` types, in place; the gradients'
-    norm, 0-d fp32."""
-    state = [exp_avg, exp_avg_sq, master, steps] if lr_tensor is None else [exp_avg, exp_avg_sq, master, steps, lr_tensor]
+          beta1: float, beta2: float, eps: float, decay: float, scale: float, most: float, skip: bool, missed: Tensor,
+          numbers: Sequence[int]) -> Tensor:
+    """``ctmr_adamw_counted``: a step of parameters without gaps, of ``counts`` values and ``elems`` types, in place; the
+    gradients' norm, 0-d fp32.  ``numbers``: the parameters' places in ``missed``; empty where all have a gradient."""
+    state = [exp_avg, exp_avg_sq, master, steps, missed, *(() if lr_tensor is None else (lr_tensor,))]
     like, sizes = _list_on_device([*state, *parameters, *gradients]), _sizes_of(tuple(counts), tuple(elems))
     norm = torch.empty((), device=like.device, dtype=torch.float32)
     desc = _lib.AdamwDesc(lr, beta1, beta2, eps, decay, scale, most, skip)
+    parameters_kept = missed.numel()
     with _on(like):
-        ws = _workspace(sizes.nbytes, like.device)
-        _lib.check(_lib.lib().ctmr_adamw(
+        nbytes = sizes.bytes_of_step(parameters_kept)
+        ws = _workspace(nbytes, like.device)
+        _lib.check(_lib.lib().ctmr_adamw_counted(
             ctypes.byref(desc), sizes.count, _addresses(parameters), _addresses(gradients), sizes.sizes, sizes.elems,
             _places(tuple(starts)), _places(tuple(master_starts)), exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
-            master.data_ptr() if master.numel() else None, steps.data_ptr(), _ptr(lr_tensor), norm.data_ptr(), ws.data_ptr(),
-            sizes.nbytes, _raw_stream(like.device)), "ctmr_adamw")
+            master.data_ptr() if master.numel() else None, steps.data_ptr(), parameters_kept,
+            _numbers(tuple(numbers)) if numbers else None, missed.data_ptr(), _ptr(lr_tensor), norm.data_ptr(), ws.data_ptr(),
+            nbytes, _raw_stream(like.device)), "ctmr_adamw_counted")
         _note_writes(parameters)
     return norm
 
