@@ -590,7 +590,7 @@ def self_attention_tokens(tokens: Tensor, weights: Mapping[str, Tensor], *, head
 
     Raises:
         ValueError: on tokens that are not (B, L, C), heads that do not divide C, positions without sections or the
-            reverse, and what ``rotary`` and ``attention`` refuse."""
+            reverse, weights with a position bias without buckets, and what ``rotary`` and ``attention`` refuse."""
     _activation(tokens, "tokens", 3)
     n, length, c = (int(s) for s in tokens.shape)
     heads = int(heads)
@@ -601,7 +601,10 @@ def self_attention_tokens(tokens: Tensor, weights: Mapping[str, Tensor], *, head
     names = [f"{prefix}.to_{m}" for m in ("q", "k", "v")]
     used = [weights[f"{m}.{part}"] for m in [*names, *([f"{prefix}.out_proj"] if include_fc else [])]
             for part in (("weight", "bias") if qkv_bias or m.endswith("out_proj") else ("weight",))]
-    table = None if buckets is None else weights[f"{prefix}.position_bias"]
+    name = f"{prefix}.position_bias"
+    if buckets is None and name in weights:
+        raise ValueError(f"{name} needs buckets, without which it would be left out")
+    table = None if buckets is None else weights[name]
     token = _graph_token(tokens, *used, table) if torch.is_grad_enabled() and tokens.is_cuda else None
     w = torch.cat([_like(weights[f"{m}.weight"], tokens, f"{m}.weight", 2) for m in names])
     b = torch.cat([_like(weights[f"{m}.bias"], tokens, f"{m}.bias", 1) for m in names]) if qkv_bias else None

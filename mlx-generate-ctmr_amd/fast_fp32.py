@@ -800,7 +800,14 @@ def self_attention_tokens(tokens: Tensor, weights: Mapping[str, Tensor], *, head
     """Q/K/V projections, multi-head self-attention and optional ``out_proj`` on ``(B, L, C)``
     tokens (``fast_fp32.self_attention_tokens``, :352-392).  32-wide heads run the HIP flash
     kernel on one fused Q/K/V projection; other head widths use PyTorch's attention on the
-    GPU, as the reference falls back to ``mx.fast.scaled_dot_product_attention``."""
+    GPU, as the reference falls back to ``mx.fast.scaled_dot_product_attention``.
+
+    Raises:
+        ValueError: on tokens that are not fp32 on the GPU, and weights with a learned position bias, which
+            ``differentiable.self_attention_tokens`` applies and this attention would leave out."""
+    if f"{prefix}.position_bias" in weights:
+        raise ValueError(f"{prefix}.position_bias needs buckets (maisi.spatial_attention or "
+                         "differentiable.self_attention_tokens); this attention has none")
     tokens = _rows(tokens, "tokens")
     n, length, c = (int(s) for s in tokens.shape)
     names = ("q", "k", "v")

@@ -100,18 +100,30 @@ def condition_embedding(timesteps: Tensor, class_labels: Optional[Tensor], spaci
 # attention (attention.py:92-160), NDHWC: tokens are the voxel rows
 # ---------------------------------------------------------------------------
 def spatial_attention(x: Tensor, weights: Mapping[str, Tensor], *, num_groups: int, eps: float,
-                      num_head_channels: int, include_fc: bool) -> Tensor:
+                      num_head_channels: int, include_fc: bool, buckets: Optional[df.PositionBuckets] = None) -> Tensor:
     """Residual self-attention over all voxels of NDHWC ``x`` (attention.py:92-160): group
     norm (HIP), tokens are the NDHWC rows as they lie, Q/K/V + flash attention + out_proj.  The
-    residual sum carries per-channel statistics for the group norm that reads it next."""
+    residual sum carries per-channel statistics for the group norm that reads it next.
+
+    ``buckets`` of the voxels (``PackedVolumes([(D, H, W)], device).buckets(...)``) add the bias
+    ``weights["attn.position_bias"]`` that ``spatial_attention_volumes`` has learned.
+
+    Raises:
+        ValueError: on channels that ``num_head_channels`` does not divide, a position bias without buckets (the
+            networks' own calls have none) and what the operators refuse."""
     n, d, h, w, c = x.shape
     if c % num_head_channels != 0:
         raise ValueError("num_channels must be divisible by num_head_channels")
     heads = c // num_head_channels
     scale = float(num_head_channels) ** -0.5
     hidden = ff.group_norm(x, weights["norm.weight"], weights["norm.bias"], num_groups=num_groups, eps=eps)
-    merged = ff.self_attention_tokens(hidden.reshape(n, d * h * w, c), weights, heads=heads, scale=scale,
-                                      include_fc=include_fc)
+    tokens = hidden.reshape(n, d * h * w, c)
+    if buckets is None:
+        merged = ff.self_attention_tokens(tokens, weights, heads=heads, scale=scale, include_fc=include_fc)
+    else:
+        with torch.no_grad():
+            merged = df.self_attention_tokens(tokens, weights, heads=heads, scale=scale, include_fc=include_fc,
+                                              buckets=buckets)
     return ff.add_with_stats(x, merged.reshape(n, d, h, w, c))
 
 
