@@ -383,29 +383,31 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
 #pragma unroll
         for (int r = 0; r < 16; ++r) ds[r] *= __builtin_amdgcn_exp2f(fmaf(s[r], c, kHalf<T> ? raise - lse : -lse));
       }
-      auto hide_keys = [&](f16v& ds) {
-        // a visible key whose values were zeroed in LDS because they are not finite: no gradient is
-        const unsigned set = partial ? odd[u] >> (4 * half) : 0u;
-        if (set)
+      // (As a function of ds or db this kept ds in memory: heads of 32 with a cap past 256 spilled 112 registers, 9 so.)
+      if (masked) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) ds[r] = (set >> (8 * (r >> 2) + (r & 3))) & 1u ? NAN : ds[r];
-        if (docs)
+        for (int which = 0; which < (ST > 0 && CAP != kNoCap ? 2 : 1); ++which) {
+          f16v& hidden = which == 0 ? ds : db;
+          // a visible key whose values were zeroed in LDS because they are not finite: no gradient is
+          const unsigned set = partial ? odd[u] >> (4 * half) : 0u;
+          if (set)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int4 other = *reinterpret_cast<const int4*>(ids + k0 + 32 * u + 4 * half + 8 * w);
-            ds[4 * w] = other.x != id ? 0.f : ds[4 * w];
-            ds[4 * w + 1] = other.y != id ? 0.f : ds[4 * w + 1];
-            ds[4 * w + 2] = other.z != id ? 0.f : ds[4 * w + 2];
-            ds[4 * w + 3] = other.w != id ? 0.f : ds[4 * w + 3];
-          }
-        if (scoring.prefixed || !docs)
+            for (int r = 0; r < 16; ++r) hidden[r] = (set >> (8 * (r >> 2) + (r & 3))) & 1u ? NAN : hidden[r];
+          if (docs)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) ds[r] = 8 * (r >> 2) + (r & 3) >= limit - at ? 0.f : ds[r];
-      };
-      if (masked) hide_keys(ds);
+            for (int w = 0; w < 4; ++w) {
+              const int4 other = *reinterpret_cast<const int4*>(ids + k0 + 32 * u + 4 * half + 8 * w);
+              hidden[4 * w] = other.x != id ? 0.f : hidden[4 * w];
+              hidden[4 * w + 1] = other.y != id ? 0.f : hidden[4 * w + 1];
+              hidden[4 * w + 2] = other.z != id ? 0.f : hidden[4 * w + 2];
+              hidden[4 * w + 3] = other.w != id ? 0.f : hidden[4 * w + 3];
+            }
+          if (scoring.prefixed || !docs)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) hidden[r] = 8 * (r >> 2) + (r & 3) >= limit - at ? 0.f : hidden[r];
+        }
+      }
       const float raised = raise;  // of db
-      if constexpr (ST > 0 && CAP != kNoCap)
-        if (masked) hide_keys(db);
       if constexpr (kHalf<T>) keep_in_range<false, ND>(ds, dq, raise);
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
