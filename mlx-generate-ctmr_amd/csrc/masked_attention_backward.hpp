@@ -262,10 +262,11 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
   const T* k = static_cast<const T*>(a.k) + b * a.kb + (h / a.group) * a.kh;
   const T* v = static_cast<const T*>(a.v) + b * a.vb + (h / a.group) * a.vh;
 
-  // The matrix units round sums of 16-bit products to one side, so each ds has a bias that the table's sums over rows and
-  // keys add up (2.5e-6 of its gradient at 4096 rows, growing with their number).  Odd rows have g and all that is made of
-  // it with the other sign, and it cancels (5e-7, at any length).
-  constexpr bool kFlips = ST > 0 && sizeof(T) == 2;
+  // The matrix units round sums of 16-bit products to one side, so each dr (and with 16-bit heads each ds) has a bias that
+  // the table's sums over rows and keys add up, the more the longer they are: of the table's gradient 2.5e-6 at 4096 rows with
+  // 16-bit heads, 8e-7 with fp32 ones and 1.4e-6 at 16384.  Odd rows have g and all that is made of it with the other
+  // sign, and it cancels (below 2e-7 of a drift from 256 to 16384 rows, heads of 32 and 128).
+  constexpr bool kFlips = ST > 0;
   const float flip = kFlips && (lane & 1) ? -1.f : 1.f;
   Frag<T> qf[NK], gf[NK];
   float delta = 0.f;
@@ -295,7 +296,12 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
   if constexpr (kFlips) {
     delta *= flip;
 #pragma unroll
-    for (int s = 0; s < NK; ++s) gf[s] = __builtin_bit_cast(Frag<T>, __builtin_bit_cast(u4, gf[s]) ^ (lane & 1 ? 0x80008000u : 0u));
+    for (int s = 0; s < NK; ++s) {
+      if constexpr (sizeof(T) == 2)
+        gf[s] = __builtin_bit_cast(Frag<T>, __builtin_bit_cast(u4, gf[s]) ^ (lane & 1 ? 0x80008000u : 0u));
+      else
+        gf[s] *= flip;
+    }
   }
   const float lse = real ? a.lse[stat] : INFINITY;
   float raise = kDsRaise<T>;
