@@ -539,7 +539,8 @@ int ctmr_masked_attention_backward(const ctmr_masked_attention_desc* desc, const
  * places outside are taken as the nearest inside.  With `same` the keys lie where the rows
  * lie and key_places is not read.  table (table_rows, q_heads) of type table_elem; its
  * values are expected below 2^20 in size like scores, or below -2^100 (-inf too), which hides
- * a pair: a row left with no key gives zeros.  NaN or inf makes NaN of the rows that see a
+ * a pair by a weight of zero (its key and value have to be finite, unlike masked ones): a row
+ * left with no key gives zeros.  NaN or inf makes NaN of the rows that see a
  * key at that distance.
  * The scale, or the cap with one, is at least 2^-20 here.
  * `fine`: 16-bit softmax weights keep twice their type's bits in their products (bf16 with an

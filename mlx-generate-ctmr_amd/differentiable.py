@@ -473,8 +473,11 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, softcap: float =
     Statistics and sums are fp32; the softmax weights, and in the gradients those of the scores, are rounded to the
     inputs' type for their products (in fp16 raised by powers of two that keep them in its range).  The bias is added in
     fp32; its gradient is summed in fp32 and fp64 from all bits of each score's gradient (17 for a table of 16 bits), and
-    where it is wanted the weights keep more of theirs, so outputs may differ in the last from those without it.  A bias below -2^100
-    (-inf too) hides its pairs; NaN or inf makes NaN of the rows that see a key at that distance.  The output has ``q``'s type and lies as ``(B, Lq, Hq, D)`` in memory, so merging the heads is a view.
+    where it is wanted the weights keep more of theirs, so outputs may differ in the last from those without it.  A bias
+    below -2^100 (-inf too) hides its pairs by their weights alone, which are zero: unlike masked places, what hidden ones
+    hold has to be finite, since 0 * NaN is NaN.  A bias of NaN or inf makes NaN of the rows that see a key at that distance.
+
+    The output has ``q``'s type and lies as ``(B, Lq, Hq, D)`` in memory, so merging the heads is a view.
 
     Raises:
         ValueError: on other types, devices or shapes, a scale that is not positive and finite, a cap that is
