@@ -454,15 +454,14 @@ __global__ __launch_bounds__(kThreads, (dq_waves<T, D, ST>())) void attention_dq
                           a.d, lane);
 }
 
-template <typename T, int D, int ST>
+template <typename T, int D>
 constexpr int dkv_waves() {
-  if (ST > 0) return D * sizeof(T) >= 256 ? 1 : D * sizeof(T) == 64 ? 4 : 2;
   return D * sizeof(T) >= 256 ? 1 : D * sizeof(T) == 64 ? 4 : 2;
 }
 
 // dk and dv: 128 keys of a key head, the query tiles of its heads streaming.
 template <typename T, int D, Cap CAP, int ST>
-__global__ __launch_bounds__(kThreads, (dkv_waves<T, D, ST>())) void attention_dkv_kernel(Args a, BiasOf<ST> bias) {
+__global__ __launch_bounds__(kThreads, (dkv_waves<T, D>())) void attention_dkv_kernel(Args a, BiasOf<ST> bias) {
   constexpr int NK = D / 16, ND = D / 32;
   typedef Tile<T, D> Lds;
   __shared__ __attribute__((aligned(16))) unsigned words0[kTile];
