@@ -750,7 +750,7 @@ class AdamW:
     Steps may be captured into a graph; ``lr`` may then be a 0-d fp32 tensor.  Replays raise no ``_version``: from the
     capture on, ``fast_fp32`` and ``maisi`` derive what they keep of the parameters (packed and fused weights) anew at each
     use, until ``fast_fp32.settle_weights`` after the last replay; a ``maisi.UNetGraph`` recorded before the capture keeps
-    the old ones.
+    the old ones, and so does a pass that is recorded before the step in one capture.
 
     Raises:
         ValueError: on an empty list, other types, parameters that are not on one GPU, share memory or have gaps in it, and
