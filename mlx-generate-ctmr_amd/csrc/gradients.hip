@@ -17,8 +17,8 @@
 //
 // Bound by memory: the norm reads each gradient once, the scaling reads and writes
 // it, a step moves 28 bytes an fp32 parameter.  240 tensors of 24 blocks of 1024 channels,
-// fp32 (403 MB): the norm 52 + 26 us (5.1 TB/s; 88 + 37 behind a step's writes), its end
-// 5, the scaling 79 + 48 (22 where the norm is below the limit), the steps 159 + 184 + 186
+// fp32 (403 MB): the norm 52 + 26 us (5.1 TB/s; 79 + 27 behind a step's writes), its end
+// 5, the scaling 79 + 48 (22 where the norm is below the limit), the steps 158 + 185 + 186
 // (2.8 GB at 5.3 TB/s).  Short lists are bound by the host: 160 tensors of 16 blocks of 301
 // channels, fp16, 105 us for 18 of kernels.
 // (Chunks of four times as many values, each workgroup's own or in turns, take the 22 us

@@ -20,12 +20,15 @@
 // type for their products, half a step of it on each term of an fp32 sum.
 //
 // Bound by the matrix products and, at their side, the exponentials: 2 x 16 heads of
-// 4096 rows, every key, bf16, both kernels: heads of 32 327 us, of 64 505 (680 TFLOP/s
-// of the five products, 950 of the seven), of 128 990; fp16 378, 568, 1147 (the powers of
+// 4096 rows, every key, bf16, both kernels: heads of 32 330 us, of 64 501 (686 TFLOP/s
+// of the five products, 960 of the seven), of 128 997; fp16 383, 581, 1160 (the powers of
 // two below: two operations a score in dk and dv, half a one in dq); fp32, 2 x 8 heads of
-// 2048 rows of 32: 252 (119 of the seven, where a library product of 8192^3 reaches 153).
+// 2048 rows of 32: 251 (120 of the seven, where a library product of 8192^3 reaches 153).
 // With a position bias on 16x16x16 and its table's gradient (position_bias.hpp): bf16, heads
-// of 32 660 us, of 64 826, of 128 1870; fp32 as above on 16x16x8 318.
+// of 32 655 us, of 64 815, of 128 1858, for a table of 16 bits 605, 761, 1800, and for one
+// without a gradient 498, 650, 1621; fp32 as above on 16x16x8 318, 276 without.  dk and dv spill
+// scalar registers there (117 to 196 of the bias' arguments, 65 to 75 without a bias), and with
+// heads of 32 and 16 bits 26 to 64 vector registers.
 //
 // fp16's range is far smaller than what ds spans, so every row of dq and every key of
 // dk (a lane's column) has a power of two of its own that ds is multiplied by: the sums
@@ -201,8 +204,8 @@ __device__ __forceinline__ void add_distances(const Bias& bias, const f16v (&dr)
 }
 
 // Waves a SIMD that the registers are kept for.  16-bit, 2 x 16 heads of 4096 rows, both kernels: heads of 32 with four
-// 327 us (a few registers spill), with three 351; heads of 64 with three for dk and dv too (20 spill) 577 us, with two
-// there 505.  With a bias dq has up to 64 more sums a lane: heads of 32 with 96 columns, 8192 rows on 32x32x8, both kernels
+// 330 us (a few registers spill), with three 351; heads of 64 with three for dk and dv too (20 spill) 577 us, with two
+// there 501.  With a bias dq has up to 64 more sums a lane: heads of 32 with 96 columns, 8192 rows on 32x32x8, both kernels
 // with two 1182 us, with three 1514 (ds in two parts).
 template <typename T, int D, int ST>
 constexpr int dq_waves() {

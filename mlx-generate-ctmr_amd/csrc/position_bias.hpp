@@ -8,10 +8,11 @@
 // them, summed, in the scores' units.  Tokens have codes, places times strides, whose
 // difference is the LDS address of both pairs' values: a score costs two subtractions, two
 // reads and an addition, whatever the places and their order (without a cap the products
-// are added to it by the matrix units).  That is what bounds the forward pass: 2 x 16 heads
-// of 64, 4096 rows on 16x16x16, bf16, 255 us where no bias takes 162: 4 LDS instructions
-// where 1 was, LDS busy for 37 % of the time, vector units for 52, matrix units for 21
-// (38); no bank conflicts.  Heads of 32 187 us (116), of 128 361 (272).
+// are added to it by the matrix units).  The forward pass is bound by the latency of these
+// reads: 2 x 16 heads of 64, 4096 rows on 16x16x16, bf16, 257 us where no bias takes 163:
+// 4 LDS instructions where 1 was, and waves wait 2.5 times as long, three of them a SIMD,
+// while no unit is full (LDS 37 % of the time, vector units 52, matrix units 21 for 38; no
+// bank conflicts).  Heads of 32 187 us (116), of 128 358 (270).
 //
 // The table's gradient is the sum of the scores' gradients ds of a head over all pairs of
 // a distance.  For a row i, ds_ij counts by the key's place on each axis, so with a
@@ -21,7 +22,7 @@
 // rows' dr are then added by distance.  o is exact in bf16 and the same for all heads: it
 // streams through LDS beside the keys.  ds goes in three bf16 parts, all of fp32's bits, or
 // two, 2^-17 of it, where the table has 16 bits (both kernels of the backward pass, heads of
-// 64, 4096 rows: 826 us, 775).
+// 64, 4096 rows: 815 us, 761).
 //
 // (The bias itself as a product too, of o_j and each row's r_i[c] = table[row_a(x - x_a(i))]
 // in parts, has no reads of single values, but r takes 24 to 64 registers and the product
