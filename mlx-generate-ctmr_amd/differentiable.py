@@ -748,8 +748,8 @@ class AdamW:
     the list's order.
 
     Steps may be captured into a graph; ``lr`` may then be a 0-d fp32 tensor.  Replays raise no ``_version``: from the
-    capture on, ``fast_fp32`` and ``maisi`` derive what they keep of the parameters (packed and fused weights) anew at each
-    use, until ``fast_fp32.settle_weights`` after the last replay; a ``maisi.UNetGraph`` recorded before the capture keeps
+    capture on (and of inference tensors from their first step on) ``fast_fp32`` and ``maisi`` derive what they keep of the
+    parameters (packed and fused weights) anew at each use, until ``fast_fp32.settle_weights`` after the last one; a ``maisi.UNetGraph`` recorded before the capture keeps
     the old ones, and so does a pass that is recorded before the step in one capture.
 
     Raises:
@@ -772,6 +772,7 @@ class AdamW:
         self._given = self._taken = self._checked(betas, eps, weight_decay, max_norm, skip_non_finite)
         self.betas, self.eps, self.weight_decay, self.max_norm, self.skip_non_finite = self._taken
         self._layouts = _layouts_of(self.parameters)
+        self._unversioned = [p for p in self.parameters if p.is_inference()]
         self._counts = tuple(p.numel() for p in self.parameters)
         self._elems = tuple(ops.ELEMENTS[p.dtype] for p in self.parameters)
         self._starts, total = self._places(self.parameters)
@@ -934,4 +935,5 @@ class AdamW:
         norm = ops.adamw(parameters, gradients, *state[:4], rate[0], *places, rate[1], *betas, eps, decay, scale, most, skip,
                          state[4], given)
         torch.autograd.graph.increment_version([*parameters, *state])
+        ops._mark_rewritten(self._unversioned)
         return norm

@@ -172,7 +172,8 @@ _retained = threading.local()
 
 def _version(t: Tensor) -> int:
     """``t._version``, or -1 for an inference tensor (created under ``torch.inference_mode``), which
-    has no version counter; such a tensor cannot be modified in place outside inference mode."""
+    has no version counter; torch modifies no such tensor in place outside inference mode, and what
+    ``differentiable.AdamW`` writes of them is marked (``ops._mark_rewritten``)."""
     return -1 if t.is_inference() else t._version
 
 

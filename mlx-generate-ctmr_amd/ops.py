@@ -975,15 +975,19 @@ def _list_on_device(tensors: Sequence[Tensor]) -> Tensor:
     return tensors[0]
 
 
-# Storages that a call recorded into a HIP graph writes, by identity.  A replay writes them without a step of their version
-# counters, so that nothing derived of them may be kept by these (``fast_fp32.cached_derived``).
+# Storages that a call recorded into a HIP graph writes, by identity, and those of inference tensors that a call wrote.  A
+# replay writes them without a step of their version counters, and inference tensors have none, so that nothing derived of
+# them may be kept by these (``fast_fp32.cached_derived``).
 _rewritten: dict[int, "weakref.ref[torch.UntypedStorage]"] = {}
 
 
 def _note_writes(tensors: Sequence[Tensor]) -> None:
     """Marks what a call writes, if it is recorded into a graph."""
-    if not torch.cuda.is_current_stream_capturing():
-        return
+    if torch.cuda.is_current_stream_capturing():
+        _mark_rewritten(tensors)
+
+
+def _mark_rewritten(tensors: Sequence[Tensor]) -> None:
     for t in tensors:
         storage = t.untyped_storage()
         key = id(storage)

@@ -57,6 +57,27 @@ def test_kept_again_once_settled(ctmr, captured):
         ff._caches.remove((cache, lock))
 
 
+def test_steps_of_inference_tensors_are_noticed(ctmr, monkeypatch):
+    """They have no version; a step marks them instead."""
+    f, ff, lock = ctmr.differentiable, ctmr.fast_fp32, threading.RLock()
+    monkeypatch.setattr(f, "_on_gpu", lambda t, name: None)
+    monkeypatch.setattr(f, "_stream_of", lambda t: None)
+    with torch.inference_mode():
+        w = torch.zeros(4)
+        monkeypatch.setattr(f.ops, "adamw", lambda *a: w.add_(1))
+    other, cache = torch.zeros(4), {}
+    o = f.AdamW([w, other])
+    kept = _derived(ff, cache, lock, w)
+    assert _derived(ff, cache, lock, w) is kept
+    try:
+        with torch.inference_mode():
+            o.step([torch.zeros(4), torch.zeros(4)])
+        assert bool((_derived(ff, cache, lock, w) == 1).all())
+        assert _derived(ff, cache, lock, other) is _derived(ff, cache, lock, other)
+    finally:
+        ctmr.ops._rewritten.clear()
+
+
 def test_marks_end_with_their_memory(ctmr, captured):
     t = torch.zeros(4)
     captured([t, t.view(2, 2)])
